@@ -1,7 +1,8 @@
-"""MI355X-native flash grouped-query attention (decode incl. paged/fp8 KV caches, causal, sliding-window, MLA and sparse-index prefill, and the causal, sliding-window and MLA prefill backward).
+"""MI355X-native flash grouped-query attention (decode incl. paged/fp8/int8 KV caches, their writing and eviction, causal, sliding-window, MLA and sparse-index prefill, and the causal, sliding-window and MLA prefill backward).
 
 The kernels live in libfgqa.so (HIP, gfx950); ``flash_gqa`` is the Python host
-interface over its C ABI (include/fgqa.h).
+interface over its C ABI (include/fgqa.h), and ``kv_cache`` that of the paged
+cache's operators (include/fgqa_kv.h).
 """
 from ._lib import FgqaError, LIB_PATH, lib, status_string  # noqa: F401
 from .flash_gqa import (  # noqa: F401
@@ -31,6 +32,11 @@ from .flash_gqa import (  # noqa: F401
     prefill_kernel_name,
     prepare_prefill,
     PreparedLaunch,
+)
+from .kv_cache import (  # noqa: F401
+    accumulate_kv_weights_paged,
+    append_kv_paged,
+    evict_kv_paged,
 )
 
 __version__ = "0.1.0"

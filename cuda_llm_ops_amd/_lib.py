@@ -1,4 +1,4 @@
-"""ctypes binding of libfgqa.so, the C ABI declared in include/fgqa.h.
+"""ctypes binding of libfgqa.so, the C ABI declared in include/fgqa.h and include/fgqa_kv.h.
 
 The library is built in-tree (``make -C cuda_llm_ops_amd/csrc`` or
 ``__graft_entry__.build()``).  Loading fails loudly when it is missing: there
@@ -186,6 +186,108 @@ class SparsePrefillArgs(ctypes.Structure):
     ]
 
 
+FGQA_KV_INT8 = 2
+
+# The fields of ``fgqa_kv_cache`` (include/fgqa_kv.h), with which the argument
+# blocks below begin (its size is a multiple of its alignment, so they lie as in
+# the nested struct).
+_KV_CACHE = [
+    ("k_cache", ctypes.c_void_p),
+    ("v_cache", ctypes.c_void_p),
+    ("k_scales", ctypes.c_void_p),
+    ("v_scales", ctypes.c_void_p),
+    ("kv_dtype", ctypes.c_int32),
+    ("num_kv_heads", ctypes.c_int32),
+    ("head_dim", ctypes.c_int32),
+    ("page_size", ctypes.c_int32),
+    ("num_pages", ctypes.c_int32),
+    ("k_scale", ctypes.c_float),
+    ("v_scale", ctypes.c_float),
+    ("k_stride", _I64x3),
+    ("v_stride", _I64x3),
+    ("k_scales_stride", _I64x2),
+    ("v_scales_stride", _I64x2),
+]
+
+
+class KvAppendArgs(ctypes.Structure):
+    """Mirror of ``fgqa_kv_append_args`` (include/fgqa_kv.h)."""
+    _fields_ = _KV_CACHE + [
+        ("k_new", ctypes.c_void_p),
+        ("v_new", ctypes.c_void_p),
+        ("k_new_stride", _I64x3),
+        ("v_new_stride", _I64x3),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("seqlens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("max_new", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+    ]
+
+
+class DecodeBlocksArgs(ctypes.Structure):
+    """Mirror of ``fgqa_decode_blocks_args`` (include/fgqa_kv.h)."""
+    _fields_ = _KV_CACHE + [
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("seqlens", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("max_seqlen", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("q_stride", _I64x2),
+        ("o_stride", _I64x2),
+        ("block_table_stride", ctypes.c_int64),
+        ("split_tokens", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class KvWeightsArgs(ctypes.Structure):
+    """Mirror of ``fgqa_kv_weights_args`` (include/fgqa_kv.h)."""
+    _fields_ = _KV_CACHE + [
+        ("q", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p),
+        ("q_stride", _I64x2),
+        ("weights_stride", _I64x2),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("seqlens", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("max_seqlen", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class KvEvictArgs(ctypes.Structure):
+    """Mirror of ``fgqa_kv_evict_args`` (include/fgqa_kv.h)."""
+    _fields_ = _KV_CACHE + [
+        ("weights", ctypes.c_void_p),
+        ("new_weights", ctypes.c_void_p),
+        ("weights_stride", _I64x2),
+        ("new_weights_stride", _I64x2),
+        ("block_table", ctypes.c_void_p),
+        ("new_block_table", ctypes.c_void_p),
+        ("block_table_stride", ctypes.c_int64),
+        ("new_block_table_stride", ctypes.c_int64),
+        ("seqlens", ctypes.c_void_p),
+        ("new_seqlens", ctypes.c_void_p),
+        ("kept", ctypes.c_void_p),
+        ("batch", ctypes.c_int32),
+        ("max_seqlen", ctypes.c_int32),
+        ("weights_len", ctypes.c_int32),
+        ("budget", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+    ]
+
+
 _FORMATS = {ctypes.c_void_p: "P", ctypes.c_int32: "i", ctypes.c_float: "f", ctypes.c_int64: "q",
             ctypes.c_size_t: "N", _I64x2: "2q", _I64x3: "3q"}
 
@@ -219,6 +321,10 @@ pack_prefill = ArgsPacker(PrefillArgs)
 pack_paged = ArgsPacker(PagedDecodeArgs)
 pack_backward = ArgsPacker(BackwardArgs)
 pack_sparse = ArgsPacker(SparsePrefillArgs)
+pack_kv_append = ArgsPacker(KvAppendArgs)
+pack_decode_blocks = ArgsPacker(DecodeBlocksArgs)
+pack_kv_weights = ArgsPacker(KvWeightsArgs)
+pack_kv_evict = ArgsPacker(KvEvictArgs)
 
 
 class FgqaError(RuntimeError):
@@ -265,6 +371,13 @@ def lib() -> ctypes.CDLL:
         L.fgqa_prefill_backward_bf16.argtypes = [ctypes.POINTER(BackwardArgs), ctypes.c_void_p]
         L.fgqa_sparse_prefill_bf16.restype = ctypes.c_int
         L.fgqa_sparse_prefill_bf16.argtypes = [ctypes.POINTER(SparsePrefillArgs), ctypes.c_void_p]
+        for name, args in (("fgqa_kv_append", KvAppendArgs), ("fgqa_decode_blocks", DecodeBlocksArgs),
+                           ("fgqa_kv_weights", KvWeightsArgs), ("fgqa_kv_evict", KvEvictArgs)):
+            getattr(L, name).restype = ctypes.c_int
+            getattr(L, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        L.fgqa_decode_blocks_workspace_bytes.restype = ctypes.c_int
+        L.fgqa_decode_blocks_workspace_bytes.argtypes = [ctypes.POINTER(DecodeBlocksArgs),
+                                                         ctypes.POINTER(ctypes.c_size_t)]
         L.fgqa_status_string.restype = ctypes.c_char_p
         L.fgqa_status_string.argtypes = [ctypes.c_int]
         L.fgqa_version.restype = ctypes.c_int

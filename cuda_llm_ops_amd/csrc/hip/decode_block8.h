@@ -1,0 +1,241 @@
+// One decode item over a paged cache of 8-bit codes with block scales (included
+// by decode_flash_gqa.hip, whose kernels share the work out and merge the items).
+//
+// The mathematics is that of dec_item, on codes: with K = sK c_K and V = sV c_V
+// (one scale per page and KV head),
+//     s_t = scale sK(t) (q . c_K[t]),   o = sum_t softmax(s)_t sV(t) c_V[t].
+// Codes are widened exactly (to bf16 for K, fp16 for V).  sK multiplies the
+// scores in fp32.  sV is folded into P, relative to the largest sV met so far
+// (vref), and P sV / vref is rounded to fp16 at 2^14 times its value: 11 bits
+// where the bf16 decode keeps 8, and no loss down to 2^-29 of the largest P.
+//
+// K never goes through LDS: lane (l16, g4) reads the 16-byte pieces 16 g4 and
+// 64 + 16 g4 of token l16's row, and the MFMA's contraction index is reordered
+// so that these are its operands (Q is loaded in the same order).  V's rows go
+// through LDS as codes, half the bytes of bf16 rows, and come back transposed
+// (ds_read_b64_tr_b8: 8 tokens of one column per lane).
+#pragma once
+
+#include "fgqa_device.h"
+#include "kv_codes.h"
+
+namespace fgqa {
+
+constexpr int kDec8RowStride = 144;   // LDS bytes of a V row: 16 rows spread over all 64 banks
+constexpr int kDec8TileBytes = kDecStep * kDec8RowStride;
+constexpr int kDec8ScaleBytes = kDecStep * 2 * 4;
+constexpr int kDec8MergeBytes = kDecWaves * 16 * kHeadDim * 4 + kDecWaves * 16 * 2 * 4;
+constexpr int kDec8WaveBytes = kDec8TileBytes + kDec8ScaleBytes;
+constexpr int kDec8SmemBytes =
+    kDecWaves * kDec8WaveBytes > kDec8MergeBytes ? kDecWaves * kDec8WaveBytes : kDec8MergeBytes;
+constexpr float kDec8PScale = 16384.f;   // P's scale in fp16
+
+__device__ __forceinline__ f32x4_t mfma16_f16(f16x8_t a, f16x8_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Transposed LDS read of bytes: within 16 lanes, lane i gets bytes 0 .. 7 of
+// column i of the 8 x 16 bytes whose row j lies at the addresses of lanes 2j
+// (columns 0 .. 7) and 2j + 1 (8 .. 15).
+__device__ __forceinline__ u32x2_t lds_read_tr8(const unsigned char* p) {
+    typedef int s32x2_t __attribute__((ext_vector_type(2)));
+    const s32x2_t v = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (__attribute__((address_space(3))) s32x2_t*)(__attribute__((address_space(3))) void*)(p));
+    return __builtin_bit_cast(u32x2_t, v);
+}
+
+// As dec_item: tokens [t_begin, t_end) (not empty, t_begin a multiple of 128)
+// of one sequence and kv head by 4 waves.
+template <int kCode>
+__device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* smem, int t_begin, int t_end, int kvh,
+                                          int b, int tid, bool whole, int64_t slot0) {
+    const int lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int l16 = lane & 15;
+    const int g4 = lane >> 4;
+    unsigned char* vl = smem + wave * kDec8WaveBytes;
+    float* sl = reinterpret_cast<float*>(vl + kDec8TileBytes);   // [32] K scales, [32] V scales
+
+    // Q^T as the B operand: lane holds Q[h = l16] at the elements that its
+    // pieces of K hold; heads >= G are zero.
+    bf16x8_t qop[4];
+    {
+        const bool hv = l16 < p.group;
+        const __bf16* qrow = p.q + b * p.q_sb + (int64_t)(kvh * p.group + (hv ? l16 : 0)) * p.q_sh;
+        const u32x4_t zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            const u32x4_t t = *reinterpret_cast<const u32x4_t*>(qrow + 64 * (kk / 2) + 16 * g4 + 8 * (kk % 2));
+            qop[kk] = as_bf16x8(hv ? t : zero);
+        }
+    }
+
+    float m_run = -INFINITY;
+    float l_run = 0.f;   // this lane's share of the rowsum of head l16
+    float vref = __uint_as_float(0x00800000u);   // largest |V scale| so far
+    f32x4_t oacc[8];
+#pragma unroll
+    for (int db = 0; db < 8; ++db) oacc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    const unsigned char* kbase = reinterpret_cast<const unsigned char*>(p.k) + kvh * p.k_sh + g4 * 16;
+    const unsigned char* vbase = reinterpret_cast<const unsigned char*>(p.v) + kvh * p.v_sh;
+    const float* kscales = p.k_scales + kvh * p.ks_sh;
+    const float* vscales = p.v_scales + kvh * p.vs_sh;
+    const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
+    const int pmask = (1 << p.page_shift) - 1;
+    const int v_row = lane >> 3, v_chunk = lane & 7;
+    const int n_steps = (t_end - t_begin + kDecStep - 1) / kDecStep;
+    for (int st = wave; st < n_steps; st += kDecWaves) {
+        const int t0 = t_begin + st * kDecStep;
+        // Tokens past the item's end reuse its last one (masked below).
+        u32x4_t kreg[2][2], vreg[4];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+            const int tok = min(t0 + 16 * tb + l16, t_end - 1);
+            const int page = min(max(bt[tok >> p.page_shift], 0), p.num_pages - 1);
+            const unsigned char* row = kbase + (int64_t)page * p.k_sb + (int64_t)(tok & pmask) * p.k_ss;
+            kreg[tb][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row));
+            kreg[tb][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row + 64));
+            if (g4 == 0) {
+                sl[16 * tb + l16] = kscales[(int64_t)page * p.ks_sp];
+                sl[kDecStep + 16 * tb + l16] = vscales[(int64_t)page * p.vs_sp];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int tok = min(t0 + 8 * r + v_row, t_end - 1);
+            const int page = min(max(bt[tok >> p.page_shift], 0), p.num_pages - 1);
+            vreg[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
+                vbase + (int64_t)page * p.v_sb + (int64_t)(tok & pmask) * p.v_ss + v_chunk * 16));
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            *reinterpret_cast<u32x4_t*>(vl + (8 * r + v_row) * kDec8RowStride + v_chunk * 16) = vreg[r];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+
+        // S^T = K Q^T (codes), K as the A operand
+        f32x4_t s[2];
+        float ks[8], vs[8];
+        float vmax = vref;
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+            s[tb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                s[tb] = mfma16(codes_to_bf16<kCode>(kreg[tb][j][0], kreg[tb][j][1]), qop[2 * j], s[tb]);
+                s[tb] = mfma16(codes_to_bf16<kCode>(kreg[tb][j][2], kreg[tb][j][3]), qop[2 * j + 1], s[tb]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                ks[4 * tb + i] = sl[16 * tb + 4 * g4 + i] * p.scale_log2;
+                vs[4 * tb + i] = sl[kDecStep + 16 * tb + 4 * g4 + i];
+                vmax = fmaxf(vmax, fabsf(vs[4 * tb + i]));
+            }
+        }
+        vmax = xor_max(xor_max(vmax, 16), 32);
+
+        // Online softmax for head l16 over tokens t0 + 16*tb + 4*g4 + i.
+        float x[8];
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int tok = t0 + (j >> 2) * 16 + g4 * 4 + (j & 3);
+            x[j] = tok < t_end ? s[j >> 2][j & 3] * ks[j] : -INFINITY;
+            tmax = fmaxf(tmax, x[j]);
+        }
+        tmax = xor_max(xor_max(tmax, 16), 32);
+        const float m_new = fmaxf(m_run, tmax);   // finite: every step holds a valid token
+        const float alpha = fast_exp2(m_run - m_new);
+        const float vinv = __builtin_amdgcn_rcpf(vmax);
+        const float oalpha = alpha * (vref * vinv);
+        const float pscale = vinv * kDec8PScale;
+        float psum = 0.f;
+        f16x8_t pop;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float pv = fast_exp2(x[j] - m_new);
+            psum += pv;
+            pop[j] = (_Float16)(pv * (vs[j] * pscale));
+        }
+        l_run = l_run * alpha + psum;
+        m_run = m_new;
+        vref = vmax;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) oacc[db] *= oalpha;
+
+        // V^T as the A operand: tokens 4*g4 + {0..3} and 16 + 4*g4 + {0..3}
+        // of column 16*db + l16, those whose P this lane holds.  Row j of the
+        // group's 8 is addressed by lanes 2j and 2j + 1.
+        const int row = l16 >> 1;
+        const unsigned char* vsrc =
+            vl + (4 * g4 + (row & 3) + 16 * (row >> 2)) * kDec8RowStride + 8 * (l16 & 1);
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+            const u32x2_t c = lds_read_tr8(vsrc + 16 * db);
+            oacc[db] = mfma16_f16(codes_to_f16<kCode>(c[0], c[1]), pop, oacc[db]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+
+    l_run = xor_sum(xor_sum(l_run, 16), 32);
+
+    // Merge the 4 waves in LDS (reusing the staging area).
+    __syncthreads();
+    float* ow = reinterpret_cast<float*>(smem);   // [wave][16][128]
+    float* mlw = ow + kDecWaves * 16 * kHeadDim;  // [wave][16][2]
+    const float oscale = vref * (1.f / kDec8PScale);
+#pragma unroll
+    for (int db = 0; db < 8; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ow[(wave * 16 + l16) * kHeadDim + db * 16 + g4 * 4 + i] = oacc[db][i] * oscale;
+    if (g4 == 0) {
+        mlw[(wave * 16 + l16) * 2 + 0] = m_run;
+        mlw[(wave * 16 + l16) * 2 + 1] = l_run;
+    }
+    __syncthreads();
+
+    const int h = tid >> 4;
+    const int d0 = (tid & 15) * 8;
+    if (h >= p.group) return;
+    float mw[kDecWaves];
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kDecWaves; ++w) {
+        mw[w] = mlw[(w * 16 + h) * 2];
+        M = fmaxf(M, mw[w]);
+    }
+    float L = 0.f;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kDecWaves; ++w) {
+        const float c = (mw[w] == -INFINITY) ? 0.f : fast_exp2(mw[w] - M);
+        L += c * mlw[(w * 16 + h) * 2 + 1];
+        const float* src = ow + (w * 16 + h) * kHeadDim + d0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += c * src[j];
+    }
+    const int qh = kvh * p.group + h;
+    if (whole) {
+        const float inv = 1.f / L;
+        bf16x8_t out;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) out[j] = (__bf16)(acc[j] * inv);
+        *reinterpret_cast<bf16x8_t*>(p.o + b * p.o_sb + qh * p.o_sh + d0) = out;
+        if (p.lse != nullptr && (tid & 15) == 0) p.lse[(int64_t)b * p.hq + qh] = M * kLn2 + logf(L);
+    } else {
+        const int64_t slot = slot0 + h;
+        float* po = p.part_o + slot * kHeadDim + d0;
+        *reinterpret_cast<f32x4_t*>(po) = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
+        *reinterpret_cast<f32x4_t*>(po + 4) = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
+        if ((tid & 15) == 0) {
+            p.part_ml[slot * 2 + 0] = M;
+            p.part_ml[slot * 2 + 1] = L;
+        }
+    }
+}
+
+}  // namespace fgqa

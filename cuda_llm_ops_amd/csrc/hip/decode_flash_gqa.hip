@@ -39,6 +39,7 @@
 
 #include "fgqa_device.h"
 #include "fgqa_internal.h"
+#include "../host/kv_plan.h"
 
 namespace fgqa {
 
@@ -68,10 +69,14 @@ struct DecodeParams {
     int page_shift;
     int num_pages;      // page indices are clamped to [0, num_pages)
     float v_scale;      // multiplies O (the fp8 V scale; 1 otherwise)
+    // block scales of an 8-bit cache, strides {page, head}
+    const float* k_scales;
+    const float* v_scales;
+    int64_t ks_sp, ks_sh, vs_sp, vs_sh;
 };
 
-// Cache layouts the decode items read.
-enum DecKv { kKvContig = 0, kKvPagedBf16 = 1, kKvPagedFp8 = 2 };
+// Cache layouts the decode items read (the last two: codes with block scales).
+enum DecKv { kKvContig = 0, kKvPagedBf16 = 1, kKvPagedFp8 = 2, kKvBlocksFp8 = 3, kKvBlocksInt8 = 4 };
 
 // 16 OCP fp8 e4m3 values -> 16 bf16 (exact: every e4m3 value is a bf16 value).
 __device__ __forceinline__ void fp8x16_to_bf16(u32x4_t in, u32x4_t* lo, u32x4_t* hi) {
@@ -423,6 +428,25 @@ __device__ __forceinline__ void dec_item(const DecodeParams& p, unsigned char* s
     }
 }
 
+}  // namespace fgqa
+
+#include "decode_block8.h"
+
+namespace fgqa {
+
+// The item of each layout, and its LDS.
+template <int kKv>
+constexpr int kDecItemSmem = kKv >= kKvBlocksFp8 ? kDec8SmemBytes : kDecSmemBytes;
+
+template <int kKv, int kSeg>
+__device__ __forceinline__ void dec_item_of(const DecodeParams& p, unsigned char* smem, int t_begin, int t_end, int kvh,
+                                            int b, int tid, bool whole, int64_t slot0) {
+    if constexpr (kKv >= kKvBlocksFp8)
+        dec_item8<kKv == kKvBlocksFp8 ? kCodeFp8 : kCodeInt8>(p, smem, t_begin, t_end, kvh, b, tid, whole, slot0);
+    else
+        dec_item<kKv, kSeg>(p, smem, t_begin, t_end, kvh, b, tid, whole, slot0);
+}
+
 // Pass 1 over the full (split, kv head, batch) grid.  kPair (an even number
 // of kv heads): 8-wave workgroups over (split, kv head pair, batch), waves 0-3
 // on kv head 2j and waves 4-7 on kv head 2j + 1, so that the two 256-byte
@@ -620,7 +644,8 @@ __device__ __forceinline__ int seq_blocks(int len) {
 template <int kKv, int kSeg = 0, bool kPair = false>
 __global__ __launch_bounds__(kPair ? 2 * kDecThreads : kDecThreads) void decode_list_kernel(DecodeParams p) {
     constexpr int kThreads = kPair ? 2 * kDecThreads : kDecThreads;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[(kPair ? 2 : 1) * kDecSmemBytes];
+    constexpr int kSmem = kDecItemSmem<kKv>;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[(kPair ? 2 : 1) * kSmem];
     // wave-uniform (readfirstlane), so the buffer resources built from the
     // head stay scalar
     const int half = kPair ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kDecThreads)) : 0;
@@ -722,7 +747,7 @@ __global__ __launch_bounds__(kPair ? 2 * kDecThreads : kDecThreads) void decode_
             slot = (int64_t)(2 * team + (blk == 0 ? 1 : 0)) * p.hkv + kvh;
         }
         __syncthreads();   // the previous item's merge buffers alias the staging area
-        dec_item<kKv, kSeg>(p, smem + half * kDecSmemBytes, t_begin, t_end, kvh, b, tid, whole, slot * p.group);
+        dec_item_of<kKv, kSeg>(p, smem + half * kSmem, t_begin, t_end, kvh, b, tid, whole, slot * p.group);
         if (p.work == nullptr) {
             g0 += (t_end - t_begin + plan::kDecodeStepRound - 1) / plan::kDecodeStepRound;
             ++b;
@@ -1038,6 +1063,8 @@ int decode_run(const fgqa_decode_args* a, void* stream, bool noalloc) {
     p.page_shift = 0;
     p.num_pages = 0;
     p.v_scale = 1.f;
+    p.k_scales = p.v_scales = nullptr;
+    p.ks_sp = p.ks_sh = p.vs_sp = p.vs_sh = 0;
     p.q = static_cast<const __bf16*>(a->q);
     p.k = static_cast<const __bf16*>(a->k);
     p.v = static_cast<const __bf16*>(a->v);
@@ -1132,14 +1159,14 @@ extern "C" int fgqa_decode_paged_workspace_bytes(const fgqa_decode_paged_args* a
     return FGQA_OK;
 }
 
-extern "C" int fgqa_decode_paged(const fgqa_decode_paged_args* a, void* stream) {
-    int st = plan::validate_paged(a);
-    if (st != FGQA_OK) return st;
-    st = plan::validate_paged_pointers(a);
-    if (st != FGQA_OK) return st;
+namespace fgqa {
+namespace {
+// The paged decode of validated arguments; `blocks`: a cache with block scales,
+// e4m3 or int8 (`a` describes the rest of the call).
+int paged_run(const fgqa_decode_paged_args* a, const fgqa_kv_cache* blocks, void* stream) {
     if (a->batch == 0) return FGQA_OK;
     DecodePlan plan;
-    st = plan::plan_paged(a, &plan);
+    int st = plan::plan_paged(a, &plan);
     if (st != FGQA_OK) return st;
 
     DecodeParams p;
@@ -1179,6 +1206,16 @@ extern "C" int fgqa_decode_paged(const fgqa_decode_paged_args* a, void* stream) 
     p.page_shift = shift;
     p.num_pages = a->num_pages;
     p.v_scale = a->v_scale;
+    p.k_scales = p.v_scales = nullptr;
+    p.ks_sp = p.ks_sh = p.vs_sp = p.vs_sh = 0;
+    if (blocks != nullptr) {
+        p.k_scales = blocks->k_scales;
+        p.v_scales = blocks->v_scales;
+        p.ks_sp = blocks->k_scales_stride[0];
+        p.ks_sh = blocks->k_scales_stride[1];
+        p.vs_sp = blocks->v_scales_stride[0];
+        p.vs_sh = blocks->v_scales_stride[1];
+    }
 
     const hipStream_t s = static_cast<hipStream_t>(stream);
     int32_t* work = nullptr;
@@ -1205,7 +1242,10 @@ extern "C" int fgqa_decode_paged(const fgqa_decode_paged_args* a, void* stream) 
                                  (int64_t)a->page_size * a->v_stride[1] * 2 < ((int64_t)1 << 31);
         const int seg = !small_pages ? 0 : a->page_size >= 32 ? 32 : a->page_size >= 4 ? a->page_size : 0;
         auto pass1 = [&] {
-            if (fp8) {
+            if (blocks != nullptr) {
+                if (blocks->kv_dtype == FGQA_KV_INT8) launch_list<kKvBlocksInt8, 0>(p, plan.nsplit, cus, s);
+                else launch_list<kKvBlocksFp8, 0>(p, plan.nsplit, cus, s);
+            } else if (fp8) {
                 switch (seg >= 8 ? seg : 0) {
                     case 32: launch_list<kKvPagedFp8, 32>(p, plan.nsplit, cus, s); break;
                     case 16: launch_list<kKvPagedFp8, 16>(p, plan.nsplit, cus, s); break;
@@ -1226,4 +1266,33 @@ extern "C" int fgqa_decode_paged(const fgqa_decode_paged_args* a, void* stream) 
     }
     if (hipGetLastError() != hipSuccess) return FGQA_ERR_HIP;
     return FGQA_OK;
+}
+
+}  // namespace
+}  // namespace fgqa
+
+extern "C" int fgqa_decode_paged(const fgqa_decode_paged_args* a, void* stream) {
+    int st = plan::validate_paged(a);
+    if (st != FGQA_OK) return st;
+    st = plan::validate_paged_pointers(a);
+    if (st != FGQA_OK) return st;
+    return paged_run(a, nullptr, stream);
+}
+
+// ---------------------------------------------------------------- 8-bit cache with block scales
+extern "C" int fgqa_decode_blocks_workspace_bytes(const fgqa_decode_blocks_args* a, size_t* bytes) {
+    if (bytes == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
+    const int st = plan::validate_decode_blocks(a);
+    if (st != FGQA_OK) return st;
+    const fgqa_decode_paged_args p = plan::as_decode_paged(a);
+    return fgqa_decode_paged_workspace_bytes(&p, bytes);
+}
+
+extern "C" int fgqa_decode_blocks(const fgqa_decode_blocks_args* a, void* stream) {
+    int st = plan::validate_decode_blocks(a);
+    if (st != FGQA_OK) return st;
+    st = plan::validate_decode_blocks_pointers(a);
+    if (st != FGQA_OK) return st;
+    const fgqa_decode_paged_args p = plan::as_decode_paged(a);
+    return paged_run(&p, &a->cache, stream);
 }

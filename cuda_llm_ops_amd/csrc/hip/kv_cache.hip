@@ -1,0 +1,708 @@
+// The paged KV cache's operators (include/fgqa_kv.h): writing tokens, the
+// attention weight of each cached token, and eviction.
+//
+// A block is one page of one KV head: page_size rows of 128 elements.  Blocks
+// in 8 bits hold codes c and one scale s, standing for s * c.  The scales that
+// are made here are powers of two, so that x / s is exact and a code has one
+// rounding, growing a block's scale rounds its int8 codes once more and its
+// e4m3 codes not at all (but where they become subnormal), and the result does
+// not depend on the order of anything.
+#include <math.h>
+
+#include "fgqa_internal.h"
+#include "kv_codes.h"
+#include "../host/kv_plan.h"
+
+namespace fgqa {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kLanesPerRow = 8;                        // 16 elements of a row each
+constexpr int kRowsPerSweep = kWave / kLanesPerRow;
+
+// The cache as the kernels take it: index 0 is K, 1 is V; strides in bytes (the scales' in elements).
+struct CacheParams {
+    unsigned char* data[2];
+    float* scales[2];      // or null
+    float scale[2];        // of the whole cache, without block scales
+    int64_t page[2], slot[2], head[2];
+    int64_t scale_page[2], scale_head[2];
+    int hkv, page_shift, num_pages;
+};
+
+CacheParams cache_params(const fgqa_kv_cache& c) {
+    CacheParams p;
+    const int elem = c.kv_dtype == FGQA_KV_BF16 ? 2 : 1;
+    const int64_t* st[2] = {c.k_stride, c.v_stride};
+    const int64_t* sc[2] = {c.k_scales_stride, c.v_scales_stride};
+    void* data[2] = {c.k, c.v};
+    float* scales[2] = {c.k_scales, c.v_scales};
+    for (int i = 0; i < 2; ++i) {
+        p.data[i] = static_cast<unsigned char*>(data[i]);
+        p.scales[i] = scales[i];
+        p.page[i] = st[i][0] * elem;
+        p.slot[i] = st[i][1] * elem;
+        p.head[i] = st[i][2] * elem;
+        p.scale_page[i] = sc[i][0];
+        p.scale_head[i] = sc[i][1];
+    }
+    p.scale[0] = c.k_scale;
+    p.scale[1] = c.v_scale;
+    p.hkv = c.num_kv_heads;
+    p.page_shift = plan::log2_of(c.page_size);
+    p.num_pages = c.num_pages;
+    return p;
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int m = 1; m < kWave; m *= 2) v = xor_max(v, m);
+    return v;
+}
+
+// x / s: exact for a power of two, else correctly rounded.
+struct Divisor {
+    float s, inv;
+    bool pow2;
+    __device__ explicit Divisor(float scale) : s(scale), inv(1.f / scale) {
+        const uint32_t b = __float_as_uint(scale);
+        pow2 = (b & 0x7fffffu) == 0 && b >= 0x00800000u && b < 0x7f000000u;
+    }
+    __device__ f32x4_t operator()(f32x4_t x) const {
+        if (pow2) return x * inv;
+        return f32x4_t{x[0] / s, x[1] / s, x[2] / s, x[3] / s};
+    }
+};
+
+// 4 bf16 of two words -> fp32.
+__device__ __forceinline__ f32x4_t bf16x4_to_f32(uint32_t w0, uint32_t w1) {
+    return f32x4_t{__uint_as_float(w0 << 16), __uint_as_float(w0 & 0xffff0000u), __uint_as_float(w1 << 16),
+                   __uint_as_float(w1 & 0xffff0000u)};
+}
+
+// How a cache of codes is scaled: not (bf16), as a whole, or block by block.
+enum Scaling { kNone, kWhole, kBlocks };
+
+// The waves that write one block and the sweeps (of 8 rows) each holds in
+// registers: pages of up to 64 rows take a wave, larger ones a workgroup, which
+// goes over pages of more than 256 rows in several rounds, reading them twice.
+template <int kSweeps, int kBlockWaves>
+struct BlockShape {
+    static constexpr int sweeps = kSweeps, waves = kBlockWaves;
+    static constexpr int rows = kSweeps * kBlockWaves * kRowsPerSweep;   // of one round
+};
+
+// The largest of the block's waves' values.
+template <typename Shape>
+__device__ __forceinline__ float block_max(float v, float* s_max) {
+    v = wave_max(v);
+    if constexpr (Shape::waves > 1) {
+        const int wave = threadIdx.x / kWave;
+        if ((threadIdx.x & (kWave - 1)) == 0) s_max[wave] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < Shape::waves; ++w) v = fmaxf(v, s_max[w]);
+    }
+    return v;
+}
+
+// ---------------------------------------------------------------- append
+struct AppendParams {
+    CacheParams c;
+    const unsigned char* x[2];       // new K, V
+    int64_t x_b[2], x_t[2], x_h[2];  // bytes
+    const int32_t* block_table;
+    int64_t bt_stride;
+    const int32_t* seqlens;
+    const int32_t* new_lens;
+    int max_new, max_tokens;
+    int pages;                       // of one sequence that new tokens can touch
+    int64_t items;                   // batch * pages * 2 * hkv
+};
+
+// One block per item: item = ((b * pages + j) * 2 + K or V) * hkv + head, heads
+// side by side as the new rows lie.
+template <int kCode, Scaling kScaling, typename Shape>
+__global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
+    __shared__ float s_max[kWaves];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    const int64_t item = (int64_t)blockIdx.x * (kWaves / Shape::waves) + wave / Shape::waves;
+    if (item >= p.items) return;
+    const int h = (int)(item % p.c.hkv);
+    const int64_t rest = item / p.c.hkv;
+    const int kv = (int)(rest & 1);
+    const int j = (int)((rest >> 1) % p.pages);
+    const int b = (int)((rest >> 1) / p.pages);
+
+    const int len = max(p.seqlens[b], 0);
+    const int want = p.new_lens != nullptr ? min(max(p.new_lens[b], 0), p.max_new) : p.max_new;
+    if (len >= p.max_tokens) return;
+    const int end = (int)min((int64_t)len + want, (int64_t)p.max_tokens);
+    const int page_at = (len >> p.c.page_shift) + j;
+    const int64_t t0 = (int64_t)page_at << p.c.page_shift;   // the page's first token
+    if (t0 >= end) return;
+    const int page_rows = 1 << p.c.page_shift;
+    const int slot0 = (int)max((int64_t)len - t0, (int64_t)0);                // new rows: slots [slot0, slot1)
+    const int slot1 = (int)min((int64_t)end - t0, (int64_t)page_rows);
+    if (slot0 >= slot1) return;
+    const int page = p.block_table[(int64_t)b * p.bt_stride + page_at];
+    if (page < 0 || page >= p.c.num_pages) return;
+
+    const int row = lane / kLanesPerRow, chunk = lane % kLanesPerRow;
+    const int first_row = (wave % Shape::waves) * Shape::sweeps * kRowsPerSweep + row;
+    // token of slot 0 in the new rows (below 0 where the sequence's older tokens are)
+    const int64_t i0 = t0 - len;
+    const unsigned char* src = p.x[kv] + b * p.x_b[kv] + h * p.x_h[kv] + chunk * 32;
+    unsigned char* dst = p.c.data[kv] + page * p.c.page[kv] + h * p.c.head[kv] + chunk * (kCode == kCodeBf16 ? 32 : 16);
+
+    u32x4_t raw[Shape::sweeps][2];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int s = 0; s < Shape::sweeps; ++s) {
+            const int slot = base + first_row + s * kRowsPerSweep;
+            raw[s][0] = raw[s][1] = u32x4_t{0u, 0u, 0u, 0u};
+            if (slot >= slot0 && slot < slot1) {
+                const u32x4_t* r = reinterpret_cast<const u32x4_t*>(src + (i0 + slot) * p.x_t[kv]);
+                raw[s][0] = r[0];
+                raw[s][1] = r[1];
+            }
+        }
+    };
+    const int begin = slot0 / Shape::rows * Shape::rows;   // rounds from the first new row's on
+    const int last = (slot1 - 1) / Shape::rows * Shape::rows;
+
+    float scale = p.c.scale[kv];
+    if constexpr (kScaling == kBlocks) {
+        float amax = 0.f;
+        for (int base = begin; base <= last; base += Shape::rows) {
+            load(base);
+#pragma unroll
+            for (int s = 0; s < Shape::sweeps; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t w = raw[s][i / 4][i % 4];
+                    amax = fmaxf(amax, fmaxf(finite_abs(__uint_as_float(w << 16)),
+                                             finite_abs(__uint_as_float(w & 0xffff0000u))));
+                }
+        }
+        scale = block_scale<kCode>(block_max<Shape>(amax, s_max));
+        float* at = p.c.scales[kv] + page * p.c.scale_page[kv] + h * p.c.scale_head[kv];
+        bool fresh = true;
+        if (slot0 > 0) {   // older tokens in the block
+            const float old = *at;
+            if (!(scale > old)) {
+                scale = old;
+                fresh = false;
+            } else {
+                const Divisor div(scale);
+                for (int base = 0; base < slot0; base += Shape::rows)
+#pragma unroll
+                    for (int s = 0; s < Shape::sweeps; ++s) {
+                        const int slot = base + first_row + s * kRowsPerSweep;
+                        if (slot >= slot0) continue;
+                        u32x4_t* r = reinterpret_cast<u32x4_t*>(dst + slot * p.c.slot[kv]);
+                        u32x4_t w = *r;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = to_codes<kCode>(div(codes_to_f32<kCode>(w[i]) * old));
+                        *r = w;
+                    }
+            }
+        }
+        if constexpr (Shape::waves > 1) __syncthreads();   // every wave has read the old scale
+        if (fresh && lane == 0 && wave % Shape::waves == 0) *at = scale;
+    }
+    const Divisor div(scale);
+    for (int base = last; base >= begin; base -= Shape::rows) {
+        if (kScaling != kBlocks || base != last) load(base);
+#pragma unroll
+        for (int s = 0; s < Shape::sweeps; ++s) {
+            const int slot = base + first_row + s * kRowsPerSweep;
+            if (slot < slot0 || slot >= slot1) continue;
+            u32x4_t* r = reinterpret_cast<u32x4_t*>(dst + slot * p.c.slot[kv]);
+            if constexpr (kCode == kCodeBf16) {
+                r[0] = raw[s][0];
+                r[1] = raw[s][1];
+            } else {
+                u32x4_t w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = to_codes<kCode>(div(bf16x4_to_f32(raw[s][i / 2][2 * (i % 2)], raw[s][i / 2][2 * (i % 2) + 1])));
+                *r = w;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- weights
+struct WeightsParams {
+    CacheParams c;
+    const __bf16* q;
+    const float* lse;
+    float* weights;
+    int64_t q_b, q_h, w_b, w_h;
+    const int32_t* block_table;
+    int64_t bt_stride;
+    const int32_t* seqlens;
+    int max_seqlen, group, chunk, chunks;
+    float scale;
+    int64_t items;   // batch * chunks * hkv
+};
+
+// One wave per item of `chunk` tokens of one KV head, 32 at a time; heads side
+// by side.  S[h][t] = Q[h][:] . K[t][:] by v_mfma_f32_16x16x32_bf16 with the 16
+// query heads (zero past the group) as rows, so that a lane holds one token's
+// scores of 4 heads and the sum over heads takes two exchanges.  The order of
+// the head dim inside the products is free as long as Q's is the same: lane
+// group g4 takes the elements that its 16-byte pieces of the rows hold.
+template <int kCode, Scaling kScaling>
+__global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    const int l16 = lane & 15, g4 = lane >> 4;
+    const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
+    if (item >= p.items) return;
+    const int kvh = (int)(item % p.c.hkv);
+    const int64_t rest = item / p.c.hkv;
+    const int b = (int)(rest / p.chunks);
+    const int t_begin = (int)(rest % p.chunks) * p.chunk;
+    const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
+    const int t_end = min(t_begin + p.chunk, len);
+    if (t_begin >= t_end) return;
+
+    constexpr int kPieces = kCode == kCodeBf16 ? 4 : 2;   // 16-byte pieces of a row that a lane holds
+    bf16x8_t qop[4];
+    {
+        const __bf16* qrow = p.q + b * p.q_b + (int64_t)(kvh * p.group + min(l16, p.group - 1)) * p.q_h;
+        const u32x4_t zero = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            const int d = kCode == kCodeBf16 ? 32 * kk + 8 * g4 : 64 * (kk / 2) + 16 * g4 + 8 * (kk % 2);
+            const u32x4_t t = *reinterpret_cast<const u32x4_t*>(qrow + d);
+            qop[kk] = as_bf16x8(l16 < p.group ? t : zero);
+        }
+    }
+    // heads past the group: exp(. - inf) = 0.  (The difference is formed before
+    // log2(e) is multiplied in: its rounding then is relative to the small
+    // exponents of the weights that count, not to the LSE's size.)
+    float neg_lse[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int g = 4 * g4 + i;
+        const float l = p.lse[(int64_t)b * p.c.hkv * p.group + kvh * p.group + min(g, p.group - 1)];
+        neg_lse[i] = g < p.group ? -l : -INFINITY;
+    }
+    const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
+    const int pmask = (1 << p.c.page_shift) - 1;
+    const unsigned char* kbase = p.c.data[0] + kvh * p.c.head[0] + g4 * 16;
+    float* wrow = p.weights + b * p.w_b + kvh * p.w_h;
+    for (int t0 = t_begin; t0 < t_end; t0 += 32) {
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+            const int tok = t0 + 16 * tb + l16;
+            const int at = min(tok, t_end - 1);   // (past the end: its last token, not stored)
+            const int page = min(max(bt[at >> p.c.page_shift], 0), p.c.num_pages - 1);
+            const unsigned char* row = kbase + page * p.c.page[0] + (at & pmask) * p.c.slot[0];
+            float ks = p.scale;
+            if constexpr (kScaling == kBlocks) ks *= p.c.scales[0][page * p.c.scale_page[0] + kvh * p.c.scale_head[0]];
+            f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) {
+                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + 64 * j);
+                if constexpr (kCode == kCodeBf16) {
+                    s = mfma16(qop[j], as_bf16x8(w), s);
+                } else {
+                    s = mfma16(qop[2 * j], codes_to_bf16<kCode>(w[0], w[1]), s);
+                    s = mfma16(qop[2 * j + 1], codes_to_bf16<kCode>(w[2], w[3]), s);
+                }
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += fast_exp2(fmaf(s[i], ks, neg_lse[i]) * kLog2e);
+            sum = xor_sum(xor_sum(sum, 16), 32);
+            if (g4 == 0 && tok < t_end) wrow[tok] += sum;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- evict
+struct EvictParams {
+    CacheParams c;
+    const float* weights;
+    float* new_weights;
+    int64_t w_b, w_h, nw_b, nw_h;
+    const int32_t* block_table;
+    const int32_t* new_table;
+    int64_t bt_stride, nt_stride;
+    const int32_t* seqlens;
+    int32_t* new_seqlens;
+    int32_t* kept;
+    int max_seqlen, weights_len, budget, recent;
+    int pages;       // new pages of a sequence at most
+    int64_t items;   // batch * pages * 2 * hkv
+};
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectWaves = kSelectThreads / kWave;
+constexpr int kBins = 2048;
+
+// Weights in their order as unsigned numbers; NaN above all, -0 as 0.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    if (w != w) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(w + 0.f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// One workgroup per (sequence, head): the `need` largest keys of the candidates
+// (tokens before the recent ones) by their digits from the top, 11, 11 and 10
+// bits: the histogram of the keys that share the digits found so far says which
+// digit the last kept key has.  Then every wave walks its part of the row in
+// order and writes what is kept.  Integer sums only: no order matters.
+__global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
+    __shared__ int s_hist[kBins];
+    __shared__ int s_wave[3][kSelectWaves];
+    __shared__ int s_found[2];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int h = (int)(blockIdx.x % (unsigned)p.c.hkv), b = (int)(blockIdx.x / (unsigned)p.c.hkv);
+    const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
+    const int count = min(len, p.budget);
+    const int recent = len > p.budget ? min(p.recent, p.budget) : len;
+    const int cand = len - recent;
+    const int need = count - recent;
+    const float* w = p.weights + b * p.w_b + h * p.w_h;
+    float* nw = p.new_weights + b * p.nw_b + h * p.nw_h;
+    int32_t* kept = p.kept + ((int64_t)b * p.c.hkv + h) * p.budget;
+    if (h == 0 && tid == 0) p.new_seqlens[b] = count;
+
+    // keys above `key` are kept, and the first `equal` of those equal to it
+    uint32_t key = 0xffffffffu;
+    int equal = 0;
+    if (need > 0) {
+        uint32_t prefix = 0, mask = 0;
+        int left = need;
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const int bins = pass == 2 ? 1024 : 2048;
+            for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < cand; i += kSelectThreads) {
+                const uint32_t k = weight_key(w[i]);
+                if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1);
+            }
+            __syncthreads();
+            // thread t: bins kBins - 1 - 2t and the one below, from the top down
+            const int hi = s_hist[kBins - 1 - 2 * tid], lo = s_hist[kBins - 2 - 2 * tid];
+            int incl = hi + lo;
+#pragma unroll
+            for (int d = 1; d < kWave; d *= 2) {
+                const int o = __shfl_up(incl, d, kWave);
+                incl += lane >= d ? o : 0;
+            }
+            if (lane == kWave - 1) s_wave[0][wave] = incl;
+            __syncthreads();
+            int before = incl - hi - lo;
+            for (int v = 0; v < wave; ++v) before += s_wave[0][v];
+            if (before < left && before + hi >= left) {
+                s_found[0] = kBins - 1 - 2 * tid;
+                s_found[1] = left - before;
+            } else if (before + hi < left && before + hi + lo >= left) {
+                s_found[0] = kBins - 2 - 2 * tid;
+                s_found[1] = left - before - hi;
+            }
+            __syncthreads();
+            prefix |= (uint32_t)s_found[0] << shift;
+            mask |= (uint32_t)(bins - 1) << shift;
+            left = s_found[1];
+            __syncthreads();
+        }
+        key = prefix;
+        equal = left;
+    }
+
+    // each wave's run of the row
+    const int run = (len + kSelectThreads - 1) / kSelectThreads * kWave;
+    const int lo = min(wave * run, len), hi = min(lo + run, len);
+    auto classify = [&](int i, float* v, bool* above, bool* same) {
+        *v = i < hi ? w[i] : 0.f;
+        const uint32_t k = weight_key(*v);
+        const bool chosen = i < cand && need > 0;
+        *above = i < hi && (i >= cand || (chosen && k > key));
+        *same = i < hi && chosen && k == key;
+    };
+    int n_above = 0, n_same = 0;
+    for (int i0 = lo; i0 < hi; i0 += kWave) {
+        float v;
+        bool above, same;
+        classify(i0 + lane, &v, &above, &same);
+        n_above += __popcll(__ballot(above));
+        n_same += __popcll(__ballot(same));
+    }
+    if (lane == 0) {
+        s_wave[1][wave] = n_above;
+        s_wave[2][wave] = n_same;
+    }
+    __syncthreads();
+    int at = 0, seen = 0;
+    for (int v = 0; v < wave; ++v) {
+        at += s_wave[1][v];
+        seen += s_wave[2][v];
+    }
+    at += min(seen, equal);
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+    for (int i0 = lo; i0 < hi; i0 += kWave) {
+        float v;
+        bool above, same;
+        classify(i0 + lane, &v, &above, &same);
+        const uint64_t m_same = __ballot(same);
+        const bool keep = above || (same && seen + __popcll(m_same & below) < equal);
+        const uint64_t m_keep = __ballot(keep);
+        if (keep) {
+            const int to = at + __popcll(m_keep & below);
+            kept[to] = i0 + lane;
+            nw[to] = v;
+        }
+        at += __popcll(m_keep);
+        seen += __popcll(m_same);
+    }
+    for (int i = count + tid; i < p.budget; i += kSelectThreads) kept[i] = -1;
+    for (int i = count + tid; i < p.weights_len; i += kSelectThreads) nw[i] = 0.f;
+}
+
+// Moves the kept tokens: one block of the new pages per item, as append_kernel,
+// its rows gathered through `kept` and the block table.
+template <int kCode, Scaling kScaling, typename Shape>
+__global__ __launch_bounds__(kThreads) void move_kernel(EvictParams p) {
+    __shared__ float s_max[kWaves];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    const int64_t item = (int64_t)blockIdx.x * (kWaves / Shape::waves) + wave / Shape::waves;
+    if (item >= p.items) return;
+    const int h = (int)(item % p.c.hkv);
+    const int64_t rest = item / p.c.hkv;
+    const int kv = (int)(rest & 1);
+    const int j = (int)((rest >> 1) % p.pages);
+    const int b = (int)((rest >> 1) / p.pages);
+    const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
+    const int rows = min(min(len, p.budget) - (j << p.c.page_shift), 1 << p.c.page_shift);
+    if (rows <= 0) return;
+    const int page = p.new_table[(int64_t)b * p.nt_stride + j];
+    if (page < 0 || page >= p.c.num_pages) return;
+
+    constexpr int kPieces = kCode == kCodeBf16 ? 2 : 1;   // 16-byte pieces of a row that a lane holds
+    const int row = lane / kLanesPerRow, chunk = lane % kLanesPerRow;
+    const int first_row = (wave % Shape::waves) * Shape::sweeps * kRowsPerSweep + row;
+    const int32_t* kept = p.kept + ((int64_t)b * p.c.hkv + h) * p.budget + (j << p.c.page_shift);
+    const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
+    const unsigned char* src = p.c.data[kv] + h * p.c.head[kv] + chunk * 16 * kPieces;
+    unsigned char* dst = p.c.data[kv] + page * p.c.page[kv] + h * p.c.head[kv] + chunk * 16 * kPieces;
+    const int pmask = (1 << p.c.page_shift) - 1;
+
+    u32x4_t raw[Shape::sweeps][kPieces];
+    float from[Shape::sweeps];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int s = 0; s < Shape::sweeps; ++s) {
+            const int slot = base + first_row + s * kRowsPerSweep;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) raw[s][i] = u32x4_t{0u, 0u, 0u, 0u};
+            from[s] = 0.f;
+            if (slot < rows) {
+                const int t = kept[slot];
+                const int old = min(max(bt[t >> p.c.page_shift], 0), p.c.num_pages - 1);
+                const u32x4_t* r = reinterpret_cast<const u32x4_t*>(src + old * p.c.page[kv] + (t & pmask) * p.c.slot[kv]);
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) raw[s][i] = r[i];
+                if constexpr (kScaling == kBlocks)
+                    from[s] = p.c.scales[kv][old * p.c.scale_page[kv] + h * p.c.scale_head[kv]];
+            }
+        }
+    };
+    const int last = (rows - 1) / Shape::rows * Shape::rows;
+    float scale = 1.f;
+    if constexpr (kScaling == kBlocks) {
+        float amax = 0.f;
+        for (int base = 0; base <= last; base += Shape::rows) {
+            load(base);
+#pragma unroll
+            for (int s = 0; s < Shape::sweeps; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4_t x = codes_to_f32<kCode>(raw[s][0][i]) * from[s];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) amax = fmaxf(amax, finite_abs(x[e]));
+                }
+        }
+        scale = block_scale<kCode>(block_max<Shape>(amax, s_max));
+        if (lane == 0 && wave % Shape::waves == 0)
+            p.c.scales[kv][page * p.c.scale_page[kv] + h * p.c.scale_head[kv]] = scale;
+    }
+    const Divisor div(scale);
+    for (int base = last; base >= 0; base -= Shape::rows) {
+        if (kScaling != kBlocks || base != last) load(base);
+#pragma unroll
+        for (int s = 0; s < Shape::sweeps; ++s) {
+            const int slot = base + first_row + s * kRowsPerSweep;
+            if (slot >= rows) continue;
+            u32x4_t* r = reinterpret_cast<u32x4_t*>(dst + slot * p.c.slot[kv]);
+            if constexpr (kScaling == kBlocks) {
+                u32x4_t w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = to_codes<kCode>(div(codes_to_f32<kCode>(raw[s][0][i]) * from[s]));
+                *r = w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) r[i] = raw[s][i];
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- launches
+// Calls f with the block shape for pages of page_size rows.
+template <typename F>
+void with_shape(int page_size, F&& f) {
+    if (page_size <= 8) f(BlockShape<1, 1>{});
+    else if (page_size <= 16) f(BlockShape<2, 1>{});
+    else if (page_size <= 32) f(BlockShape<4, 1>{});
+    else if (page_size <= 64) f(BlockShape<8, 1>{});
+    else if (page_size <= 128) f(BlockShape<4, 4>{});
+    else f(BlockShape<8, 4>{});
+}
+
+template <typename Shape>
+unsigned block_grid(int64_t items) {
+    return (unsigned)ceil_div(items, kWaves / Shape::waves);
+}
+
+template <int kCode, Scaling kScaling>
+void launch_append(const AppendParams& p, int page_size, hipStream_t s) {
+    with_shape(page_size, [&](auto shape) {
+        using Shape = decltype(shape);
+        hipLaunchKernelGGL((append_kernel<kCode, kScaling, Shape>), dim3(block_grid<Shape>(p.items)), dim3(kThreads), 0,
+                           s, p);
+    });
+}
+
+template <int kCode, Scaling kScaling>
+void launch_move(const EvictParams& p, int page_size, hipStream_t s) {
+    with_shape(page_size, [&](auto shape) {
+        using Shape = decltype(shape);
+        hipLaunchKernelGGL((move_kernel<kCode, kScaling, Shape>), dim3(block_grid<Shape>(p.items)), dim3(kThreads), 0, s,
+                           p);
+    });
+}
+
+}  // namespace
+}  // namespace fgqa
+
+using namespace fgqa;
+
+extern "C" int fgqa_kv_append(const fgqa_kv_append_args* a, void* stream) {
+    const int st = plan::validate_kv_append(a);
+    if (st != FGQA_OK) return st;
+    if (a->batch == 0 || a->max_new == 0 || a->max_pages == 0) return FGQA_OK;
+    AppendParams p;
+    p.c = cache_params(a->cache);
+    const void* x[2] = {a->k_new, a->v_new};
+    const int64_t* xs[2] = {a->k_new_stride, a->v_new_stride};
+    for (int i = 0; i < 2; ++i) {
+        p.x[i] = static_cast<const unsigned char*>(x[i]);
+        p.x_b[i] = xs[i][0] * 2;
+        p.x_t[i] = xs[i][1] * 2;
+        p.x_h[i] = xs[i][2] * 2;
+    }
+    p.block_table = a->block_table;
+    p.bt_stride = a->block_table_stride;
+    p.seqlens = a->seqlens;
+    p.new_lens = a->new_lens;
+    p.max_new = a->max_new;
+    p.max_tokens = a->max_pages * a->cache.page_size;
+    p.pages = (int)plan::append_pages(a->max_new, a->cache.page_size);
+    p.items = (int64_t)a->batch * p.pages * 2 * p.c.hkv;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const int page = a->cache.page_size;
+    const bool blocks = a->cache.k_scales != nullptr;
+    if (a->cache.kv_dtype == FGQA_KV_BF16) launch_append<kCodeBf16, kNone>(p, page, s);
+    else if (a->cache.kv_dtype == FGQA_KV_INT8) launch_append<kCodeInt8, kBlocks>(p, page, s);
+    else if (blocks) launch_append<kCodeFp8, kBlocks>(p, page, s);
+    else launch_append<kCodeFp8, kWhole>(p, page, s);
+    return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
+}
+
+extern "C" int fgqa_kv_weights(const fgqa_kv_weights_args* a, void* stream) {
+    const int st = plan::validate_kv_weights(a);
+    if (st != FGQA_OK) return st;
+    if (a->batch == 0 || a->max_seqlen == 0) return FGQA_OK;
+    WeightsParams p;
+    p.c = cache_params(a->cache);
+    p.q = static_cast<const __bf16*>(a->q);
+    p.lse = a->lse;
+    p.weights = a->weights;
+    p.q_b = a->q_stride[0];
+    p.q_h = a->q_stride[1];
+    p.w_b = a->weights_stride[0];
+    p.w_h = a->weights_stride[1];
+    p.block_table = a->block_table;
+    p.bt_stride = a->block_table_stride;
+    p.seqlens = a->seqlens;
+    p.max_seqlen = a->max_seqlen;
+    p.group = a->num_q_heads / p.c.hkv;
+    p.chunk = plan::weights_chunk(a->batch, p.c.hkv, a->max_seqlen);
+    p.chunks = (int)ceil_div(a->max_seqlen, p.chunk);
+    p.items = (int64_t)a->batch * p.chunks * p.c.hkv;
+    const bool blocks = a->cache.k_scales != nullptr;
+    const bool whole = a->cache.kv_dtype == FGQA_KV_FP8_E4M3 && !blocks;
+    p.scale = a->scale * (whole ? a->cache.k_scale : 1.f);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const dim3 grid((unsigned)ceil_div(p.items, kWaves));
+    if (a->cache.kv_dtype == FGQA_KV_BF16)
+        hipLaunchKernelGGL((weights_kernel<kCodeBf16, kNone>), grid, dim3(kThreads), 0, s, p);
+    else if (a->cache.kv_dtype == FGQA_KV_INT8)
+        hipLaunchKernelGGL((weights_kernel<kCodeInt8, kBlocks>), grid, dim3(kThreads), 0, s, p);
+    else if (blocks)
+        hipLaunchKernelGGL((weights_kernel<kCodeFp8, kBlocks>), grid, dim3(kThreads), 0, s, p);
+    else
+        hipLaunchKernelGGL((weights_kernel<kCodeFp8, kWhole>), grid, dim3(kThreads), 0, s, p);
+    return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
+}
+
+extern "C" int fgqa_kv_evict(const fgqa_kv_evict_args* a, void* stream) {
+    const int st = plan::validate_kv_evict(a);
+    if (st != FGQA_OK) return st;
+    if (a->batch == 0) return FGQA_OK;
+    EvictParams p;
+    p.c = cache_params(a->cache);
+    p.weights = a->weights;
+    p.new_weights = a->new_weights;
+    p.w_b = a->weights_stride[0];
+    p.w_h = a->weights_stride[1];
+    p.nw_b = a->new_weights_stride[0];
+    p.nw_h = a->new_weights_stride[1];
+    p.block_table = a->block_table;
+    p.new_table = a->new_block_table;
+    p.bt_stride = a->block_table_stride;
+    p.nt_stride = a->new_block_table_stride;
+    p.seqlens = a->seqlens;
+    p.new_seqlens = a->new_seqlens;
+    p.kept = a->kept;
+    p.max_seqlen = a->max_seqlen;
+    p.weights_len = a->weights_len;
+    p.budget = a->budget;
+    p.recent = a->recent;
+    const int most = a->budget < a->max_seqlen ? a->budget : a->max_seqlen;
+    p.pages = (int)ceil_div(most, a->cache.page_size);
+    p.items = (int64_t)a->batch * p.pages * 2 * p.c.hkv;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(select_kernel, dim3((unsigned)a->batch * (unsigned)p.c.hkv), dim3(kSelectThreads), 0, s, p);
+    if (p.items > 0) {
+        const int page = a->cache.page_size;
+        if (a->cache.kv_dtype == FGQA_KV_BF16) launch_move<kCodeBf16, kNone>(p, page, s);
+        else if (a->cache.kv_dtype == FGQA_KV_INT8) launch_move<kCodeInt8, kBlocks>(p, page, s);
+        else if (a->cache.k_scales != nullptr) launch_move<kCodeFp8, kBlocks>(p, page, s);
+        else launch_move<kCodeFp8, kWhole>(p, page, s);
+    }
+    return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
+}

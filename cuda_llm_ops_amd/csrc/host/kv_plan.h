@@ -1,0 +1,38 @@
+// Host-only argument validation of the paged KV cache's C ABI (include/fgqa_kv.h),
+// apart from HIP like fgqa_plan.h, so that the CPU tests build it with sanitizers.
+#pragma once
+
+#include "fgqa_kv.h"
+#include "fgqa_plan.h"
+
+namespace fgqa {
+namespace plan {
+
+// Sizes and addresses of a call; FGQA_OK with batch (or what it would write)
+// zero, where nothing is launched and no address is looked at.
+int validate_kv_append(const fgqa_kv_append_args* a);
+int validate_kv_weights(const fgqa_kv_weights_args* a);
+int validate_kv_evict(const fgqa_kv_evict_args* a);
+
+// The block-scaled decode's cache and scales; then what fgqa_decode_paged
+// checks, on its arguments for the same call (an e4m3 cache: the same element size).
+int validate_decode_blocks(const fgqa_decode_blocks_args* a);
+int validate_decode_blocks_pointers(const fgqa_decode_blocks_args* a);
+fgqa_decode_paged_args as_decode_paged(const fgqa_decode_blocks_args* a);
+
+inline int log2_of(int power_of_two) {
+    int shift = 0;
+    while ((1 << shift) < power_of_two) ++shift;
+    return shift;
+}
+
+// Most pages of one sequence that `max_new` tokens in a row touch.
+inline int64_t append_pages(int64_t max_new, int64_t page_size) { return (max_new + page_size - 2) / page_size + 1; }
+
+// Tokens of a wave's item in the weights kernel (a multiple of 32): as many as
+// leave the chip kWeightsItems items, from 512 down to 64.
+constexpr int kWeightsItems = 8192;
+int weights_chunk(int64_t batch, int64_t num_kv_heads, int64_t max_seqlen);
+
+}  // namespace plan
+}  // namespace fgqa

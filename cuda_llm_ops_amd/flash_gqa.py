@@ -14,7 +14,8 @@ Two families of entry points:
   K/V ``[B,S,Hkv,D]``, decode_flash_gqa_kernel.cuh:28-38) and of the new C++
   prefill entry point (BSHD):
     - ``decode_flash_gqa_bshd``  (adds per-sequence lengths and an LSE output)
-    - ``decode_flash_gqa_paged`` (paged KV cache with a block table, bf16 or fp8 e4m3)
+    - ``decode_flash_gqa_paged`` (paged KV cache with a block table, bf16, fp8 e4m3 or int8;
+      ``kv_cache`` writes such a cache and evicts from it)
     - ``flash_gqa_forward_bshd``
     - ``flash_gqa_backward_bshd``
 
@@ -24,6 +25,7 @@ through ``fgqa_decode_bf16`` / ``fgqa_prefill_bf16`` / ``fgqa_prefill_backward_b
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import operator
 
@@ -272,6 +274,53 @@ def _paged_prepare(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_
     return a, out, (q, k_cache, v_cache, block_table, seqlens, out, lse, workspace)
 
 
+def _has_block_scales(k_cache, k_scale, v_scale) -> bool:
+    return isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor) or k_cache.dtype == torch.int8
+
+
+@functools.lru_cache(maxsize=256)
+def _blocks_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, split_tokens) -> int:
+    return paged_decode_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, split_tokens=split_tokens)
+
+
+def _prepare_blocks(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse, max_seqlen,
+                    split_tokens, workspace):
+    """The paged decode over a cache with block scales, validated."""
+    if q.dtype != torch.bfloat16:
+        raise ValueError("paged decode expects a bf16 query")
+    if q.dim() != 3:
+        raise ValueError("expected q [B,Hq,D] and k_cache/v_cache [num_pages, page_size, Hkv, D]")
+    cache = kv_cache.cache_fields(k_cache, v_cache, k_scale, v_scale)
+    B, Hq, D = q.shape
+    num_pages, page_size, Hkv, _ = k_cache.shape
+    if k_cache.shape[3] != D:
+        raise ValueError("the caches' head_dim must match Q")
+    if Hq % Hkv != 0:
+        raise ValueError("Query heads must be divisible by KV heads")
+    table_stride = kv_cache.check_table(block_table, B, "block_table")
+    kv_cache.check_lens(seqlens, B, "seqlens")
+    max_seqlen = kv_cache.check_max_seqlen(max_seqlen, block_table, page_size)
+    if out is not None and (out.shape != (B, Hq, D) or out.dtype != torch.bfloat16 or not _kernel_ready(out)):
+        raise ValueError("out must be a bf16 [B, Hq, D] tensor with contiguous rows")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, Hq) or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous fp32 [B, Hq] tensor")
+    kv_cache.check_device(q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens, out, lse, workspace)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    q = _prep(q)
+    if out is None:
+        out = torch.empty((B, Hq, D), device=q.device, dtype=torch.bfloat16)
+    if workspace is None and B > 0:
+        workspace = torch.empty(_blocks_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, int(split_tokens)),
+                                device=q.device, dtype=torch.uint8)
+    a = _lib.pack_decode_blocks(
+        *cache, _ptr(q), _ptr(out), _ptr(lse), _ptr(block_table), _ptr(seqlens), B, max_seqlen, Hq, float(scale),
+        *q.stride()[:2], *out.stride()[:2], table_stride, int(split_tokens), *_workspace(workspace))
+    return kv_cache.DeviceLaunch(_lib.lib().fgqa_decode_blocks, a,
+                                 (q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens, out, lse, workspace), out,
+                                 "fgqa_decode_blocks", q.device)
+
+
 def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None, k_scale=1.0, v_scale=1.0,
                            out=None, lse=None, max_seqlen=None, split_tokens=0, workspace=None):
     """Single-token GQA decode over a paged KV cache.
@@ -281,7 +330,16 @@ def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None
     block_table: int32 [B, max_pages] (token t of sequence b is slot
     t % page_size of page block_table[b, t // page_size]); seqlens: int32 [B].
     page_size must be a power of two.  Returns ``out`` (bf16 [B, Hq, D]).
+
+    k_scale, v_scale: numbers, or fp32 tensors [num_pages, Hkv] with a scale for
+    each page of each KV head, as ``append_kv_paged`` writes them; the caches then
+    are float8_e4m3fn or int8 (int8 ones always have such scales).  Without a
+    ``workspace`` that form takes one from torch's allocator, so its calls on
+    different streams, and captured ones, may overlap.
     """
+    if _has_block_scales(k_cache, k_scale, v_scale):
+        return _prepare_blocks(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse,
+                               max_seqlen, split_tokens, workspace)()
     a, out, _keep = _paged_prepare(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out,
                                    lse, max_seqlen, split_tokens, workspace)
     _lib.check(_lib.lib().fgqa_decode_paged(ctypes.byref(a), _stream()), "fgqa_decode_paged")
@@ -291,6 +349,9 @@ def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None
 def prepare_decode_paged(q, k_cache, v_cache, block_table, seqlens, scale=None, k_scale=1.0, v_scale=1.0,
                          out=None, lse=None, max_seqlen=None, split_tokens=0, workspace=None):
     """``decode_flash_gqa_paged`` validated once; returns a ``PreparedLaunch``."""
+    if _has_block_scales(k_cache, k_scale, v_scale):
+        return _prepare_blocks(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse,
+                               max_seqlen, split_tokens, workspace)
     a, out, keep = _paged_prepare(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse,
                                   max_seqlen, split_tokens, workspace)
     return PreparedLaunch(_lib.lib().fgqa_decode_paged, a, keep, out, "fgqa_decode_paged")
@@ -1203,3 +1264,7 @@ def launch_flash_sgqa_forward_bf16_kernel(q, k, v, sparse_kv_indices, num_sparse
     if squeeze_output:
         return out_b.squeeze(0), lse_b.squeeze(0)
     return out_b, lse_b
+
+
+# (kv_cache builds on the helpers above)
+from . import kv_cache  # noqa: E402
