@@ -297,6 +297,10 @@ def evict_kv_paged(k_cache, v_cache, block_table, seqlens, weights, new_block_ta
     if kept is not None and (kept.dtype != torch.int32 or kept.shape != (B, Hkv, budget) or not kept.is_contiguous()):
         raise ValueError("kept must be a contiguous int32 [B, Hkv, budget] tensor")
     _check_written(k_cache, v_cache, k_scale, v_scale, new_weights)
+    given = [t for t in (new_seqlens, new_weights, kept) if t is not None]
+    if any(_meet(t, x) for i, t in enumerate(given)
+           for x in (*given[:i], weights, seqlens, block_table, new_block_table)):
+        raise ValueError("new_seqlens, new_weights and kept must be apart from each other and from the inputs")
     check_device(k_cache, v_cache, block_table, seqlens, weights, new_block_table, k_scale, v_scale, new_seqlens,
                  new_weights, kept)
     dev = k_cache.device
@@ -306,11 +310,6 @@ def evict_kv_paged(k_cache, v_cache, block_table, seqlens, weights, new_block_ta
         new_weights = torch.empty((B, Hkv, W), device=dev, dtype=torch.float32)
     if kept is None:
         kept = torch.empty((B, Hkv, budget), device=dev, dtype=torch.int32)
-    outs = (new_seqlens, new_weights, kept)
-    ins = (weights, seqlens, block_table, new_block_table)
-    if any(_meet(o, i) for o in outs for i in ins) or _meet(new_weights, kept) or _meet(new_seqlens, kept) \
-            or _meet(new_seqlens, new_weights):
-        raise ValueError("new_seqlens, new_weights and kept must be apart from each other and from the inputs")
     a = _lib.pack_kv_evict(*cache, _ptr(weights), _ptr(new_weights), *weights.stride()[:2], *new_weights.stride()[:2],
                            _ptr(block_table), _ptr(new_block_table), table_stride, new_stride, _ptr(seqlens),
                            _ptr(new_seqlens), _ptr(kept), B, max_seqlen, W, budget, recent)

@@ -6,4 +6,5 @@
 #include "FlashGQA/decode_flash_gqa_kernel.h"
 #include "FlashGQA/flash_gqa_backward_kernel.h"
 #include "FlashGQA/flash_gqa_forward_kernel.h"
+#include "FlashGQA/kv_cache_kernel.h"
 #include "Utils/utils.h"

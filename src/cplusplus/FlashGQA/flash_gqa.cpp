@@ -47,6 +47,11 @@ fgqa_decode_args contiguous_decode(const bf16_t* q, const bf16_t* k, const bf16_
 }
 }  // namespace
 
+// (the paged cache's entry points, kv_cache.cpp, report through the same status)
+namespace fgqa_cpp {
+__attribute__((visibility("hidden"))) void set_last_status(int status) { g_last_status = status; }
+}  // namespace fgqa_cpp
+
 void LaunchFlashGqaBf16Kernel(const bf16_t* q, const bf16_t* k, const bf16_t* v, float scale, bf16_t* o,
                               float* oIntermediate, int batchSize, int seqLength, int numQueryHeads,
                               int numKvHeads, int headDim) {
