@@ -44,9 +44,23 @@ __device__ __forceinline__ u32x2_t lds_read_tr8(const unsigned char* p) {
     return __builtin_bit_cast(u32x2_t, v);
 }
 
+// The loads of one 32-token step, and the scales of its tokens' blocks: of the
+// step's 16-token halves (kSeg > 0), or of this lane's two K rows (kSeg 0).
+struct Step8 {
+    u32x4_t k[2][2];   // token 16 tb + l16: pieces 16 g4 and 64 + 16 g4
+    u32x4_t v[4];      // row 8 r + lane / 8, piece lane % 8
+    float ks[2], vs[2];
+};
+
 // As dec_item: tokens [t_begin, t_end) (not empty, t_begin a multiple of 128)
-// of one sequence and kv head by 4 waves.
-template <int kCode>
+// of one sequence and kv head by 4 waves.  Two steps' loads are in flight per
+// wave: a step of codes is half the bytes of a bf16 one.
+// kSeg (32 or 16, for pages of at least that many rows whose bytes stay below
+// 2^31): a step is one or two page segments, read through buffer resources that
+// end at the item's last token (rows past it are zeros), their pages and scales
+// taken 64 segments at a time from one vector load each.  0: any pages, a lookup
+// and a 64-bit address per row.
+template <int kCode, int kSeg>
 __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* smem, int t_begin, int t_end, int kvh,
                                           int b, int tid, bool whole, int64_t slot0) {
     const int lane = tid & (kWave - 1);
@@ -54,7 +68,7 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
     const int l16 = lane & 15;
     const int g4 = lane >> 4;
     unsigned char* vl = smem + wave * kDec8WaveBytes;
-    float* sl = reinterpret_cast<float*>(vl + kDec8TileBytes);   // [32] K scales, [32] V scales
+    float* sl = reinterpret_cast<float*>(vl + kDec8TileBytes);   // kSeg 0: [32] K scales, [32] V scales
 
     // Q^T as the B operand: lane holds Q[h = l16] at the elements that its
     // pieces of K hold; heads >= G are zero.
@@ -77,73 +91,154 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
 #pragma unroll
     for (int db = 0; db < 8; ++db) oacc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-    const unsigned char* kbase = reinterpret_cast<const unsigned char*>(p.k) + kvh * p.k_sh + g4 * 16;
+    const unsigned char* kbase = reinterpret_cast<const unsigned char*>(p.k) + kvh * p.k_sh;
     const unsigned char* vbase = reinterpret_cast<const unsigned char*>(p.v) + kvh * p.v_sh;
     const float* kscales = p.k_scales + kvh * p.ks_sh;
     const float* vscales = p.v_scales + kvh * p.vs_sh;
     const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
     const int pmask = (1 << p.page_shift) - 1;
     const int v_row = lane >> 3, v_chunk = lane & 7;
+    const int t_end_u = __builtin_amdgcn_readfirstlane(t_end);
     const int n_steps = (t_end - t_begin + kDecStep - 1) / kDecStep;
-    for (int st = wave; st < n_steps; st += kDecWaves) {
-        const int t0 = t_begin + st * kDecStep;
-        // Tokens past the item's end reuse its last one (masked below).
-        u32x4_t kreg[2][2], vreg[4];
+
+    // kSeg > 0
+    constexpr int kSegs = kSeg > 0 ? kDecStep / kSeg : 1;
+    const uint32_t kss = (uint32_t)p.k_ss, vss = (uint32_t)p.v_ss;
+    [[maybe_unused]] const uint32_t koff = (uint32_t)l16 * kss + g4 * 16;
+    [[maybe_unused]] const uint32_t voff = (uint32_t)v_row * vss + v_chunk * 16;
+    [[maybe_unused]] int pt_page = 0, pt_first = -kWave;   // lane l: the wave's segment pt_first + l
+    [[maybe_unused]] float pt_ks = 0.f, pt_vs = 0.f;
+    [[maybe_unused]] auto pt_load = [&](int first) {
+        const int n = first + lane;
+        const int tok = min(t_begin + (wave + kDecWaves * (n / kSegs)) * kDecStep + kSeg * (n % kSegs), t_end_u - 1);
+        pt_page = min(max(bt[tok >> p.page_shift], 0), p.num_pages - 1);
+        pt_ks = kscales[(int64_t)pt_page * p.ks_sp];
+        pt_vs = vscales[(int64_t)pt_page * p.vs_sp];
+        pt_first = first;
+    };
+    // kSeg 0: the table's entries are loaded two steps before they are used, and
+    // before the rows of the step between: vector loads complete in order, so
+    // waiting for them then waits for no row that is not needed yet.
+    [[maybe_unused]] int pg[2][6];   // of the K rows (2) and V rows (4)
+    [[maybe_unused]] auto fetch_pages = [&](int s, int (&to)[6]) {
+        const int t0 = t_begin + s * kDecStep;
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb) {
-            const int tok = min(t0 + 16 * tb + l16, t_end - 1);
-            const int page = min(max(bt[tok >> p.page_shift], 0), p.num_pages - 1);
-            const unsigned char* row = kbase + (int64_t)page * p.k_sb + (int64_t)(tok & pmask) * p.k_ss;
-            kreg[tb][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row));
-            kreg[tb][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row + 64));
-            if (g4 == 0) {
-                sl[16 * tb + l16] = kscales[(int64_t)page * p.ks_sp];
-                sl[kDecStep + 16 * tb + l16] = vscales[(int64_t)page * p.vs_sp];
+        for (int tb = 0; tb < 2; ++tb) to[tb] = bt[min(t0 + 16 * tb + l16, t_end - 1) >> p.page_shift];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to[2 + r] = bt[min(t0 + 8 * r + v_row, t_end - 1) >> p.page_shift];
+    };
+    auto load_step = [&](int s, Step8& x, [[maybe_unused]] const int (&pages)[6]) {
+        const int t0 = t_begin + s * kDecStep;
+        if constexpr (kSeg > 0) {
+            const int n0 = ((s - wave) / kDecWaves) * kSegs;   // the wave's first segment of step s
+            if (n0 + kSegs > pt_first + kWave) pt_load(n0);
+#pragma unroll
+            for (int g = 0; g < kSegs; ++g) {
+                const int at = n0 - pt_first + g;
+                const int64_t page = __builtin_amdgcn_readlane(pt_page, at);
+                x.ks[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pt_ks), at));
+                x.vs[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pt_vs), at));
+                const int tok = t0 + kSeg * g;
+                const int nv = min(kSeg, t_end_u - tok);   // rows before the item's end
+                const uint32_t slot = (uint32_t)(tok & pmask);
+                const __amdgpu_buffer_rsrc_t kr =
+                    make_rsrc(kbase + page * p.k_sb + slot * kss, nv > 0 ? (uint32_t)(nv - 1) * kss + kHeadDim : 0u);
+                const __amdgpu_buffer_rsrc_t vr =
+                    make_rsrc(vbase + page * p.v_sb + slot * vss, nv > 0 ? (uint32_t)(nv - 1) * vss + kHeadDim : 0u);
+#pragma unroll
+                for (int i = 0; i < 2 / kSegs; ++i) {
+                    const int tb = g * (2 / kSegs) + i;
+                    x.k[tb][0] = buf_load16_nt(kr, koff + (uint32_t)(16 * i) * kss);
+                    x.k[tb][1] = buf_load16_nt(kr, koff + (uint32_t)(16 * i) * kss + 64);
+                }
+#pragma unroll
+                for (int i = 0; i < 4 / kSegs; ++i)
+                    x.v[g * (4 / kSegs) + i] = buf_load16_nt(vr, voff + (uint32_t)(8 * i) * vss);
+            }
+            if constexpr (kSegs == 1) {
+                x.ks[1] = x.ks[0];
+                x.vs[1] = x.vs[0];
+            }
+        } else {
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb) {
+                const int slot = min(t0 + 16 * tb + l16, t_end - 1) & pmask;
+                const int64_t page = min(max(pages[tb], 0), p.num_pages - 1);
+                const unsigned char* row = kbase + page * p.k_sb + (int64_t)slot * p.k_ss + g4 * 16;
+                x.k[tb][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row));
+                x.k[tb][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row + 64));
+                x.ks[tb] = kscales[page * p.ks_sp];
+                x.vs[tb] = vscales[page * p.vs_sp];
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int slot = min(t0 + 8 * r + v_row, t_end - 1) & pmask;
+                const int64_t page = min(max(pages[2 + r], 0), p.num_pages - 1);
+                x.v[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
+                    vbase + page * p.v_sb + (int64_t)slot * p.v_ss + v_chunk * 16));
             }
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int tok = min(t0 + 8 * r + v_row, t_end - 1);
-            const int page = min(max(bt[tok >> p.page_shift], 0), p.num_pages - 1);
-            vreg[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
-                vbase + (int64_t)page * p.v_sb + (int64_t)(tok & pmask) * p.v_ss + v_chunk * 16));
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<u32x4_t*>(vl + (8 * r + v_row) * kDec8RowStride + v_chunk * 16) = vreg[r];
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
 
-        // S^T = K Q^T (codes), K as the A operand
-        f32x4_t s[2];
+    // One step; its registers are free for the next loads once `reload` is called.
+    auto compute = [&](int st, Step8& x, auto&& reload) {
+        const int t0 = t_begin + st * kDecStep;
         float ks[8], vs[8];
         float vmax = vref;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            *reinterpret_cast<u32x4_t*>(vl + (8 * r + v_row) * kDec8RowStride + v_chunk * 16) = x.v[r];
+        if constexpr (kSeg == 0) {
+            if (g4 == 0) {
+#pragma unroll
+                for (int tb = 0; tb < 2; ++tb) {
+                    sl[16 * tb + l16] = x.ks[tb];
+                    sl[kDecStep + 16 * tb + l16] = x.vs[tb];
+                }
+            }
+        }
+        // S^T = K Q^T (codes), K as the A operand
+        f32x4_t s[2];
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
             s[tb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                s[tb] = mfma16(codes_to_bf16<kCode>(kreg[tb][j][0], kreg[tb][j][1]), qop[2 * j], s[tb]);
-                s[tb] = mfma16(codes_to_bf16<kCode>(kreg[tb][j][2], kreg[tb][j][3]), qop[2 * j + 1], s[tb]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                ks[4 * tb + i] = sl[16 * tb + 4 * g4 + i] * p.scale_log2;
-                vs[4 * tb + i] = sl[kDecStep + 16 * tb + 4 * g4 + i];
-                vmax = fmaxf(vmax, fabsf(vs[4 * tb + i]));
+                s[tb] = mfma16(codes_to_bf16<kCode>(x.k[tb][j][0], x.k[tb][j][1]), qop[2 * j], s[tb]);
+                s[tb] = mfma16(codes_to_bf16<kCode>(x.k[tb][j][2], x.k[tb][j][3]), qop[2 * j + 1], s[tb]);
             }
         }
-        vmax = xor_max(xor_max(vmax, 16), 32);
+        const float ks_half[2] = {x.ks[0], x.ks[1]}, vs_half[2] = {x.vs[0], x.vs[1]};
+        reload();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if constexpr (kSeg > 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                ks[j] = ks_half[j / 4] * p.scale_log2;
+                vs[j] = vs_half[j / 4];
+            }
+            vmax = fmaxf(vmax, fmaxf(fabsf(vs_half[0]), fabsf(vs_half[1])));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = 16 * (j / 4) + 4 * g4 + j % 4;
+                ks[j] = sl[at] * p.scale_log2;
+                vs[j] = sl[kDecStep + at];
+                vmax = fmaxf(vmax, fabsf(vs[j]));
+            }
+            vmax = xor_max(xor_max(vmax, 16), 32);
+        }
 
         // Online softmax for head l16 over tokens t0 + 16*tb + 4*g4 + i.
-        float x[8];
+        float y[8];
         float tmax = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int tok = t0 + (j >> 2) * 16 + g4 * 4 + (j & 3);
-            x[j] = tok < t_end ? s[j >> 2][j & 3] * ks[j] : -INFINITY;
-            tmax = fmaxf(tmax, x[j]);
+            y[j] = tok < t_end ? s[j >> 2][j & 3] * ks[j] : -INFINITY;
+            tmax = fmaxf(tmax, y[j]);
         }
         tmax = xor_max(xor_max(tmax, 16), 32);
         const float m_new = fmaxf(m_run, tmax);   // finite: every step holds a valid token
@@ -155,7 +250,7 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         f16x8_t pop;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float pv = fast_exp2(x[j] - m_new);
+            const float pv = fast_exp2(y[j] - m_new);
             psum += pv;
             pop[j] = (_Float16)(pv * (vs[j] * pscale));
         }
@@ -179,6 +274,21 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+
+    Step8 step_a, step_b;
+    auto load_if = [&](int s, Step8& x, int (&pages)[6], int (&next)[6]) {
+        if (kSeg == 0 && s + kDecWaves < n_steps) fetch_pages(s + kDecWaves, next);
+        if (s < n_steps) load_step(s, x, pages);
+    };
+    int st = wave;
+    if (kSeg == 0 && st < n_steps) fetch_pages(st, pg[0]);
+    load_if(st, step_a, pg[0], pg[1]);
+    load_if(st + kDecWaves, step_b, pg[1], pg[0]);
+    for (; st < n_steps; st += 2 * kDecWaves) {
+        compute(st, step_a, [&] { load_if(st + 2 * kDecWaves, step_a, pg[0], pg[1]); });
+        if (st + kDecWaves < n_steps)
+            compute(st + kDecWaves, step_b, [&] { load_if(st + 3 * kDecWaves, step_b, pg[1], pg[0]); });
     }
 
     l_run = xor_sum(xor_sum(l_run, 16), 32);

@@ -37,6 +37,8 @@
 // each row's page and form its 64-bit address.
 #include <math.h>
 
+#include <type_traits>
+
 #include "fgqa_device.h"
 #include "fgqa_internal.h"
 #include "../host/kv_plan.h"
@@ -442,7 +444,7 @@ template <int kKv, int kSeg>
 __device__ __forceinline__ void dec_item_of(const DecodeParams& p, unsigned char* smem, int t_begin, int t_end, int kvh,
                                             int b, int tid, bool whole, int64_t slot0) {
     if constexpr (kKv >= kKvBlocksFp8)
-        dec_item8<kKv == kKvBlocksFp8 ? kCodeFp8 : kCodeInt8>(p, smem, t_begin, t_end, kvh, b, tid, whole, slot0);
+        dec_item8<kKv == kKvBlocksFp8 ? kCodeFp8 : kCodeInt8, kSeg>(p, smem, t_begin, t_end, kvh, b, tid, whole, slot0);
     else
         dec_item<kKv, kSeg>(p, smem, t_begin, t_end, kvh, b, tid, whole, slot0);
 }
@@ -1243,8 +1245,15 @@ int paged_run(const fgqa_decode_paged_args* a, const fgqa_kv_cache* blocks, void
         const int seg = !small_pages ? 0 : a->page_size >= 32 ? 32 : a->page_size >= 4 ? a->page_size : 0;
         auto pass1 = [&] {
             if (blocks != nullptr) {
-                if (blocks->kv_dtype == FGQA_KV_INT8) launch_list<kKvBlocksInt8, 0>(p, plan.nsplit, cus, s);
-                else launch_list<kKvBlocksFp8, 0>(p, plan.nsplit, cus, s);
+                auto launch = [&](auto kv) {
+                    switch (seg >= 16 ? seg : 0) {
+                        case 32: launch_list<decltype(kv)::value, 32>(p, plan.nsplit, cus, s); break;
+                        case 16: launch_list<decltype(kv)::value, 16>(p, plan.nsplit, cus, s); break;
+                        default: launch_list<decltype(kv)::value, 0>(p, plan.nsplit, cus, s); break;
+                    }
+                };
+                if (blocks->kv_dtype == FGQA_KV_INT8) launch(std::integral_constant<int, kKvBlocksInt8>{});
+                else launch(std::integral_constant<int, kKvBlocksFp8>{});
             } else if (fp8) {
                 switch (seg >= 8 ? seg : 0) {
                     case 32: launch_list<kKvPagedFp8, 32>(p, plan.nsplit, cus, s); break;

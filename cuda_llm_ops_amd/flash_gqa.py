@@ -283,42 +283,49 @@ def _blocks_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, split_tokens) -> 
     return paged_decode_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, split_tokens=split_tokens)
 
 
-def _prepare_blocks(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse, max_seqlen,
-                    split_tokens, workspace):
-    """The paged decode over a cache with block scales, validated."""
-    if q.dtype != torch.bfloat16:
+def _blocks_args(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse, max_seqlen,
+                 split_tokens, workspace):
+    """The paged decode over a cache with block scales, validated: (argument
+    block's bytes, out, the device's index, what they point at)."""
+    if q.dtype is not torch.bfloat16:
         raise ValueError("paged decode expects a bf16 query")
     if q.dim() != 3:
         raise ValueError("expected q [B,Hq,D] and k_cache/v_cache [num_pages, page_size, Hkv, D]")
-    cache = kv_cache.cache_fields(k_cache, v_cache, k_scale, v_scale)
+    cache, _ = kv_cache.cache_fields(k_cache, v_cache, k_scale, v_scale)
     B, Hq, D = q.shape
-    num_pages, page_size, Hkv, _ = k_cache.shape
-    if k_cache.shape[3] != D:
+    _, page_size, Hkv, _ = k_cache.shape
+    if D != 128:
         raise ValueError("the caches' head_dim must match Q")
     if Hq % Hkv != 0:
         raise ValueError("Query heads must be divisible by KV heads")
-    table_stride = kv_cache.check_table(block_table, B, "block_table")
+    pages, table_stride = kv_cache.check_table(block_table, B, "block_table")
     kv_cache.check_lens(seqlens, B, "seqlens")
-    max_seqlen = kv_cache.check_max_seqlen(max_seqlen, block_table, page_size)
+    tokens = pages * page_size
+    max_seqlen = tokens if max_seqlen is None else kv_cache.check_max_seqlen(max_seqlen, tokens)
+    split_tokens = int(split_tokens)
+    if not 0 <= split_tokens < 1 << 31:
+        raise ValueError("split_tokens must not be negative (and be below 2^31)")
+    given = [t for t in (out, lse, workspace) if t is not None]
     if out is not None and (out.shape != (B, Hq, D) or out.dtype != torch.bfloat16 or not _kernel_ready(out)):
         raise ValueError("out must be a bf16 [B, Hq, D] tensor with contiguous rows")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, Hq) or not lse.is_contiguous()):
-        raise ValueError("lse must be a contiguous fp32 [B, Hq] tensor")
-    kv_cache.check_device(q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens, out, lse, workspace)
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
+    lse_ptr = 0
+    if lse is not None:
+        if lse.dtype is not torch.float32 or lse.shape != (B, Hq) or not lse.is_contiguous():
+            raise ValueError("lse must be a contiguous fp32 [B, Hq] tensor")
+        lse_ptr = lse.data_ptr()
+    dev = kv_cache.check_device(q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens, *given)
     q = _prep(q)
     if out is None:
         out = torch.empty((B, Hq, D), device=q.device, dtype=torch.bfloat16)
     if workspace is None and B > 0:
-        workspace = torch.empty(_blocks_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, int(split_tokens)),
+        workspace = torch.empty(_blocks_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, split_tokens),
                                 device=q.device, dtype=torch.uint8)
-    a = _lib.pack_decode_blocks(
-        *cache, _ptr(q), _ptr(out), _ptr(lse), _ptr(block_table), _ptr(seqlens), B, max_seqlen, Hq, float(scale),
-        *q.stride()[:2], *out.stride()[:2], table_stride, int(split_tokens), *_workspace(workspace))
-    return kv_cache.DeviceLaunch(_lib.lib().fgqa_decode_blocks, a,
-                                 (q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens, out, lse, workspace), out,
-                                 "fgqa_decode_blocks", q.device)
+    qst, ost = q.stride(), out.stride()
+    packed = _lib.pack_decode_blocks.bytes(
+        *cache, q.data_ptr(), out.data_ptr(), lse_ptr, block_table.data_ptr(), seqlens.data_ptr(), B, max_seqlen, Hq,
+        1.0 / math.sqrt(D) if scale is None else float(scale), qst[0], qst[1], ost[0], ost[1], table_stride,
+        split_tokens, *_workspace(workspace))
+    return packed, out, dev, (q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens, out, lse, workspace)
 
 
 def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None, k_scale=1.0, v_scale=1.0,
@@ -338,8 +345,10 @@ def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None
     different streams, and captured ones, may overlap.
     """
     if _has_block_scales(k_cache, k_scale, v_scale):
-        return _prepare_blocks(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse,
-                               max_seqlen, split_tokens, workspace)()
+        packed, out, dev, _keep = _blocks_args(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out,
+                                               lse, max_seqlen, split_tokens, workspace)
+        kv_cache.launch(_lib.lib().fgqa_decode_blocks, packed, dev, "fgqa_decode_blocks")
+        return out
     a, out, _keep = _paged_prepare(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out,
                                    lse, max_seqlen, split_tokens, workspace)
     _lib.check(_lib.lib().fgqa_decode_paged(ctypes.byref(a), _stream()), "fgqa_decode_paged")
@@ -350,8 +359,9 @@ def prepare_decode_paged(q, k_cache, v_cache, block_table, seqlens, scale=None, 
                          out=None, lse=None, max_seqlen=None, split_tokens=0, workspace=None):
     """``decode_flash_gqa_paged`` validated once; returns a ``PreparedLaunch``."""
     if _has_block_scales(k_cache, k_scale, v_scale):
-        return _prepare_blocks(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse,
-                               max_seqlen, split_tokens, workspace)
+        packed, out, dev, keep = _blocks_args(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out,
+                                              lse, max_seqlen, split_tokens, workspace)
+        return kv_cache.DeviceLaunch(_lib.lib().fgqa_decode_blocks, packed, keep, out, "fgqa_decode_blocks", dev)
     a, out, keep = _paged_prepare(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse,
                                   max_seqlen, split_tokens, workspace)
     return PreparedLaunch(_lib.lib().fgqa_decode_paged, a, keep, out, "fgqa_decode_paged")
