@@ -9,11 +9,19 @@
 // (vref), and P sV / vref is rounded to fp16 at 2^14 times its value: 11 bits
 // where the bf16 decode keeps 8, and no loss down to 2^-29 of the largest P.
 //
-// K never goes through LDS: lane (l16, g4) reads the 16-byte pieces 16 g4 and
-// 64 + 16 g4 of token l16's row, and the MFMA's contraction index is reordered
-// so that these are its operands (Q is loaded in the same order).  V's rows go
-// through LDS as codes, half the bytes of bf16 rows, and come back transposed
-// (ds_read_b64_tr_b8: 8 tokens of one column per lane).
+// K and V rows are loaded whole, 8 lanes of 16 bytes a row, and staged in LDS
+// as codes, half the bytes of bf16 rows.  (Reading K's MFMA operand straight
+// from memory touches each 128-byte row twice, 64 bytes at a time: 381 us instead
+// of 357 for the loads alone of 1M tokens of 8 heads.)  V comes back transposed
+// (ds_read_b64_tr_b8: 8 tokens of one column per lane).  The K operand's
+// contraction index is reordered so that a lane's 16-byte pieces 16 g4 and
+// 64 + 16 g4 of a row are two operands each (Q is loaded in the same order).
+//
+// Four heads a workgroup of 8 waves where they divide by 4: the rows of a token
+// lie side by side over its heads, and what limits the stream is how much of
+// them is read together (loads alone, 64-token pages in random order: 5.95,
+// 6.59 and 7.00 TB/s with 1, 2 and 4 heads a workgroup; one step or three in
+// flight per wave change nothing).
 #pragma once
 
 #include "fgqa_device.h"
@@ -21,13 +29,13 @@
 
 namespace fgqa {
 
-constexpr int kDec8RowStride = 144;   // LDS bytes of a V row: 16 rows spread over all 64 banks
+constexpr int kDec8RowStride = 144;   // LDS bytes of a row: 16 rows spread over all 64 banks
 constexpr int kDec8TileBytes = kDecStep * kDec8RowStride;
-constexpr int kDec8ScaleBytes = kDecStep * 2 * 4;
-constexpr int kDec8MergeBytes = kDecWaves * 16 * kHeadDim * 4 + kDecWaves * 16 * 2 * 4;
-constexpr int kDec8WaveBytes = kDec8TileBytes + kDec8ScaleBytes;
-constexpr int kDec8SmemBytes =
-    kDecWaves * kDec8WaveBytes > kDec8MergeBytes ? kDecWaves * kDec8WaveBytes : kDec8MergeBytes;
+constexpr int kDec8WaveBytes = 2 * kDec8TileBytes + kDecStep * 2 * 4;   // K, V, their scales
+constexpr int dec8_smem_bytes(int waves) {
+    const int merge = waves * 16 * kHeadDim * 4 + waves * 16 * 2 * 4;
+    return waves * kDec8WaveBytes > merge ? waves * kDec8WaveBytes : merge;
+}
 constexpr float kDec8PScale = 16384.f;   // P's scale in fp16
 
 __device__ __forceinline__ f32x4_t mfma16_f16(f16x8_t a, f16x8_t b, f32x4_t c) {
@@ -44,30 +52,31 @@ __device__ __forceinline__ u32x2_t lds_read_tr8(const unsigned char* p) {
     return __builtin_bit_cast(u32x2_t, v);
 }
 
-// The loads of one 32-token step, and the scales of its tokens' blocks: of the
-// step's 16-token halves (kSeg > 0), or of this lane's two K rows (kSeg 0).
+// The loads of one 32-token step, row 8 r + lane / 8 and piece lane % 8 each, and
+// the scales of its tokens' blocks: of the step's kSegs segments, or (kSeg 0) of
+// this lane's rows.
 struct Step8 {
-    u32x4_t k[2][2];   // token 16 tb + l16: pieces 16 g4 and 64 + 16 g4
-    u32x4_t v[4];      // row 8 r + lane / 8, piece lane % 8
-    float ks[2], vs[2];
+    u32x4_t k[4], v[4];
+    float ks[4], vs[4];
 };
 
 // As dec_item: tokens [t_begin, t_end) (not empty, t_begin a multiple of 128)
-// of one sequence and kv head by 4 waves.  Two steps' loads are in flight per
-// wave: a step of codes is half the bytes of a bf16 one.
-// kSeg (32 or 16, for pages of at least that many rows whose bytes stay below
-// 2^31): a step is one or two page segments, read through buffer resources that
+// of one sequence and kv head, by kNw waves.  Two steps' loads are in flight per
+// wave.
+// kSeg (32, 16 or 8, for pages of at least that many rows whose bytes stay below
+// 2^31): a step is 1, 2 or 4 page segments, read through buffer resources that
 // end at the item's last token (rows past it are zeros), their pages and scales
 // taken 64 segments at a time from one vector load each.  0: any pages, a lookup
 // and a 64-bit address per row.
-template <int kCode, int kSeg>
+template <int kCode, int kSeg, int kNw>
 __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* smem, int t_begin, int t_end, int kvh,
                                           int b, int tid, bool whole, int64_t slot0) {
     const int lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int l16 = lane & 15;
     const int g4 = lane >> 4;
-    unsigned char* vl = smem + wave * kDec8WaveBytes;
+    unsigned char* kl = smem + wave * kDec8WaveBytes;
+    unsigned char* vl = kl + kDec8TileBytes;
     float* sl = reinterpret_cast<float*>(vl + kDec8TileBytes);   // kSeg 0: [32] K scales, [32] V scales
 
     // Q^T as the B operand: lane holds Q[h = l16] at the elements that its
@@ -97,20 +106,20 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
     const float* vscales = p.v_scales + kvh * p.vs_sh;
     const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
     const int pmask = (1 << p.page_shift) - 1;
-    const int v_row = lane >> 3, v_chunk = lane & 7;
+    const int row8 = lane >> 3, piece = lane & 7;
     const int t_end_u = __builtin_amdgcn_readfirstlane(t_end);
     const int n_steps = (t_end - t_begin + kDecStep - 1) / kDecStep;
 
     // kSeg > 0
     constexpr int kSegs = kSeg > 0 ? kDecStep / kSeg : 1;
     const uint32_t kss = (uint32_t)p.k_ss, vss = (uint32_t)p.v_ss;
-    [[maybe_unused]] const uint32_t koff = (uint32_t)l16 * kss + g4 * 16;
-    [[maybe_unused]] const uint32_t voff = (uint32_t)v_row * vss + v_chunk * 16;
+    [[maybe_unused]] const uint32_t koff = (uint32_t)row8 * kss + piece * 16;
+    [[maybe_unused]] const uint32_t voff = (uint32_t)row8 * vss + piece * 16;
     [[maybe_unused]] int pt_page = 0, pt_first = -kWave;   // lane l: the wave's segment pt_first + l
     [[maybe_unused]] float pt_ks = 0.f, pt_vs = 0.f;
     [[maybe_unused]] auto pt_load = [&](int first) {
         const int n = first + lane;
-        const int tok = min(t_begin + (wave + kDecWaves * (n / kSegs)) * kDecStep + kSeg * (n % kSegs), t_end_u - 1);
+        const int tok = min(t_begin + (wave + kNw * (n / kSegs)) * kDecStep + kSeg * (n % kSegs), t_end_u - 1);
         pt_page = min(max(bt[tok >> p.page_shift], 0), p.num_pages - 1);
         pt_ks = kscales[(int64_t)pt_page * p.ks_sp];
         pt_vs = vscales[(int64_t)pt_page * p.vs_sp];
@@ -119,18 +128,16 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
     // kSeg 0: the table's entries are loaded two steps before they are used, and
     // before the rows of the step between: vector loads complete in order, so
     // waiting for them then waits for no row that is not needed yet.
-    [[maybe_unused]] int pg[2][6];   // of the K rows (2) and V rows (4)
-    [[maybe_unused]] auto fetch_pages = [&](int s, int (&to)[6]) {
+    [[maybe_unused]] int pg[2][4];   // of the lane's rows
+    [[maybe_unused]] auto fetch_pages = [&](int s, int (&to)[4]) {
         const int t0 = t_begin + s * kDecStep;
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb) to[tb] = bt[min(t0 + 16 * tb + l16, t_end - 1) >> p.page_shift];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) to[2 + r] = bt[min(t0 + 8 * r + v_row, t_end - 1) >> p.page_shift];
+        for (int r = 0; r < 4; ++r) to[r] = bt[min(t0 + 8 * r + row8, t_end - 1) >> p.page_shift];
     };
-    auto load_step = [&](int s, Step8& x, [[maybe_unused]] const int (&pages)[6]) {
+    auto load_step = [&](int s, Step8& x, [[maybe_unused]] const int (&pages)[4]) {
         const int t0 = t_begin + s * kDecStep;
         if constexpr (kSeg > 0) {
-            const int n0 = ((s - wave) / kDecWaves) * kSegs;   // the wave's first segment of step s
+            const int n0 = ((s - wave) / kNw) * kSegs;   // the wave's first segment of step s
             if (n0 + kSegs > pt_first + kWave) pt_load(n0);
 #pragma unroll
             for (int g = 0; g < kSegs; ++g) {
@@ -146,36 +153,23 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
                 const __amdgpu_buffer_rsrc_t vr =
                     make_rsrc(vbase + page * p.v_sb + slot * vss, nv > 0 ? (uint32_t)(nv - 1) * vss + kHeadDim : 0u);
 #pragma unroll
-                for (int i = 0; i < 2 / kSegs; ++i) {
-                    const int tb = g * (2 / kSegs) + i;
-                    x.k[tb][0] = buf_load16_nt(kr, koff + (uint32_t)(16 * i) * kss);
-                    x.k[tb][1] = buf_load16_nt(kr, koff + (uint32_t)(16 * i) * kss + 64);
-                }
+                for (int i = 0; i < 4 / kSegs; ++i)
+                    x.k[g * (4 / kSegs) + i] = buf_load16_nt(kr, koff + (uint32_t)(8 * i) * kss);
 #pragma unroll
                 for (int i = 0; i < 4 / kSegs; ++i)
                     x.v[g * (4 / kSegs) + i] = buf_load16_nt(vr, voff + (uint32_t)(8 * i) * vss);
             }
-            if constexpr (kSegs == 1) {
-                x.ks[1] = x.ks[0];
-                x.vs[1] = x.vs[0];
-            }
         } else {
 #pragma unroll
-            for (int tb = 0; tb < 2; ++tb) {
-                const int slot = min(t0 + 16 * tb + l16, t_end - 1) & pmask;
-                const int64_t page = min(max(pages[tb], 0), p.num_pages - 1);
-                const unsigned char* row = kbase + page * p.k_sb + (int64_t)slot * p.k_ss + g4 * 16;
-                x.k[tb][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row));
-                x.k[tb][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(row + 64));
-                x.ks[tb] = kscales[page * p.ks_sp];
-                x.vs[tb] = vscales[page * p.vs_sp];
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int slot = min(t0 + 8 * r + v_row, t_end - 1) & pmask;
-                const int64_t page = min(max(pages[2 + r], 0), p.num_pages - 1);
-                x.v[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
-                    vbase + page * p.v_sb + (int64_t)slot * p.v_ss + v_chunk * 16));
+            for (int r = 0; r < 4; ++r) {   // (past the item's end: its last token)
+                const int64_t slot = min(t0 + 8 * r + row8, t_end - 1) & pmask;
+                const int64_t page = min(max(pages[r], 0), p.num_pages - 1);
+                x.k[r] = __builtin_nontemporal_load(
+                    reinterpret_cast<const u32x4_t*>(kbase + page * p.k_sb + slot * p.k_ss + piece * 16));
+                x.v[r] = __builtin_nontemporal_load(
+                    reinterpret_cast<const u32x4_t*>(vbase + page * p.v_sb + slot * p.v_ss + piece * 16));
+                x.ks[r] = kscales[page * p.ks_sp];
+                x.vs[r] = vscales[page * p.vs_sp];
             }
         }
     };
@@ -183,20 +177,31 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
     // One step; its registers are free for the next loads once `reload` is called.
     auto compute = [&](int st, Step8& x, auto&& reload) {
         const int t0 = t_begin + st * kDecStep;
-        float ks[8], vs[8];
-        float vmax = vref;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            *reinterpret_cast<u32x4_t*>(vl + (8 * r + v_row) * kDec8RowStride + v_chunk * 16) = x.v[r];
+        for (int r = 0; r < 4; ++r) {
+            *reinterpret_cast<u32x4_t*>(kl + (8 * r + row8) * kDec8RowStride + piece * 16) = x.k[r];
+            *reinterpret_cast<u32x4_t*>(vl + (8 * r + row8) * kDec8RowStride + piece * 16) = x.v[r];
+        }
         if constexpr (kSeg == 0) {
-            if (g4 == 0) {
+            if (piece == 0) {
 #pragma unroll
-                for (int tb = 0; tb < 2; ++tb) {
-                    sl[16 * tb + l16] = x.ks[tb];
-                    sl[kDecStep + 16 * tb + l16] = x.vs[tb];
+                for (int r = 0; r < 4; ++r) {
+                    sl[8 * r + row8] = x.ks[r];
+                    sl[kDecStep + 8 * r + row8] = x.vs[r];
                 }
             }
         }
+        float ks_seg[4], vs_seg[4];
+#pragma unroll
+        for (int g = 0; g < kSegs; ++g) {
+            ks_seg[g] = x.ks[g];
+            vs_seg[g] = x.vs[g];
+        }
+        reload();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+
         // S^T = K Q^T (codes), K as the A operand
         f32x4_t s[2];
 #pragma unroll
@@ -204,22 +209,30 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
             s[tb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                s[tb] = mfma16(codes_to_bf16<kCode>(x.k[tb][j][0], x.k[tb][j][1]), qop[2 * j], s[tb]);
-                s[tb] = mfma16(codes_to_bf16<kCode>(x.k[tb][j][2], x.k[tb][j][3]), qop[2 * j + 1], s[tb]);
+                const u32x4_t c =
+                    *reinterpret_cast<const u32x4_t*>(kl + (16 * tb + l16) * kDec8RowStride + 64 * j + 16 * g4);
+                s[tb] = mfma16(codes_to_bf16<kCode>(c[0], c[1]), qop[2 * j], s[tb]);
+                s[tb] = mfma16(codes_to_bf16<kCode>(c[2], c[3]), qop[2 * j + 1], s[tb]);
             }
         }
-        const float ks_half[2] = {x.ks[0], x.ks[1]}, vs_half[2] = {x.vs[0], x.vs[1]};
-        reload();
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        // scales of tokens t0 + 16*tb + 4*g4 + i
+        float ks[8], vs[8];
+        float vmax = vref;
         if constexpr (kSeg > 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                ks[j] = ks_half[j / 4] * p.scale_log2;
-                vs[j] = vs_half[j / 4];
+            for (int tb = 0; tb < 2; ++tb) {
+                const int g = kSegs == 1 ? 0 : kSegs == 2 ? tb : 2 * tb;
+                const bool second = kSegs == 4 && g4 >= 2;
+                const float k1 = second ? ks_seg[kSegs == 4 ? g + 1 : g] : ks_seg[g];
+                const float v1 = second ? vs_seg[kSegs == 4 ? g + 1 : g] : vs_seg[g];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    ks[4 * tb + i] = k1 * p.scale_log2;
+                    vs[4 * tb + i] = v1;
+                }
             }
-            vmax = fmaxf(vmax, fmaxf(fabsf(vs_half[0]), fabsf(vs_half[1])));
+#pragma unroll
+            for (int g = 0; g < kSegs; ++g) vmax = fmaxf(vmax, fabsf(vs_seg[g]));
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -277,26 +290,25 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
     };
 
     Step8 step_a, step_b;
-    auto load_if = [&](int s, Step8& x, int (&pages)[6], int (&next)[6]) {
-        if (kSeg == 0 && s + kDecWaves < n_steps) fetch_pages(s + kDecWaves, next);
+    auto load_if = [&](int s, Step8& x, int (&pages)[4], int (&next)[4]) {
+        if (kSeg == 0 && s + kNw < n_steps) fetch_pages(s + kNw, next);
         if (s < n_steps) load_step(s, x, pages);
     };
     int st = wave;
     if (kSeg == 0 && st < n_steps) fetch_pages(st, pg[0]);
     load_if(st, step_a, pg[0], pg[1]);
-    load_if(st + kDecWaves, step_b, pg[1], pg[0]);
-    for (; st < n_steps; st += 2 * kDecWaves) {
-        compute(st, step_a, [&] { load_if(st + 2 * kDecWaves, step_a, pg[0], pg[1]); });
-        if (st + kDecWaves < n_steps)
-            compute(st + kDecWaves, step_b, [&] { load_if(st + 3 * kDecWaves, step_b, pg[1], pg[0]); });
+    load_if(st + kNw, step_b, pg[1], pg[0]);
+    for (; st < n_steps; st += 2 * kNw) {
+        compute(st, step_a, [&] { load_if(st + 2 * kNw, step_a, pg[0], pg[1]); });
+        if (st + kNw < n_steps) compute(st + kNw, step_b, [&] { load_if(st + 3 * kNw, step_b, pg[1], pg[0]); });
     }
 
     l_run = xor_sum(xor_sum(l_run, 16), 32);
 
-    // Merge the 4 waves in LDS (reusing the staging area).
+    // Merge the waves in LDS (reusing the staging area).
     __syncthreads();
     float* ow = reinterpret_cast<float*>(smem);   // [wave][16][128]
-    float* mlw = ow + kDecWaves * 16 * kHeadDim;  // [wave][16][2]
+    float* mlw = ow + kNw * 16 * kHeadDim;        // [wave][16][2]
     const float oscale = vref * (1.f / kDec8PScale);
 #pragma unroll
     for (int db = 0; db < 8; ++db)
@@ -308,42 +320,42 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
     }
     __syncthreads();
 
-    const int h = tid >> 4;
     const int d0 = (tid & 15) * 8;
-    if (h >= p.group) return;
-    float mw[kDecWaves];
-    float M = -INFINITY;
+    for (int h = tid >> 4; h < p.group; h += kNw * 4) {
+        float mw[kNw];
+        float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kDecWaves; ++w) {
-        mw[w] = mlw[(w * 16 + h) * 2];
-        M = fmaxf(M, mw[w]);
-    }
-    float L = 0.f;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < kNw; ++w) {
+            mw[w] = mlw[(w * 16 + h) * 2];
+            M = fmaxf(M, mw[w]);
+        }
+        float L = 0.f;
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kDecWaves; ++w) {
-        const float c = (mw[w] == -INFINITY) ? 0.f : fast_exp2(mw[w] - M);
-        L += c * mlw[(w * 16 + h) * 2 + 1];
-        const float* src = ow + (w * 16 + h) * kHeadDim + d0;
+        for (int w = 0; w < kNw; ++w) {
+            const float c = (mw[w] == -INFINITY) ? 0.f : fast_exp2(mw[w] - M);
+            L += c * mlw[(w * 16 + h) * 2 + 1];
+            const float* src = ow + (w * 16 + h) * kHeadDim + d0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += c * src[j];
-    }
-    const int qh = kvh * p.group + h;
-    if (whole) {
-        const float inv = 1.f / L;
-        bf16x8_t out;
+            for (int j = 0; j < 8; ++j) acc[j] += c * src[j];
+        }
+        const int qh = kvh * p.group + h;
+        if (whole) {
+            const float inv = 1.f / L;
+            bf16x8_t out;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) out[j] = (__bf16)(acc[j] * inv);
-        *reinterpret_cast<bf16x8_t*>(p.o + b * p.o_sb + qh * p.o_sh + d0) = out;
-        if (p.lse != nullptr && (tid & 15) == 0) p.lse[(int64_t)b * p.hq + qh] = M * kLn2 + logf(L);
-    } else {
-        const int64_t slot = slot0 + h;
-        float* po = p.part_o + slot * kHeadDim + d0;
-        *reinterpret_cast<f32x4_t*>(po) = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
-        *reinterpret_cast<f32x4_t*>(po + 4) = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
-        if ((tid & 15) == 0) {
-            p.part_ml[slot * 2 + 0] = M;
-            p.part_ml[slot * 2 + 1] = L;
+            for (int j = 0; j < 8; ++j) out[j] = (__bf16)(acc[j] * inv);
+            *reinterpret_cast<bf16x8_t*>(p.o + b * p.o_sb + qh * p.o_sh + d0) = out;
+            if (p.lse != nullptr && (tid & 15) == 0) p.lse[(int64_t)b * p.hq + qh] = M * kLn2 + logf(L);
+        } else {
+            const int64_t slot = slot0 + h;
+            float* po = p.part_o + slot * kHeadDim + d0;
+            *reinterpret_cast<f32x4_t*>(po) = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
+            *reinterpret_cast<f32x4_t*>(po + 4) = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
+            if ((tid & 15) == 0) {
+                p.part_ml[slot * 2 + 0] = M;
+                p.part_ml[slot * 2 + 1] = L;
+            }
         }
     }
 }

@@ -436,15 +436,16 @@ __device__ __forceinline__ void dec_item(const DecodeParams& p, unsigned char* s
 
 namespace fgqa {
 
-// The item of each layout, and its LDS.
-template <int kKv>
-constexpr int kDecItemSmem = kKv >= kKvBlocksFp8 ? kDec8SmemBytes : kDecSmemBytes;
+// The item of each layout, and its LDS, for kNw waves.
+template <int kKv, int kNw>
+constexpr int kDecItemSmem = kKv >= kKvBlocksFp8 ? dec8_smem_bytes(kNw) : kDecSmemBytes;
 
-template <int kKv, int kSeg>
+template <int kKv, int kSeg, int kNw>
 __device__ __forceinline__ void dec_item_of(const DecodeParams& p, unsigned char* smem, int t_begin, int t_end, int kvh,
                                             int b, int tid, bool whole, int64_t slot0) {
     if constexpr (kKv >= kKvBlocksFp8)
-        dec_item8<kKv == kKvBlocksFp8 ? kCodeFp8 : kCodeInt8, kSeg>(p, smem, t_begin, t_end, kvh, b, tid, whole, slot0);
+        dec_item8<kKv == kKvBlocksFp8 ? kCodeFp8 : kCodeInt8, kSeg, kNw>(p, smem, t_begin, t_end, kvh, b, tid, whole,
+                                                                         slot0);
     else
         dec_item<kKv, kSeg>(p, smem, t_begin, t_end, kvh, b, tid, whole, slot0);
 }
@@ -643,16 +644,24 @@ __device__ __forceinline__ int seq_blocks(int len) {
     return (len + plan::kDecodeStepRound - 1) / plan::kDecodeStepRound;
 }
 
-template <int kKv, int kSeg = 0, bool kPair = false>
-__global__ __launch_bounds__(kPair ? 2 * kDecThreads : kDecThreads) void decode_list_kernel(DecodeParams p) {
-    constexpr int kThreads = kPair ? 2 * kDecThreads : kDecThreads;
-    constexpr int kSmem = kDecItemSmem<kKv>;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[(kPair ? 2 : 1) * kSmem];
+//
+// kHeads: adjacent kv heads of a workgroup, 1 or such a pair of 4 waves each, or
+// (8-bit caches with block scales) 4 of 2 waves each.
+template <int kHeads>
+constexpr int kListWaves = kHeads == 4 ? 2 : kDecWaves;   // of one head
+
+template <int kKv, int kSeg = 0, int kHeads = 1>
+__global__ __launch_bounds__(kHeads* kListWaves<kHeads>* kWave) void decode_list_kernel(DecodeParams p) {
+    constexpr int kNw = kListWaves<kHeads>;
+    constexpr int kItemThreads = kNw * kWave;
+    constexpr int kThreads = kHeads * kItemThreads;
+    constexpr int kSmem = kDecItemSmem<kKv, kNw>;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kHeads * kSmem];
     // wave-uniform (readfirstlane), so the buffer resources built from the
     // head stay scalar
-    const int half = kPair ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kDecThreads)) : 0;
-    const int per_entry = kPair ? p.hkv / 2 : p.hkv;
-    const int tid = (int)threadIdx.x - half * kDecThreads;
+    const int half = kHeads > 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kItemThreads)) : 0;
+    const int per_entry = p.hkv / kHeads;
+    const int tid = (int)threadIdx.x - half * kItemThreads;
     // work list: items blockIdx.x, + gridDim.x, ...
     int item = blockIdx.x;
     const int n_items = p.work != nullptr ? p.work[0] * per_entry : 0;
@@ -729,7 +738,7 @@ __global__ __launch_bounds__(kPair ? 2 * kDecThreads : kDecThreads) void decode_
             t_begin = split * p.chunk;
             t_end = min(t_begin + p.chunk, clamp_len(p, b));
             whole = p.nsplit == 1;
-            kvh = kPair ? 2 * kvh + half : kvh;
+            kvh = kHeads * kvh + half;
             slot = ((int64_t)b * p.hkv + kvh) * p.nsplit + split;
             item += gridDim.x;
         } else {
@@ -745,11 +754,11 @@ __global__ __launch_bounds__(kPair ? 2 * kDecThreads : kDecThreads) void decode_
             t_end = min((blk + n) * plan::kDecodeStepRound, len);
             whole = n == nb;
             kvh = blockIdx.x % per_entry;
-            kvh = kPair ? 2 * kvh + half : kvh;
+            kvh = kHeads * kvh + half;
             slot = (int64_t)(2 * team + (blk == 0 ? 1 : 0)) * p.hkv + kvh;
         }
         __syncthreads();   // the previous item's merge buffers alias the staging area
-        dec_item_of<kKv, kSeg>(p, smem + half * kSmem, t_begin, t_end, kvh, b, tid, whole, slot * p.group);
+        dec_item_of<kKv, kSeg, kNw>(p, smem + half * kSmem, t_begin, t_end, kvh, b, tid, whole, slot * p.group);
         if (p.work == nullptr) {
             g0 += (t_end - t_begin + plan::kDecodeStepRound - 1) / plan::kDecodeStepRound;
             ++b;
@@ -760,19 +769,26 @@ __global__ __launch_bounds__(kPair ? 2 * kDecThreads : kDecThreads) void decode_
 
 // Launches pass 1 over a ragged batch: the head-pair form (one 8-wave
 // workgroup per CU) when the kv heads pair up, else two 4-wave workgroups per
-// CU.  A work list's grid never exceeds what the CUs hold at once; the teams fill
+// CU; over blocks with scales 4 heads per 8-wave workgroup where they divide.  A
+// work list's grid never exceeds what the CUs hold at once; the teams fill
 // 256 CUs (kDecodeItemSlots), and on fewer they run in more than one round.
+template <int kKv, int kSeg, int kHeads>
+static void launch_list_heads(const DecodeParams& p, int nsplit, int cus, hipStream_t s) {
+    const int per_entry = p.hkv / kHeads;
+    const int64_t items = (int64_t)p.batch * nsplit * per_entry;   // most the list can hold
+    const int64_t slots = (int64_t)(kHeads == 1 ? 2 : 1) * cus;
+    const int grid = p.teams > 0 ? p.teams * per_entry : (int)(items < slots ? items : slots);
+    hipLaunchKernelGGL((decode_list_kernel<kKv, kSeg, kHeads>), dim3(grid), dim3(kHeads * kListWaves<kHeads> * kWave), 0, s,
+                       p);
+}
+
 template <int kKv, int kSeg>
 static void launch_list(const DecodeParams& p, int nsplit, int cus, hipStream_t s) {
-    const bool pair = (p.hkv % 2) == 0;
-    const int per_entry = pair ? p.hkv / 2 : p.hkv;
-    const int64_t items = (int64_t)p.batch * nsplit * per_entry;   // most the list can hold
-    const int64_t slots = (int64_t)(pair ? 1 : 2) * cus;
-    const int grid = p.teams > 0 ? p.teams * per_entry : (int)(items < slots ? items : slots);
-    if (pair)
-        hipLaunchKernelGGL((decode_list_kernel<kKv, kSeg, true>), dim3(grid), dim3(2 * kDecThreads), 0, s, p);
-    else
-        hipLaunchKernelGGL((decode_list_kernel<kKv, kSeg, false>), dim3(grid), dim3(kDecThreads), 0, s, p);
+    if constexpr (kKv >= kKvBlocksFp8) {
+        if (p.hkv % 4 == 0) return launch_list_heads<kKv, kSeg, 4>(p, nsplit, cus, s);
+    }
+    if (p.hkv % 2 == 0) launch_list_heads<kKv, kSeg, 2>(p, nsplit, cus, s);
+    else launch_list_heads<kKv, kSeg, 1>(p, nsplit, cus, s);
 }
 
 // Log-sum-exp merge of the partials of each (sequence, query head): 16 lanes
@@ -1168,7 +1184,7 @@ namespace {
 int paged_run(const fgqa_decode_paged_args* a, const fgqa_kv_cache* blocks, void* stream) {
     if (a->batch == 0) return FGQA_OK;
     DecodePlan plan;
-    int st = plan::plan_paged(a, &plan);
+    int st = plan::plan_paged(a, &plan, blocks != nullptr ? plan::block_item_slots(a->num_kv_heads) : plan::kDecodeItemSlots);
     if (st != FGQA_OK) return st;
 
     DecodeParams p;
@@ -1246,9 +1262,10 @@ int paged_run(const fgqa_decode_paged_args* a, const fgqa_kv_cache* blocks, void
         auto pass1 = [&] {
             if (blocks != nullptr) {
                 auto launch = [&](auto kv) {
-                    switch (seg >= 16 ? seg : 0) {
+                    switch (seg >= 8 ? seg : 0) {
                         case 32: launch_list<decltype(kv)::value, 32>(p, plan.nsplit, cus, s); break;
                         case 16: launch_list<decltype(kv)::value, 16>(p, plan.nsplit, cus, s); break;
+                        case 8: launch_list<decltype(kv)::value, 8>(p, plan.nsplit, cus, s); break;
                         default: launch_list<decltype(kv)::value, 0>(p, plan.nsplit, cus, s); break;
                     }
                 };
@@ -1294,7 +1311,11 @@ extern "C" int fgqa_decode_blocks_workspace_bytes(const fgqa_decode_blocks_args*
     const int st = plan::validate_decode_blocks(a);
     if (st != FGQA_OK) return st;
     const fgqa_decode_paged_args p = plan::as_decode_paged(a);
-    return fgqa_decode_paged_workspace_bytes(&p, bytes);
+    DecodePlan plan;
+    const int planned = plan::plan_paged(&p, &plan, plan::block_item_slots(p.num_kv_heads));
+    if (planned != FGQA_OK) return planned;
+    *bytes = plan.ws_bytes;
+    return FGQA_OK;
 }
 
 extern "C" int fgqa_decode_blocks(const fgqa_decode_blocks_args* a, void* stream) {

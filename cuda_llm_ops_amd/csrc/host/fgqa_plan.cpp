@@ -145,11 +145,11 @@ int plan_decode(const DecodeShape& a, int cus, DecodePlan* plan) {
     plan->least_bytes = plan->ws_bytes;
     plan->teams = 0;
     plan->team_ml_off = plan->team_prefix_off = 0;
-    if (plan->list && a.split_tokens == 0 && a.num_kv_heads <= kDecodeItemSlots) {
+    if (plan->list && a.split_tokens == 0 && a.num_kv_heads <= a.item_slots) {
         // (the list's size stays the least that a caller's scratch needs, so
         // that which calls fit a scratch does not depend on how the batch is
         // shared out)
-        plan->teams = kDecodeItemSlots / a.num_kv_heads;
+        plan->teams = a.item_slots / a.num_kv_heads;
         const i128 rows = (i128)2 * plan->teams * a.num_q_heads;
         plan->team_ml_off = round256(rows * kHeadDim * 4);
         plan->team_prefix_off = plan->team_ml_off + round256(rows * 2 * 4);
@@ -208,8 +208,8 @@ int validate_paged_pointers(const fgqa_decode_paged_args* a) {
     return FGQA_OK;
 }
 
-int plan_paged(const fgqa_decode_paged_args* a, DecodePlan* plan) {
-    const DecodeShape shape{a->batch, a->max_seqlen, a->num_q_heads, a->num_kv_heads, a->split_tokens, true};
+int plan_paged(const fgqa_decode_paged_args* a, DecodePlan* plan, int item_slots) {
+    const DecodeShape shape{a->batch, a->max_seqlen, a->num_q_heads, a->num_kv_heads, a->split_tokens, true, item_slots};
     if (!list_batch(shape)) return FGQA_ERR_UNSUPPORTED;
     const int st = plan_decode(shape, 0, plan);
     if (st != FGQA_OK) return st;

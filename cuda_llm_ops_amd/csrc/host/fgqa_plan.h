@@ -50,13 +50,14 @@ constexpr int kDecodeItemCost = 128;
 struct DecodeShape {
     int batch, max_seqlen, num_q_heads, num_kv_heads, split_tokens;
     bool ragged;   // per-sequence lengths are given
+    int item_slots = kDecodeItemSlots;   // of a ragged batch's teams
 };
 
 struct DecodePlan {
     int chunk;            // tokens per split (a multiple of kDecodeStepRound)
     int nsplit;           // splits per sequence
     bool list;            // ragged batch: teams, or (split length given) a device-built work list of non-empty splits
-    int teams;            // ragged batch without a given split length, at most kDecodeItemSlots kv heads: its
+    int teams;            // ragged batch without a given split length, at most item_slots kv heads: its
                           // teams (else 0)
     size_t part_o_bytes;  // fp32 partial O of every split (nsplit > 1)
     size_t part_ml_bytes; // their (max, sum)
@@ -89,7 +90,7 @@ int validate_paged_pointers(const fgqa_decode_paged_args* a);
 // The paged decode always runs the work-list kernel (it needs no CU count): a
 // shape the list cannot index (batch >= 2^15 or >= 2^16 splits) is
 // FGQA_ERR_UNSUPPORTED.
-int plan_paged(const fgqa_decode_paged_args* a, DecodePlan* plan);
+int plan_paged(const fgqa_decode_paged_args* a, DecodePlan* plan, int item_slots = kDecodeItemSlots);
 
 // ---------------------------------------------------------------- prefill
 constexpr int kPrefillMaxSplit = 128;     // most unit pairs whose units a launch may split

@@ -20,6 +20,10 @@ int validate_decode_blocks(const fgqa_decode_blocks_args* a);
 int validate_decode_blocks_pointers(const fgqa_decode_blocks_args* a);
 fgqa_decode_paged_args as_decode_paged(const fgqa_decode_blocks_args* a);
 
+// Heads' items that the chip holds at once in the block-scaled decode: 256 CUs
+// times 4 heads of 2 waves, or 2 of 4.
+constexpr int block_item_slots(int num_kv_heads) { return num_kv_heads % 4 == 0 ? 1024 : kDecodeItemSlots; }
+
 inline int log2_of(int power_of_two) {
     int shift = 0;
     while ((1 << shift) < power_of_two) ++shift;

@@ -280,7 +280,14 @@ def _has_block_scales(k_cache, k_scale, v_scale) -> bool:
 
 @functools.lru_cache(maxsize=256)
 def _blocks_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, split_tokens) -> int:
-    return paged_decode_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, split_tokens=split_tokens)
+    a = _lib.DecodeBlocksArgs()
+    a.kv_dtype, a.num_kv_heads, a.head_dim, a.page_size, a.num_pages = _lib.FGQA_KV_INT8, Hkv, 128, page_size, 1
+    a.batch, a.max_seqlen, a.num_q_heads, a.scale, a.split_tokens = B, max_seqlen, Hq, 1.0, split_tokens
+    a.block_table_stride = -(-max_seqlen // page_size)
+    n = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().fgqa_decode_blocks_workspace_bytes(ctypes.byref(a), ctypes.byref(n)),
+               "fgqa_decode_blocks_workspace_bytes")
+    return int(n.value)
 
 
 def _blocks_args(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse, max_seqlen,

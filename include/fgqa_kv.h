@@ -96,9 +96,9 @@ int fgqa_kv_append(const fgqa_kv_append_args* args, void* stream);
 /*
  * fgqa_decode_paged over a cache with block scales (e4m3 or int8): scores use
  * q.c * k_scales[page][head] * scale, and O sums p * c * v_scales[page][head].
- * q, o, lse, block_table, seqlens, scale, split_tokens, workspace: as there;
- * the workspace is that of fgqa_decode_paged for the same sizes.  Codes are
- * widened exactly; P is rounded to fp16 (11 bits) for P.V, sums are fp32.
+ * q, o, lse, block_table, seqlens, scale, split_tokens, workspace: as there.
+ * Codes are widened exactly; P is rounded to fp16 (11 bits) for P.V, sums are
+ * fp32.
  */
 typedef struct fgqa_decode_blocks_args {
     fgqa_kv_cache cache;

@@ -242,4 +242,5 @@ def test_c_abi_refuses_before_launch():
     a.batch, a.max_seqlen, a.num_q_heads, a.block_table_stride, a.scale = 2, 4096, 32, 256, 0.1
     assert L.fgqa_decode_blocks_workspace_bytes(ctypes.byref(a), None) == _lib.FGQA_ERR_INVALID_ARGUMENT
     assert L.fgqa_decode_blocks_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == 0
-    assert n.value == fg.paged_decode_workspace_bytes(2, 4096, 32, 8, 16)
+    # 128 teams of 8 heads: two partials of 32 rows (512 + 8 bytes) each, and the sequences' prefix
+    assert n.value == 2 * 128 * 32 * 520 + 3 * 8
