@@ -250,14 +250,25 @@ struct WeightsParams {
     int64_t items;   // batch * chunks * hkv
 };
 
-// One wave per item of `chunk` tokens of one KV head, 32 at a time; heads side
-// by side.  S[h][t] = Q[h][:] . K[t][:] by v_mfma_f32_16x16x32_bf16 with the 16
-// query heads (zero past the group) as rows, so that a lane holds one token's
-// scores of 4 heads and the sum over heads takes two exchanges.  The order of
-// the head dim inside the products is free as long as Q's is the same: lane
-// group g4 takes the elements that its 16-byte pieces of the rows hold.
-template <int kCode, Scaling kScaling>
+// One wave per item of `chunk` tokens of one KV head, 32 at a time; the waves of
+// a workgroup take adjacent heads, so that a token's rows, which lie side by
+// side, are read together.  Rows are loaded whole (8 lanes of 16 bytes for codes,
+// 16 for bf16), two steps ahead, and staged in LDS as they are.
+// S[h][t] = Q[h][:] . K[t][:] by v_mfma_f32_16x16x32_bf16 with the 16 query heads
+// (zero past the group) as rows: a lane holds one token's scores of 4 heads, and
+// the sum over heads takes two exchanges of lane groups.  The order of the head
+// dim inside the products is free as long as Q's is the same: lane group g4
+// takes the elements of the 16-byte pieces that it reads.
+// kSeg (32, 16 or 8): page segments as in the block-scaled decode; 0: any pages.
+template <int kCode, Scaling kScaling, int kSeg>
 __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
+    constexpr int kStep = 32;
+    constexpr int kRowBytes = kCode == kCodeBf16 ? 256 : 128;
+    constexpr int kLanes = kRowBytes / 16;          // of a row
+    constexpr int kRows = kWave / kLanes;           // of one load instruction
+    constexpr int kLoads = kStep / kRows;           // of a step
+    constexpr int kStride = kRowBytes + 16;         // LDS bytes of a row: 16 rows spread over all banks
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kWaves * kStep * kStride];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
     const int l16 = lane & 15, g4 = lane >> 4;
@@ -268,10 +279,27 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
     const int b = (int)(rest / p.chunks);
     const int t_begin = (int)(rest % p.chunks) * p.chunk;
     const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
-    const int t_end = min(t_begin + p.chunk, len);
+    const int t_end = __builtin_amdgcn_readfirstlane(min(t_begin + p.chunk, len));
     if (t_begin >= t_end) return;
 
-    constexpr int kPieces = kCode == kCodeBf16 ? 4 : 2;   // 16-byte pieces of a row that a lane holds
+    const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
+    const int pmask = (1 << p.c.page_shift) - 1;
+    const unsigned char* kbase = p.c.data[0] + kvh * p.c.head[0];
+    const float* scales = p.c.scales[0] + kvh * p.c.scale_head[0];
+    float* wrow = p.weights + b * p.w_b + kvh * p.w_h;
+    unsigned char* kl = smem + wave * kStep * kStride;
+    const int row = lane / kLanes, piece = lane % kLanes;
+    const int n_steps = (t_end - t_begin + kStep - 1) / kStep;
+
+    // Segment l of the item (at most 64) has its page and scale in lane l.
+    constexpr int kSegs = kSeg > 0 ? kStep / kSeg : 1;
+    constexpr int kPer = kLoads / kSegs;
+    [[maybe_unused]] int seg_page = 0;
+    [[maybe_unused]] float seg_scale = p.scale;
+    if constexpr (kSeg > 0) {
+        seg_page = min(max(bt[min(t_begin + kSeg * lane, t_end - 1) >> p.c.page_shift], 0), p.c.num_pages - 1);
+        if constexpr (kScaling == kBlocks) seg_scale *= scales[(int64_t)seg_page * p.c.scale_page[0]];
+    }
     bf16x8_t qop[4];
     {
         const __bf16* qrow = p.q + b * p.q_b + (int64_t)(kvh * p.group + min(l16, p.group - 1)) * p.q_h;
@@ -293,36 +321,110 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
         const float l = p.lse[(int64_t)b * p.c.hkv * p.group + kvh * p.group + min(g, p.group - 1)];
         neg_lse[i] = g < p.group ? -l : -INFINITY;
     }
-    const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
-    const int pmask = (1 << p.c.page_shift) - 1;
-    const unsigned char* kbase = p.c.data[0] + kvh * p.c.head[0] + g4 * 16;
-    float* wrow = p.weights + b * p.w_b + kvh * p.w_h;
-    for (int t0 = t_begin; t0 < t_end; t0 += 32) {
+
+    struct Step {
+        u32x4_t k[kLoads];
+        float scale[2];   // kSeg 0: of tokens l16 and 16 + l16
+        float w;          // old weight of token lane (below 32)
+    };
+    const uint32_t kss = (uint32_t)p.c.slot[0];
+    [[maybe_unused]] const uint32_t koff = (uint32_t)row * kss + piece * 16;
+    auto load = [&](int s, Step& x) {
+        const int t0 = t_begin + s * kStep;
+        if constexpr (kSeg > 0) {
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb) {
-            const int tok = t0 + 16 * tb + l16;
-            const int at = min(tok, t_end - 1);   // (past the end: its last token, not stored)
-            const int page = min(max(bt[at >> p.c.page_shift], 0), p.c.num_pages - 1);
-            const unsigned char* row = kbase + page * p.c.page[0] + (at & pmask) * p.c.slot[0];
-            float ks = p.scale;
-            if constexpr (kScaling == kBlocks) ks *= p.c.scales[0][page * p.c.scale_page[0] + kvh * p.c.scale_head[0]];
-            f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+            for (int g = 0; g < kSegs; ++g) {
+                const int64_t page = __builtin_amdgcn_readlane(seg_page, s * kSegs + g);
+                const int tok = t0 + kSeg * g;
+                const int nv = min(kSeg, t_end - tok);   // rows before the item's end; the others read as zeros
+                const __amdgpu_buffer_rsrc_t r =
+                    make_rsrc(kbase + page * p.c.page[0] + (uint32_t)(tok & pmask) * kss,
+                              nv > 0 ? (uint32_t)(nv - 1) * kss + kRowBytes : 0u);
 #pragma unroll
-            for (int j = 0; j < kPieces; ++j) {
-                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + 64 * j);
-                if constexpr (kCode == kCodeBf16) {
-                    s = mfma16(qop[j], as_bf16x8(w), s);
-                } else {
-                    s = mfma16(qop[2 * j], codes_to_bf16<kCode>(w[0], w[1]), s);
-                    s = mfma16(qop[2 * j + 1], codes_to_bf16<kCode>(w[2], w[3]), s);
+                for (int i = 0; i < kPer; ++i) x.k[g * kPer + i] = buf_load16_nt(r, koff + (uint32_t)(kRows * i) * kss);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {   // (past the end: its last token, not stored)
+                const int tok = min(t0 + kRows * i + row, t_end - 1);
+                const int64_t page = min(max(bt[tok >> p.c.page_shift], 0), p.c.num_pages - 1);
+                x.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
+                    kbase + page * p.c.page[0] + (tok & pmask) * p.c.slot[0] + piece * 16));
+            }
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb) {
+                x.scale[tb] = p.scale;
+                if constexpr (kScaling == kBlocks) {
+                    const int tok = min(t0 + 16 * tb + l16, t_end - 1);
+                    const int64_t page = min(max(bt[tok >> p.c.page_shift], 0), p.c.num_pages - 1);
+                    x.scale[tb] *= scales[page * p.c.scale_page[0]];
                 }
             }
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum += fast_exp2(fmaf(s[i], ks, neg_lse[i]) * kLog2e);
-            sum = xor_sum(xor_sum(sum, 16), 32);
-            if (g4 == 0 && tok < t_end) wrow[tok] += sum;
         }
+        x.w = wrow[min(t0 + (lane & 31), t_end - 1)];
+    };
+    auto compute = [&](int s, Step& x, auto&& reload) {
+        const int t0 = t_begin + s * kStep;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            *reinterpret_cast<u32x4_t*>(kl + (kRows * i + row) * kStride + piece * 16) = x.k[i];
+        const float old = x.w;
+        float scale[2];
+        if constexpr (kSeg > 0) {
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb) {
+                auto of = [&](int g) {
+                    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(seg_scale), s * kSegs + g));
+                };
+                if constexpr (kSegs == 1) scale[tb] = of(0);
+                else if constexpr (kSegs == 2) scale[tb] = of(tb);
+                else scale[tb] = l16 < 8 ? of(2 * tb) : of(2 * tb + 1);
+            }
+        } else {
+            scale[0] = x.scale[0];
+            scale[1] = x.scale[1];
+        }
+        reload();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        float sum[2];
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+            f32x4_t c = {0.f, 0.f, 0.f, 0.f};
+            const unsigned char* src = kl + (16 * tb + l16) * kStride + 16 * g4;
+#pragma unroll
+            for (int j = 0; j < kRowBytes / 64; ++j) {
+                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(src + 64 * j);
+                if constexpr (kCode == kCodeBf16) {
+                    c = mfma16(qop[j], as_bf16x8(w), c);
+                } else {
+                    c = mfma16(qop[2 * j], codes_to_bf16<kCode>(w[0], w[1]), c);
+                    c = mfma16(qop[2 * j + 1], codes_to_bf16<kCode>(w[2], w[3]), c);
+                }
+            }
+            sum[tb] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[tb] += fast_exp2(fmaf(c[i], scale[tb], neg_lse[i]) * kLog2e);
+        }
+        // over the lane groups: groups 0 and 1 get the sums of tokens l16 and 16 + l16
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum[0]), __float_as_uint(sum[1]), false, false);
+        const float total = half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+        const int tok = t0 + lane;
+        if (lane < kStep && tok < t_end) wrow[tok] = old + total;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    Step a, c;
+    auto load_if = [&](int s, Step& x) {
+        if (s < n_steps) load(s, x);
+    };
+    load_if(0, a);
+    load_if(1, c);
+    for (int s = 0; s < n_steps; s += 2) {
+        compute(s, a, [&] { load_if(s + 2, a); });
+        if (s + 1 < n_steps) compute(s + 1, c, [&] { load_if(s + 3, c); });
     }
 }
 
@@ -587,6 +689,15 @@ void launch_append(const AppendParams& p, int page_size, hipStream_t s) {
 }
 
 template <int kCode, Scaling kScaling>
+void launch_weights(const WeightsParams& p, int page_size, hipStream_t s) {
+    const dim3 grid((unsigned)ceil_div(p.items, kWaves)), block(kThreads);
+    if (page_size >= 32) hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 32>), grid, block, 0, s, p);
+    else if (page_size == 16) hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 16>), grid, block, 0, s, p);
+    else if (page_size == 8) hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 8>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 0>), grid, block, 0, s, p);
+}
+
+template <int kCode, Scaling kScaling>
 void launch_move(const EvictParams& p, int page_size, hipStream_t s) {
     with_shape(page_size, [&](auto shape) {
         using Shape = decltype(shape);
@@ -657,15 +768,12 @@ extern "C" int fgqa_kv_weights(const fgqa_kv_weights_args* a, void* stream) {
     const bool whole = a->cache.kv_dtype == FGQA_KV_FP8_E4M3 && !blocks;
     p.scale = a->scale * (whole ? a->cache.k_scale : 1.f);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)ceil_div(p.items, kWaves));
-    if (a->cache.kv_dtype == FGQA_KV_BF16)
-        hipLaunchKernelGGL((weights_kernel<kCodeBf16, kNone>), grid, dim3(kThreads), 0, s, p);
-    else if (a->cache.kv_dtype == FGQA_KV_INT8)
-        hipLaunchKernelGGL((weights_kernel<kCodeInt8, kBlocks>), grid, dim3(kThreads), 0, s, p);
-    else if (blocks)
-        hipLaunchKernelGGL((weights_kernel<kCodeFp8, kBlocks>), grid, dim3(kThreads), 0, s, p);
-    else
-        hipLaunchKernelGGL((weights_kernel<kCodeFp8, kWhole>), grid, dim3(kThreads), 0, s, p);
+    // Page segments of at least 8 rows, where a page's bytes stay below 2^31.
+    const int page = (int64_t)a->cache.page_size * p.c.slot[0] < ((int64_t)1 << 31) ? a->cache.page_size : 1;
+    if (a->cache.kv_dtype == FGQA_KV_BF16) launch_weights<kCodeBf16, kNone>(p, page, s);
+    else if (a->cache.kv_dtype == FGQA_KV_INT8) launch_weights<kCodeInt8, kBlocks>(p, page, s);
+    else if (blocks) launch_weights<kCodeFp8, kBlocks>(p, page, s);
+    else launch_weights<kCodeFp8, kWhole>(p, page, s);
     return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
 }
 
