@@ -245,15 +245,17 @@ struct WeightsParams {
     const int32_t* block_table;
     int64_t bt_stride;
     const int32_t* seqlens;
-    int max_seqlen, group, chunk, chunks;
+    int max_seqlen, group, chunks;
     float scale;
     int64_t items;   // batch * chunks * hkv
 };
 
-// One wave per item of `chunk` tokens of one KV head, 32 at a time; the waves of
-// a workgroup take adjacent heads, so that a token's rows, which lie side by
-// side, are read together.  Rows are loaded whole (8 lanes of 16 bytes for codes,
-// 16 for bf16), two steps ahead, and staged in LDS as they are.
+// One wave per 64 tokens of one KV head, two steps of 32; the waves of a workgroup
+// take adjacent heads, so that a token's rows, which lie side by side, are read
+// together.  (64 tokens an item are never slower than more, and small calls fill
+// the chip; items of 32: 108 us for 92, 64 sequences of up to 16384.)  Rows are
+// loaded whole (8 lanes of 16 bytes for codes, 16 for bf16), both steps at once,
+// and staged in LDS as they are.
 // S[h][t] = Q[h][:] . K[t][:] by v_mfma_f32_16x16x32_bf16 with the 16 query heads
 // (zero past the group) as rows: a lane holds one token's scores of 4 heads, and
 // the sum over heads takes two exchanges of lane groups.  The order of the head
@@ -272,14 +274,14 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
     const int l16 = lane & 15, g4 = lane >> 4;
-    const int64_t item = (int64_t)blockIdx.x * kWaves + wave;
-    if (item >= p.items) return;
-    const int kvh = (int)(item % p.c.hkv);
-    const int64_t rest = item / p.c.hkv;
-    const int b = (int)(rest / p.chunks);
-    const int t_begin = (int)(rest % p.chunks) * p.chunk;
+    const uint32_t item = blockIdx.x * (uint32_t)kWaves + (uint32_t)wave;
+    if (item >= (uint32_t)p.items) return;
+    const int kvh = (int)(item % (uint32_t)p.c.hkv);
+    const uint32_t rest = item / (uint32_t)p.c.hkv;
+    const int b = (int)(rest / (uint32_t)p.chunks);
+    const int t_begin = (int)(rest % (uint32_t)p.chunks) * plan::kWeightsTokens;
     const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
-    const int t_end = __builtin_amdgcn_readfirstlane(min(t_begin + p.chunk, len));
+    const int t_end = __builtin_amdgcn_readfirstlane(min(t_begin + plan::kWeightsTokens, len));
     if (t_begin >= t_end) return;
 
     const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
@@ -291,7 +293,7 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
     const int row = lane / kLanes, piece = lane % kLanes;
     const int n_steps = (t_end - t_begin + kStep - 1) / kStep;
 
-    // Segment l of the item (at most 64) has its page and scale in lane l.
+    // Segment l of the item (at most 8) has its page and scale in lane l.
     constexpr int kSegs = kSeg > 0 ? kStep / kSeg : 1;
     constexpr int kPer = kLoads / kSegs;
     [[maybe_unused]] int seg_page = 0;
@@ -363,7 +365,7 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
         }
         x.w = wrow[min(t0 + (lane & 31), t_end - 1)];
     };
-    auto compute = [&](int s, Step& x, auto&& reload) {
+    auto compute = [&](int s, const Step& x) {
         const int t0 = t_begin + s * kStep;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i)
@@ -384,7 +386,6 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
             scale[0] = x.scale[0];
             scale[1] = x.scale[1];
         }
-        reload();
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -416,16 +417,12 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
-    Step a, c;
-    auto load_if = [&](int s, Step& x) {
-        if (s < n_steps) load(s, x);
-    };
-    load_if(0, a);
-    load_if(1, c);
-    for (int s = 0; s < n_steps; s += 2) {
-        compute(s, a, [&] { load_if(s + 2, a); });
-        if (s + 1 < n_steps) compute(s + 1, c, [&] { load_if(s + 3, c); });
-    }
+    static_assert(plan::kWeightsTokens == 2 * kStep, "two steps an item");
+    Step first, second;
+    load(0, first);
+    if (n_steps > 1) load(1, second);
+    compute(0, first);
+    if (n_steps > 1) compute(1, second);
 }
 
 // ---------------------------------------------------------------- evict
@@ -761,8 +758,7 @@ extern "C" int fgqa_kv_weights(const fgqa_kv_weights_args* a, void* stream) {
     p.seqlens = a->seqlens;
     p.max_seqlen = a->max_seqlen;
     p.group = a->num_q_heads / p.c.hkv;
-    p.chunk = plan::weights_chunk(a->batch, p.c.hkv, a->max_seqlen);
-    p.chunks = (int)ceil_div(a->max_seqlen, p.chunk);
+    p.chunks = (int)ceil_div(a->max_seqlen, plan::kWeightsTokens);
     p.items = (int64_t)a->batch * p.chunks * p.c.hkv;
     const bool blocks = a->cache.k_scales != nullptr;
     const bool whole = a->cache.kv_dtype == FGQA_KV_FP8_E4M3 && !blocks;

@@ -95,13 +95,6 @@ int validate_kv_append(const fgqa_kv_append_args* a) {
     return validate_cache_pointers(a->cache, true);
 }
 
-int weights_chunk(int64_t batch, int64_t num_kv_heads, int64_t max_seqlen) {
-    const i128 per_item = (i128)batch * num_kv_heads * max_seqlen / kWeightsItems;
-    int chunk = 512;
-    while (chunk > 64 && chunk > per_item) chunk /= 2;
-    return chunk;
-}
-
 int validate_kv_weights(const fgqa_kv_weights_args* a) {
     if (a == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
     const int st = validate_cache(a->cache, false, false);
@@ -121,7 +114,7 @@ int validate_kv_weights(const fgqa_kv_weights_args* a) {
     const int64_t bn[1] = {a->batch};
     if (!extent_ok(qn, a->q_stride) || !extent_ok(wn, ws) || !extent_ok(bn, &a->block_table_stride))
         return FGQA_ERR_UNSUPPORTED;
-    if (!grid_ok((i128)a->batch * a->cache.num_kv_heads * (a->max_seqlen / 64 + 1))) return FGQA_ERR_UNSUPPORTED;
+    if (!grid_ok((i128)a->batch * a->cache.num_kv_heads * ceil_div(a->max_seqlen, kWeightsTokens))) return FGQA_ERR_UNSUPPORTED;
     if (a->batch == 0 || a->max_seqlen == 0) return FGQA_OK;
     if (a->q == nullptr || a->lse == nullptr || a->weights == nullptr || a->block_table == nullptr ||
         a->seqlens == nullptr)

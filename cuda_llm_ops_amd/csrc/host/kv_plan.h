@@ -33,10 +33,7 @@ inline int log2_of(int power_of_two) {
 // Most pages of one sequence that `max_new` tokens in a row touch.
 inline int64_t append_pages(int64_t max_new, int64_t page_size) { return (max_new + page_size - 2) / page_size + 1; }
 
-// Tokens of a wave's item in the weights kernel (a multiple of 32): as many as
-// leave the chip kWeightsItems items, from 512 down to 64.
-constexpr int kWeightsItems = 8192;
-int weights_chunk(int64_t batch, int64_t num_kv_heads, int64_t max_seqlen);
+constexpr int kWeightsTokens = 64;   // of a wave's item in the weights kernel
 
 }  // namespace plan
 }  // namespace fgqa

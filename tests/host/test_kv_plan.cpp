@@ -275,11 +275,7 @@ static void test_weights() {
     WEIGHTS(a.batch = 0; a.q = nullptr, OK);
     WEIGHTS(a.max_seqlen = 0; a.weights = nullptr, OK);
     WEIGHTS(a.max_seqlen = INT_MAX; a.block_table_stride = INT_MAX, NOT);
-    for (int64_t tokens = 1; tokens < (1 << 30); tokens = tokens * 3 + 1) {
-        const int c = plan::weights_chunk(1, 8, tokens);
-        CHECK(c >= 64 && c <= 512 && c % 32 == 0);
-    }
-    CHECK(plan::weights_chunk(INT_MAX, INT_MAX, INT_MAX) == 512);
+    WEIGHTS(a.batch = 1 << 20; a.max_seqlen = 64 << 8; a.block_table_stride = 1 << 20, NOT);   // 2^31 items
 }
 
 static void test_evict() {
@@ -409,8 +405,8 @@ static void fuzz() {
         CHECK(plan::validate_kv_evict(&e) <= 0);
         CHECK(fgqa_decode_blocks(&d, nullptr) <= 0);
         if (plan::validate_kv_weights(&w) == OK && w.batch > 0 && w.max_seqlen > 0) {
-            const int chunk = plan::weights_chunk(w.batch, w.cache.num_kv_heads, w.max_seqlen);
-            CHECK((__int128)w.batch * w.cache.num_kv_heads * ceil_div(w.max_seqlen, chunk) < ((int64_t)1 << 31));
+            CHECK((__int128)w.batch * w.cache.num_kv_heads * ceil_div(w.max_seqlen, plan::kWeightsTokens) <
+                  ((int64_t)1 << 31));
         }
     }
 }
