@@ -458,6 +458,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // bits: the histogram of the keys that share the digits found so far says which
 // digit the last kept key has.  Then every wave walks its part of the row in
 // order and writes what is kept.  Integer sums only: no order matters.
+// kPer: weights of the row that a thread holds in registers, read once, all loads
+// in flight together; 0 for longer rows, which every pass reads again.
+template <int kPer>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     __shared__ int s_hist[kBins];
     __shared__ int s_wave[3][kSelectWaves];
@@ -475,6 +478,29 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     int32_t* kept = p.kept + ((int64_t)b * p.c.hkv + h) * p.budget;
     if (h == 0 && tid == 0) p.new_seqlens[b] = count;
 
+    // each wave's run of the row, in order; f(index, weight) for 64 of it at a
+    // time, with indices at or past `hi` where the run ends
+    const int run = (len + kSelectThreads - 1) / kSelectThreads * kWave;
+    const int lo = min(wave * run, len), hi = min(lo + run, len);
+    constexpr int kBatch = kPer > 0 ? kPer : 8;
+    float held[kBatch];
+    auto read = [&](int i0) {
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s) {
+            const int i = i0 + s * kWave + lane;
+            held[s] = i < hi ? w[i] : 0.f;
+        }
+    };
+    auto each = [&](auto&& f) {
+        for (int i0 = lo; i0 < hi; i0 += kBatch * kWave) {
+            if (kPer == 0) read(i0);
+#pragma unroll
+            for (int s = 0; s < kBatch; ++s)
+                if (i0 + s * kWave < hi) f(i0 + s * kWave + lane, held[s]);
+        }
+    };
+    if (kPer > 0) read(lo);
+
     // keys above `key` are kept, and the first `equal` of those equal to it
     uint32_t key = 0xffffffffu;
     int equal = 0;
@@ -487,14 +513,14 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
             const int bins = pass == 2 ? 1024 : 2048;
             for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
             __syncthreads();
-            for (int i = tid; i < cand; i += kSelectThreads) {
-                const uint32_t k = weight_key(w[i]);
-                if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1);
-            }
+            each([&](int i, float v) {
+                const uint32_t k = weight_key(v);
+                if (i < cand && i < hi && (k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1);
+            });
             __syncthreads();
             // thread t: bins kBins - 1 - 2t and the one below, from the top down
-            const int hi = s_hist[kBins - 1 - 2 * tid], lo = s_hist[kBins - 2 - 2 * tid];
-            int incl = hi + lo;
+            const int top = s_hist[kBins - 1 - 2 * tid], next = s_hist[kBins - 2 - 2 * tid];
+            int incl = top + next;
 #pragma unroll
             for (int d = 1; d < kWave; d *= 2) {
                 const int o = __shfl_up(incl, d, kWave);
@@ -502,14 +528,14 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
             }
             if (lane == kWave - 1) s_wave[0][wave] = incl;
             __syncthreads();
-            int before = incl - hi - lo;
+            int before = incl - top - next;
             for (int v = 0; v < wave; ++v) before += s_wave[0][v];
-            if (before < left && before + hi >= left) {
+            if (before < left && before + top >= left) {
                 s_found[0] = kBins - 1 - 2 * tid;
                 s_found[1] = left - before;
-            } else if (before + hi < left && before + hi + lo >= left) {
+            } else if (before + top < left && before + top + next >= left) {
                 s_found[0] = kBins - 2 - 2 * tid;
-                s_found[1] = left - before - hi;
+                s_found[1] = left - before - top;
             }
             __syncthreads();
             prefix |= (uint32_t)s_found[0] << shift;
@@ -521,24 +547,13 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
         equal = left;
     }
 
-    // each wave's run of the row
-    const int run = (len + kSelectThreads - 1) / kSelectThreads * kWave;
-    const int lo = min(wave * run, len), hi = min(lo + run, len);
-    auto classify = [&](int i, float* v, bool* above, bool* same) {
-        *v = i < hi ? w[i] : 0.f;
-        const uint32_t k = weight_key(*v);
-        const bool chosen = i < cand && need > 0;
-        *above = i < hi && (i >= cand || (chosen && k > key));
-        *same = i < hi && chosen && k == key;
-    };
+    auto above = [&](int i, float v) { return i < hi && (i >= cand || (need > 0 && weight_key(v) > key)); };
+    auto same = [&](int i, float v) { return i < hi && i < cand && need > 0 && weight_key(v) == key; };
     int n_above = 0, n_same = 0;
-    for (int i0 = lo; i0 < hi; i0 += kWave) {
-        float v;
-        bool above, same;
-        classify(i0 + lane, &v, &above, &same);
-        n_above += __popcll(__ballot(above));
-        n_same += __popcll(__ballot(same));
-    }
+    each([&](int i, float v) {
+        n_above += __popcll(__ballot(above(i, v)));
+        n_same += __popcll(__ballot(same(i, v)));
+    });
     if (lane == 0) {
         s_wave[1][wave] = n_above;
         s_wave[2][wave] = n_same;
@@ -551,21 +566,19 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     }
     at += min(seen, equal);
     const uint64_t below = ((uint64_t)1 << lane) - 1;
-    for (int i0 = lo; i0 < hi; i0 += kWave) {
-        float v;
-        bool above, same;
-        classify(i0 + lane, &v, &above, &same);
-        const uint64_t m_same = __ballot(same);
-        const bool keep = above || (same && seen + __popcll(m_same & below) < equal);
+    each([&](int i, float v) {
+        const bool eq = same(i, v);
+        const uint64_t m_same = __ballot(eq);
+        const bool keep = above(i, v) || (eq && seen + __popcll(m_same & below) < equal);
         const uint64_t m_keep = __ballot(keep);
         if (keep) {
             const int to = at + __popcll(m_keep & below);
-            kept[to] = i0 + lane;
+            kept[to] = i;
             nw[to] = v;
         }
         at += __popcll(m_keep);
         seen += __popcll(m_same);
-    }
+    });
     for (int i = count + tid; i < p.budget; i += kSelectThreads) kept[i] = -1;
     for (int i = count + tid; i < p.weights_len; i += kSelectThreads) nw[i] = 0.f;
 }
@@ -599,24 +612,27 @@ __global__ __launch_bounds__(kThreads) void move_kernel(EvictParams p) {
     unsigned char* dst = p.c.data[kv] + page * p.c.page[kv] + h * p.c.head[kv] + chunk * 16 * kPieces;
     const int pmask = (1 << p.c.page_shift) - 1;
 
+    // A wave's rows of a round: lane l looks up row l (its place and scale), and
+    // the lanes of a row get them from there, so that all rows load together.
+    static_assert(Shape::sweeps * kRowsPerSweep <= kWave, "a lane for each of the wave's rows");
     u32x4_t raw[Shape::sweeps][kPieces];
     float from[Shape::sweeps];
     auto load = [&](int base) {
+        const int slot_l = min(base + (wave % Shape::waves) * Shape::sweeps * kRowsPerSweep + lane, rows - 1);
+        const int t = kept[slot_l];
+        const int64_t old = min(max(bt[t >> p.c.page_shift], 0), p.c.num_pages - 1);
+        const int64_t place = old * p.c.page[kv] + (t & pmask) * p.c.slot[kv];
+        float scale_l = 0.f;
+        if constexpr (kScaling == kBlocks) scale_l = p.c.scales[kv][old * p.c.scale_page[kv] + h * p.c.scale_head[kv]];
 #pragma unroll
         for (int s = 0; s < Shape::sweeps; ++s) {
-            const int slot = base + first_row + s * kRowsPerSweep;
+            const int from_lane = s * kRowsPerSweep + row;
+            const uint32_t lo = __shfl((int)place, from_lane, kWave), hi = __shfl((int)(place >> 32), from_lane, kWave);
+            const u32x4_t* r =
+                reinterpret_cast<const u32x4_t*>(src + (int64_t)(((uint64_t)hi << 32) | lo));
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) raw[s][i] = u32x4_t{0u, 0u, 0u, 0u};
-            from[s] = 0.f;
-            if (slot < rows) {
-                const int t = kept[slot];
-                const int old = min(max(bt[t >> p.c.page_shift], 0), p.c.num_pages - 1);
-                const u32x4_t* r = reinterpret_cast<const u32x4_t*>(src + old * p.c.page[kv] + (t & pmask) * p.c.slot[kv]);
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i) raw[s][i] = r[i];
-                if constexpr (kScaling == kBlocks)
-                    from[s] = p.c.scales[kv][old * p.c.scale_page[kv] + h * p.c.scale_head[kv]];
-            }
+            for (int i = 0; i < kPieces; ++i) raw[s][i] = __builtin_nontemporal_load(r + i);   // (past the end: the last row)
+            if constexpr (kScaling == kBlocks) from[s] = __shfl(scale_l, from_lane, kWave);
         }
     };
     const int last = (rows - 1) / Shape::rows * Shape::rows;
@@ -800,7 +816,10 @@ extern "C" int fgqa_kv_evict(const fgqa_kv_evict_args* a, void* stream) {
     p.pages = (int)ceil_div(most, a->cache.page_size);
     p.items = (int64_t)a->batch * p.pages * 2 * p.c.hkv;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(select_kernel, dim3((unsigned)a->batch * (unsigned)p.c.hkv), dim3(kSelectThreads), 0, s, p);
+    const dim3 grid((unsigned)a->batch * (unsigned)p.c.hkv), block(kSelectThreads);
+    if (a->max_seqlen <= 8 * kSelectThreads) hipLaunchKernelGGL(select_kernel<8>, grid, block, 0, s, p);
+    else if (a->max_seqlen <= 32 * kSelectThreads) hipLaunchKernelGGL(select_kernel<32>, grid, block, 0, s, p);
+    else hipLaunchKernelGGL(select_kernel<0>, grid, block, 0, s, p);
     if (p.items > 0) {
         const int page = a->cache.page_size;
         if (a->cache.kv_dtype == FGQA_KV_BF16) launch_move<kCodeBf16, kNone>(p, page, s);
