@@ -445,26 +445,57 @@ struct EvictParams {
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / kWave;
 constexpr int kBins = 2048;
+constexpr int kListMax = 256;
 
-// Weights in their order as unsigned numbers; NaN above all, -0 as 0.
+// Weights in their order as unsigned numbers above 0; NaN above all, -0 as 0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
-    if (w != w) return 0xffffffffu;
     const uint32_t b = __float_as_uint(w + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const uint32_t k = b ^ (uint32_t)(((int32_t)b >> 31) | (int32_t)0x80000000);
+    return w != w ? 0xffffffffu : k;
+}
+
+// The weight of a key (of -0 and of a NaN: 0 and a NaN).
+__device__ __forceinline__ float weight_of_key(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? (k == 0xffffffffu ? 0x7fc00000u : k ^ 0x80000000u) : ~k);
+}
+
+// Lanes of m before this one.
+__device__ __forceinline__ uint32_t lanes_below(uint64_t m) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+
+// dst[from, to) = value, 16 bytes at a time where they are aligned.
+template <typename T>
+__device__ __forceinline__ void fill_row(T* dst, int from, int to, T value) {
+    static_assert(sizeof(T) == 4, "");
+    typedef T vec __attribute__((ext_vector_type(4)));
+    const int tid = threadIdx.x;
+    const int head = min(from + (int)((0 - (reinterpret_cast<uintptr_t>(dst + from) >> 2)) & 3), to);
+    const int vecs = (to - head) / 4;
+    if (tid < head - from) dst[from + tid] = value;
+    for (int i = tid; i < vecs; i += kSelectThreads)
+        reinterpret_cast<vec*>(dst + head)[i] = vec{value, value, value, value};
+    if (tid < to - head - 4 * vecs) dst[head + 4 * vecs + tid] = value;
 }
 
 // One workgroup per (sequence, head): the `need` largest keys of the candidates
 // (tokens before the recent ones) by their digits from the top, 11, 11 and 10
 // bits: the histogram of the keys that share the digits found so far says which
-// digit the last kept key has.  Then every wave walks its part of the row in
-// order and writes what is kept.  Integer sums only: no order matters.
-// kPer: weights of the row that a thread holds in registers, read once, all loads
-// in flight together; 0 for longer rows, which every pass reads again.
+// digit the last kept key has.  (After the first digit each wave puts the keys
+// that have it in a list, and takes the others from there where it is long
+// enough.)  Then every wave walks its
+// part of the candidates in order and writes what is kept.  Integer sums only: no
+// order matters.
+// kPer: candidates that a thread holds in registers, read once, all loads in
+// flight together; 0 for longer rows, which every pass reads again.
+// Few rows leave most of the chip idle: splitting a row over workgroups would
+// take a launch for each pass, about what a pass takes.
 template <int kPer>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     __shared__ int s_hist[kBins];
     __shared__ int s_wave[3][kSelectWaves];
     __shared__ int s_found[2];
+    __shared__ uint32_t s_list[kSelectWaves][kListMax];
     const int tid = threadIdx.x, lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int h = (int)(blockIdx.x % (unsigned)p.c.hkv), b = (int)(blockIdx.x / (unsigned)p.c.hkv);
@@ -476,111 +507,145 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     const float* w = p.weights + b * p.w_b + h * p.w_h;
     float* nw = p.new_weights + b * p.nw_b + h * p.nw_h;
     int32_t* kept = p.kept + ((int64_t)b * p.c.hkv + h) * p.budget;
-    if (h == 0 && tid == 0) p.new_seqlens[b] = count;
 
-    // each wave's run of the row, in order; f(index, weight) for 64 of it at a
-    // time, with indices at or past `hi` where the run ends
-    const int run = (len + kSelectThreads - 1) / kSelectThreads * kWave;
-    const int lo = min(wave * run, len), hi = min(lo + run, len);
+    // each wave's run of the candidates, in order; f(index, key) for 64 of them at
+    // a time, the key 0, which no weight has, where the run has ended
+    const int run = (cand + kSelectThreads - 1) / kSelectThreads * kWave;
+    const int lo = min(wave * run, cand), hi = min(lo + run, cand);
     constexpr int kBatch = kPer > 0 ? kPer : 8;
-    float held[kBatch];
+    uint32_t keys[kBatch];
     auto read = [&](int i0) {
+        float v[kBatch];
 #pragma unroll
         for (int s = 0; s < kBatch; ++s) {
             const int i = i0 + s * kWave + lane;
-            held[s] = i < hi ? w[i] : 0.f;
+            v[s] = i < hi ? w[i] : 0.f;
         }
+#pragma unroll
+        for (int s = 0; s < kBatch; ++s) keys[s] = i0 + s * kWave + lane < hi ? weight_key(v[s]) : 0u;
     };
     auto each = [&](auto&& f) {
         for (int i0 = lo; i0 < hi; i0 += kBatch * kWave) {
             if (kPer == 0) read(i0);
 #pragma unroll
-            for (int s = 0; s < kBatch; ++s)
-                if (i0 + s * kWave < hi) f(i0 + s * kWave + lane, held[s]);
+            for (int s = 0; s < kBatch; s += 4) {
+                if (i0 + s * kWave >= hi) break;
+#pragma unroll
+                for (int e = s; e < s + 4; ++e) f(i0 + e * kWave + lane, keys[e]);
+            }
         }
     };
-    if (kPer > 0) read(lo);
+    if (kPer > 0 && need > 0) read(lo);
 
-    // keys above `key` are kept, and the first `equal` of those equal to it
-    uint32_t key = 0xffffffffu;
-    int equal = 0;
-    if (need > 0) {
-        uint32_t prefix = 0, mask = 0;
-        int left = need;
+    // what needs no choice: the recent tokens, and what lies behind the kept ones
+    if (h == 0 && tid == 0) p.new_seqlens[b] = count;
+    for (int i = tid; i < recent; i += kSelectThreads) {
+        kept[need + i] = cand + i;
+        nw[need + i] = w[cand + i];
+    }
+    fill_row(kept, count, p.budget, (int32_t)-1);
+    fill_row(nw, count, p.weights_len, 0.f);
+    if (need <= 0) return;
+
+    // keys above `prefix` are kept, and the first `left` of those equal to it
+    uint32_t prefix = 0;
+    int left = need;
+    int listed = 0;   // of this wave
 #pragma unroll
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-            const int bins = pass == 2 ? 1024 : 2048;
-            for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
-            __syncthreads();
-            each([&](int i, float v) {
-                const uint32_t k = weight_key(v);
-                if (i < cand && i < hi && (k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1);
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const int bins = pass == 2 ? 1024 : 2048;
+        const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
+        for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
+        __syncthreads();
+        auto add = [&](uint32_t k) { atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1); };
+        if (pass == 0) {
+            each([&](int, uint32_t k) {
+                if (k != 0u) add(k);
             });
-            __syncthreads();
-            // thread t: bins kBins - 1 - 2t and the one below, from the top down
-            const int top = s_hist[kBins - 1 - 2 * tid], next = s_hist[kBins - 2 - 2 * tid];
-            int incl = top + next;
-#pragma unroll
-            for (int d = 1; d < kWave; d *= 2) {
-                const int o = __shfl_up(incl, d, kWave);
-                incl += lane >= d ? o : 0;
+        } else {
+            if (pass == 1) {
+                each([&](int, uint32_t k) {
+                    const uint64_t m = __ballot((k >> 21) == prefix >> 21);
+                    if (m == 0) return;
+                    const int at = listed + (int)lanes_below(m);
+                    if (((m >> lane) & 1) && at < kListMax) s_list[wave][at] = k;
+                    listed += __popcll(m);
+                });
             }
-            if (lane == kWave - 1) s_wave[0][wave] = incl;
-            __syncthreads();
-            int before = incl - top - next;
-            for (int v = 0; v < wave; ++v) before += s_wave[0][v];
-            if (before < left && before + top >= left) {
-                s_found[0] = kBins - 1 - 2 * tid;
-                s_found[1] = left - before;
-            } else if (before + top < left && before + top + next >= left) {
-                s_found[0] = kBins - 2 - 2 * tid;
-                s_found[1] = left - before - top;
+            if (listed <= kListMax) {
+                for (int i = lane; i < listed; i += kWave) {
+                    const uint32_t k = s_list[wave][i];
+                    if ((k & mask) == prefix) add(k);
+                }
+            } else {
+                each([&](int, uint32_t k) {
+                    if ((k & mask) == prefix) add(k);
+                });
             }
-            __syncthreads();
-            prefix |= (uint32_t)s_found[0] << shift;
-            mask |= (uint32_t)(bins - 1) << shift;
-            left = s_found[1];
-            __syncthreads();
         }
-        key = prefix;
-        equal = left;
+        __syncthreads();
+        // thread t: bins kBins - 1 - 2t and the one below, from the top down
+        const int top = s_hist[kBins - 1 - 2 * tid], next = s_hist[kBins - 2 - 2 * tid];
+        int incl = top + next;
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) {
+            const int o = __shfl_up(incl, d, kWave);
+            incl += lane >= d ? o : 0;
+        }
+        if (lane == kWave - 1) s_wave[0][wave] = incl;
+        __syncthreads();
+        int before = incl - top - next;
+#pragma unroll
+        for (int v = 0; v < kSelectWaves; ++v) before += v < wave ? s_wave[0][v] : 0;
+        if (before < left && before + top >= left) {
+            s_found[0] = kBins - 1 - 2 * tid;
+            s_found[1] = left - before;
+        } else if (before + top < left && before + top + next >= left) {
+            s_found[0] = kBins - 2 - 2 * tid;
+            s_found[1] = left - before - top;
+        }
+        __syncthreads();
+        prefix |= (uint32_t)s_found[0] << shift;
+        left = s_found[1];
     }
 
-    auto above = [&](int i, float v) { return i < hi && (i >= cand || (need > 0 && weight_key(v) > key)); };
-    auto same = [&](int i, float v) { return i < hi && i < cand && need > 0 && weight_key(v) == key; };
     int n_above = 0, n_same = 0;
-    each([&](int i, float v) {
-        n_above += __popcll(__ballot(above(i, v)));
-        n_same += __popcll(__ballot(same(i, v)));
+    each([&](int, uint32_t k) {
+        n_above += k > prefix ? 1 : 0;
+        n_same += k == prefix ? 1 : 0;
     });
+#pragma unroll
+    for (int m = 1; m < kWave; m *= 2) {
+        n_above += __shfl_xor(n_above, m, kWave);
+        n_same += __shfl_xor(n_same, m, kWave);
+    }
     if (lane == 0) {
         s_wave[1][wave] = n_above;
         s_wave[2][wave] = n_same;
     }
     __syncthreads();
     int at = 0, seen = 0;
-    for (int v = 0; v < wave; ++v) {
-        at += s_wave[1][v];
-        seen += s_wave[2][v];
+#pragma unroll
+    for (int v = 0; v < kSelectWaves; ++v) {
+        at += v < wave ? s_wave[1][v] : 0;
+        seen += v < wave ? s_wave[2][v] : 0;
     }
-    at += min(seen, equal);
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
-    each([&](int i, float v) {
-        const bool eq = same(i, v);
-        const uint64_t m_same = __ballot(eq);
-        const bool keep = above(i, v) || (eq && seen + __popcll(m_same & below) < equal);
-        const uint64_t m_keep = __ballot(keep);
-        if (keep) {
-            const int to = at + __popcll(m_keep & below);
-            kept[to] = i;
-            nw[to] = v;
+    at += min(seen, left);
+    each([&](int i, uint32_t k) {
+        uint64_t keep = __ballot(k > prefix);
+        const uint64_t same = __ballot(k == prefix);
+        if (same != 0) {
+            keep |= __ballot(k == prefix && seen + (int)lanes_below(same) < left);
+            seen += __popcll(same);
         }
-        at += __popcll(m_keep);
-        seen += __popcll(m_same);
+        if ((keep >> lane) & 1) {
+            const int to = at + (int)lanes_below(keep);
+            kept[to] = i;
+            nw[to] = weight_of_key(k);
+        }
+        at += __popcll(keep);
     });
-    for (int i = count + tid; i < p.budget; i += kSelectThreads) kept[i] = -1;
-    for (int i = count + tid; i < p.weights_len; i += kSelectThreads) nw[i] = 0.f;
 }
 
 // Moves the kept tokens: one block of the new pages per item, as append_kernel,
