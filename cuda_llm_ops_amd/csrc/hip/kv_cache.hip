@@ -55,6 +55,8 @@ CacheParams cache_params(const fgqa_kv_cache& c) {
     return p;
 }
 
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int m = 1; m < kWave; m *= 2) v = xor_max(v, m);
@@ -165,8 +167,8 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
             raw[s][0] = raw[s][1] = u32x4_t{0u, 0u, 0u, 0u};
             if (slot >= slot0 && slot < slot1) {
                 const u32x4_t* r = reinterpret_cast<const u32x4_t*>(src + (i0 + slot) * p.x_t[kv]);
-                raw[s][0] = r[0];
-                raw[s][1] = r[1];
+                raw[s][0] = __builtin_nontemporal_load(r);
+                raw[s][1] = __builtin_nontemporal_load(r + 1);
             }
         }
     };
@@ -174,20 +176,41 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
     const int last = (slot1 - 1) / Shape::rows * Shape::rows;
 
     float scale = p.c.scale[kv];
+    [[maybe_unused]] bool all_finite = false;
     if constexpr (kScaling == kBlocks) {
-        float amax = 0.f;
+        // Without a sign bf16 values order as 16-bit numbers, infinities and NaN
+        // above all others; only a block that has such takes the maximum again
+        // without them.
+        u16x2_t most = {0, 0};
         for (int base = begin; base <= last; base += Shape::rows) {
             load(base);
 #pragma unroll
             for (int s = 0; s < Shape::sweeps; ++s)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t w = raw[s][i / 4][i % 4];
-                    amax = fmaxf(amax, fmaxf(finite_abs(__uint_as_float(w << 16)),
-                                             finite_abs(__uint_as_float(w & 0xffff0000u))));
-                }
+                for (int i = 0; i < 8; ++i)
+                    most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, raw[s][i / 4][i % 4] & 0x7fff7fffu));
         }
-        scale = block_scale<kCode>(block_max<Shape>(amax, s_max));
+        const uint32_t top = min((uint32_t)max(most[0], most[1]), 0x7f80u);   // (NaN as inf: a maximum would drop it)
+        float amax = block_max<Shape>(__uint_as_float(top << 16), s_max);
+        all_finite = amax < INFINITY;
+        if (!all_finite) {
+            amax = 0.f;
+            for (int base = last; base >= begin; base -= Shape::rows) {
+                if (base != last) load(base);
+#pragma unroll
+                for (int s = 0; s < Shape::sweeps; ++s)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t w = raw[s][i / 4][i % 4];
+                        amax = fmaxf(amax, fmaxf(finite_abs(__uint_as_float(w << 16)),
+                                                 finite_abs(__uint_as_float(w & 0xffff0000u))));
+                    }
+            }
+            if (begin != last) load(last);
+            if constexpr (Shape::waves > 1) __syncthreads();   // s_max has been read
+            amax = block_max<Shape>(amax, s_max);
+        }
+        scale = block_scale<kCode>(amax);
         float* at = p.c.scales[kv] + page * p.c.scale_page[kv] + h * p.c.scale_head[kv];
         bool fresh = true;
         if (slot0 > 0) {   // older tokens in the block
@@ -225,6 +248,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
                 r[0] = raw[s][0];
                 r[1] = raw[s][1];
             } else {
+                if (kScaling == kBlocks && all_finite && div.pow2) {
+                    __builtin_nontemporal_store(finite_to_codes<kCode>(raw[s], scale, div.inv), r);
+                    continue;
+                }
                 u32x4_t w;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)

@@ -114,6 +114,35 @@ __device__ __forceinline__ uint32_t to_codes(f32x4_t y) {
     }
 }
 
+// 16 finite bf16 values (two 16-byte pieces) / s -> 16 codes, for a power of two s
+// that brings them inside the codes' range, so nothing saturates: x / s is exact
+// and rounds once.  e4m3: the conversion divides by the power of two itself.
+// int8: 1.5 * 2^23 + x / s rounds to a whole number whose low byte is the code.
+template <int kCode>
+__device__ __forceinline__ u32x4_t finite_to_codes(const u32x4_t (&x)[2], float s, float inv) {
+    u32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w0 = x[i / 2][2 * (i % 2)], w1 = x[i / 2][2 * (i % 2) + 1];
+        if constexpr (kCode == kCodeFp8) {
+            typedef short s16x2_t __attribute__((ext_vector_type(2)));
+            s16x2_t c = {0, 0};
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2_t, w0), s, false);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2_t, w1), s, true);
+            r[i] = __builtin_bit_cast(uint32_t, c);
+        } else {
+            const float magic = 12582912.f;
+            const uint32_t a = __float_as_uint(fmaf(__uint_as_float(w0 << 16), inv, magic));
+            const uint32_t b = __float_as_uint(fmaf(__uint_as_float(w0 & 0xffff0000u), inv, magic));
+            const uint32_t c = __float_as_uint(fmaf(__uint_as_float(w1 << 16), inv, magic));
+            const uint32_t d = __float_as_uint(fmaf(__uint_as_float(w1 & 0xffff0000u), inv, magic));
+            r[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u),
+                                         0x05040100u);
+        }
+    }
+    return r;
+}
+
 __device__ __forceinline__ float finite_abs(float x) {
     const float a = fabsf(x);
     return a < INFINITY ? a : 0.f;   // (false for NaN)
