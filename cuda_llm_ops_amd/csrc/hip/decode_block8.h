@@ -32,8 +32,9 @@ namespace fgqa {
 constexpr int kDec8RowStride = 144;   // LDS bytes of a row: 16 rows spread over all 64 banks
 constexpr int kDec8TileBytes = kDecStep * kDec8RowStride;
 constexpr int kDec8WaveBytes = 2 * kDec8TileBytes + kDecStep * 2 * 4;   // K, V, their scales
+constexpr int kDec8MergeStride = kHeadDim + 4;   // floats of a merged row: 16 rows spread over all 64 banks
 constexpr int dec8_smem_bytes(int waves) {
-    const int merge = waves * 16 * kHeadDim * 4 + waves * 16 * 2 * 4;
+    const int merge = waves * 16 * kDec8MergeStride * 4 + waves * 16 * 2 * 4;
     return waves * kDec8WaveBytes > merge ? waves * kDec8WaveBytes : merge;
 }
 constexpr float kDec8PScale = 16384.f;   // P's scale in fp16
@@ -241,23 +242,27 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
                 vs[j] = sl[kDecStep + at];
                 vmax = fmaxf(vmax, fabsf(vs[j]));
             }
-            vmax = xor_max(xor_max(vmax, 16), 32);
+            vmax = groups_max(vmax);
         }
 
         // Online softmax for head l16 over tokens t0 + 16*tb + 4*g4 + i.
         float y[8];
         float tmax = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int tok = t0 + (j >> 2) * 16 + g4 * 4 + (j & 3);
-            y[j] = tok < t_end ? s[j >> 2][j & 3] * ks[j] : -INFINITY;
-            tmax = fmaxf(tmax, y[j]);
+        for (int j = 0; j < 8; ++j) y[j] = s[j >> 2][j & 3] * ks[j];
+        if (t0 + kDecStep > t_end_u) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (t0 + (j >> 2) * 16 + g4 * 4 + (j & 3) >= t_end) y[j] = -INFINITY;
         }
-        tmax = xor_max(xor_max(tmax, 16), 32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tmax = fmaxf(tmax, y[j]);
+        tmax = groups_max(tmax);
         const float m_new = fmaxf(m_run, tmax);   // finite: every step holds a valid token
         const float alpha = fast_exp2(m_run - m_new);
         const float vinv = __builtin_amdgcn_rcpf(vmax);
-        const float oalpha = alpha * (vref * vinv);
+        // (exactly 1 where nothing changed: vref * (1 / vref) need not be)
+        const float oalpha = alpha * (vmax > vref ? vref * vinv : 1.f);
         const float pscale = vinv * kDec8PScale;
         float psum = 0.f;
         f16x8_t pop;
@@ -270,8 +275,11 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         l_run = l_run * alpha + psum;
         m_run = m_new;
         vref = vmax;
+        // (most steps raise neither maximum)
+        if (__any(oalpha != 1.f)) {
 #pragma unroll
-        for (int db = 0; db < 8; ++db) oacc[db] *= oalpha;
+            for (int db = 0; db < 8; ++db) oacc[db] *= oalpha;
+        }
 
         // V^T as the A operand: tokens 4*g4 + {0..3} and 16 + 4*g4 + {0..3}
         // of column 16*db + l16, those whose P this lane holds.  Row j of the
@@ -303,17 +311,16 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         if (st + kNw < n_steps) compute(st + kNw, step_b, [&] { load_if(st + 3 * kNw, step_b, pg[1], pg[0]); });
     }
 
-    l_run = xor_sum(xor_sum(l_run, 16), 32);
+    l_run = groups_sum(l_run);
 
     // Merge the waves in LDS (reusing the staging area).
     __syncthreads();
-    float* ow = reinterpret_cast<float*>(smem);   // [wave][16][128]
-    float* mlw = ow + kNw * 16 * kHeadDim;        // [wave][16][2]
+    float* ow = reinterpret_cast<float*>(smem);       // [wave][16][kDec8MergeStride]
+    float* mlw = ow + kNw * 16 * kDec8MergeStride;    // [wave][16][2]
     const float oscale = vref * (1.f / kDec8PScale);
 #pragma unroll
     for (int db = 0; db < 8; ++db)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ow[(wave * 16 + l16) * kHeadDim + db * 16 + g4 * 4 + i] = oacc[db][i] * oscale;
+        *reinterpret_cast<f32x4_t*>(ow + (wave * 16 + l16) * kDec8MergeStride + db * 16 + g4 * 4) = oacc[db] * oscale;
     if (g4 == 0) {
         mlw[(wave * 16 + l16) * 2 + 0] = m_run;
         mlw[(wave * 16 + l16) * 2 + 1] = l_run;
@@ -335,7 +342,7 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         for (int w = 0; w < kNw; ++w) {
             const float c = (mw[w] == -INFINITY) ? 0.f : fast_exp2(mw[w] - M);
             L += c * mlw[(w * 16 + h) * 2 + 1];
-            const float* src = ow + (w * 16 + h) * kHeadDim + d0;
+            const float* src = ow + (w * 16 + h) * kDec8MergeStride + d0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[j] += c * src[j];
         }

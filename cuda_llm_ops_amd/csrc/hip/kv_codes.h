@@ -143,6 +143,17 @@ __device__ __forceinline__ u32x4_t finite_to_codes(const u32x4_t (&x)[2], float 
     return r;
 }
 
+// Over the wave's four groups of 16 lanes, in every lane: v_permlane16_swap and
+// v_permlane32_swap, without the LDS round trips of a shuffle.
+__device__ __forceinline__ float groups_max(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 __device__ __forceinline__ float finite_abs(float x) {
     const float a = fabsf(x);
     return a < INFINITY ? a : 0.f;   // (false for NaN)
