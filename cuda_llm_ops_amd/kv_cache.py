@@ -61,8 +61,6 @@ def launch(fn, packed, device, where):
 # read each property of a tensor once and name what is wrong only afterwards.)
 def _rows_apart(t) -> bool:
     """No two elements of t share memory (an expanded tensor's do)."""
-    if t.is_contiguous():
-        return True
     end = 1   # elements that the dims so far span
     for st, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if st < end:
@@ -73,7 +71,7 @@ def _rows_apart(t) -> bool:
 
 def _check_written(*ts):
     for t in ts:
-        if not _rows_apart(t):
+        if not (t.is_contiguous() or _rows_apart(t)):
             raise ValueError("a tensor that is written must not overlap itself (expanded dims)")
 
 
@@ -239,10 +237,12 @@ def append_kv_paged(k, v, k_cache, v_cache, block_table, seqlens, new_lens=None,
     dev = check_device(k, v, block_table, seqlens, *written)
     if new_lens is not None:
         check_device(k, new_lens)
-    k, v = _prep(k), _prep(v)
-    ks, vs = k.stride(), v.stride()
+    kp, vp, ks, vs = k.data_ptr(), v.data_ptr(), k.stride(), v.stride()
+    if kp & 15 or vp & 15 or ks[3] != 1 or vs[3] != 1 or (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 7:
+        k, v = _prep(k), _prep(v)
+        kp, vp, ks, vs = k.data_ptr(), v.data_ptr(), k.stride(), v.stride()
     packed = _lib.pack_kv_append.bytes(
-        *cache, k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], block_table.data_ptr(),
+        *cache, kp, vp, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], block_table.data_ptr(),
         table_stride, seqlens.data_ptr(), new, B, N, pages)
     launch(_lib.lib().fgqa_kv_append, packed, dev, "fgqa_kv_append")
     return k_cache, v_cache
