@@ -258,8 +258,10 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
 #pragma unroll
         for (int j = 0; j < 8; ++j) tmax = fmaxf(tmax, y[j]);
         tmax = groups_max(tmax);
-        const float m_new = fmaxf(m_run, tmax);   // finite: every step holds a valid token
-        const float alpha = fast_exp2(m_run - m_new);
+        const float m_new = fmaxf(m_run, tmax);
+        // (-inf, no score above it yet: what is subtracted has to be a number)
+        const float m_sub = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = fast_exp2(m_run - m_sub);
         const float vinv = __builtin_amdgcn_rcpf(vmax);
         // (exactly 1 where nothing changed: vref * (1 / vref) need not be)
         const float oalpha = alpha * (vmax > vref ? vref * vinv : 1.f);
@@ -268,7 +270,7 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         f16x8_t pop;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float pv = fast_exp2(y[j] - m_new);
+            const float pv = fast_exp2(y[j] - m_sub);
             psum += pv;
             pop[j] = (_Float16)(pv * (vs[j] * pscale));
         }

@@ -120,7 +120,7 @@ struct AppendParams {
     const int32_t* new_lens;
     int max_new, max_tokens;
     int pages;                       // of one sequence that new tokens can touch
-    int64_t items;                   // batch * pages * 2 * hkv
+    uint32_t items;                  // batch * pages * 2 * hkv, below 2^31
 };
 
 // One block per item: item = ((b * pages + j) * 2 + K or V) * hkv + head, heads
@@ -130,13 +130,13 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
     __shared__ float s_max[kWaves];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
-    const int64_t item = (int64_t)blockIdx.x * (kWaves / Shape::waves) + wave / Shape::waves;
+    const uint32_t item = blockIdx.x * (uint32_t)(kWaves / Shape::waves) + (uint32_t)(wave / Shape::waves);
     if (item >= p.items) return;
-    const int h = (int)(item % p.c.hkv);
-    const int64_t rest = item / p.c.hkv;
+    const int h = (int)(item % (uint32_t)p.c.hkv);
+    const uint32_t rest = item / (uint32_t)p.c.hkv;
     const int kv = (int)(rest & 1);
-    const int j = (int)((rest >> 1) % p.pages);
-    const int b = (int)((rest >> 1) / p.pages);
+    const int j = (int)((rest >> 1) % (uint32_t)p.pages);
+    const int b = (int)((rest >> 1) / (uint32_t)p.pages);
 
     const int len = max(p.seqlens[b], 0);
     const int want = p.new_lens != nullptr ? min(max(p.new_lens[b], 0), p.max_new) : p.max_new;
@@ -274,7 +274,7 @@ struct WeightsParams {
     const int32_t* seqlens;
     int max_seqlen, group, chunks;
     float scale;
-    int64_t items;   // batch * chunks * hkv
+    uint32_t items;   // batch * chunks * hkv, below 2^31
 };
 
 // One wave per 64 tokens of one KV head, two steps of 32; the waves of a workgroup
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
     const int l16 = lane & 15, g4 = lane >> 4;
     const uint32_t item = blockIdx.x * (uint32_t)kWaves + (uint32_t)wave;
-    if (item >= (uint32_t)p.items) return;
+    if (item >= p.items) return;
     const int kvh = (int)(item % (uint32_t)p.c.hkv);
     const uint32_t rest = item / (uint32_t)p.c.hkv;
     const int b = (int)(rest / (uint32_t)p.chunks);
@@ -466,7 +466,7 @@ struct EvictParams {
     int32_t* kept;
     int max_seqlen, weights_len, budget, recent;
     int pages;       // new pages of a sequence at most
-    int64_t items;   // batch * pages * 2 * hkv
+    uint32_t items;  // batch * pages * 2 * hkv, below 2^31
 };
 
 constexpr int kSelectThreads = 1024;
@@ -682,13 +682,13 @@ __global__ __launch_bounds__(kThreads) void move_kernel(EvictParams p) {
     __shared__ float s_max[kWaves];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
-    const int64_t item = (int64_t)blockIdx.x * (kWaves / Shape::waves) + wave / Shape::waves;
+    const uint32_t item = blockIdx.x * (uint32_t)(kWaves / Shape::waves) + (uint32_t)(wave / Shape::waves);
     if (item >= p.items) return;
-    const int h = (int)(item % p.c.hkv);
-    const int64_t rest = item / p.c.hkv;
+    const int h = (int)(item % (uint32_t)p.c.hkv);
+    const uint32_t rest = item / (uint32_t)p.c.hkv;
     const int kv = (int)(rest & 1);
-    const int j = (int)((rest >> 1) % p.pages);
-    const int b = (int)((rest >> 1) / p.pages);
+    const int j = (int)((rest >> 1) % (uint32_t)p.pages);
+    const int b = (int)((rest >> 1) / (uint32_t)p.pages);
     const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
     const int rows = min(min(len, p.budget) - (j << p.c.page_shift), 1 << p.c.page_shift);
     if (rows <= 0) return;
@@ -837,7 +837,7 @@ extern "C" int fgqa_kv_append(const fgqa_kv_append_args* a, void* stream) {
     p.max_new = a->max_new;
     p.max_tokens = a->max_pages * a->cache.page_size;
     p.pages = (int)plan::append_pages(a->max_new, a->cache.page_size);
-    p.items = (int64_t)a->batch * p.pages * 2 * p.c.hkv;
+    p.items = (uint32_t)((int64_t)a->batch * p.pages * 2 * p.c.hkv);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const int page = a->cache.page_size;
     const bool blocks = a->cache.k_scales != nullptr;
@@ -867,7 +867,7 @@ extern "C" int fgqa_kv_weights(const fgqa_kv_weights_args* a, void* stream) {
     p.max_seqlen = a->max_seqlen;
     p.group = a->num_q_heads / p.c.hkv;
     p.chunks = (int)ceil_div(a->max_seqlen, plan::kWeightsTokens);
-    p.items = (int64_t)a->batch * p.chunks * p.c.hkv;
+    p.items = (uint32_t)((int64_t)a->batch * p.chunks * p.c.hkv);
     const bool blocks = a->cache.k_scales != nullptr;
     const bool whole = a->cache.kv_dtype == FGQA_KV_FP8_E4M3 && !blocks;
     p.scale = a->scale * (whole ? a->cache.k_scale : 1.f);
@@ -906,7 +906,7 @@ extern "C" int fgqa_kv_evict(const fgqa_kv_evict_args* a, void* stream) {
     p.recent = a->recent;
     const int most = a->budget < a->max_seqlen ? a->budget : a->max_seqlen;
     p.pages = (int)ceil_div(most, a->cache.page_size);
-    p.items = (int64_t)a->batch * p.pages * 2 * p.c.hkv;
+    p.items = (uint32_t)((int64_t)a->batch * p.pages * 2 * p.c.hkv);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid((unsigned)a->batch * (unsigned)p.c.hkv), block(kSelectThreads);
     if (a->max_seqlen <= 8 * kSelectThreads) hipLaunchKernelGGL(select_kernel<8>, grid, block, 0, s, p);

@@ -348,6 +348,57 @@ def test_decode_same_bits_as_the_whole_cache_scale(cuda):
     assert (whole.float() - blocks.float()).abs().max() <= v * (2.0 ** -8 + 2.0 ** -11) + 2 * 2.0 ** -8 * blocks.float().abs().max()
 
 
+@pytest.mark.parametrize("P", [4, 16, 64])
+def test_decode_scores_of_minus_infinity(cuda, P):
+    """Keys whose scores overflow to -inf get nothing, wherever they lie; a row of
+    such keys alone is NaN, as the formula has it."""
+    torch = _torch()
+    rng = np.random.default_rng(82)
+    width = -(-300 // P)
+    c = Cache(cuda, rng, "int8", 2 * width, P, 1)
+    table, lens = _table(rng, 2, width, 2 * width), [300, 40]
+    alive = np.zeros(300, bool)
+    alive[140:150] = alive[299] = True
+    # 3e38 * -1 * 64 / sqrt(128) is past fp32's range; the alive keys' products are 0
+    raw = c.t[0].view(torch.uint8)
+    raw[:, :, 0, 7] = 0xff
+    for t in np.flatnonzero(alive):
+        raw[int(table[0, t // P]), t % P, 0, 7] = 0
+    c.s[0].fill_(64.0)
+    q = _x(rng, 2, 2, 128)
+    q[:, 0, :] = 0.0
+    q[:, 0, 7] = 3e38
+    lse = torch.empty((2, 2), device=cuda)
+    o = _fg().decode_flash_gqa_paged(q.to(cuda), c.t[0], c.t[1], _i32(cuda, table), _i32(cuda, lens), lse=lse, **c.scales)
+    torch.cuda.synchronize()
+    v = ref.gather(c.n[1], c.sn[1], table, 0, 300, 0)[alive].mean(axis=0)
+    size = np.abs(ref.gather(c.n[1], c.sn[1], table, 0, 300, 0)[alive]).mean(axis=0)
+    got = o[0, 0].float().cpu().double().numpy()
+    # equal P's of 1 round to nothing; sums of 11 terms and two products in fp32, O to bf16
+    assert np.all(np.abs(got - v) <= 2.0 ** -8 * np.abs(v) + 2.0 ** -20 * size)
+    assert abs(float(lse[0, 0]) - math.log(11)) <= 2.0 ** -21
+    assert bool(o[1, 0].isnan().all())           # no key of row 1 is alive
+
+
+def test_decode_least_workspace(cuda):
+    """A caller's workspace that holds 4096-token splits only, one that holds the
+    even sharing, and one too small."""
+    torch = _torch()
+    fg = _fg()
+    rng = np.random.default_rng(83)
+    c = Cache(cuda, rng, "e4m3", 300, 64, 4)
+    table, lens = _table(rng, 2, 150, 300), [9500, 4097]
+    q = _x(rng, 2, 16, 128)
+    n = -(-9600 // 4096)
+    least = -(-2 * 16 * n * 512 // 256) * 256 + -(-2 * 16 * n * 8 // 256) * 256 + 4 * (1 + 2 * n)
+    for size in (least, 64 << 20):
+        ws = torch.empty(size, dtype=torch.uint8, device=cuda)
+        _decode(cuda, c, q, table, lens, f"workspace {size}", workspace=ws)
+    with pytest.raises(fg.FgqaError):
+        fg.decode_flash_gqa_paged(q.to(cuda), c.t[0], c.t[1], _i32(cuda, table), _i32(cuda, lens), workspace=ws[:least - 4],
+                                  **c.scales)
+
+
 @pytest.mark.parametrize("what", ["append", "decode", "weights", "evict"])
 def test_offsets_past_32_bits(cuda, what):
     """Pages that begin past 4 GiB of a cache."""
@@ -679,3 +730,73 @@ def test_two_streams_at_once(cuda):
         for a, b in zip(alone, got):
             for x, y in zip(a, b):
                 assert torch.equal(x, y)
+
+
+# ------------------------------------------------------------------ C++ operator layer
+def test_cplusplus_entry_points(cuda):
+    """The C++ entry points on the default stream against the Python functions: the same bits."""
+    import ctypes
+    import subprocess
+
+    import cuda_llm_ops_amd._lib as L
+    torch = _torch()
+    fg = _fg()
+
+    class Kv(ctypes.Structure):   # KvCache (kv_cache_kernel.h)
+        _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ks", ctypes.c_void_p), ("vs", ctypes.c_void_p),
+                    ("type", ctypes.c_int), ("pages", ctypes.c_int), ("page", ctypes.c_int), ("heads", ctypes.c_int),
+                    ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
+
+    syms = subprocess.run(["nm", "-D", "--defined-only", L.LIB_PATH], check=True, capture_output=True, text=True).stdout
+    lib = L.lib()
+
+    def entry(name):
+        return getattr(lib, next(w.split()[-1] for w in syms.splitlines() if f"{len(name)}{name}R" in w))
+
+    status = getattr(lib, next(w.split()[-1] for w in syms.splitlines() if "FlashGqaGetLastStatus" in w))
+    rng = np.random.default_rng(400)
+    B, H, Hq, P, pages = 2, 2, 8, 16, 30
+    c = Cache(cuda, rng, "int8", pages, P, H)
+    table = _i32(cuda, _table(rng, B, 10, 20))
+    new_table = _i32(cuda, 20 + np.arange(10).reshape(2, 5))
+    lens, news = _i32(cuda, [100, 37]), _i32(cuda, [5, 3])
+    x = _x(rng, B, 5, H, 128).to(cuda)
+    q = _x(rng, B, Hq, 128).to(cuda)
+    P_ = lambda t: ctypes.c_void_p(0 if t is None else t.data_ptr())  # noqa: E731
+    f32, i32 = ctypes.c_float, ctypes.c_int
+    results = []
+    for cpp in (False, True):
+        k, v, ks, vs = c.t[0].clone(), c.t[1].clone(), c.s[0].clone(), c.s[1].clone()
+        o = torch.empty((B, Hq, 128), dtype=torch.bfloat16, device=cuda)
+        lse, w = torch.empty((B, Hq), device=cuda), torch.zeros((B, H, 10 * P), device=cuda)
+        nw, kept, nl = torch.empty_like(w), torch.empty((B, H, 70), dtype=torch.int32, device=cuda), torch.empty_like(lens)
+        torch.cuda.synchronize()
+        after = lens + news
+        if cpp:
+            torch.cuda.synchronize()
+            kv = Kv(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), 2, pages, P, H, 1.0, 1.0)
+            ref_kv = ctypes.byref(kv)
+            entry("LaunchKvCacheAppendKernel")(ref_kv, P_(x), P_(x), P_(table), P_(lens), P_(news), i32(B), i32(5), i32(10))
+            assert status() == 0
+            entry("LaunchFlashGqaBf16KernelPagedBlocks")(ref_kv, P_(q), f32(SCALE), P_(o), P_(lse), P_(table), P_(after),
+                                                         i32(B), i32(10), i32(Hq))
+            assert status() == 0
+            entry("LaunchKvCacheWeightsKernel")(ref_kv, P_(q), f32(SCALE), P_(lse), P_(w), P_(table), P_(after), i32(B),
+                                                i32(10), i32(Hq))
+            assert status() == 0
+            entry("LaunchKvCacheEvictKernel")(ref_kv, P_(w), P_(nw), P_(table), P_(new_table), P_(after), P_(nl), P_(kept),
+                                              i32(70), i32(8), i32(B), i32(10), i32(5))
+            assert status() == 0
+            entry("LaunchKvCacheEvictKernel")(ref_kv, P_(w), P_(nw), P_(table), P_(new_table), P_(after), P_(nl), P_(kept),
+                                              i32(0), i32(8), i32(B), i32(10), i32(5))
+            assert status() == L.FGQA_ERR_INVALID_ARGUMENT
+        else:
+            sc = dict(k_scale=ks, v_scale=vs)
+            fg.append_kv_paged(x, x, k, v, table, lens, new_lens=news, **sc)
+            fg.decode_flash_gqa_paged(q, k, v, table, after, out=o, lse=lse, **sc)
+            fg.accumulate_kv_weights_paged(q, k, lse, table, after, w, k_scale=ks)
+            fg.evict_kv_paged(k, v, table, after, w, new_table, 70, 8, new_seqlens=nl, new_weights=nw, kept=kept, **sc)
+        torch.cuda.synchronize()
+        results.append([t.clone() for t in (k, v, ks, vs, o.view(torch.int16), lse, w, nw, kept, nl)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
