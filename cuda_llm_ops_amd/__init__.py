@@ -4,7 +4,7 @@ The kernels live in libfgqa.so (HIP, gfx950); ``flash_gqa`` is the Python host
 interface over its C ABI (include/fgqa.h), and ``kv_cache`` that of the paged
 cache's operators (include/fgqa_kv.h).
 """
-from ._lib import FgqaError, LIB_PATH, lib, status_string  # noqa: F401
+from ._lib import FgqaError, LIB_PATH, lib, native, status_string  # noqa: F401
 from .flash_gqa import (  # noqa: F401
     backward_workspace_bytes,
     decode_flash_gqa_bshd,

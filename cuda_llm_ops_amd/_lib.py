@@ -1,4 +1,5 @@
-"""ctypes binding of libfgqa.so, the C ABI declared in include/fgqa.h and include/fgqa_kv.h.
+"""ctypes binding of libfgqa.so, the C ABI declared in include/fgqa.h, and the native
+module that binds include/fgqa_kv.h.
 
 The library is built in-tree (``make -C cuda_llm_ops_amd/csrc`` or
 ``__graft_entry__.build()``).  Loading fails loudly when it is missing: there
@@ -7,11 +8,13 @@ is no fallback implementation of any entry point.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libfgqa.so")
+NATIVE_PATH = os.path.join(_HERE, "lib", "_kv_native.so")
 
 FGQA_OK = 0
 FGQA_ERR_INVALID_ARGUMENT = -1
@@ -186,108 +189,6 @@ class SparsePrefillArgs(ctypes.Structure):
     ]
 
 
-FGQA_KV_INT8 = 2
-
-# The fields of ``fgqa_kv_cache`` (include/fgqa_kv.h), with which the argument
-# blocks below begin (its size is a multiple of its alignment, so they lie as in
-# the nested struct).
-_KV_CACHE = [
-    ("k_cache", ctypes.c_void_p),
-    ("v_cache", ctypes.c_void_p),
-    ("k_scales", ctypes.c_void_p),
-    ("v_scales", ctypes.c_void_p),
-    ("kv_dtype", ctypes.c_int32),
-    ("num_kv_heads", ctypes.c_int32),
-    ("head_dim", ctypes.c_int32),
-    ("page_size", ctypes.c_int32),
-    ("num_pages", ctypes.c_int32),
-    ("k_scale", ctypes.c_float),
-    ("v_scale", ctypes.c_float),
-    ("k_stride", _I64x3),
-    ("v_stride", _I64x3),
-    ("k_scales_stride", _I64x2),
-    ("v_scales_stride", _I64x2),
-]
-
-
-class KvAppendArgs(ctypes.Structure):
-    """Mirror of ``fgqa_kv_append_args`` (include/fgqa_kv.h)."""
-    _fields_ = _KV_CACHE + [
-        ("k_new", ctypes.c_void_p),
-        ("v_new", ctypes.c_void_p),
-        ("k_new_stride", _I64x3),
-        ("v_new_stride", _I64x3),
-        ("block_table", ctypes.c_void_p),
-        ("block_table_stride", ctypes.c_int64),
-        ("seqlens", ctypes.c_void_p),
-        ("new_lens", ctypes.c_void_p),
-        ("batch", ctypes.c_int32),
-        ("max_new", ctypes.c_int32),
-        ("max_pages", ctypes.c_int32),
-    ]
-
-
-class DecodeBlocksArgs(ctypes.Structure):
-    """Mirror of ``fgqa_decode_blocks_args`` (include/fgqa_kv.h)."""
-    _fields_ = _KV_CACHE + [
-        ("q", ctypes.c_void_p),
-        ("o", ctypes.c_void_p),
-        ("lse", ctypes.c_void_p),
-        ("block_table", ctypes.c_void_p),
-        ("seqlens", ctypes.c_void_p),
-        ("batch", ctypes.c_int32),
-        ("max_seqlen", ctypes.c_int32),
-        ("num_q_heads", ctypes.c_int32),
-        ("scale", ctypes.c_float),
-        ("q_stride", _I64x2),
-        ("o_stride", _I64x2),
-        ("block_table_stride", ctypes.c_int64),
-        ("split_tokens", ctypes.c_int32),
-        ("workspace", ctypes.c_void_p),
-        ("workspace_bytes", ctypes.c_size_t),
-    ]
-
-
-class KvWeightsArgs(ctypes.Structure):
-    """Mirror of ``fgqa_kv_weights_args`` (include/fgqa_kv.h)."""
-    _fields_ = _KV_CACHE + [
-        ("q", ctypes.c_void_p),
-        ("lse", ctypes.c_void_p),
-        ("weights", ctypes.c_void_p),
-        ("q_stride", _I64x2),
-        ("weights_stride", _I64x2),
-        ("block_table", ctypes.c_void_p),
-        ("block_table_stride", ctypes.c_int64),
-        ("seqlens", ctypes.c_void_p),
-        ("batch", ctypes.c_int32),
-        ("max_seqlen", ctypes.c_int32),
-        ("num_q_heads", ctypes.c_int32),
-        ("scale", ctypes.c_float),
-    ]
-
-
-class KvEvictArgs(ctypes.Structure):
-    """Mirror of ``fgqa_kv_evict_args`` (include/fgqa_kv.h)."""
-    _fields_ = _KV_CACHE + [
-        ("weights", ctypes.c_void_p),
-        ("new_weights", ctypes.c_void_p),
-        ("weights_stride", _I64x2),
-        ("new_weights_stride", _I64x2),
-        ("block_table", ctypes.c_void_p),
-        ("new_block_table", ctypes.c_void_p),
-        ("block_table_stride", ctypes.c_int64),
-        ("new_block_table_stride", ctypes.c_int64),
-        ("seqlens", ctypes.c_void_p),
-        ("new_seqlens", ctypes.c_void_p),
-        ("kept", ctypes.c_void_p),
-        ("batch", ctypes.c_int32),
-        ("max_seqlen", ctypes.c_int32),
-        ("weights_len", ctypes.c_int32),
-        ("budget", ctypes.c_int32),
-        ("recent", ctypes.c_int32),
-    ]
-
-
 _FORMATS = {ctypes.c_void_p: "P", ctypes.c_int32: "i", ctypes.c_float: "f", ctypes.c_int64: "q",
             ctypes.c_size_t: "N", _I64x2: "2q", _I64x3: "3q"}
 
@@ -301,10 +202,6 @@ class ArgsPacker:
         self._cls = cls
         self._struct = struct.Struct("@" + "".join(_FORMATS[t] for _, t in cls._fields_) + "0P")
         assert self._struct.size == ctypes.sizeof(cls)
-        # The block as bytes, for entry points bound with a plain address
-        # argument: no ctypes object is made (0.7 us).  A value that its field
-        # cannot hold raises.
-        self.bytes = self._struct.pack
 
     def __call__(self, *values):
         try:
@@ -325,10 +222,6 @@ pack_prefill = ArgsPacker(PrefillArgs)
 pack_paged = ArgsPacker(PagedDecodeArgs)
 pack_backward = ArgsPacker(BackwardArgs)
 pack_sparse = ArgsPacker(SparsePrefillArgs)
-pack_kv_append = ArgsPacker(KvAppendArgs)
-pack_decode_blocks = ArgsPacker(DecodeBlocksArgs)
-pack_kv_weights = ArgsPacker(KvWeightsArgs)
-pack_kv_evict = ArgsPacker(KvEvictArgs)
 
 
 class FgqaError(RuntimeError):
@@ -375,13 +268,10 @@ def lib() -> ctypes.CDLL:
         L.fgqa_prefill_backward_bf16.argtypes = [ctypes.POINTER(BackwardArgs), ctypes.c_void_p]
         L.fgqa_sparse_prefill_bf16.restype = ctypes.c_int
         L.fgqa_sparse_prefill_bf16.argtypes = [ctypes.POINTER(SparsePrefillArgs), ctypes.c_void_p]
-        # (a plain address: the argument block's bytes, or byref of its ctypes mirror)
-        for name in ("fgqa_kv_append", "fgqa_decode_blocks", "fgqa_kv_weights", "fgqa_kv_evict"):
-            getattr(L, name).restype = ctypes.c_int
-            getattr(L, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
-        L.fgqa_decode_blocks_workspace_bytes.restype = ctypes.c_int
-        L.fgqa_decode_blocks_workspace_bytes.argtypes = [ctypes.POINTER(DecodeBlocksArgs),
-                                                         ctypes.POINTER(ctypes.c_size_t)]
+        # include/fgqa_kv.h: the native module calls these but for a prepared
+        # decode, whose argument block is kept as bytes
+        L.fgqa_decode_blocks.restype = ctypes.c_int
+        L.fgqa_decode_blocks.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         L.fgqa_status_string.restype = ctypes.c_char_p
         L.fgqa_status_string.argtypes = [ctypes.c_int]
         L.fgqa_version.restype = ctypes.c_int
@@ -390,6 +280,29 @@ def lib() -> ctypes.CDLL:
         L.fgqa_clock_sample.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
         _lib = L
     return _lib
+
+
+_native = None
+
+
+def native():
+    """Load the paged KV cache's native module (once).  Raises if it has not been built."""
+    global _native
+    if _native is None:
+        if not os.path.exists(NATIVE_PATH):
+            raise ImportError(
+                f"{NATIVE_PATH} is missing: build it with `make -C cuda_llm_ops_amd/csrc python` "
+                "or __graft_entry__.build(); there is no fallback path")
+        lib()
+        import torch
+        spec = importlib.util.spec_from_file_location("cuda_llm_ops_amd._kv_native", NATIVE_PATH)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        m.bind(getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device,
+               getattr(torch._C, "_cuda_getCurrentRawStream", None)
+               or (lambda device: torch.cuda.current_stream(device).cuda_stream), FgqaError)
+        _native = m
+    return _native
 
 
 def status_string(status: int) -> str:

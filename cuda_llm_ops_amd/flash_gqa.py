@@ -25,7 +25,6 @@ through ``fgqa_decode_bf16`` / ``fgqa_prefill_bf16`` / ``fgqa_prefill_backward_b
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 import operator
 
@@ -278,63 +277,6 @@ def _has_block_scales(k_cache, k_scale, v_scale) -> bool:
     return isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor) or k_cache.dtype == torch.int8
 
 
-@functools.lru_cache(maxsize=256)
-def _blocks_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, split_tokens) -> int:
-    a = _lib.DecodeBlocksArgs()
-    a.kv_dtype, a.num_kv_heads, a.head_dim, a.page_size, a.num_pages = _lib.FGQA_KV_INT8, Hkv, 128, page_size, 1
-    a.batch, a.max_seqlen, a.num_q_heads, a.scale, a.split_tokens = B, max_seqlen, Hq, 1.0, split_tokens
-    a.block_table_stride = -(-max_seqlen // page_size)
-    n = ctypes.c_size_t(0)
-    _lib.check(_lib.lib().fgqa_decode_blocks_workspace_bytes(ctypes.byref(a), ctypes.byref(n)),
-               "fgqa_decode_blocks_workspace_bytes")
-    return int(n.value)
-
-
-def _blocks_args(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse, max_seqlen,
-                 split_tokens, workspace):
-    """The paged decode over a cache with block scales, validated: (argument
-    block's bytes, out, the device's index, what they point at)."""
-    if q.dtype is not torch.bfloat16:
-        raise ValueError("paged decode expects a bf16 query")
-    if q.dim() != 3:
-        raise ValueError("expected q [B,Hq,D] and k_cache/v_cache [num_pages, page_size, Hkv, D]")
-    cache, _ = kv_cache.cache_fields(k_cache, v_cache, k_scale, v_scale)
-    B, Hq, D = q.shape
-    _, page_size, Hkv, _ = k_cache.shape
-    if D != 128:
-        raise ValueError("the caches' head_dim must match Q")
-    if Hq % Hkv != 0:
-        raise ValueError("Query heads must be divisible by KV heads")
-    pages, table_stride = kv_cache.check_table(block_table, B, "block_table")
-    kv_cache.check_lens(seqlens, B, "seqlens")
-    tokens = pages * page_size
-    max_seqlen = tokens if max_seqlen is None else kv_cache.check_max_seqlen(max_seqlen, tokens)
-    split_tokens = int(split_tokens)
-    if not 0 <= split_tokens < 1 << 31:
-        raise ValueError("split_tokens must not be negative (and be below 2^31)")
-    given = [t for t in (out, lse, workspace) if t is not None]
-    if out is not None and (out.shape != (B, Hq, D) or out.dtype != torch.bfloat16 or not _kernel_ready(out)):
-        raise ValueError("out must be a bf16 [B, Hq, D] tensor with contiguous rows")
-    lse_ptr = 0
-    if lse is not None:
-        if lse.dtype is not torch.float32 or lse.shape != (B, Hq) or not lse.is_contiguous():
-            raise ValueError("lse must be a contiguous fp32 [B, Hq] tensor")
-        lse_ptr = lse.data_ptr()
-    dev = kv_cache.check_device(q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens, *given)
-    q = _prep(q)
-    if out is None:
-        out = torch.empty((B, Hq, D), device=q.device, dtype=torch.bfloat16)
-    if workspace is None and B > 0:
-        workspace = torch.empty(_blocks_workspace_bytes(B, max_seqlen, Hq, Hkv, page_size, split_tokens),
-                                device=q.device, dtype=torch.uint8)
-    qst, ost = q.stride(), out.stride()
-    packed = _lib.pack_decode_blocks.bytes(
-        *cache, q.data_ptr(), out.data_ptr(), lse_ptr, block_table.data_ptr(), seqlens.data_ptr(), B, max_seqlen, Hq,
-        1.0 / math.sqrt(D) if scale is None else float(scale), qst[0], qst[1], ost[0], ost[1], table_stride,
-        split_tokens, *_workspace(workspace))
-    return packed, out, dev, (q, k_cache, v_cache, k_scale, v_scale, block_table, seqlens, out, lse, workspace)
-
-
 def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None, k_scale=1.0, v_scale=1.0,
                            out=None, lse=None, max_seqlen=None, split_tokens=0, workspace=None):
     """Single-token GQA decode over a paged KV cache.
@@ -352,10 +294,8 @@ def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None
     different streams, and captured ones, may overlap.
     """
     if _has_block_scales(k_cache, k_scale, v_scale):
-        packed, out, dev, _keep = _blocks_args(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out,
-                                               lse, max_seqlen, split_tokens, workspace)
-        kv_cache.launch(_lib.lib().fgqa_decode_blocks, packed, dev, "fgqa_decode_blocks")
-        return out
+        return kv_cache.call_native("decode", q, q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out,
+                                    lse, max_seqlen, split_tokens, workspace, False)
     a, out, _keep = _paged_prepare(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out,
                                    lse, max_seqlen, split_tokens, workspace)
     _lib.check(_lib.lib().fgqa_decode_paged(ctypes.byref(a), _stream()), "fgqa_decode_paged")
@@ -366,8 +306,10 @@ def prepare_decode_paged(q, k_cache, v_cache, block_table, seqlens, scale=None, 
                          out=None, lse=None, max_seqlen=None, split_tokens=0, workspace=None):
     """``decode_flash_gqa_paged`` validated once; returns a ``PreparedLaunch``."""
     if _has_block_scales(k_cache, k_scale, v_scale):
-        packed, out, dev, keep = _blocks_args(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out,
-                                              lse, max_seqlen, split_tokens, workspace)
+        packed, out, dev, *made = kv_cache.call_native("decode", q, q, k_cache, v_cache, block_table, seqlens, scale,
+                                                       k_scale, v_scale, out, lse, max_seqlen, split_tokens, workspace,
+                                                       True)
+        keep = (k_cache, v_cache, block_table, seqlens, k_scale, v_scale, out, lse, *made)
         return kv_cache.DeviceLaunch(_lib.lib().fgqa_decode_blocks, packed, keep, out, "fgqa_decode_blocks", dev)
     a, out, keep = _paged_prepare(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_scale, out, lse,
                                   max_seqlen, split_tokens, workspace)

@@ -314,6 +314,20 @@ static void test_decode() {
     DECODE(a.cache.k_stride[1] += 8, NOT);
     DECODE(a.num_q_heads = 17 * kHeads, NOT);
     DECODE(a.batch = 0; a.q = nullptr; a.cache.k_scales = nullptr, OK);
+    // 2 sequences of 4096 tokens, 8 heads: 128 teams of two partials of 32 rows
+    // (512 + 8 bytes) each, and the sequences' prefix; 2 heads: 256 teams
+    {
+        fgqa_decode_blocks_args a = decode_args();
+        a.batch = 2;
+        a.max_seqlen = 4096;
+        a.block_table_stride = 256;
+        fgqa_decode_paged_args p = plan::as_decode_paged(&a);
+        plan::DecodePlan pl;
+        CHECK(plan::plan_paged(&p, &pl, plan::block_item_slots(8)) == OK && pl.teams == 128 &&
+              pl.ws_bytes == 2 * 128 * 32 * 520 + 3 * 8);
+        p.num_kv_heads = 2;
+        CHECK(plan::plan_paged(&p, &pl, plan::block_item_slots(2)) == OK && pl.teams == 256);
+    }
     // a cache without the 8-bit types of the C ABI before
     fgqa_decode_blocks_args a = decode_args();
     fgqa_decode_paged_args p = plan::as_decode_paged(&a);

@@ -39,29 +39,6 @@ def test_exported():
         assert re.search(rf"\bT {d}\(", syms), d
 
 
-@pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")
-def test_binding_matches_the_header(tmp_path):
-    """Size and every field's offset of the argument blocks, from a C program over the header."""
-    structs = {"fgqa_kv_append_args": _lib.KvAppendArgs, "fgqa_decode_blocks_args": _lib.DecodeBlocksArgs,
-               "fgqa_kv_weights_args": _lib.KvWeightsArgs, "fgqa_kv_evict_args": _lib.KvEvictArgs}
-    names = {"k_cache": "cache.k", "v_cache": "cache.v"}
-    names.update({f: "cache." + f for f, _ in _lib._KV_CACHE if f not in names})
-    lines, want = [], []
-    for c, cls in structs.items():
-        lines.append(f'printf("%zu\\n", sizeof({c}));')
-        want.append(ctypes.sizeof(cls))
-        for f, _ in cls._fields_:
-            lines.append(f'printf("%zu\\n", offsetof({c}, {names.get(f, f)}));')
-            want.append(getattr(cls, f).offset)
-    src = tmp_path / "layout.c"
-    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "fgqa_kv.h"\nint main(void) {\n'
-                   + "\n".join(lines) + "\nreturn 0; }\n")
-    exe = tmp_path / "layout"
-    subprocess.run(["gcc", "-I" + os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
-    got = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
-    assert [int(x) for x in got] == want
-
-
 # ------------------------------------------------------------------ refusals
 BF, F8 = torch.bfloat16, torch.float8_e4m3fn
 
@@ -230,17 +207,32 @@ def test_evict_refuses_outputs_over_inputs():
         _evict(weights=wide[:384].view(2, 4, 48), new_weights=wide[10:].view(2, 4, 48))
 
 
-def test_c_abi_refuses_before_launch():
-    """The statuses come from the library itself (null arguments and a bf16 cache for the block-scaled decode)."""
+def test_c_abi_refuses_null_arguments():
     L = _lib.lib()
-    for f in (L.fgqa_kv_append, L.fgqa_decode_blocks, L.fgqa_kv_weights, L.fgqa_kv_evict):
+    for name in ("fgqa_kv_append", "fgqa_decode_blocks", "fgqa_kv_weights", "fgqa_kv_evict"):
+        f = getattr(L, name)
+        f.restype = ctypes.c_int
+        f.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         assert f(None, None) == _lib.FGQA_ERR_INVALID_ARGUMENT
-    a = _lib.DecodeBlocksArgs()
-    n = ctypes.c_size_t(0)
-    assert L.fgqa_decode_blocks_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == _lib.FGQA_ERR_INVALID_ARGUMENT
-    a.kv_dtype, a.num_kv_heads, a.head_dim, a.page_size, a.num_pages = _lib.FGQA_KV_INT8, 8, 128, 16, 4
-    a.batch, a.max_seqlen, a.num_q_heads, a.block_table_stride, a.scale = 2, 4096, 32, 256, 0.1
-    assert L.fgqa_decode_blocks_workspace_bytes(ctypes.byref(a), None) == _lib.FGQA_ERR_INVALID_ARGUMENT
-    assert L.fgqa_decode_blocks_workspace_bytes(ctypes.byref(a), ctypes.byref(n)) == 0
-    # 128 teams of 8 heads: two partials of 32 rows (512 + 8 bytes) each, and the sequences' prefix
-    assert n.value == 2 * 128 * 32 * 520 + 3 * 8
+
+
+def test_arguments_of_other_types():
+    """What is no tensor, number or whole number; too large numbers; sparse tensors; wrong argument counts."""
+    with pytest.raises(TypeError, match="block_table must be a tensor"):
+        _append(block_table=[[0]])
+    with pytest.raises(TypeError):
+        _append(k_cache=_cache(10, 16, 4, 128, dtype=F8), v_cache=_cache(10, 16, 4, 128, dtype=F8), k_scale="1", v_scale=1.0)
+    with pytest.raises(TypeError):
+        _weights(max_seqlen=[3])
+    with pytest.raises(ValueError, match="budget"):
+        _evict(budget=2 ** 40)
+    with pytest.raises(ValueError, match="budget"):
+        _evict(budget=2 ** 80)
+    with pytest.raises(ValueError, match="finite"):
+        _append(k_cache=_cache(10, 16, 4, 128, dtype=F8), v_cache=_cache(10, 16, 4, 128, dtype=F8), k_scale=1e300, v_scale=1.0)
+    with pytest.raises(ValueError, match="split_tokens"):
+        _decode(split_tokens=-1)
+    with pytest.raises((RuntimeError, ValueError)):
+        _append(block_table=torch.zeros(2, 5, dtype=torch.int32).to_sparse())
+    with pytest.raises(TypeError, match="arguments"):
+        fg.native().append(1, 2)
