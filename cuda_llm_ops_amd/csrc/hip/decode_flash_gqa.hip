@@ -491,33 +491,6 @@ __global__ __launch_bounds__(kPair ? 2 * kDecThreads : kDecThreads) void decode_
 constexpr int kPlanThreads = 256;
 constexpr int kPlanSortMax = 1024;   // remainders kept in LDS and length-sorted up to this batch size
 
-// The value of the lane that DPP control kCtrl names, 0 where there is none or
-// the row is not in kRows.
-template <int kCtrl, int kRows, typename T>
-__device__ __forceinline__ T dpp_or_0(T v) {
-    if constexpr (sizeof(T) == 8) {
-        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xF, true);
-        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), kCtrl, kRows, 0xF, true);
-        return (T)(((uint64_t)hi << 32) | lo);
-    } else {
-        return __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xF, true);
-    }
-}
-
-// Folds each lane's value with those of all lanes before it (0: neutral): row
-// shifts by 1, 2, 4 and 8, then the rows' last lanes broadcast to the rows
-// after them.  (With LDS shuffles instead, two per step for a 64-bit sum, a
-// ragged decode of 13 us took 0.3 us longer.)
-template <typename T, typename F>
-__device__ __forceinline__ T wave_fold(T v, F&& f) {
-    v = f(v, dpp_or_0<0x111, 0xF>(v));
-    v = f(v, dpp_or_0<0x112, 0xF>(v));
-    v = f(v, dpp_or_0<0x114, 0xF>(v));
-    v = f(v, dpp_or_0<0x118, 0xF>(v));
-    v = f(v, dpp_or_0<0x142, 0xA>(v));
-    return f(v, dpp_or_0<0x143, 0xC>(v));
-}
-
 // Exclusive prefix sum of one value per thread over a workgroup of kThreads.
 // kAgain: another scan in s_wave follows (else a barrier does before s_wave's
 // memory is written again).
@@ -610,7 +583,8 @@ __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(DecodeParams 
 // sequences are nearly as even (kWholeSlack), a team takes `per` of them in a
 // row, and nothing is left to combine.
 //
-// A split length given by the caller keeps the work list (p.work): a fixed
+// A split length given by the caller keeps the work list (p.work; not over blocks
+// with scales, whose splits run in decode_blocks_split_kernel): a fixed
 // grid walks its entries, each once per kv head or pair (the head fastest, so
 // heads of one split run together).
 //
@@ -657,6 +631,7 @@ __global__ __launch_bounds__(kHeads* kListWaves<kHeads>* kWave) void decode_list
     constexpr int kThreads = kHeads * kItemThreads;
     constexpr int kSmem = kDecItemSmem<kKv, kNw>;
     __shared__ __attribute__((aligned(16))) unsigned char smem[kHeads * kSmem];
+    const bool listed = kKv < kKvBlocksFp8 && p.work != nullptr;   // (over blocks with scales: teams)
     // wave-uniform (readfirstlane), so the buffer resources built from the
     // head stay scalar
     const int half = kHeads > 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kItemThreads)) : 0;
@@ -664,13 +639,13 @@ __global__ __launch_bounds__(kHeads* kListWaves<kHeads>* kWave) void decode_list
     const int tid = (int)threadIdx.x - half * kItemThreads;
     // work list: items blockIdx.x, + gridDim.x, ...
     int item = blockIdx.x;
-    const int n_items = p.work != nullptr ? p.work[0] * per_entry : 0;
+    const int n_items = listed ? p.work[0] * per_entry : 0;
     // teams: blocks [g0, g1) of the batch, the first of them block `blk` of
     // sequence b, and none of sequence b_end
     const int team = blockIdx.x / per_entry;
     int64_t g0 = 0, g1 = 0;
     int b = 0, b_end = p.batch, blk = 0;
-    if (p.work == nullptr) {
+    if (!listed) {
         int64_t* s_wave = reinterpret_cast<int64_t*>(smem);
         int* s_pos = reinterpret_cast<int*>(s_wave + kThreads / kWave);
         int* s_max = s_pos + 2;   // per wave
@@ -729,7 +704,7 @@ __global__ __launch_bounds__(kHeads* kListWaves<kHeads>* kWave) void decode_list
         int kvh, t_begin, t_end;
         bool whole;
         int64_t slot;
-        if (p.work != nullptr) {
+        if (listed) {
             if (item >= n_items) break;
             const int e = p.work[1 + item / per_entry];
             kvh = item % per_entry;
@@ -759,7 +734,7 @@ __global__ __launch_bounds__(kHeads* kListWaves<kHeads>* kWave) void decode_list
         }
         __syncthreads();   // the previous item's merge buffers alias the staging area
         dec_item_of<kKv, kSeg, kNw>(p, smem + half * kSmem, t_begin, t_end, kvh, b, tid, whole, slot * p.group);
-        if (p.work == nullptr) {
+        if (!listed) {
             g0 += (t_end - t_begin + plan::kDecodeStepRound - 1) / plan::kDecodeStepRound;
             ++b;
             blk = 0;
@@ -789,6 +764,35 @@ static void launch_list(const DecodeParams& p, int nsplit, int cus, hipStream_t 
     }
     if (p.hkv % 2 == 0) launch_list_heads<kKv, kSeg, 2>(p, nsplit, cus, s);
     else launch_list_heads<kKv, kSeg, 1>(p, nsplit, cus, s);
+}
+
+// Pass 1 over a cache with block scales in splits (a small batch, a given split
+// length or too small a workspace for teams): one 8-wave workgroup per (split, kv
+// head) of each sequence, heads side by side.  It finds its tokens from one
+// length, where a team first scans all of them, and has 8 waves for them, not 2 or
+// 4.  Latency bounds it: 128 tokens take 5 us in all, 128 more of them each about
+// 1.2 us, a combine 4.
+template <int kKv, int kSeg>
+__global__ __launch_bounds__(2 * kDecThreads) void decode_blocks_split_kernel(DecodeParams p) {
+    constexpr int kNw = 2 * kDecWaves;
+    __shared__ __attribute__((aligned(16))) unsigned char smem[kDecItemSmem<kKv, kNw>];
+    const int kvh = (int)(blockIdx.x % (uint32_t)p.hkv);
+    const uint32_t rest = blockIdx.x / (uint32_t)p.hkv;
+    const int split = (int)(rest % (uint32_t)p.nsplit), b = (int)(rest / (uint32_t)p.nsplit);
+    const int tid = threadIdx.x;
+    const int len = clamp_len(p, b);
+    const int t_begin = split * p.chunk;
+    if (t_begin < len) {
+        dec_item_of<kKv, kSeg, kNw>(p, smem, t_begin, min(t_begin + p.chunk, len), kvh, b, tid, p.nsplit == 1,
+                                    (((int64_t)b * p.hkv + kvh) * p.nsplit + split) * p.group);
+    } else if (p.nsplit == 1 && (tid >> 4) < p.group) {   // (with splits the combine writes them)
+        const int qh = kvh * p.group + (tid >> 4);
+        bf16x8_t z;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = (__bf16)0.f;
+        *reinterpret_cast<bf16x8_t*>(p.o + b * p.o_sb + qh * p.o_sh + (tid & 15) * 8) = z;
+        if (p.lse != nullptr && (tid & 15) == 0) p.lse[(int64_t)b * p.hq + qh] = -INFINITY;
+    }
 }
 
 // Log-sum-exp merge of the partials of each (sequence, query head): 16 lanes
@@ -1179,12 +1183,40 @@ extern "C" int fgqa_decode_paged_workspace_bytes(const fgqa_decode_paged_args* a
 
 namespace fgqa {
 namespace {
+// Pages of at least one load instruction's rows (4 bf16, 8 fp8) whose
+// bytes stay below 2^31: page segments of min(page, 32) rows, each
+// read through one buffer resource (at BASELINE config 3's lengths
+// with 16- and 64-token pages: bf16 -4 %, fp8 with head pairs -1 to
+// -2 % against the per-row form).
+int page_segment(const fgqa_decode_paged_args* a) {
+    const bool small_pages = (int64_t)a->page_size * a->k_stride[1] * 2 < ((int64_t)1 << 31) &&
+                             (int64_t)a->page_size * a->v_stride[1] * 2 < ((int64_t)1 << 31);
+    return !small_pages ? 0 : a->page_size >= 32 ? 32 : a->page_size >= 4 ? a->page_size : 0;
+}
+
+template <int kKv>
+void launch_blocks_split(const DecodeParams& p, int seg, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)p.batch * p.nsplit * p.hkv)), block(2 * kDecThreads);
+    switch (seg >= 8 ? seg : 0) {
+        case 32: hipLaunchKernelGGL((decode_blocks_split_kernel<kKv, 32>), grid, block, 0, s, p); break;
+        case 16: hipLaunchKernelGGL((decode_blocks_split_kernel<kKv, 16>), grid, block, 0, s, p); break;
+        case 8: hipLaunchKernelGGL((decode_blocks_split_kernel<kKv, 8>), grid, block, 0, s, p); break;
+        default: hipLaunchKernelGGL((decode_blocks_split_kernel<kKv, 0>), grid, block, 0, s, p); break;
+    }
+    if (p.nsplit > 1) launch_combine<false>(p, p.nsplit, s);
+}
+
+// The plan of a block-scaled decode: with teams, or (plan->teams 0) in splits.
+int plan_blocks(const fgqa_decode_paged_args* a, DecodePlan* plan) {
+    return plan::plan_blocks(a, device_cu_count(), plan);
+}
+
 // The paged decode of validated arguments; `blocks`: a cache with block scales,
 // e4m3 or int8 (`a` describes the rest of the call).
 int paged_run(const fgqa_decode_paged_args* a, const fgqa_kv_cache* blocks, void* stream) {
     if (a->batch == 0) return FGQA_OK;
     DecodePlan plan;
-    int st = plan::plan_paged(a, &plan, blocks != nullptr ? plan::block_item_slots(a->num_kv_heads) : plan::kDecodeItemSlots);
+    int st = blocks != nullptr ? plan_blocks(a, &plan) : plan::plan_paged(a, &plan);
     if (st != FGQA_OK) return st;
 
     DecodeParams p;
@@ -1250,15 +1282,13 @@ int paged_run(const fgqa_decode_paged_args* a, const fgqa_kv_cache* blocks, void
     } else {
         const int cus = device_cu_count();
         if (cus <= 0) return FGQA_ERR_HIP;
-        // Pages of at least one load instruction's rows (4 bf16, 8 fp8) whose
-        // bytes stay below 2^31: page segments of min(page, 32) rows, each
-        // read through one buffer resource (at BASELINE config 3's lengths
-        // with 16- and 64-token pages: bf16 -4 %, fp8 with head pairs -1 to
-        // -2 % against the per-row form).
         const bool fp8 = a->kv_dtype == FGQA_KV_FP8_E4M3;
-        const bool small_pages = (int64_t)a->page_size * a->k_stride[1] * 2 < ((int64_t)1 << 31) &&
-                                 (int64_t)a->page_size * a->v_stride[1] * 2 < ((int64_t)1 << 31);
-        const int seg = !small_pages ? 0 : a->page_size >= 32 ? 32 : a->page_size >= 4 ? a->page_size : 0;
+        const int seg = page_segment(a);
+        if (blocks != nullptr && p.teams == 0) {
+            if (blocks->kv_dtype == FGQA_KV_INT8) launch_blocks_split<kKvBlocksInt8>(p, seg, s);
+            else launch_blocks_split<kKvBlocksFp8>(p, seg, s);
+            return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
+        }
         auto pass1 = [&] {
             if (blocks != nullptr) {
                 auto launch = [&](auto kv) {
@@ -1312,7 +1342,7 @@ extern "C" int fgqa_decode_blocks_workspace_bytes(const fgqa_decode_blocks_args*
     if (st != FGQA_OK) return st;
     const fgqa_decode_paged_args p = plan::as_decode_paged(a);
     DecodePlan plan;
-    const int planned = plan::plan_paged(&p, &plan, plan::block_item_slots(p.num_kv_heads));
+    const int planned = plan_blocks(&p, &plan);
     if (planned != FGQA_OK) return planned;
     *bytes = plan.ws_bytes;
     return FGQA_OK;

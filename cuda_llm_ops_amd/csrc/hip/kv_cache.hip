@@ -519,7 +519,7 @@ __device__ __forceinline__ void fill_row(T* dst, int from, int to, T value) {
 // take a launch for each pass, about what a pass takes.
 template <int kPer>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
-    __shared__ int s_hist[kBins];
+    __shared__ __attribute__((aligned(16))) int s_hist[kBins];
     __shared__ int s_wave[3][kSelectWaves];
     __shared__ int s_found[2];
     __shared__ uint32_t s_list[kSelectWaves][kListMax];
@@ -578,13 +578,13 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     uint32_t prefix = 0;
     int left = need;
     int listed = 0;   // of this wave
+    for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
+    __syncthreads();
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const int bins = pass == 2 ? 1024 : 2048;
         const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-        for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
-        __syncthreads();
         auto add = [&](uint32_t k) { atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1); };
         if (pass == 0) {
             each([&](int, uint32_t k) {
@@ -612,14 +612,12 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
             }
         }
         __syncthreads();
-        // thread t: bins kBins - 1 - 2t and the one below, from the top down
-        const int top = s_hist[kBins - 1 - 2 * tid], next = s_hist[kBins - 2 - 2 * tid];
-        int incl = top + next;
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const int o = __shfl_up(incl, d, kWave);
-            incl += lane >= d ? o : 0;
-        }
+        // thread t: bins kBins - 2 - 2t and the one above, from the top down, left
+        // zero for the next pass
+        int2* pair = reinterpret_cast<int2*>(s_hist) + (kBins / 2 - 1 - tid);
+        const int top = pair->y, next = pair->x;
+        *pair = int2{0, 0};
+        const int incl = wave_fold(top + next, [](int x, int y) { return x + y; });
         if (lane == kWave - 1) s_wave[0][wave] = incl;
         __syncthreads();
         int before = incl - top - next;

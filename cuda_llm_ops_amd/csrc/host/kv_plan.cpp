@@ -198,6 +198,43 @@ fgqa_decode_paged_args as_decode_paged(const fgqa_decode_blocks_args* a) {
     return p;
 }
 
+// Splits of the tokens that a CU gets of a full batch, so that one round of
+// workgroups runs, down to a step of 8 waves; no splits where the sequences are
+// at most kSplitSlack longer (the combine's launch costs what those take).  Hq / Hkv,
+// 16-token pages, lengths up to S, us teams / splits: 16 / 1, 1 x 512 11.4 / 5.8; 32 / 8,
+// 4 x 1024 16.3 / 9.2, 1 x 32768 17.8 / 14.4, 16 x 4096 30.2 / 27.4.  Teams share
+// out uneven lengths, and 4 heads of theirs read side by side: they are taken
+// for more than kSplitMost tokens a CU (16 x 8192 39.8 / 45.5, 128 x 2048 61.9 / 72.2;
+// 28 / 4, 64 x 4096 the other way, 41.3 / 35.8) or two workgroups a CU (32 / 8, 128
+// x 512 25.2 / 28.7).
+int blocks_split(int64_t batch, int64_t num_kv_heads, int64_t max_seqlen, int cus) {
+    constexpr int64_t kSplitMost = 2048, kSplitSlack = 512;
+    const i128 heads = (i128)batch * num_kv_heads;
+    const i128 tokens = heads * max_seqlen;
+    if (max_seqlen <= 0 || tokens > (i128)kSplitMost * cus || heads > 2 * (i128)cus) return 0;
+    const int64_t step = kDecodeStepRound;   // what 4 waves take at a time
+    const int64_t chunk = ceil_div(ceil_div((int64_t)tokens, cus), step) * step;
+    return (int)(max_seqlen <= chunk + kSplitSlack ? ceil_div(max_seqlen, step) * step : chunk);
+}
+
+int plan_blocks(const fgqa_decode_paged_args* a, int cus, DecodePlan* plan) {
+    fgqa_decode_paged_args split = *a;
+    if (a->split_tokens == 0)
+        split.split_tokens = blocks_split(a->batch, a->num_kv_heads, a->max_seqlen, cus > 0 ? cus : 256);
+    int st;
+    if (split.split_tokens > 0) {
+        st = plan_paged(&split, plan);
+        if (st != FGQA_OK) return st;
+        plan->list = false;
+        plan->ws_bytes = plan->least_bytes = plan->part_o_bytes + plan->part_ml_bytes;
+    } else {
+        st = plan_paged(a, plan, block_item_slots(a->num_kv_heads));
+        if (st != FGQA_OK) return st;
+    }
+    // workgroups of the split form
+    return grid_ok((i128)a->batch * plan->nsplit * a->num_kv_heads) ? FGQA_OK : FGQA_ERR_UNSUPPORTED;
+}
+
 int validate_decode_blocks(const fgqa_decode_blocks_args* a) {
     if (a == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
     if (a->cache.kv_dtype != FGQA_KV_FP8_E4M3 && a->cache.kv_dtype != FGQA_KV_INT8) return FGQA_ERR_INVALID_ARGUMENT;

@@ -24,6 +24,16 @@ fgqa_decode_paged_args as_decode_paged(const fgqa_decode_blocks_args* a);
 // times 4 heads of 2 waves, or 2 of 4.
 constexpr int block_item_slots(int num_kv_heads) { return num_kv_heads % 4 == 0 ? 1024 : kDecodeItemSlots; }
 
+// Tokens per split of a block-scaled decode without a given length on a device of
+// `cus` CUs, or 0: the batch shared out evenly over teams.
+int blocks_split(int64_t batch, int64_t num_kv_heads, int64_t max_seqlen, int cus);
+
+// The plan of a block-scaled decode on a device of `cus` CUs (0, unknown: 256, what
+// the teams are made for): splits of the given length or of blocks_split() (teams
+// 0, no work list), or teams, which become splits where the workspace holds only
+// those (fit_workspace).
+int plan_blocks(const fgqa_decode_paged_args* a, int cus, DecodePlan* plan);
+
 inline int log2_of(int power_of_two) {
     int shift = 0;
     while ((1 << shift) < power_of_two) ++shift;

@@ -314,20 +314,43 @@ static void test_decode() {
     DECODE(a.cache.k_stride[1] += 8, NOT);
     DECODE(a.num_q_heads = 17 * kHeads, NOT);
     DECODE(a.batch = 0; a.q = nullptr; a.cache.k_scales = nullptr, OK);
-    // 2 sequences of 4096 tokens, 8 heads: 128 teams of two partials of 32 rows
+    // 64 sequences of 16384 tokens, 8 heads: 128 teams of two partials of 32 rows
     // (512 + 8 bytes) each, and the sequences' prefix; 2 heads: 256 teams
     {
         fgqa_decode_blocks_args a = decode_args();
-        a.batch = 2;
-        a.max_seqlen = 4096;
-        a.block_table_stride = 256;
+        a.batch = 64;
+        a.max_seqlen = 16384;
+        a.block_table_stride = 1024;
         fgqa_decode_paged_args p = plan::as_decode_paged(&a);
         plan::DecodePlan pl;
-        CHECK(plan::plan_paged(&p, &pl, plan::block_item_slots(8)) == OK && pl.teams == 128 &&
-              pl.ws_bytes == 2 * 128 * 32 * 520 + 3 * 8);
+        CHECK(plan::plan_blocks(&p, 256, &pl) == OK && pl.teams == 128 && pl.least_bytes <= pl.ws_bytes);
         p.num_kv_heads = 2;
-        CHECK(plan::plan_paged(&p, &pl, plan::block_item_slots(2)) == OK && pl.teams == 256);
+        CHECK(plan::plan_blocks(&p, 256, &pl) == OK && pl.teams == 256);
+        // splits: of a length given, of the whole sequence (nothing to merge), of an even share
+        p.split_tokens = 1000;
+        CHECK(plan::plan_blocks(&p, 256, &pl) == OK && pl.teams == 0 && !pl.list && pl.chunk == 1024 && pl.nsplit == 16 &&
+              pl.ws_bytes == (size_t)64 * 32 * 16 * 520 && pl.least_bytes == pl.ws_bytes);
+        p.split_tokens = 0;
+        p.batch = 8;
+        p.max_seqlen = 640;
+        CHECK(plan::plan_blocks(&p, 256, &pl) == OK && pl.teams == 0 && pl.nsplit == 1 && pl.ws_bytes == 0);
+        p.max_seqlen = 8000;
+        CHECK(plan::plan_blocks(&p, 0, &pl) == OK && pl.teams == 0 && pl.chunk == 512 && pl.nsplit == 16);
+        p.max_seqlen = 0;
+        CHECK(plan::plan_blocks(&p, 256, &pl) == OK);
+        // more workgroups than a grid has
+        p.batch = 32000;
+        p.max_seqlen = 16384;
+        p.split_tokens = 1;
+        p.num_kv_heads = p.num_q_heads = 1 << 14;
+        CHECK(plan::plan_blocks(&p, 256, &pl) == NOT);
     }
+    CHECK(plan::blocks_split(1, 1, 0, 256) == 0 && plan::blocks_split(1, 1, 1, 256) == 128);
+    CHECK(plan::blocks_split(1, 8, 640, 256) == 640 && plan::blocks_split(1, 8, 641, 256) == 128);
+    CHECK(plan::blocks_split(64, 8, 1024, 256) == 1024 && plan::blocks_split(64, 8, 1025, 256) == 0);
+    CHECK(plan::blocks_split(65, 8, 128, 256) == 0 && plan::blocks_split(64, 8, 128, 256) == 128);
+    CHECK(plan::blocks_split(1, 1, 524288, 256) == 2048 && plan::blocks_split(1, 1, 524289, 256) == 0);
+    CHECK(plan::blocks_split(INT_MAX, INT_MAX, INT_MAX, 256) == 0);
     // a cache without the 8-bit types of the C ABI before
     fgqa_decode_blocks_args a = decode_args();
     fgqa_decode_paged_args p = plan::as_decode_paged(&a);

@@ -229,13 +229,29 @@ def _check_decode(c, q, table, lens, got_o, got_lse, what):
     assert np.all(d <= e), f"{what}: lse off by {d.max()}"
 
 
+def _for_teams(cuda, table, P, H):
+    """The block table with room for so many tokens that a decode without a given
+    split length shares the batch out over teams, not in splits (more than
+    2048 tokens of a head per CU); the entries that no sequence reaches are garbage."""
+    cus = _torch().cuda.get_device_properties(cuda).multi_processor_count
+    width = (2048 * cus // (len(table) * H) + P) // P
+    wide = np.random.default_rng(5).integers(-9, 10 ** 9, size=(len(table), width))
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
 def _decode(cuda, c, q, table, lens, what, **kw):
+    """One decode, and one over teams where no argument settles the form."""
     torch = _torch()
-    lse = torch.full(q.shape[:2], float("nan"), dtype=torch.float32, device=cuda)
-    o = _fg().decode_flash_gqa_paged(q.to(cuda), c.t[0], c.t[1], _i32(cuda, table), _i32(cuda, lens), lse=lse, **c.scales,
-                                     **kw)
-    torch.cuda.synchronize()
-    _check_decode(c, q, table, lens, o, lse, what)
+    tables = [table]
+    if not {"split_tokens", "workspace", "max_seqlen"} & kw.keys():
+        tables.append(_for_teams(cuda, table, c.t[0].shape[1], c.t[0].shape[2]))
+    for form, t in zip(("", " in teams"), tables):
+        lse = torch.full(q.shape[:2], float("nan"), dtype=torch.float32, device=cuda)
+        o = _fg().decode_flash_gqa_paged(q.to(cuda), c.t[0], c.t[1], _i32(cuda, t), _i32(cuda, lens), lse=lse,
+                                         **c.scales, **kw)
+        torch.cuda.synchronize()
+        _check_decode(c, q, table, lens, o, lse, what + form)
     return o, lse
 
 
@@ -263,7 +279,8 @@ def test_decode_heads_and_splits(cuda, G, H, dtype):
     c = Cache(cuda, rng, dtype, 4 * 75 + 1, 16, H)
     table = _table(rng, 4, 75, 4 * 75 + 1)
     q = _x(rng, 4, G * H, 128)
-    for split in (0, 128, 512):
+    _decode(cuda, c, q, table, lens, what)
+    for split in (128, 512):
         _decode(cuda, c, q, table, lens, f"{what} split={split}", split_tokens=split)
 
 
@@ -348,8 +365,9 @@ def test_decode_same_bits_as_the_whole_cache_scale(cuda):
     assert (whole.float() - blocks.float()).abs().max() <= v * (2.0 ** -8 + 2.0 ** -11) + 2 * 2.0 ** -8 * blocks.float().abs().max()
 
 
+@pytest.mark.parametrize("teams", [False, True])
 @pytest.mark.parametrize("P", [4, 16, 64])
-def test_decode_scores_of_minus_infinity(cuda, P):
+def test_decode_scores_of_minus_infinity(cuda, P, teams):
     """Keys whose scores overflow to -inf get nothing, wherever they lie; a row of
     such keys alone is NaN, as the formula has it."""
     torch = _torch()
@@ -369,7 +387,8 @@ def test_decode_scores_of_minus_infinity(cuda, P):
     q[:, 0, :] = 0.0
     q[:, 0, 7] = 3e38
     lse = torch.empty((2, 2), device=cuda)
-    o = _fg().decode_flash_gqa_paged(q.to(cuda), c.t[0], c.t[1], _i32(cuda, table), _i32(cuda, lens), lse=lse, **c.scales)
+    of = _for_teams(cuda, table, P, 1) if teams else table
+    o = _fg().decode_flash_gqa_paged(q.to(cuda), c.t[0], c.t[1], _i32(cuda, of), _i32(cuda, lens), lse=lse, **c.scales)
     torch.cuda.synchronize()
     v = ref.gather(c.n[1], c.sn[1], table, 0, 300, 0)[alive].mean(axis=0)
     size = np.abs(ref.gather(c.n[1], c.sn[1], table, 0, 300, 0)[alive]).mean(axis=0)
@@ -380,6 +399,28 @@ def test_decode_scores_of_minus_infinity(cuda, P):
     assert bool(o[1, 0].isnan().all())           # no key of row 1 is alive
 
 
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("B,H,S", [(1, 8, 640), (1, 8, 641), (3, 1, 5000), (16, 4, 1024), (16, 4, 1025), (64, 8, 130),
+                                   (65, 8, 130), (8, 8, 8192), (8, 8, 8200), (300, 1, 40)])
+def test_decode_forms(cuda, B, H, S, dtype):
+    """Either side of where sequences are split, and shared out over teams: the
+    lengths 0, 1 and the longest among them."""
+    what = f"decode B={B} Hkv={H} S={S} {dtype}"
+    print(what, flush=True)
+    rng = np.random.default_rng(B + S)
+    lens = rng.integers(1, min(S, 700) + 1, size=B)
+    lens[0] = S
+    lens[1:3] = (0, 1)[:max(0, min(2, B - 1))]
+    width = -(-S // 64)
+    pages = int(sum(-(-n // 64) for n in lens)) + 1
+    c = Cache(cuda, rng, dtype, pages, 64, H)
+    table, at = np.zeros((B, width), np.int32), rng.permutation(pages)
+    for b, n in enumerate(lens):
+        table[b, :-(-n // 64)], at = at[:-(-n // 64)], at[-(-n // 64):]
+    q = _x(rng, B, 3 * H, 128)
+    _decode(cuda, c, q, table, lens.tolist(), what, max_seqlen=S)
+
+
 def test_decode_least_workspace(cuda):
     """A caller's workspace that holds 4096-token splits only, one that holds the
     even sharing, and one too small."""
@@ -387,9 +428,9 @@ def test_decode_least_workspace(cuda):
     fg = _fg()
     rng = np.random.default_rng(83)
     c = Cache(cuda, rng, "e4m3", 300, 64, 4)
-    table, lens = _table(rng, 2, 150, 300), [9500, 4097]
+    table, lens = _for_teams(cuda, _table(rng, 2, 150, 300), 64, 4), [9500, 4097]
     q = _x(rng, 2, 16, 128)
-    n = -(-9600 // 4096)
+    n = -(-table.shape[1] * 64 // 4096)
     least = -(-2 * 16 * n * 512 // 256) * 256 + -(-2 * 16 * n * 8 // 256) * 256 + 4 * (1 + 2 * n)
     for size in (least, 64 << 20):
         ws = torch.empty(size, dtype=torch.uint8, device=cuda)
