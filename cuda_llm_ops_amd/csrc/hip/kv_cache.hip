@@ -7,6 +7,7 @@
 // rounding, growing a block's scale rounds its int8 codes once more and its
 // e4m3 codes not at all (but where they become subnormal), and the result does
 // not depend on the order of anything.
+#include <algorithm>
 #include <math.h>
 
 #include "fgqa_internal.h"
@@ -466,13 +467,13 @@ struct EvictParams {
     int32_t* kept;
     int max_seqlen, weights_len, budget, recent;
     int pages;       // new pages of a sequence at most
+    int parts;       // workgroups per row of the selection
     uint32_t items;  // batch * pages * 2 * hkv, below 2^31
 };
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWaves = kSelectThreads / kWave;
 constexpr int kBins = 2048;
-constexpr int kListMax = 256;
 
 // Weights in their order as unsigned numbers above 0; NaN above all, -0 as 0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -491,41 +492,45 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t m) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
 }
 
-// dst[from, to) = value, 16 bytes at a time where they are aligned.
+// dst[from, to) = value by `threads` threads, 16 bytes at a time where they are aligned.
 template <typename T>
-__device__ __forceinline__ void fill_row(T* dst, int from, int to, T value) {
+__device__ __forceinline__ void fill_row(T* dst, int from, int to, T value, int thread, int threads) {
     static_assert(sizeof(T) == 4, "");
     typedef T vec __attribute__((ext_vector_type(4)));
-    const int tid = threadIdx.x;
     const int head = min(from + (int)((0 - (reinterpret_cast<uintptr_t>(dst + from) >> 2)) & 3), to);
     const int vecs = (to - head) / 4;
-    if (tid < head - from) dst[from + tid] = value;
-    for (int i = tid; i < vecs; i += kSelectThreads)
-        reinterpret_cast<vec*>(dst + head)[i] = vec{value, value, value, value};
-    if (tid < to - head - 4 * vecs) dst[head + 4 * vecs + tid] = value;
+    if (thread < head - from) dst[from + thread] = value;
+    for (int i = thread; i < vecs; i += threads) reinterpret_cast<vec*>(dst + head)[i] = vec{value, value, value, value};
+    if (thread < to - head - 4 * vecs) dst[head + 4 * vecs + thread] = value;
 }
 
 // One workgroup per (sequence, head): the `need` largest keys of the candidates
 // (tokens before the recent ones) by their digits from the top, 11, 11 and 10
 // bits: the histogram of the keys that share the digits found so far says which
-// digit the last kept key has.  (After the first digit each wave puts the keys
-// that have it in a list, and takes the others from there where it is long
-// enough.)  Then every wave walks its
-// part of the candidates in order and writes what is kept.  Integer sums only: no
-// order matters.
-// kPer: candidates that a thread holds in registers, read once, all loads in
-// flight together; 0 for longer rows, which every pass reads again.
-// Few rows leave most of the chip idle: splitting a row over workgroups would
-// take a launch for each pass, about what a pass takes.
-template <int kPer>
+// digit the last kept key has.  Then every wave walks its part of the candidates
+// in order and writes what is kept.  Integer sums only: no order matters.
+// kHeld: candidates whose keys are held in LDS, read once, all loads in
+// flight together; 0 for longer rows, which every pass reads again.  (In 32
+// registers of a thread instead, whose passes cannot be loops, 23.3 us where LDS
+// took 22.1.)
+// The vector units of a row's one CU bound it: an operation on each of 32K keys
+// takes 0.2 us, the first histogram 3.5.  Shared out over workgroups, the
+// histograms would take a launch for each pass, about what a pass takes; but
+// where there are fewer rows than CUs, `parts` workgroups find the same
+// threshold, and each writes its part of every wave's steps.  8 rows of 32K: 17.2
+// us (22.1 in one part), 256 of 8K 13.7, 4 of 600 7.1, 3 launches' worth of
+// latency: loads, three scans, stores.
+template <int kHeld>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
+    __shared__ __attribute__((aligned(16))) uint32_t s_keys[kHeld > 0 ? kHeld : 4];
     __shared__ __attribute__((aligned(16))) int s_hist[kBins];
-    __shared__ int s_wave[3][kSelectWaves];
+    __shared__ __attribute__((aligned(16))) int s_wave[3][kSelectWaves];
     __shared__ int s_found[2];
-    __shared__ uint32_t s_list[kSelectWaves][kListMax];
     const int tid = threadIdx.x, lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int h = (int)(blockIdx.x % (unsigned)p.c.hkv), b = (int)(blockIdx.x / (unsigned)p.c.hkv);
+    const int part = (int)(blockIdx.x % (unsigned)p.parts);
+    const unsigned row = blockIdx.x / (unsigned)p.parts;
+    const int h = (int)(row % (unsigned)p.c.hkv), b = (int)(row / (unsigned)p.c.hkv);
     const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
     const int count = min(len, p.budget);
     const int recent = len > p.budget ? min(p.recent, p.budget) : len;
@@ -535,82 +540,102 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     float* nw = p.new_weights + b * p.nw_b + h * p.nw_h;
     int32_t* kept = p.kept + ((int64_t)b * p.c.hkv + h) * p.budget;
 
-    // each wave's run of the candidates, in order; f(index, key) for 64 of them at
-    // a time, the key 0, which no weight has, where the run has ended
-    const int run = (cand + kSelectThreads - 1) / kSelectThreads * kWave;
-    const int lo = min(wave * run, cand), hi = min(lo + run, cand);
-    constexpr int kBatch = kPer > 0 ? kPer : 8;
-    uint32_t keys[kBatch];
-    auto read = [&](int i0) {
-        float v[kBatch];
-#pragma unroll
-        for (int s = 0; s < kBatch; ++s) {
-            const int i = i0 + s * kWave + lane;
-            v[s] = i < hi ? w[i] : 0.f;
-        }
-#pragma unroll
-        for (int s = 0; s < kBatch; ++s) keys[s] = i0 + s * kWave + lane < hi ? weight_key(v[s]) : 0u;
+    // each wave's run of the candidates: steps of 4 in a row per lane, the key 0,
+    // which no weight has, past the end
+    const int steps = (int)(((unsigned)cand + kSelectThreads * 4 - 1) / (kSelectThreads * 4));
+    const int lo = wave * steps * (kWave * 4) + lane * 4;
+    // 4 weights from i on; past the row's end the last 4, which to_keys puts in place
+    // (no load in a branch, where each would be waited for)
+    auto read = [&](int i) -> f32x4_t {
+        typedef f32x4_t loose __attribute__((aligned(4)));
+        if (cand >= 4) return *reinterpret_cast<const loose*>(w + min(i, cand - 4));
+        return f32x4_t{w[0], w[min(1, cand - 1)], w[cand - 1], 0.f};
     };
-    auto each = [&](auto&& f) {
-        for (int i0 = lo; i0 < hi; i0 += kBatch * kWave) {
-            if (kPer == 0) read(i0);
+    auto to_keys = [&](int i, f32x4_t v) {
+        const int over = cand >= 4 ? i - (cand - 4) : i;   // of 4, how many lie past the end
+        if (over > 0) v = f32x4_t{over == 1 ? v[1] : over == 2 ? v[2] : v[3], over == 1 ? v[2] : v[3], v[3], 0.f};
+        u32x4_t k;
 #pragma unroll
-            for (int s = 0; s < kBatch; s += 4) {
-                if (i0 + s * kWave >= hi) break;
+        for (int e = 0; e < 4; ++e) k[e] = i + e < cand ? weight_key(v[e]) : 0u;
+        return k;
+    };
+    // f(index of the first, keys) for each of these steps of the wave's, in order
+    auto each = [&](int from, int end, auto&& f) {
+        if constexpr (kHeld > 0) {
+            for (int s = from; s < end; ++s) {
+                const int i = lo + s * (kWave * 4);
+                f(i, *reinterpret_cast<const u32x4_t*>(s_keys + i));
+            }
+        } else {
+            constexpr int kBatch = 4;
+            for (int s = from; s < end; s += kBatch) {
+                f32x4_t v[kBatch];
 #pragma unroll
-                for (int e = s; e < s + 4; ++e) f(i0 + e * kWave + lane, keys[e]);
+                for (int e = 0; e < kBatch; ++e) v[e] = s + e < end ? read(lo + (s + e) * (kWave * 4)) : f32x4_t{};
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e)
+                    if (s + e < end) {
+                        const int i = lo + (s + e) * (kWave * 4);
+                        f(i, to_keys(i, v[e]));
+                    }
             }
         }
     };
-    if (kPer > 0 && need > 0) read(lo);
+    auto waves_before = [&](const int* of_waves) {   // their sum over the waves before this one
+        int x = 0;
+#pragma unroll
+        for (int v = 0; v < kSelectWaves; v += 4) {
+            const int4 q = *reinterpret_cast<const int4*>(of_waves + v);
+            x += (v < wave ? q.x : 0) + (v + 1 < wave ? q.y : 0) + (v + 2 < wave ? q.z : 0) + (v + 3 < wave ? q.w : 0);
+        }
+        return x;
+    };
+    constexpr int kMost = kHeld / (kSelectThreads * 4);   // steps of a held row
+    f32x4_t raw[kMost > 0 ? kMost : 1];
+    if (kHeld > 0 && need > 0) {
+#pragma unroll
+        for (int s = 0; s < kMost; ++s)
+            if (s < steps) raw[s] = read(lo + s * (kWave * 4));
+    }
 
     // what needs no choice: the recent tokens, and what lies behind the kept ones
-    if (h == 0 && tid == 0) p.new_seqlens[b] = count;
-    for (int i = tid; i < recent; i += kSelectThreads) {
+    const int at_thread = part * kSelectThreads + tid, threads = p.parts * kSelectThreads;
+    if (h == 0 && at_thread == 0) p.new_seqlens[b] = count;
+    for (int i = at_thread; i < recent; i += threads) {
         kept[need + i] = cand + i;
         nw[need + i] = w[cand + i];
     }
-    fill_row(kept, count, p.budget, (int32_t)-1);
-    fill_row(nw, count, p.weights_len, 0.f);
-    if (need <= 0) return;
+    auto fill = [&] {
+        fill_row(kept, count, p.budget, (int32_t)-1, at_thread, threads);
+        fill_row(nw, count, p.weights_len, 0.f, at_thread, threads);
+    };
+    if (need <= 0) return fill();
+
+    for (int i = tid; i < kBins / 4; i += kSelectThreads) reinterpret_cast<int4*>(s_hist)[i] = int4{0, 0, 0, 0};
+    if constexpr (kHeld > 0) {
+#pragma unroll
+        for (int s = 0; s < kMost; ++s) {
+            const int i = lo + s * (kWave * 4);
+            if (s < steps) *reinterpret_cast<u32x4_t*>(s_keys + i) = to_keys(i, raw[s]);
+        }
+    }
+    fill();   // (after the loads: a wait for those would wait for its stores too)
+    __syncthreads();
 
     // keys above `prefix` are kept, and the first `left` of those equal to it
     uint32_t prefix = 0;
     int left = need;
-    int listed = 0;   // of this wave
-    for (int i = tid; i < kBins; i += kSelectThreads) s_hist[i] = 0;
-    __syncthreads();
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const int bins = pass == 2 ? 1024 : 2048;
+        const uint32_t digits = pass == 2 ? 1023u : 2047u;
         const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-        auto add = [&](uint32_t k) { atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1); };
-        if (pass == 0) {
-            each([&](int, uint32_t k) {
-                if (k != 0u) add(k);
-            });
-        } else {
-            if (pass == 1) {
-                each([&](int, uint32_t k) {
-                    const uint64_t m = __ballot((k >> 21) == prefix >> 21);
-                    if (m == 0) return;
-                    const int at = listed + (int)lanes_below(m);
-                    if (((m >> lane) & 1) && at < kListMax) s_list[wave][at] = k;
-                    listed += __popcll(m);
-                });
-            }
-            if (listed <= kListMax) {
-                for (int i = lane; i < listed; i += kWave) {
-                    const uint32_t k = s_list[wave][i];
-                    if ((k & mask) == prefix) add(k);
-                }
-            } else {
-                each([&](int, uint32_t k) {
-                    if ((k & mask) == prefix) add(k);
-                });
-            }
-        }
+        each(0, steps, [&](int, u32x4_t k) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (pass == 0 ? k[e] != 0u : (k[e] & mask) == prefix)   // (no weight's key has the top digit 0)
+                    atomicAdd(&s_hist[(k[e] >> shift) & digits], 1);
+        });
         __syncthreads();
         // thread t: bins kBins - 2 - 2t and the one above, from the top down, left
         // zero for the next pass
@@ -620,9 +645,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
         const int incl = wave_fold(top + next, [](int x, int y) { return x + y; });
         if (lane == kWave - 1) s_wave[0][wave] = incl;
         __syncthreads();
-        int before = incl - top - next;
-#pragma unroll
-        for (int v = 0; v < kSelectWaves; ++v) before += v < wave ? s_wave[0][v] : 0;
+        const int before = incl - top - next + waves_before(s_wave[0]);
         if (before < left && before + top >= left) {
             s_found[0] = kBins - 1 - 2 * tid;
             s_found[1] = left - before;
@@ -635,41 +658,65 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
         left = s_found[1];
     }
 
+    // of this wave, and before its steps of this part
+    const int first = (int)((int64_t)part * steps / p.parts), end = (int)((int64_t)(part + 1) * steps / p.parts);
     int n_above = 0, n_same = 0;
-    each([&](int, uint32_t k) {
-        n_above += k > prefix ? 1 : 0;
-        n_same += k == prefix ? 1 : 0;
-    });
+    int above_before = 0, same_before = 0;
+    each(0, steps, [&](int i, u32x4_t k) {
+        const bool here = i - lo >= first * (kWave * 4);
 #pragma unroll
-    for (int m = 1; m < kWave; m *= 2) {
-        n_above += __shfl_xor(n_above, m, kWave);
-        n_same += __shfl_xor(n_same, m, kWave);
-    }
+        for (int e = 0; e < 4; ++e) {
+            n_above += __popcll(__ballot(k[e] > prefix));
+            n_same += __popcll(__ballot(k[e] == prefix));
+        }
+        above_before = here ? above_before : n_above;
+        same_before = here ? same_before : n_same;
+    });
     if (lane == 0) {
         s_wave[1][wave] = n_above;
         s_wave[2][wave] = n_same;
     }
     __syncthreads();
-    int at = 0, seen = 0;
+    int seen = __builtin_amdgcn_readfirstlane(waves_before(s_wave[2])) + same_before;
+    int at = __builtin_amdgcn_readfirstlane(waves_before(s_wave[1])) + above_before + min(seen, left);
+    each(first, end, [&](int i, u32x4_t k) {
+        // ties: the first of them in the lanes before, then in this lane's order
+        bool keep[4];
+        uint64_t same[4];
+        bool any = false;
 #pragma unroll
-    for (int v = 0; v < kSelectWaves; ++v) {
-        at += v < wave ? s_wave[1][v] : 0;
-        seen += v < wave ? s_wave[2][v] : 0;
-    }
-    at += min(seen, left);
-    each([&](int i, uint32_t k) {
-        uint64_t keep = __ballot(k > prefix);
-        const uint64_t same = __ballot(k == prefix);
-        if (same != 0) {
-            keep |= __ballot(k == prefix && seen + (int)lanes_below(same) < left);
-            seen += __popcll(same);
+        for (int e = 0; e < 4; ++e) {
+            keep[e] = k[e] > prefix;
+            same[e] = __ballot(k[e] == prefix);
+            any |= same[e] != 0;
         }
-        if ((keep >> lane) & 1) {
-            const int to = at + (int)lanes_below(keep);
-            kept[to] = i;
-            nw[to] = weight_of_key(k);
+        if (any) {
+            int tie = seen;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                tie += (int)lanes_below(same[e]);
+                seen += __popcll(same[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                keep[e] = keep[e] || (k[e] == prefix && tie < left);
+                tie += k[e] == prefix ? 1 : 0;
+            }
         }
-        at += __popcll(keep);
+        int to = at;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint64_t m = __ballot(keep[e]);
+            to += (int)lanes_below(m);
+            at += __popcll(m);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (keep[e]) {
+                kept[to] = i + e;
+                nw[to] = weight_of_key(k[e]);
+                ++to;
+            }
     });
 }
 
@@ -906,9 +953,13 @@ extern "C" int fgqa_kv_evict(const fgqa_kv_evict_args* a, void* stream) {
     p.pages = (int)ceil_div(most, a->cache.page_size);
     p.items = (uint32_t)((int64_t)a->batch * p.pages * 2 * p.c.hkv);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)a->batch * (unsigned)p.c.hkv), block(kSelectThreads);
-    if (a->max_seqlen <= 8 * kSelectThreads) hipLaunchKernelGGL(select_kernel<8>, grid, block, 0, s, p);
-    else if (a->max_seqlen <= 32 * kSelectThreads) hipLaunchKernelGGL(select_kernel<32>, grid, block, 0, s, p);
+    const int64_t rows = (int64_t)a->batch * p.c.hkv;
+    const int cus = device_cu_count();
+    if (cus <= 0) return FGQA_ERR_HIP;
+    p.parts = (int)std::max<int64_t>(1, std::min(cus / rows, ceil_div(a->max_seqlen, 4 * kSelectThreads)));
+    const dim3 grid((unsigned)(rows * p.parts)), block(kSelectThreads);
+    if (a->max_seqlen <= 8 * kSelectThreads) hipLaunchKernelGGL(select_kernel<8 * kSelectThreads>, grid, block, 0, s, p);
+    else if (a->max_seqlen <= 32 * kSelectThreads) hipLaunchKernelGGL(select_kernel<32 * kSelectThreads>, grid, block, 0, s, p);
     else hipLaunchKernelGGL(select_kernel<0>, grid, block, 0, s, p);
     if (p.items > 0) {
         const int page = a->cache.page_size;

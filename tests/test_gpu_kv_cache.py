@@ -652,6 +652,46 @@ def test_evict_long_row(cuda):
     assert got[0] is lens and got[1] is out and got[2] is kept
 
 
+@pytest.mark.parametrize("n", [8192, 8193, 20000, 32768, 32769])
+@pytest.mark.parametrize("ties", [False, True])
+def test_evict_few_rows(cuda, n, ties):
+    """Rows that several workgroups share, at the ends of what one holds, beside a
+    short sequence, one of candidates 1 past a multiple of 4 and one that is cut to its recent tokens."""
+    torch = _torch()
+    rng = np.random.default_rng(n)
+    lens = [n, 5 + 128, n - 2, 129]
+    budget, recent, P = 1999, 128, 512
+    width, nwidth = -(-n // P), -(-budget // P)
+    pages = 4 * (width + nwidth)
+    c = Cache(cuda, rng, "int8", pages, P, 1)
+    both = _table(rng, 4, width + nwidth, pages)
+    w = rng.integers(0, 9, size=(4, 1, n)) if ties else rng.exponential(size=(4, 1, n))
+    _evict(cuda, c, both[:, :width], both[:, width:], lens, torch.from_numpy(w.astype(np.float32)).to(cuda), budget, recent,
+           f"few rows n={n} ties={ties}")
+    w = torch.from_numpy(w[:, :, :n].astype(np.float32)).to(cuda)
+    for budget in (1, 130, n - 3):   # the candidates' last vector of 4 in every place
+        if -(-budget // P) <= nwidth:
+            _evict(cuda, c, both[:, :width], both[:, width:], lens, w, budget, min(budget, recent), f"n={n} budget={budget}")
+
+
+@pytest.mark.parametrize("cand", [1, 2, 3, 4, 5, 6, 7, 63, 257, 4095, 4097])
+def test_evict_candidates_past_the_last_vector(cuda, cand):
+    """Candidates in every place of the last 4; what lies behind them is larger."""
+    torch = _torch()
+    rng = np.random.default_rng(cand)
+    recent, P = 3, 64
+    n = cand + recent
+    budget = recent + max(1, cand // 2)
+    if budget >= n:
+        n, recent, budget = cand + 1, 1, 1
+    width, nwidth = -(-n // P), -(-budget // P)
+    c = Cache(cuda, rng, "e4m3", width + nwidth, P, 1)
+    both = _table(rng, 1, width + nwidth, width + nwidth)
+    w = rng.exponential(size=(1, 1, n + 5)).astype(np.float32)
+    w[:, :, n - recent:] = 1e30
+    _evict(cuda, c, both[:, :width], both[:, width:], [n], torch.from_numpy(w).to(cuda), budget, recent, f"candidates {cand}")
+
+
 def test_evict_pages_outside(cuda):
     """New pages outside the cache are not written; old entries are clamped."""
     torch = _torch()
