@@ -96,7 +96,9 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
 
     float m_run = -INFINITY;
     float l_run = 0.f;   // this lane's share of the rowsum of head l16
-    float vref = __uint_as_float(0x00800000u);   // largest |V scale| so far
+    // largest |V scale| so far, and 2^-112 at least: 2^14 / vref is a number (blocks
+    // of zeros have the scale 2^-126)
+    float vref = __uint_as_float(0x07800000u);
     f32x4_t oacc[8];
 #pragma unroll
     for (int db = 0; db < 8; ++db) oacc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};

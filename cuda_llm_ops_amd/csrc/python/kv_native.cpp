@@ -122,6 +122,11 @@ bool meet(const at::Tensor& a, const at::Tensor& b) {
     return reinterpret_cast<uintptr_t>(address(a)) < end(b) && reinterpret_cast<uintptr_t>(address(b)) < end(a);
 }
 
+// Caches that are written: not one memory for both (interleaved ones are two).
+void check_caches_apart(const at::Tensor& k, const at::Tensor& v) {
+    if (k.numel() > 0 && address(k) == address(v)) refuse("k_cache and v_cache must be apart");
+}
+
 // All tensors of a call live on one GPU.
 struct Device {
     int64_t index = -1;
@@ -314,6 +319,9 @@ PyObject* append(PyObject* const* o) {
     check_written(kc);
     check_written(vc);
     check_written_scales(o[7], o[8]);
+    check_caches_apart(kc, vc);
+    for (const at::Tensor* t : {&k, &v})
+        if (meet(*t, kc) || meet(*t, vc)) refuse("K and V must be apart from the caches");
     Device dev;
     for (const at::Tensor* t : {&k, &v, &kc, &vc, &table, &lens}) dev.add(*t);
     for (int i = 6; i < 9; ++i) dev.add_if(o[i]);
@@ -360,6 +368,7 @@ PyObject* decode(PyObject* const* o) {
         out = tensor(o[8], "out");
         if (out.scalar_type() != at::kBFloat16 || out.sizes() != q.sizes() || !kernel_ready(out))
             refuse("out must be a bf16 [B, Hq, D] tensor with contiguous rows");
+        check_written(out);
     }
     if (o[9] != Py_None) {
         const at::Tensor& lse = tensor(o[9], "lse");
@@ -428,6 +437,7 @@ PyObject* weights(PyObject* const* o) {
     a.max_seqlen = check_max_seqlen(o[8], tokens, std::min(tokens, W));
     if (W < a.max_seqlen) refuse("weights must hold max_seqlen tokens");
     check_written(w);
+    if (meet(w, lse) || meet(w, q) || meet(w, table) || meet(w, lens)) refuse("weights must be apart from the inputs");
     Device dev;
     for (const at::Tensor* t : {&q, &kc, &lse, &table, &lens, &w}) dev.add(*t);
     dev.add_if(o[7]);
@@ -475,6 +485,7 @@ PyObject* evict(PyObject* const* o) {
     check_written(kc);
     check_written(vc);
     check_written_scales(o[8], o[9]);
+    check_caches_apart(kc, vc);
     at::Tensor given[3];   // new_seqlens, new_weights, kept
     if (o[10] != Py_None) {
         given[0] = tensor(o[10], "new_seqlens");

@@ -274,7 +274,9 @@ def _paged_prepare(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_
 
 
 def _has_block_scales(k_cache, k_scale, v_scale) -> bool:
-    return isinstance(k_scale, torch.Tensor) or isinstance(v_scale, torch.Tensor) or k_cache.dtype == torch.int8
+    # (a tensor of one element that is no [num_pages, Hkv] stands for a number)
+    return k_cache.dtype == torch.int8 or any(
+        isinstance(s, torch.Tensor) and (s.numel() != 1 or s.shape == k_cache.shape[::2]) for s in (k_scale, v_scale))
 
 
 def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None, k_scale=1.0, v_scale=1.0,

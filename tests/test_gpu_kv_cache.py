@@ -331,6 +331,26 @@ def test_decode_garbage_outside_the_sequences(cuda, dtype):
         _decode(cuda, c, q, far, lens, f"garbage P={P} {dtype}")
 
 
+@pytest.mark.parametrize("dtype", ["e4m3", "int8"])
+@pytest.mark.parametrize("P", [4, 16, 64])
+def test_decode_blocks_of_zeros(cuda, P, dtype):
+    """Blocks of zeros, whose scale is 2^-126, alone and before and after others."""
+    rng = np.random.default_rng(75)
+    lens = [200, 3 * P, 150, 1]
+    width = -(-200 // P)
+    c = Cache(cuda, rng, dtype, 4 * width, P, 2)
+    table = _table(rng, 4, width, 4 * width)
+    zero = [table[0], table[1][:1], table[2][1:], table[3]]
+    for i in range(2):
+        for p in np.concatenate(zero):
+            c.t[i].view(_torch().uint8)[int(p)] = 0
+            c.s[i][int(p)] = 2.0 ** -126
+            c.n[i][p] = 0
+            c.sn[i][p] = 2.0 ** -126
+    o, _ = _decode(cuda, c, _x(rng, 4, 8, 128), table, lens, f"zeros P={P} {dtype}")
+    assert not o[0].any() and not o[3].any()
+
+
 def test_decode_strided_and_prepared(cuda):
     """Wider caches, scales and queries; an output view; a prepared launch."""
     torch = _torch()

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import cuda_llm_ops_amd as fg
-from cuda_llm_ops_amd import _lib
+from cuda_llm_ops_amd import _lib, flash_gqa
 from tests.test_host_sanitizers import HOST, ROOT, _build_and_run
 
 HEADER = os.path.join(ROOT, "include", "fgqa_kv.h")
@@ -205,6 +205,39 @@ def test_evict_refuses_outputs_over_inputs():
     wide = torch.zeros(2 * 4 * 48 + 10, dtype=torch.float32)
     with pytest.raises(ValueError, match="apart"):
         _evict(weights=wide[:384].view(2, 4, 48), new_weights=wide[10:].view(2, 4, 48))
+
+
+def test_refuses_written_tensors_over_others():
+    k = _cache(10, 16, 4, 128)
+    with pytest.raises(ValueError, match="apart"):
+        _append(k_cache=k, v_cache=k)
+    with pytest.raises(ValueError, match="apart"):
+        _evict(k_cache=k, v_cache=k)
+    k = _cache(10, 16, 4, 128, dtype=BF)
+    with pytest.raises(ValueError, match="apart"):
+        _append(k=k[:2, :3], k_cache=k, v_cache=k.clone(), k_scale=1.0, v_scale=1.0)
+    both = _cache(10, 2, 16, 4, 128)   # interleaved caches are two memories
+    with pytest.raises(ValueError, match="GPU"):
+        _append(k_cache=both[:, 0], v_cache=both[:, 1])
+    w = torch.zeros(2, 4, 80)
+    with pytest.raises(ValueError, match="apart"):
+        _weights(weights=w, lse=w[0, 0, :16].view(2, 8))
+    with pytest.raises(ValueError, match="overlap itself"):
+        _decode(out=torch.zeros(1, 8, 128, dtype=BF).expand(2, 8, 128))
+
+
+def test_scales_that_stand_for_a_number():
+    """Tensors of one element beside an fp8 cache of more blocks stay numbers; a cache
+    of one block takes them as its scales."""
+    c = _cache(10, 16, 4, 128, dtype=F8)
+    one = torch.tensor(0.5)
+    for s in (one, one.view(1), one.view(1, 1)):
+        assert not flash_gqa._has_block_scales(c, s, s)
+        assert not flash_gqa._has_block_scales(c, 1.0, s)
+    assert flash_gqa._has_block_scales(c[:1, :, :1], one.view(1, 1), one.view(1, 1))
+    assert flash_gqa._has_block_scales(c, torch.ones(10, 4), torch.ones(10, 4))
+    assert flash_gqa._has_block_scales(_cache(10, 16, 4, 128), 1.0, 1.0)
+    assert not flash_gqa._has_block_scales(c, 0.5, 2)
 
 
 def test_c_abi_refuses_null_arguments():
