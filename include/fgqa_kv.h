@@ -27,8 +27,8 @@ extern "C" {
  *   k_scales, v_scales   fp32 [num_pages, num_kv_heads], strides {page, head} in
  *             elements: the scale of each block, one page of one KV head, whose
  *             codes c stand for c * scale.  Both or neither (NULL); required
- *             with FGQA_KV_INT8, NULL with FGQA_KV_BF16.  Scales are finite and
- *             positive (the append and the eviction write powers of two).
+ *             with FGQA_KV_INT8, NULL with FGQA_KV_BF16.  Scales are positive
+ *             and at most 2^126 (the append and the eviction write powers of two).
  *   k_scale, v_scale     one scale for a whole FGQA_KV_FP8_E4M3 cache without
  *             block scales (finite, and above 0 where tokens are written);
  *             ignored otherwise.
@@ -98,7 +98,10 @@ int fgqa_kv_append(const fgqa_kv_append_args* args, void* stream);
  * q.c * k_scales[page][head] * scale, and O sums p * c * v_scales[page][head].
  * q, o, lse, block_table, seqlens, scale, split_tokens, workspace: as there.
  * Codes are widened exactly; P is rounded to fp16 (11 bits) for P.V, sums are
- * fp32.
+ * fp32.  Sequences are cut into splits of split_tokens or, where that is 0, as
+ * the batch's size asks: outputs may differ in rounding between batches, not
+ * between runs of one.  A call whose sequences run whole needs no workspace
+ * (fgqa_decode_blocks_workspace_bytes gives 0).
  */
 typedef struct fgqa_decode_blocks_args {
     fgqa_kv_cache cache;
@@ -167,6 +170,7 @@ int fgqa_kv_weights(const fgqa_kv_weights_args* args, void* stream);
  *   weights      fp32 [B, Hkv, at least max_seqlen], strides {b, h}
  *   new_weights  fp32 [B, Hkv, weights_len], strides {b, h}: the kept tokens'
  *                weights, then zeros to weights_len (>= max_seqlen)
+ *                (of older tokens, -0 as 0 and a NaN as some NaN)
  *   kept         int32 [B, Hkv, budget], contiguous; -1 past the kept tokens
  *   new_seqlens  int32 [B]: min(n, budget)
  *   block_table, seqlens, max_seqlen: as fgqa_decode_paged
