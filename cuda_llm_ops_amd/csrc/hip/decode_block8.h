@@ -21,7 +21,9 @@
 // lie side by side over its heads, and what limits the stream is how much of
 // them is read together (loads alone, 64-token pages in random order: 5.95,
 // 6.59 and 7.00 TB/s with 1, 2 and 4 heads a workgroup; one step or three in
-// flight per wave change nothing).
+// flight per wave change nothing).  The read stream bounds it: 64 sequences of up to
+// 32768 tokens, 64 / 8 heads, e4m3 pages of 64: 2155 MB in 327 us, 6.6 TB/s, and 4 to 7
+// for the combine.
 #pragma once
 
 #include "fgqa_device.h"

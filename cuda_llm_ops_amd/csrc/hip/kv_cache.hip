@@ -4,9 +4,8 @@
 // A block is one page of one KV head: page_size rows of 128 elements.  Blocks
 // in 8 bits hold codes c and one scale s, standing for s * c.  The scales that
 // are made here are powers of two, so that x / s is exact and a code has one
-// rounding, growing a block's scale rounds its int8 codes once more and its
-// e4m3 codes not at all (but where they become subnormal), and the result does
-// not depend on the order of anything.
+// rounding, and growing a block's scale rounds its int8 codes once more and its
+// e4m3 codes not at all (but where they become subnormal).
 #include <algorithm>
 #include <math.h>
 
@@ -125,7 +124,10 @@ struct AppendParams {
 };
 
 // One block per item: item = ((b * pages + j) * 2 + K or V) * hkv + head, heads
-// side by side as the new rows lie.
+// side by side as the new rows lie.  Memory bounds it: the rows stay in registers
+// between their maximum and their codes, so each is read once (pages of more than
+// 256 rows: twice).  2 x 16384 tokens of 8 heads into e4m3 pages of 64: 155 MB in 35 us,
+// 4.4 TB/s where a copy runs at 4.9.  64 single tokens: 4.5 us, a launch.
 template <int kCode, Scaling kScaling, typename Shape>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
     __shared__ float s_max[kWaves];
@@ -281,7 +283,9 @@ struct WeightsParams {
 // One wave per 64 tokens of one KV head, two steps of 32; the waves of a workgroup
 // take adjacent heads, so that a token's rows, which lie side by side, are read
 // together.  (64 tokens an item are never slower than more, and small calls fill
-// the chip; items of 32: 108 us for 92, 64 sequences of up to 16384.)  Rows are
+// the chip; items of 32: 108 us for 92, 64 sequences of up to 16384.)  Memory
+// bounds it: those 64 sequences, 64 / 8 heads, e4m3, 499 MB in 89 us, 5.6 TB/s; the
+// stores of the weights between the reads of K cost 13 of them.  Rows are
 // loaded whole (8 lanes of 16 bytes for codes, 16 for bf16), both steps at once,
 // and staged in LDS as they are.
 // S[h][t] = Q[h][:] . K[t][:] by v_mfma_f32_16x16x32_bf16 with the 16 query heads
@@ -721,7 +725,9 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
 }
 
 // Moves the kept tokens: one block of the new pages per item, as append_kernel,
-// its rows gathered through `kept` and the block table.
+// its rows gathered through `kept` and the block table.  Memory bounds it: 32
+// sequences cut to 4000 tokens, 8 heads, e4m3 pages of 64: 530 MB in 111 us, 4.8 TB/s,
+// the rate of a copy.
 template <int kCode, Scaling kScaling, typename Shape>
 __global__ __launch_bounds__(kThreads) void move_kernel(EvictParams p) {
     __shared__ float s_max[kWaves];

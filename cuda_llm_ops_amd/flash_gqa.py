@@ -274,9 +274,13 @@ def _paged_prepare(q, k_cache, v_cache, block_table, seqlens, scale, k_scale, v_
 
 
 def _has_block_scales(k_cache, k_scale, v_scale) -> bool:
+    if k_cache.dtype == torch.int8:
+        return True
+    if isinstance(k_scale, float) and isinstance(v_scale, float):
+        return False
     # (a tensor of one element that is no [num_pages, Hkv] stands for a number)
-    return k_cache.dtype == torch.int8 or any(
-        isinstance(s, torch.Tensor) and (s.numel() != 1 or s.shape == k_cache.shape[::2]) for s in (k_scale, v_scale))
+    return any(isinstance(s, torch.Tensor) and (s.numel() != 1 or s.shape == k_cache.shape[::2])
+               for s in (k_scale, v_scale))
 
 
 def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None, k_scale=1.0, v_scale=1.0,
