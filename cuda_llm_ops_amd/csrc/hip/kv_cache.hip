@@ -275,12 +275,14 @@ struct WeightsParams {
     const int32_t* block_table;
     int64_t bt_stride;
     const int32_t* seqlens;
-    int max_seqlen, group, chunks;
+    int max_seqlen, group;
+    int waves;        // of one (sequence, head)
     float scale;
-    uint32_t items;   // batch * chunks * hkv, below 2^31
+    uint32_t items;   // batch * waves * hkv
 };
 
-// One wave per 64 tokens of one KV head, two steps of 32; the waves of a workgroup
+// One wave per 64 tokens of one KV head (plan::weights_waves: or several such
+// items), two steps of 32; the waves of a workgroup
 // take adjacent heads, so that a token's rows, which lie side by side, are read
 // together.  (64 tokens an item are never slower than more, and small calls fill
 // the chip; items of 32: 108 us for 92, 64 sequences of up to 16384.)  Memory
@@ -294,7 +296,8 @@ struct WeightsParams {
 // dim inside the products is free as long as Q's is the same: lane group g4
 // takes the elements of the 16-byte pieces that it reads.
 // kSeg (32, 16 or 8): page segments as in the block-scaled decode; 0: any pages.
-template <int kCode, Scaling kScaling, int kSeg>
+// kTurns: a wave takes several items (the loop costs calls of an item a wave 1.5 to 3 %).
+template <int kCode, Scaling kScaling, int kSeg, bool kTurns>
 __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
     constexpr int kStep = 32;
     constexpr int kRowBytes = kCode == kCodeBf16 ? 256 : 128;
@@ -310,11 +313,11 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
     if (item >= p.items) return;
     const int kvh = (int)(item % (uint32_t)p.c.hkv);
     const uint32_t rest = item / (uint32_t)p.c.hkv;
-    const int b = (int)(rest / (uint32_t)p.chunks);
-    const int t_begin = (int)(rest % (uint32_t)p.chunks) * plan::kWeightsTokens;
-    const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
-    const int t_end = __builtin_amdgcn_readfirstlane(min(t_begin + plan::kWeightsTokens, len));
-    if (t_begin >= t_end) return;
+    const int b = (int)(rest / (uint32_t)p.waves);
+    const int first_item = (int)(rest % (uint32_t)p.waves);
+    const int len = __builtin_amdgcn_readfirstlane(min(max(p.seqlens[b], 0), p.max_seqlen));
+    const int n_items = (len + plan::kWeightsTokens - 1) / plan::kWeightsTokens;
+    if (first_item >= n_items) return;
 
     const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
     const int pmask = (1 << p.c.page_shift) - 1;
@@ -323,17 +326,22 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
     float* wrow = p.weights + b * p.w_b + kvh * p.w_h;
     unsigned char* kl = smem + wave * kStep * kStride;
     const int row = lane / kLanes, piece = lane % kLanes;
-    const int n_steps = (t_end - t_begin + kStep - 1) / kStep;
 
     // Segment l of the item (at most 8) has its page and scale in lane l.
     constexpr int kSegs = kSeg > 0 ? kStep / kSeg : 1;
     constexpr int kPer = kLoads / kSegs;
+    int t_begin = 0, t_end = 0;
     [[maybe_unused]] int seg_page = 0;
     [[maybe_unused]] float seg_scale = p.scale;
-    if constexpr (kSeg > 0) {
-        seg_page = min(max(bt[min(t_begin + kSeg * lane, t_end - 1) >> p.c.page_shift], 0), p.c.num_pages - 1);
-        if constexpr (kScaling == kBlocks) seg_scale *= scales[(int64_t)seg_page * p.c.scale_page[0]];
-    }
+    auto begin = [&](int item) {
+        t_begin = item * plan::kWeightsTokens;
+        t_end = min(t_begin + plan::kWeightsTokens, len);
+        if constexpr (kSeg > 0) {
+            seg_page = min(max(bt[min(t_begin + kSeg * lane, t_end - 1) >> p.c.page_shift], 0), p.c.num_pages - 1);
+            if constexpr (kScaling == kBlocks) seg_scale = p.scale * scales[(int64_t)seg_page * p.c.scale_page[0]];
+        }
+    };
+    begin(first_item);
     bf16x8_t qop[4];
     {
         const __bf16* qrow = p.q + b * p.q_b + (int64_t)(kvh * p.group + min(l16, p.group - 1)) * p.q_h;
@@ -450,11 +458,18 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
     static_assert(plan::kWeightsTokens == 2 * kStep, "two steps an item");
-    Step first, second;
-    load(0, first);
-    if (n_steps > 1) load(1, second);
-    compute(0, first);
-    if (n_steps > 1) compute(1, second);
+    for (int item = first_item;;) {
+        const bool two = t_begin + kStep < t_end;
+        Step first, second;
+        load(0, first);
+        if (two) load(1, second);
+        compute(0, first);
+        if (two) compute(1, second);
+        if constexpr (!kTurns) break;
+        item += p.waves;
+        if (item >= n_items) break;
+        begin(item);
+    }
 }
 
 // ---------------------------------------------------------------- evict
@@ -822,6 +837,7 @@ __global__ __launch_bounds__(kThreads) void move_kernel(EvictParams p) {
 // Calls f with the block shape for pages of page_size rows.
 template <typename F>
 void with_shape(int page_size, F&& f) {
+    static_assert(plan::kWavePageRows == 64, "larger pages take a workgroup");
     if (page_size <= 8) f(BlockShape<1, 1>{});
     else if (page_size <= 16) f(BlockShape<2, 1>{});
     else if (page_size <= 32) f(BlockShape<4, 1>{});
@@ -844,13 +860,19 @@ void launch_append(const AppendParams& p, int page_size, hipStream_t s) {
     });
 }
 
+template <int kCode, Scaling kScaling, bool kTurns>
+void launch_weights_pages(const WeightsParams& p, int page_size, hipStream_t s) {
+    const dim3 grid((unsigned)ceil_div(p.items, kWaves)), block(kThreads);
+    if (page_size >= 32) hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 32, kTurns>), grid, block, 0, s, p);
+    else if (page_size == 16) hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 16, kTurns>), grid, block, 0, s, p);
+    else if (page_size == 8) hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 8, kTurns>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 0, kTurns>), grid, block, 0, s, p);
+}
+
 template <int kCode, Scaling kScaling>
 void launch_weights(const WeightsParams& p, int page_size, hipStream_t s) {
-    const dim3 grid((unsigned)ceil_div(p.items, kWaves)), block(kThreads);
-    if (page_size >= 32) hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 32>), grid, block, 0, s, p);
-    else if (page_size == 16) hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 16>), grid, block, 0, s, p);
-    else if (page_size == 8) hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 8>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((weights_kernel<kCode, kScaling, 0>), grid, block, 0, s, p);
+    if ((int64_t)p.waves * plan::kWeightsTokens < p.max_seqlen) launch_weights_pages<kCode, kScaling, true>(p, page_size, s);
+    else launch_weights_pages<kCode, kScaling, false>(p, page_size, s);
 }
 
 template <int kCode, Scaling kScaling>
@@ -917,8 +939,8 @@ extern "C" int fgqa_kv_weights(const fgqa_kv_weights_args* a, void* stream) {
     p.seqlens = a->seqlens;
     p.max_seqlen = a->max_seqlen;
     p.group = a->num_q_heads / p.c.hkv;
-    p.chunks = (int)ceil_div(a->max_seqlen, plan::kWeightsTokens);
-    p.items = (uint32_t)((int64_t)a->batch * p.chunks * p.c.hkv);
+    p.waves = plan::weights_waves(a->batch, p.c.hkv, a->max_seqlen);
+    p.items = (uint32_t)((int64_t)a->batch * p.waves * p.c.hkv);
     const bool blocks = a->cache.k_scales != nullptr;
     const bool whole = a->cache.kv_dtype == FGQA_KV_FP8_E4M3 && !blocks;
     p.scale = a->scale * (whole ? a->cache.k_scale : 1.f);

@@ -68,7 +68,15 @@ int validate_cache_pointers(const fgqa_kv_cache& c, bool with_v) {
     return FGQA_OK;
 }
 
-bool grid_ok(i128 workgroups) { return workgroups < kLim31; }
+// A launch has fewer than 2^31 workgroups and 2^32 threads.
+bool grid_ok(i128 workgroups, int threads) {
+    return workgroups < kLim31 && workgroups * threads < ((i128)1 << 32);
+}
+
+// Blocks of the append's and the eviction's pages.
+bool blocks_ok(i128 blocks, int page_size) {
+    return blocks < kLim31 && grid_ok(page_size <= kWavePageRows ? (blocks + 3) / 4 : blocks, 256);
+}
 }  // namespace
 
 int validate_kv_append(const fgqa_kv_append_args* a) {
@@ -82,7 +90,8 @@ int validate_kv_append(const fgqa_kv_append_args* a) {
     const int64_t bn[1] = {a->batch};
     if (!extent_ok(n, a->k_new_stride) || !extent_ok(n, a->v_new_stride) || !extent_ok(bn, &a->block_table_stride))
         return FGQA_ERR_UNSUPPORTED;
-    if (!grid_ok((i128)a->batch * append_pages(a->max_new, a->cache.page_size) * 2 * a->cache.num_kv_heads))
+    if (!blocks_ok((i128)a->batch * append_pages(a->max_new, a->cache.page_size) * 2 * a->cache.num_kv_heads,
+                   a->cache.page_size))
         return FGQA_ERR_UNSUPPORTED;
     if (a->batch == 0 || a->max_new == 0 || a->max_pages == 0) return FGQA_OK;
     if (a->k_new == nullptr || a->v_new == nullptr || a->block_table == nullptr || a->seqlens == nullptr)
@@ -114,8 +123,10 @@ int validate_kv_weights(const fgqa_kv_weights_args* a) {
     const int64_t bn[1] = {a->batch};
     if (!extent_ok(qn, a->q_stride) || !extent_ok(wn, ws) || !extent_ok(bn, &a->block_table_stride))
         return FGQA_ERR_UNSUPPORTED;
-    if (!grid_ok((i128)a->batch * a->cache.num_kv_heads * ceil_div(a->max_seqlen, kWeightsTokens))) return FGQA_ERR_UNSUPPORTED;
     if (a->batch == 0 || a->max_seqlen == 0) return FGQA_OK;
+    if (!grid_ok(((i128)a->batch * a->cache.num_kv_heads * weights_waves(a->batch, a->cache.num_kv_heads, a->max_seqlen) + 3) / 4,
+                 256))
+        return FGQA_ERR_UNSUPPORTED;
     if (a->q == nullptr || a->lse == nullptr || a->weights == nullptr || a->block_table == nullptr ||
         a->seqlens == nullptr)
         return FGQA_ERR_INVALID_ARGUMENT;
@@ -148,7 +159,8 @@ int validate_kv_evict(const fgqa_kv_evict_args* a) {
         !extent_ok(bn, &a->new_block_table_stride) ||
         (i128)a->batch * a->cache.num_kv_heads * a->budget >= ((i128)1 << 60))
         return FGQA_ERR_UNSUPPORTED;
-    if (!grid_ok((i128)a->batch * a->cache.num_kv_heads * 2 * (ceil_div(most, a->cache.page_size) + 1)))
+    const i128 rows = (i128)a->batch * a->cache.num_kv_heads;
+    if (!grid_ok(rows, 1024) || !blocks_ok(rows * 2 * ceil_div(most, a->cache.page_size), a->cache.page_size))
         return FGQA_ERR_UNSUPPORTED;
     if (a->batch == 0) return FGQA_OK;
     if (a->seqlens == nullptr || a->new_seqlens == nullptr || a->kept == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
@@ -221,18 +233,16 @@ int plan_blocks(const fgqa_decode_paged_args* a, int cus, DecodePlan* plan) {
     fgqa_decode_paged_args split = *a;
     if (a->split_tokens == 0)
         split.split_tokens = blocks_split(a->batch, a->num_kv_heads, a->max_seqlen, cus > 0 ? cus : 256);
-    int st;
-    if (split.split_tokens > 0) {
-        st = plan_paged(&split, plan);
-        if (st != FGQA_OK) return st;
-        plan->list = false;
-        plan->ws_bytes = plan->least_bytes = plan->part_o_bytes + plan->part_ml_bytes;
-    } else {
-        st = plan_paged(a, plan, block_item_slots(a->num_kv_heads));
-        if (st != FGQA_OK) return st;
+    const int st = split.split_tokens > 0 ? plan_paged(&split, plan) : plan_paged(a, plan, block_item_slots(a->num_kv_heads));
+    if (st != FGQA_OK) return st;
+    const bool splits = grid_ok((i128)a->batch * plan->nsplit * a->num_kv_heads, 512);
+    if (plan->teams > 0) {
+        if (!splits) plan->least_bytes = plan->ws_bytes;   // teams or nothing
+        return FGQA_OK;
     }
-    // workgroups of the split form
-    return grid_ok((i128)a->batch * plan->nsplit * a->num_kv_heads) ? FGQA_OK : FGQA_ERR_UNSUPPORTED;
+    plan->list = false;
+    plan->ws_bytes = plan->least_bytes = plan->part_o_bytes + plan->part_ml_bytes;
+    return splits ? FGQA_OK : FGQA_ERR_UNSUPPORTED;
 }
 
 int validate_decode_blocks(const fgqa_decode_blocks_args* a) {

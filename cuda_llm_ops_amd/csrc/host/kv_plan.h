@@ -45,5 +45,20 @@ inline int64_t append_pages(int64_t max_new, int64_t page_size) { return (max_ne
 
 constexpr int kWeightsTokens = 64;   // of a wave's item in the weights kernel
 
+// Waves of one (sequence, KV head) in the weights kernel, each of which takes every
+// so many-th item: one an item, but kWeightsWaves in all (where a batch needs no
+// more than one each).  What decides is a capacity far above the lengths, whose
+// empty waves only end: 64 sequences of up to 2048 tokens, 8 heads, take 17 us with
+// max_seqlen 2048, and with 131072 took 100 at an item a wave.
+constexpr int64_t kWeightsWaves = 1 << 17;
+inline int weights_waves(int64_t batch, int64_t num_kv_heads, int64_t max_seqlen) {
+    const int64_t items = ceil_div(max_seqlen, kWeightsTokens), rows = batch * num_kv_heads;
+    const int64_t most = rows >= kWeightsWaves ? 1 : kWeightsWaves / rows;
+    return (int)(items < most ? items : most);
+}
+
+// A block of the append and the eviction is a wave's, or a workgroup's of 4.
+constexpr int kWavePageRows = 64;
+
 }  // namespace plan
 }  // namespace fgqa

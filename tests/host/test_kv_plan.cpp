@@ -275,7 +275,12 @@ static void test_weights() {
     WEIGHTS(a.batch = 0; a.q = nullptr, OK);
     WEIGHTS(a.max_seqlen = 0; a.weights = nullptr, OK);
     WEIGHTS(a.max_seqlen = INT_MAX; a.block_table_stride = INT_MAX, NOT);
-    WEIGHTS(a.batch = 1 << 20; a.max_seqlen = 64 << 8; a.block_table_stride = 1 << 20, NOT);   // 2^31 items
+    WEIGHTS(a.batch = 1 << 20; a.max_seqlen = 64 << 8; a.block_table_stride = 1 << 20, OK);   // a wave a row
+    WEIGHTS(a.batch = (1 << 23) - 1, OK);
+    WEIGHTS(a.batch = 1 << 23, NOT);   // 2^32 threads
+    CHECK(plan::weights_waves(1, 1, 1) == 1 && plan::weights_waves(1, 1, 65) == 2 && plan::weights_waves(64, 8, 16384) == 256);
+    CHECK(plan::weights_waves(64, 8, 16385) == 256 && plan::weights_waves(3, 8, 1 << 30) == (1 << 17) / 24);
+    CHECK(plan::weights_waves(1 << 17, 1, 1 << 30) == 1 && plan::weights_waves(INT_MAX, INT_MAX, 1 << 30) == 1);
 }
 
 static void test_evict() {
@@ -300,6 +305,11 @@ static void test_evict() {
     EVICT(a.batch = 0; a.kept = nullptr, OK);
     EVICT(a.max_seqlen = 0; a.weights = nullptr; a.block_table = nullptr; a.cache.k = nullptr, OK);
     EVICT(a.batch = INT_MAX, NOT);
+    EVICT(a.batch = (1 << 19) - 1, OK);
+    EVICT(a.batch = 1 << 19, NOT);                                               // rows of 1024 threads
+    EVICT(a.batch = 1 << 18; a.max_seqlen = 0, OK);
+    EVICT(a.batch = 1 << 18; a.budget = 1 << 20; a.weights_len = a.max_seqlen = 16 * 16;
+          a.block_table_stride = a.new_block_table_stride = 1 << 20, NOT);       // 2^26 blocks of 16 rows
 }
 
 static void test_decode() {
@@ -442,8 +452,8 @@ static void fuzz() {
         CHECK(plan::validate_kv_evict(&e) <= 0);
         CHECK(fgqa_decode_blocks(&d, nullptr) <= 0);
         if (plan::validate_kv_weights(&w) == OK && w.batch > 0 && w.max_seqlen > 0) {
-            CHECK((__int128)w.batch * w.cache.num_kv_heads * ceil_div(w.max_seqlen, plan::kWeightsTokens) <
-                  ((int64_t)1 << 31));
+            const int waves = plan::weights_waves(w.batch, w.cache.num_kv_heads, w.max_seqlen);
+            CHECK(waves >= 1 && (__int128)w.batch * w.cache.num_kv_heads * waves * 64 < ((int64_t)1 << 32));
         }
     }
 }

@@ -557,6 +557,27 @@ def test_weights_heads(cuda, G, H, dtype):
     _weights(cuda, c, _x(rng, 2, G * H, 128), table, lens, lse, wide[:, 1:, 3:], f"heads {G} {H} {dtype}")
 
 
+@pytest.mark.parametrize("dtype,P", [("int8", 8), ("bf16", 4), ("e4m3", 64)])
+def test_weights_several_items_a_wave(cuda, dtype, P):
+    """More items than waves: a sequence's waves take items in turn, up to its length."""
+    torch = _torch()
+    rng = np.random.default_rng(130)
+    B, W = 1024, 4500   # 64 waves a row: 4096 tokens
+    lens = rng.integers(0, 4, size=B)
+    lens[[3, 500, 1023]] = (4500, 4096, 4161)
+    width = -(-W // P)
+    need = [-(-int(n) // P) for n in lens]
+    pages = sum(need) + 1
+    c = Cache(cuda, rng, dtype, pages, P, 2, scales=dtype != "bf16")
+    table, at = np.full((B, width), -1, np.int32), rng.permutation(pages)
+    for b, n in enumerate(need):
+        table[b, :n], at = at[:n], at[n:]
+    q = _x(rng, B, 4, 128)
+    lse = torch.from_numpy(rng.uniform(3, 12, size=(B, 4)).astype(np.float32)).to(cuda)
+    w = torch.from_numpy(rng.uniform(0, 1, size=(B, 2, W)).astype(np.float32)).to(cuda)
+    _weights(cuda, c, q, table, lens.tolist(), lse, w, f"several items {dtype} P={P}", max_seqlen=W)
+
+
 def test_weights_sum_to_the_query_heads(cuda):
     """With the decode's LSE the weights of a step are a softmax's: they add up to
     G; a long sequence and one of a single token."""
