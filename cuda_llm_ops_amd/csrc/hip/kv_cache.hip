@@ -537,8 +537,9 @@ __device__ __forceinline__ void fill_row(T* dst, int from, int to, T value, int 
 // histograms would take a launch for each pass, about what a pass takes; but
 // where there are fewer rows than CUs, `parts` workgroups find the same
 // threshold, and each writes its part of every wave's steps.  8 rows of 32K: 17.2
-// us (22.1 in one part), 256 of 8K 13.7, 4 of 600 7.1, 3 launches' worth of
-// latency: loads, three scans, stores.
+// us (22.1 in one part), 256 of 8K 13.2, 4 of 600 6.9: the latency of loads, three
+// histograms and their scans, and stores (the passes in a loop of one body: 0.8 us
+// more).
 template <int kHeld>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     __shared__ __attribute__((aligned(16))) uint32_t s_keys[kHeld > 0 ? kHeld : 4];
@@ -678,7 +679,8 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     }
 
     // of this wave, and before its steps of this part
-    const int first = (int)((int64_t)part * steps / p.parts), end = (int)((int64_t)(part + 1) * steps / p.parts);
+    const int first = p.parts == 1 ? 0 : (int)((unsigned)(part * steps) / (unsigned)p.parts);
+    const int end = p.parts == 1 ? steps : (int)((unsigned)((part + 1) * steps) / (unsigned)p.parts);
     int n_above = 0, n_same = 0;
     int above_before = 0, same_before = 0;
     each(0, steps, [&](int i, u32x4_t k) {
