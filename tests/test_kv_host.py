@@ -12,7 +12,7 @@ import pytest
 import torch
 
 import cuda_llm_ops_amd as fg
-from cuda_llm_ops_amd import _lib, flash_gqa
+from cuda_llm_ops_amd import _lib, flash_gqa, kv_cache
 from tests.test_host_sanitizers import HOST, ROOT, _build_and_run
 
 HEADER = os.path.join(ROOT, "include", "fgqa_kv.h")
@@ -269,3 +269,32 @@ def test_arguments_of_other_types():
         _append(block_table=torch.zeros(2, 5, dtype=torch.int32).to_sparse())
     with pytest.raises(TypeError, match="arguments"):
         fg.native().append(1, 2)
+
+
+def test_calls_for_another_device(monkeypatch):
+    """A call whose tensors live on another device runs again with that one current."""
+    seen, now = [], [0]
+
+    class Native:
+        @staticmethod
+        def append(*args):
+            seen.append((now[0], args))
+            return NotImplemented if now[0] != 1 else None
+
+    class Current:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            now[0] = self.device
+
+        def __exit__(self, *_):
+            now[0] = 0
+
+    class On1:
+        device = 1
+
+    monkeypatch.setattr(_lib, "native", lambda: Native)
+    monkeypatch.setattr(torch.cuda, "device", Current)
+    assert kv_cache.call_native("append", On1, 3, 4) is None
+    assert seen == [(0, (3, 4)), (1, (3, 4))] and now == [0]
