@@ -854,6 +854,52 @@ def test_two_streams_at_once(cuda):
                 assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("teams", [False, True])
+def test_two_graphs_at_once(cuda, teams):
+    """Two captured decodes (in splits or over teams, merged through a workspace) and
+    evictions (a row shared by several workgroups), replayed on two streams at once
+    with eager work between the replays."""
+    torch = _torch()
+    fg = _fg()
+    rng = np.random.default_rng(330)
+    P, n = 64, 9000
+    c = Cache(cuda, rng, "int8", 2 * 180, P, 4)
+    both = _table(rng, 2, 180, 360)
+    tables = [_for_teams(cuda, both[i:i + 1, :141], P, 4) if teams else both[i:i + 1, :141] for i in range(2)]
+    args = [(_x(rng, 1, 16, 128).to(cuda), _i32(cuda, tables[i]), _i32(cuda, [n - 77 * i]), _i32(cuda, both[i:i + 1, 141:]))
+            for i in range(2)]
+    w = torch.from_numpy(rng.exponential(size=(2, 4, n)).astype(np.float32)).to(cuda)
+
+    def work(i):
+        q, table, lens, new = args[i]
+        o = fg.decode_flash_gqa_paged(q, c.t[0], c.t[1], table, lens, **c.scales)
+        return (o,) + fg.evict_kv_paged(c.t[0], c.t[1], table, lens, w[i:i + 1], new, budget=2000, recent=100,
+                                        max_seqlen=n, **c.scales)
+
+    alone = [work(0), work(1)]
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g):
+            outs.append(work(i))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for r in range(6):
+        for got in outs:
+            for x in got:
+                x.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(alone, outs):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y), f"replay {r}"
+        for a, b in zip(alone, [work(0), work(1)]):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y)
+
+
 # ------------------------------------------------------------------ C++ operator layer
 def test_cplusplus_entry_points(cuda):
     """The C++ entry points on the default stream against the Python functions: the same bits."""
