@@ -385,9 +385,9 @@ def test_decode_same_bits_as_the_whole_cache_scale(cuda):
     assert (whole.float() - blocks.float()).abs().max() <= v * (2.0 ** -8 + 2.0 ** -11) + 2 * 2.0 ** -8 * blocks.float().abs().max()
 
 
-@pytest.mark.parametrize("teams", [False, True])
+@pytest.mark.parametrize("form", ["whole", "splits", "teams"])
 @pytest.mark.parametrize("P", [4, 16, 64])
-def test_decode_scores_of_minus_infinity(cuda, P, teams):
+def test_decode_scores_of_minus_infinity(cuda, P, form):
     """Keys whose scores overflow to -inf get nothing, wherever they lie; a row of
     such keys alone is NaN, as the formula has it."""
     torch = _torch()
@@ -407,8 +407,9 @@ def test_decode_scores_of_minus_infinity(cuda, P, teams):
     q[:, 0, :] = 0.0
     q[:, 0, 7] = 3e38
     lse = torch.empty((2, 2), device=cuda)
-    of = _for_teams(cuda, table, P, 1) if teams else table
-    o = _fg().decode_flash_gqa_paged(q.to(cuda), c.t[0], c.t[1], _i32(cuda, of), _i32(cuda, lens), lse=lse, **c.scales)
+    of = _for_teams(cuda, table, P, 1) if form == "teams" else table
+    o = _fg().decode_flash_gqa_paged(q.to(cuda), c.t[0], c.t[1], _i32(cuda, of), _i32(cuda, lens), lse=lse,
+                                     split_tokens=128 if form == "splits" else 0, **c.scales)
     torch.cuda.synchronize()
     v = ref.gather(c.n[1], c.sn[1], table, 0, 300, 0)[alive].mean(axis=0)
     size = np.abs(ref.gather(c.n[1], c.sn[1], table, 0, 300, 0)[alive]).mean(axis=0)
