@@ -5,9 +5,11 @@
 // (one scale per page and KV head),
 //     s_t = scale sK(t) (q . c_K[t]),   o = sum_t softmax(s)_t sV(t) c_V[t].
 // Codes are widened exactly (to bf16 for K, fp16 for V).  sK multiplies the
-// scores in fp32.  sV is folded into P, relative to the largest sV met so far
-// (vref), and P sV / vref is rounded to fp16 at 2^14 times its value: 11 bits
-// where the bf16 decode keeps 8, and no loss down to 2^-29 of the largest P.
+// scores in fp32.  sV is folded into P in fp32, and P sV is rounded to fp16 at 2^14
+// times its ratio to the head's largest P sV so far (vref): 11 bits where the bf16
+// decode keeps 8, and no less down to 2^-28 of that largest.  (Relative to the
+// largest sV instead, a block of a far larger scale took the bits of the tokens that
+// get the attention, whatever it got itself.)
 //
 // K and V rows are loaded whole, 8 lanes of 16 bytes a row, and staged in LDS
 // as codes, half the bytes of bf16 rows.  (Reading K's MFMA operand straight
@@ -98,9 +100,10 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
 
     float m_run = -INFINITY;
     float l_run = 0.f;   // this lane's share of the rowsum of head l16
-    // largest |V scale| so far, and 2^-112 at least: 2^14 / vref is a number (blocks
-    // of zeros have the scale 2^-126)
-    float vref = __uint_as_float(0x07800000u);
+    // head l16's largest P sV so far, P relative to m_run, and 2^-112 at least: 2^14 /
+    // vref is a number (blocks of zeros have the scale 2^-126)
+    constexpr uint32_t kLeastRef = 0x07800000u;
+    float vref = __uint_as_float(kLeastRef);
     f32x4_t oacc[8];
 #pragma unroll
     for (int db = 0; db < 8; ++db) oacc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -222,7 +225,6 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         }
         // scales of tokens t0 + 16*tb + 4*g4 + i
         float ks[8], vs[8];
-        float vmax = vref;
         if constexpr (kSeg > 0) {
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb) {
@@ -236,17 +238,13 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
                     vs[4 * tb + i] = v1;
                 }
             }
-#pragma unroll
-            for (int g = 0; g < kSegs; ++g) vmax = fmaxf(vmax, fabsf(vs_seg[g]));
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int at = 16 * (j / 4) + 4 * g4 + j % 4;
                 ks[j] = sl[at] * p.scale_log2;
                 vs[j] = sl[kDecStep + at];
-                vmax = fmaxf(vmax, fabsf(vs[j]));
             }
-            vmax = groups_max(vmax);
         }
 
         // Online softmax for head l16 over tokens t0 + 16*tb + 4*g4 + i.
@@ -266,22 +264,29 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         // (-inf, no score above it yet: what is subtracted has to be a number)
         const float m_sub = m_new == -INFINITY ? 0.f : m_new;
         const float alpha = fast_exp2(m_run - m_sub);
-        const float vinv = __builtin_amdgcn_rcpf(vmax);
-        // (exactly 1 where nothing changed: vref * (1 / vref) need not be)
-        const float oalpha = alpha * (vmax > vref ? vref * vinv : 1.f);
-        const float pscale = vinv * kDec8PScale;
         float psum = 0.f;
-        f16x8_t pop;
+        float pv[8], pmax = __uint_as_float(kLeastRef);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float pv = fast_exp2(y[j] - m_sub);
-            psum += pv;
-            pop[j] = (_Float16)(pv * (vs[j] * pscale));
+            const float e = fast_exp2(y[j] - m_sub);
+            psum += e;
+            pv[j] = e * vs[j];
+            pmax = fmaxf(pmax, pv[j]);
         }
+        pmax = groups_max(pmax);
+        // The sums so far are relative to vref, which a larger m_run lowers with them:
+        // only a larger P sV rescales them (or vref at its least).
+        const float vold = vref * alpha;
+        vref = fmaxf(vold, pmax);
+        const float vinv = __builtin_amdgcn_rcpf(vref);
+        // (exactly 1 where nothing changed: vref * (1 / vref) need not be)
+        const float oalpha = vref > vold ? vold * vinv : 1.f;
+        f16x8_t pop;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pop[j] = (_Float16)(pv[j] * (vinv * kDec8PScale));
         l_run = l_run * alpha + psum;
         m_run = m_new;
-        vref = vmax;
-        // (most steps raise neither maximum)
+        // (most steps raise no head's largest)
         if (__any(oalpha != 1.f)) {
 #pragma unroll
             for (int db = 0; db < 8; ++db) oacc[db] *= oalpha;
