@@ -5,11 +5,12 @@
 // (one scale per page and KV head),
 //     s_t = scale sK(t) (q . c_K[t]),   o = sum_t softmax(s)_t sV(t) c_V[t].
 // Codes are widened exactly (to bf16 for K, fp16 for V).  sK multiplies the
-// scores in fp32.  sV is folded into P in fp32, and P sV is rounded to fp16 at 2^14
-// times its ratio to the head's largest P sV so far (vref): 11 bits where the bf16
-// decode keeps 8, and no less down to 2^-28 of that largest.  (Relative to the
+// scores in fp32.  sV is folded into P in fp32, and P sV, at 2^14 times its ratio to
+// the head's largest so far (vref), is held in two fp16 numbers, its rounding and
+// what that leaves: 22 bits, and down to 2^-39 of the largest.  (Relative to the
 // largest sV instead, a block of a far larger scale took the bits of the tokens that
-// get the attention, whatever it got itself.)
+// get the attention, whatever it got itself.  One fp16 number alone moves one bf16
+// output in a dozen to its neighbour; the second one's MFMAs run beside the loads.)
 //
 // K and V rows are loaded whole, 8 lanes of 16 bytes a row, and staged in LDS
 // as codes, half the bytes of bf16 rows.  (Reading K's MFMA operand straight
@@ -281,9 +282,13 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         const float vinv = __builtin_amdgcn_rcpf(vref);
         // (exactly 1 where nothing changed: vref * (1 / vref) need not be)
         const float oalpha = vref > vold ? vold * vinv : 1.f;
-        f16x8_t pop;
+        f16x8_t pop, plo;   // P sV: rounded, and the rest
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pop[j] = (_Float16)(pv[j] * (vinv * kDec8PScale));
+        for (int j = 0; j < 8; ++j) {
+            const float x = pv[j] * (vinv * kDec8PScale);
+            pop[j] = (_Float16)x;
+            plo[j] = (_Float16)(x - (float)pop[j]);
+        }
         l_run = l_run * alpha + psum;
         m_run = m_new;
         // (most steps raise no head's largest)
@@ -298,10 +303,19 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
         const int row = l16 >> 1;
         const unsigned char* vsrc =
             vl + (4 * g4 + (row & 3) + 16 * (row >> 2)) * kDec8RowStride + 8 * (l16 & 1);
+        // (4 columns at a time: a column's second product waits for its first)
 #pragma unroll
-        for (int db = 0; db < 8; ++db) {
-            const u32x2_t c = lds_read_tr8(vsrc + 16 * db);
-            oacc[db] = mfma16_f16(codes_to_f16<kCode>(c[0], c[1]), pop, oacc[db]);
+        for (int d4 = 0; d4 < 8; d4 += 4) {
+            f16x8_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u32x2_t c = lds_read_tr8(vsrc + 16 * (d4 + i));
+                v[i] = codes_to_f16<kCode>(c[0], c[1]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) oacc[d4 + i] = mfma16_f16(v[i], pop, oacc[d4 + i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) oacc[d4 + i] = mfma16_f16(v[i], plo, oacc[d4 + i]);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();

@@ -97,8 +97,8 @@ int fgqa_kv_append(const fgqa_kv_append_args* args, void* stream);
  * fgqa_decode_paged over a cache with block scales (e4m3 or int8): scores use
  * q.c * k_scales[page][head] * scale, and O sums p * c * v_scales[page][head].
  * q, o, lse, block_table, seqlens, scale, split_tokens, workspace: as there.
- * Codes are widened exactly; P is rounded to fp16 (11 bits) for P.V, sums are
- * fp32.  Sequences are cut into splits of split_tokens or, where that is 0, as
+ * Codes are widened exactly; P times the V scale is held in two fp16 numbers (22
+ * bits) for P.V, sums are fp32.  Sequences are cut into splits of split_tokens or, where that is 0, as
  * the batch's size asks: outputs may differ in rounding between batches, not
  * between runs of one.  A call whose sequences run whole needs no workspace
  * (fgqa_decode_blocks_workspace_bytes gives 0).
