@@ -353,17 +353,21 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
             qop[kk] = as_bf16x8(l16 < p.group ? t : zero);
         }
     }
-    // Heads past the group are left out of the sum (their products are 0 * k, NaN
-    // where a bf16 key holds an infinity).  (exp(s - lse): the difference is formed
-    // before log2(e) is multiplied in: its rounding then is relative to the small
-    // exponents of the weights that count, not to the LSE's size.)
+    // Heads past the group: exp(. - inf) = 0.  Their products are 0 * k, NaN where a
+    // bf16 key holds an infinity, so bf16 ones are also left out of the sum.  (8-bit
+    // keys hold none, and with a NaN the other heads' are NaN too.  Left out there
+    // as well, 64 sequences of up to 16384 take 90.7 us for 88.6.)
+    // (The difference is formed before log2(e) is multiplied in: its rounding then
+    // is relative to the small exponents of the weights that count, not to the
+    // LSE's size.)
     float neg_lse[4];
-    bool in_group[4];
+    [[maybe_unused]] bool in_group[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int g = 4 * g4 + i;
+        const float l = p.lse[(int64_t)b * p.c.hkv * p.group + kvh * p.group + min(g, p.group - 1)];
         in_group[i] = g < p.group;
-        neg_lse[i] = -p.lse[(int64_t)b * p.c.hkv * p.group + kvh * p.group + min(g, p.group - 1)];
+        neg_lse[i] = in_group[i] ? -l : -INFINITY;
     }
 
     struct Step {
@@ -450,7 +454,7 @@ __global__ __launch_bounds__(kThreads) void weights_kernel(WeightsParams p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float e = fast_exp2(fmaf(c[i], scale[tb], neg_lse[i]) * kLog2e);
-                sum[tb] += in_group[i] ? e : 0.f;
+                sum[tb] += kCode != kCodeBf16 || in_group[i] ? e : 0.f;
             }
         }
         // over the lane groups: groups 0 and 1 get the sums of tokens l16 and 16 + l16
