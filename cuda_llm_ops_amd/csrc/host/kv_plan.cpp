@@ -68,6 +68,11 @@ int validate_cache_pointers(const fgqa_kv_cache& c, bool with_v) {
     return FGQA_OK;
 }
 
+// K's and V's data and block scales, which the call writes, are not the same memory.
+bool written_apart(const fgqa_kv_cache& c) {
+    return c.k != c.v && (c.k_scales == nullptr || c.k_scales != c.v_scales);
+}
+
 // A launch has fewer than 2^31 workgroups and 2^32 threads.
 bool grid_ok(i128 workgroups, int threads) {
     return workgroups < kLim31 && workgroups * threads < ((i128)1 << 32);
@@ -101,7 +106,9 @@ int validate_kv_append(const fgqa_kv_append_args* a) {
         return FGQA_ERR_UNSUPPORTED;
     for (int i = 0; i < 3; ++i)
         if ((a->k_new_stride[i] & 7) || (a->v_new_stride[i] & 7)) return FGQA_ERR_UNSUPPORTED;
-    return validate_cache_pointers(a->cache, true);
+    const int pointers = validate_cache_pointers(a->cache, true);
+    if (pointers != FGQA_OK) return pointers;
+    return written_apart(a->cache) ? FGQA_OK : FGQA_ERR_INVALID_ARGUMENT;
 }
 
 int validate_kv_weights(const fgqa_kv_weights_args* a) {
@@ -173,7 +180,9 @@ int validate_kv_evict(const fgqa_kv_evict_args* a) {
     if (a->weights == nullptr || a->block_table == nullptr || a->new_block_table == nullptr)
         return FGQA_ERR_INVALID_ARGUMENT;
     if (!aligned4(a->weights) || !aligned4(a->block_table) || !aligned4(a->new_block_table)) return FGQA_ERR_UNSUPPORTED;
-    return validate_cache_pointers(a->cache, true);
+    const int pointers = validate_cache_pointers(a->cache, true);
+    if (pointers != FGQA_OK) return pointers;
+    return written_apart(a->cache) ? FGQA_OK : FGQA_ERR_INVALID_ARGUMENT;
 }
 
 fgqa_decode_paged_args as_decode_paged(const fgqa_decode_blocks_args* a) {

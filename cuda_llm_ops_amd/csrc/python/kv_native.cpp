@@ -26,6 +26,7 @@
 #include <utility>
 #include <vector>
 
+#include "../host/kv_apart.h"
 #include "fgqa_kv.h"
 
 namespace {
@@ -122,9 +123,22 @@ bool meet(const at::Tensor& a, const at::Tensor& b) {
     return reinterpret_cast<uintptr_t>(address(a)) < end(b) && reinterpret_cast<uintptr_t>(address(b)) < end(a);
 }
 
-// Caches that are written: not one memory for both (interleaved ones are two).
-void check_caches_apart(const at::Tensor& k, const at::Tensor& v) {
-    if (k.numel() > 0 && address(k) == address(v)) refuse("k_cache and v_cache must be apart");
+// Elements of a and b share memory: exactly for views of equal strides (interleaved
+// ones are two memories), by their address ranges for others.  Neither overlaps itself.
+bool share(const at::Tensor& a, const at::Tensor& b) {
+    if (!meet(a, b)) return false;
+    if (a.sizes() != b.sizes()) return true;
+    for (int64_t i = 0; i < a.dim(); ++i)
+        if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return true;
+    return fgqa::plan::views_meet(reinterpret_cast<uintptr_t>(address(a)), reinterpret_cast<uintptr_t>(address(b)),
+                                  a.sizes().data(), a.strides().data(), (int)a.dim(), (int64_t)a.element_size());
+}
+
+// Caches and block scales that are written: K's and V's lie apart.
+void check_apart(const at::Tensor& k, const at::Tensor& v, PyObject* k_scale, PyObject* v_scale) {
+    if (share(k, v)) refuse("k_cache and v_cache must be apart");
+    if (is_tensor(k_scale) && is_tensor(v_scale) && share(THPVariable_Unpack(k_scale), THPVariable_Unpack(v_scale)))
+        refuse("k_scale and v_scale must be apart");
 }
 
 // All tensors of a call live on one GPU.
@@ -319,7 +333,7 @@ PyObject* append(PyObject* const* o) {
     check_written(kc);
     check_written(vc);
     check_written_scales(o[7], o[8]);
-    check_caches_apart(kc, vc);
+    check_apart(kc, vc, o[7], o[8]);
     for (const at::Tensor* t : {&k, &v})
         if (meet(*t, kc) || meet(*t, vc)) refuse("K and V must be apart from the caches");
     Device dev;
@@ -485,7 +499,7 @@ PyObject* evict(PyObject* const* o) {
     check_written(kc);
     check_written(vc);
     check_written_scales(o[8], o[9]);
-    check_caches_apart(kc, vc);
+    check_apart(kc, vc, o[8], o[9]);
     at::Tensor given[3];   // new_seqlens, new_weights, kept
     if (o[10] != Py_None) {
         given[0] = tensor(o[10], "new_seqlens");

@@ -29,6 +29,8 @@ extern "C" {
  *             codes c stand for c * scale.  Both or neither (NULL); required
  *             with FGQA_KV_INT8, NULL with FGQA_KV_BF16.  Scales are positive
  *             and at most 2^126 (the append and the eviction write powers of two).
+ *             K's and V's data and scales lie apart where a call writes them (one
+ *             address for both is refused there); the decode takes shared ones.
  *   k_scale, v_scale     one scale for a whole FGQA_KV_FP8_E4M3 cache without
  *             block scales (finite, and above 0 where tokens are written);
  *             ignored otherwise.
