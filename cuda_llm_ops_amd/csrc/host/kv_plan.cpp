@@ -172,12 +172,14 @@ int validate_kv_evict(const fgqa_kv_evict_args* a) {
     if (a->batch == 0) return FGQA_OK;
     if (a->seqlens == nullptr || a->new_seqlens == nullptr || a->kept == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
     if (!aligned4(a->seqlens) || !aligned4(a->new_seqlens) || !aligned4(a->kept)) return FGQA_ERR_UNSUPPORTED;
+    // (workgroups write outputs while others still read these)
+    if (a->new_seqlens == a->seqlens || a->new_seqlens == a->kept) return FGQA_ERR_INVALID_ARGUMENT;
     if (a->weights_len > 0) {
         if (a->new_weights == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
         if (!aligned4(a->new_weights)) return FGQA_ERR_UNSUPPORTED;
     }
     if (a->max_seqlen == 0) return FGQA_OK;
-    if (a->weights == nullptr || a->block_table == nullptr || a->new_block_table == nullptr)
+    if (a->weights == nullptr || a->block_table == nullptr || a->new_block_table == nullptr || a->weights == a->new_weights)
         return FGQA_ERR_INVALID_ARGUMENT;
     if (!aligned4(a->weights) || !aligned4(a->block_table) || !aligned4(a->new_block_table)) return FGQA_ERR_UNSUPPORTED;
     const int pointers = validate_cache_pointers(a->cache, true);

@@ -23,6 +23,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstring>
+#include <initializer_list>
 #include <utility>
 #include <vector>
 
@@ -132,6 +133,13 @@ bool share(const at::Tensor& a, const at::Tensor& b) {
         if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return true;
     return fgqa::plan::views_meet(reinterpret_cast<uintptr_t>(address(a)), reinterpret_cast<uintptr_t>(address(b)),
                                   a.sizes().data(), a.strides().data(), (int)a.dim(), (int64_t)a.element_size());
+}
+
+// t and the caches or block scales o (others are numbers) share address ranges.
+bool meet_any(const at::Tensor& t, std::initializer_list<PyObject*> o) {
+    for (PyObject* x : o)
+        if (is_tensor(x) && meet(t, THPVariable_Unpack(x))) return true;
+    return false;
 }
 
 // Caches and block scales that are written: K's and V's lie apart.
@@ -451,7 +459,7 @@ PyObject* weights(PyObject* const* o) {
     a.max_seqlen = check_max_seqlen(o[8], tokens, std::min(tokens, W));
     if (W < a.max_seqlen) refuse("weights must hold max_seqlen tokens");
     check_written(w);
-    if (meet(w, lse) || meet(w, q) || meet(w, table) || meet(w, lens)) refuse("weights must be apart from the inputs");
+    if (meet(w, lse) || meet(w, q) || meet(w, table) || meet(w, lens) || meet_any(w, {o[1], o[7]})) refuse("weights must be apart from the inputs");
     Device dev;
     for (const at::Tensor* t : {&q, &kc, &lse, &table, &lens, &w}) dev.add(*t);
     dev.add_if(o[7]);
@@ -500,6 +508,7 @@ PyObject* evict(PyObject* const* o) {
     check_written(vc);
     check_written_scales(o[8], o[9]);
     check_apart(kc, vc, o[8], o[9]);
+    if (meet_any(w, {o[0], o[1], o[8], o[9]})) refuse("weights must be apart from the caches and scales");
     at::Tensor given[3];   // new_seqlens, new_weights, kept
     if (o[10] != Py_None) {
         given[0] = tensor(o[10], "new_seqlens");
@@ -519,7 +528,8 @@ PyObject* evict(PyObject* const* o) {
     }
     for (int i = 0; i < 3; ++i) {
         if (!given[i].defined()) continue;
-        bool met = meet(given[i], w) || meet(given[i], lens) || meet(given[i], table) || meet(given[i], new_table);
+        bool met = meet(given[i], w) || meet(given[i], lens) || meet(given[i], table) || meet(given[i], new_table) ||
+                   meet_any(given[i], {o[0], o[1], o[8], o[9]});
         for (int j = 0; j < i; ++j) met = met || (given[j].defined() && meet(given[i], given[j]));
         if (met) refuse("new_seqlens, new_weights and kept must be apart from each other and from the inputs");
     }

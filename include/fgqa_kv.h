@@ -184,7 +184,8 @@ int fgqa_kv_weights(const fgqa_kv_weights_args* args, void* stream);
  * Slots behind the last kept token keep their bytes.
  *
  * The new pages must be apart from all pages that the call reads, and not
- * shared between its sequences; new_weights and kept apart from weights.
+ * shared between its sequences; new_seqlens, new_weights and kept apart from each
+ * other and from all that the call reads (weights or seqlens in place are refused).
  * The old pages are left as they are, so pages shared with other sequences stay valid.
  */
 typedef struct fgqa_kv_evict_args {
