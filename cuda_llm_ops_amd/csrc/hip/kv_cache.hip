@@ -494,6 +494,8 @@ struct EvictParams {
     int32_t* new_seqlens;
     int32_t* kept;
     int max_seqlen, weights_len, budget, recent;
+    int max_tokens;  // lengths are clamped to it; tokens from max_seqlen on have no weight
+    int most;        // tokens of a sequence that are kept: the budget, or what its new pages hold
     int pages;       // new pages of a sequence at most
     int parts;       // workgroups per row of the selection
     uint32_t items;  // batch * pages * 2 * hkv, below 2^31
@@ -560,9 +562,10 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     const int part = (int)(blockIdx.x % (unsigned)p.parts);
     const unsigned row = blockIdx.x / (unsigned)p.parts;
     const int h = (int)(row % (unsigned)p.c.hkv), b = (int)(row / (unsigned)p.c.hkv);
-    const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
-    const int count = min(len, p.budget);
-    const int recent = len > p.budget ? min(p.recent, p.budget) : len;
+    const int len = min(max(p.seqlens[b], 0), p.max_tokens);
+    const int count = min(len, p.most);
+    // (tokens without a weight count as recent: the candidates all have one)
+    const int recent = len > p.most ? min(max(p.recent, len - p.max_seqlen), p.most) : len;
     const int cand = len - recent;
     const int need = count - recent;
     const float* w = p.weights + b * p.w_b + h * p.w_h;
@@ -632,7 +635,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
     if (h == 0 && at_thread == 0) p.new_seqlens[b] = count;
     for (int i = at_thread; i < recent; i += threads) {
         kept[need + i] = cand + i;
-        nw[need + i] = w[cand + i];
+        if (need + i < p.weights_len) nw[need + i] = cand + i < p.max_seqlen ? w[cand + i] : 0.f;
     }
     auto fill = [&] {
         fill_row(kept, count, p.budget, (int32_t)-1, at_thread, threads);
@@ -766,8 +769,8 @@ __global__ __launch_bounds__(kThreads) void move_kernel(EvictParams p) {
     const int kv = (int)(rest & 1);
     const int j = (int)((rest >> 1) % (uint32_t)p.pages);
     const int b = (int)((rest >> 1) / (uint32_t)p.pages);
-    const int len = min(max(p.seqlens[b], 0), p.max_seqlen);
-    const int rows = min(min(len, p.budget) - (j << p.c.page_shift), 1 << p.c.page_shift);
+    const int len = min(max(p.seqlens[b], 0), p.max_tokens);
+    const int rows = min(min(len, p.most) - (j << p.c.page_shift), 1 << p.c.page_shift);
     if (rows <= 0) return;
     const int page = p.new_table[(int64_t)b * p.nt_stride + j];
     if (page < 0 || page >= p.c.num_pages) return;
@@ -988,8 +991,9 @@ extern "C" int fgqa_kv_evict(const fgqa_kv_evict_args* a, void* stream) {
     p.weights_len = a->weights_len;
     p.budget = a->budget;
     p.recent = a->recent;
-    const int most = a->budget < a->max_seqlen ? a->budget : a->max_seqlen;
-    p.pages = (int)ceil_div(most, a->cache.page_size);
+    p.max_tokens = plan::evict_tokens(*a);
+    p.most = plan::evict_most(*a);
+    p.pages = (int)ceil_div(std::min(p.most, p.max_tokens), a->cache.page_size);
     p.items = (uint32_t)((int64_t)a->batch * p.pages * 2 * p.c.hkv);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t rows = (int64_t)a->batch * p.c.hkv;

@@ -147,17 +147,19 @@ int validate_kv_evict(const fgqa_kv_evict_args* a) {
     if (a == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
     const int st = validate_cache(a->cache, true, false);
     if (st != FGQA_OK) return st;
-    if (a->batch < 0 || a->max_seqlen < 0 || a->weights_len < a->max_seqlen || a->budget <= 0 || a->recent < 0)
+    if (a->batch < 0 || a->max_seqlen < 0 || a->weights_len < a->max_seqlen || a->budget <= 0 || a->recent < 0 ||
+        a->max_tokens < 0 || a->new_tokens < 0)
         return FGQA_ERR_INVALID_ARGUMENT;
     if (a->block_table_stride < 0 || a->new_block_table_stride < 0 || !non_negative(a->weights_stride) ||
         !non_negative(a->new_weights_stride))
         return FGQA_ERR_INVALID_ARGUMENT;
-    const int64_t most = a->budget < a->max_seqlen ? a->budget : a->max_seqlen;
+    const int64_t longest = evict_tokens(*a);
+    const int64_t most = evict_most(*a) < longest ? evict_most(*a) : longest;
     // the block tables' rows cover the tokens
-    if ((i128)a->max_seqlen > (i128)a->block_table_stride * a->cache.page_size ||
+    if ((i128)longest > (i128)a->block_table_stride * a->cache.page_size ||
         (i128)most > (i128)a->new_block_table_stride * a->cache.page_size)
         return FGQA_ERR_INVALID_ARGUMENT;
-    if (a->weights_len > kMaxTokens || a->budget > kMaxTokens) return FGQA_ERR_UNSUPPORTED;
+    if (a->weights_len > kMaxTokens || a->budget > kMaxTokens || longest > kMaxTokens) return FGQA_ERR_UNSUPPORTED;
     const int64_t wn[3] = {a->batch, a->cache.num_kv_heads, a->weights_len};
     const int64_t ws[3] = {a->weights_stride[0], a->weights_stride[1], 1};
     const int64_t ns[3] = {a->new_weights_stride[0], a->new_weights_stride[1], 1};
@@ -178,9 +180,9 @@ int validate_kv_evict(const fgqa_kv_evict_args* a) {
         if (a->new_weights == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
         if (!aligned4(a->new_weights)) return FGQA_ERR_UNSUPPORTED;
     }
-    if (a->max_seqlen == 0) return FGQA_OK;
-    if (a->weights == nullptr || a->block_table == nullptr || a->new_block_table == nullptr || a->weights == a->new_weights)
-        return FGQA_ERR_INVALID_ARGUMENT;
+    if (longest == 0) return FGQA_OK;
+    if (a->block_table == nullptr || a->new_block_table == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
+    if (a->max_seqlen > 0 && (a->weights == nullptr || a->weights == a->new_weights)) return FGQA_ERR_INVALID_ARGUMENT;
     if (!aligned4(a->weights) || !aligned4(a->block_table) || !aligned4(a->new_block_table)) return FGQA_ERR_UNSUPPORTED;
     const int pointers = validate_cache_pointers(a->cache, true);
     if (pointers != FGQA_OK) return pointers;

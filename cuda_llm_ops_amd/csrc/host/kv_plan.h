@@ -40,6 +40,12 @@ inline int log2_of(int power_of_two) {
     return shift;
 }
 
+// Tokens an eviction leaves of the longest sequence at most, and its longest length.
+inline int evict_tokens(const fgqa_kv_evict_args& a) { return a.max_tokens > a.max_seqlen ? a.max_tokens : a.max_seqlen; }
+inline int evict_most(const fgqa_kv_evict_args& a) {
+    return a.new_tokens > 0 && a.new_tokens < a.budget ? a.new_tokens : a.budget;
+}
+
 // Most pages of one sequence that `max_new` tokens in a row touch.
 inline int64_t append_pages(int64_t max_new, int64_t page_size) { return (max_new + page_size - 2) / page_size + 1; }
 

@@ -86,7 +86,7 @@ def accumulate_kv_weights_paged(q, k_cache, lse, block_table, seqlens, weights, 
 
     q: bf16 [B, Hq, 128]; lse: fp32 [B, Hq], as ``decode_flash_gqa_paged`` writes it
     for this q; weights: fp32 [B, Hkv, W], W >= max_seqlen (by default the block
-    table's tokens or W, whichever is less)."""
+    table's tokens or W, whichever is less: tokens from W on have no weight)."""
     call_native("weights", q, q, k_cache, lse, block_table, seqlens, weights, scale, k_scale, max_seqlen)
     return weights
 
@@ -101,9 +101,10 @@ def evict_kv_paged(k_cache, v_cache, block_table, seqlens, weights, new_block_ta
     counts as larger than any number), in order; a sequence of up to ``budget`` tokens keeps all.  Token
     kept[b, h, i] becomes token i, in page new_block_table[b, i // page_size].
 
-    weights: fp32 [B, Hkv, W], W >= max_seqlen (by default the block table's tokens
-    or W, whichever is less); new_block_table: int32 [B, pages] for
-    min(budget, max_seqlen) tokens.  new_seqlens: int32 [B]; new_weights: fp32
+    weights: fp32 [B, Hkv, W]; tokens from W on have none and are kept as the recent
+    ones are.  With a ``max_seqlen`` (at most W), lengths are clamped to it.
+    new_block_table: int32 [B, pages] for min(budget, W or max_seqlen) tokens; longer
+    sequences are cut to what it holds.  new_seqlens: int32 [B]; new_weights: fp32
     [B, Hkv, W], the kept tokens' weights, then zeros; kept: int32
     [B, Hkv, budget], -1 past the kept tokens (each allocated when None).
 

@@ -164,7 +164,8 @@ int fgqa_kv_weights(const fgqa_kv_weights_args* args, void* stream);
  * weights, and moves those to new pages.
  *
  * A sequence of n <= budget tokens keeps all.  A longer one keeps its last
- * `recent` tokens (at most budget) and, of those before, the budget - recent of
+ * `recent` tokens (at most budget; tokens at or past max_seqlen, which have no
+ * weight, all count as recent) and, of those before, the budget - recent of
  * largest weight; of equal weights the one of lower index, NaN counting as
  * larger than any number.  Kept tokens stay in order: token kept[b][h][i] becomes token i,
  * in page new_block_table[b][i / page_size].
@@ -172,12 +173,18 @@ int fgqa_kv_weights(const fgqa_kv_weights_args* args, void* stream);
  *   weights      fp32 [B, Hkv, at least max_seqlen], strides {b, h}
  *   new_weights  fp32 [B, Hkv, weights_len], strides {b, h}: the kept tokens'
  *                weights, then zeros to weights_len (>= max_seqlen)
- *                (of older tokens, -0 as 0 and a NaN as some NaN)
+ *                (of older tokens, -0 as 0 and a NaN as some NaN,
+ *                and 0 of tokens without one; tokens past weights_len have none)
  *   kept         int32 [B, Hkv, budget], contiguous; -1 past the kept tokens
  *   new_seqlens  int32 [B]: min(n, budget)
- *   block_table, seqlens, max_seqlen: as fgqa_decode_paged
- *   new_block_table  int32 [B, at least min(budget, max_seqlen) / page_size rounded up].
- *                Pages outside [0, num_pages) are not written.
+ *   block_table, seqlens: as fgqa_decode_paged.
+ *   max_seqlen   tokens that have weights.  Lengths are clamped to it, or to
+ *                max_tokens where that is more: max_tokens is what a row of the block
+ *                table holds (0: max_seqlen).
+ *   new_block_table  int32 [B, at least min(budget, longest sequence) / page_size
+ *                rounded up].  Pages outside [0, num_pages) are not written.
+ *                new_tokens: tokens its rows have pages for, where that can be less
+ *                (0: enough); sequences are cut to them as if they were the budget.
  *
  * Blocks with scales are scaled anew, as fgqa_kv_append scales new tokens (from
  * the values that the kept codes stand for); other caches' bytes are copied.
@@ -206,6 +213,8 @@ typedef struct fgqa_kv_evict_args {
     int32_t weights_len;
     int32_t budget;
     int32_t recent;
+    int32_t max_tokens;
+    int32_t new_tokens;
 } fgqa_kv_evict_args;
 
 int fgqa_kv_evict(const fgqa_kv_evict_args* args, void* stream);
