@@ -222,7 +222,9 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
                 scale = old;
                 fresh = false;
             } else {
-                const Divisor div(scale);
+                // (codes times old / scale: codes times old can pass fp32's largest
+                // number.  old / scale is exact, or 0 to every code.)
+                const float ratio = old * (1.f / scale);
                 for (int base = 0; base < slot0; base += Shape::rows)
 #pragma unroll
                     for (int s = 0; s < Shape::sweeps; ++s) {
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendParams p) {
                         u32x4_t* r = reinterpret_cast<u32x4_t*>(dst + slot * p.c.slot[kv]);
                         u32x4_t w = *r;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = to_codes<kCode>(div(codes_to_f32<kCode>(w[i]) * old));
+                        for (int i = 0; i < 4; ++i) w[i] = to_codes<kCode>(codes_to_f32<kCode>(w[i]) * ratio);
                         *r = w;
                     }
             }
@@ -819,14 +821,16 @@ __global__ __launch_bounds__(kThreads) void move_kernel(EvictParams p) {
                 for (int i = 0; i < 4; ++i) {
                     const f32x4_t x = codes_to_f32<kCode>(raw[s][0][i]) * from[s];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) amax = fmaxf(amax, finite_abs(x[e]));
+                    for (int e = 0; e < 4; ++e) amax = fmaxf(amax, capped_abs(x[e]));
                 }
         }
         scale = block_scale<kCode>(block_max<Shape>(amax, s_max));
         if (lane == 0 && wave % Shape::waves == 0)
             p.c.scales[kv][page * p.c.scale_page[kv] + h * p.c.scale_head[kv]] = scale;
     }
-    const Divisor div(scale);
+    // (codes times from / scale, as the append's older ones; past fp32's largest number
+    // only for rows whose codes are all 0)
+    const float inv = 1.f / scale;
     for (int base = last; base >= 0; base -= Shape::rows) {
         if (kScaling != kBlocks || base != last) load(base);
 #pragma unroll
@@ -835,9 +839,10 @@ __global__ __launch_bounds__(kThreads) void move_kernel(EvictParams p) {
             if (slot >= rows) continue;
             u32x4_t* r = reinterpret_cast<u32x4_t*>(dst + slot * p.c.slot[kv]);
             if constexpr (kScaling == kBlocks) {
+                const float ratio = fminf(from[s] * inv, kLargest);
                 u32x4_t w;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = to_codes<kCode>(div(codes_to_f32<kCode>(raw[s][0][i]) * from[s]));
+                for (int i = 0; i < 4; ++i) w[i] = to_codes<kCode>(codes_to_f32<kCode>(raw[s][0][i]) * ratio);
                 *r = w;
             } else {
 #pragma unroll

@@ -13,6 +13,7 @@ enum KvCode { kCodeBf16 = 0, kCodeFp8 = 1, kCodeInt8 = 2 };
 
 constexpr float kFp8Max = 448.f;
 constexpr float kInt8Max = 127.f;
+constexpr float kLargest = 3.40282347e38f;   // of fp32
 
 // Byte i of w as a signed number.
 template <int i>
@@ -157,6 +158,13 @@ __device__ __forceinline__ float groups_sum(float v) {
 __device__ __forceinline__ float finite_abs(float x) {
     const float a = fabsf(x);
     return a < INFINITY ? a : 0.f;   // (false for NaN)
+}
+
+// |x| of a code times a scale, NaN as 0.  Codes are finite, so an infinite product is
+// a number past fp32's largest: the largest bf16 number, 1.992 * 2^127, is held as
+// 2^128.  It counts as the largest, whose scale is the same.
+__device__ __forceinline__ float capped_abs(float x) {
+    return x == x ? fminf(fabsf(x), kLargest) : 0.f;
 }
 
 }  // namespace fgqa
