@@ -227,11 +227,24 @@ void check_cache(const at::Tensor& t, const char* name, int* dtype) {
         refuse("%s must be 16-byte aligned, with strides in multiples of 16 bytes", name);
 }
 
+// A tensor of one element stands for a number, unless it is all block scales of a
+// cache of one page and head.
+bool may_be_number(PyObject* o) { return !is_tensor(o) || THPVariable_Unpack(o).numel() == 1; }
+bool may_be_blocks(PyObject* o, const at::Tensor& cache) {
+    if (!is_tensor(o)) return false;
+    const at::Tensor& s = THPVariable_Unpack(o);
+    return s.scalar_type() == at::kFloat && s.dim() == 2 && s.size(0) == cache.size(0) && s.size(1) == cache.size(2) &&
+           s.device() == cache.device();
+}
+
+PyObject* blocks_or_none(const float* scales, PyObject* o) { return scales != nullptr ? o : Py_None; }
+
 // k_scale or v_scale: block scales (returned) or one for the cache.
-float* check_scale(PyObject* o, const at::Tensor& cache, int dtype, const char* name, float* whole, int64_t (&st)[2]) {
+float* check_scale(PyObject* o, bool as_number, const at::Tensor& cache, int dtype, const char* name, float* whole,
+                   int64_t (&st)[2]) {
     *whole = 1.f;
     st[0] = st[1] = 0;
-    if (is_tensor(o)) {
+    if (is_tensor(o) && !as_number) {
         const at::Tensor& s = THPVariable_Unpack(o);
         if (dtype == FGQA_KV_BF16) refuse("bf16 caches have no block scales");
         if (s.scalar_type() != at::kFloat || s.dim() != 2 || s.size(0) != cache.size(0) || s.size(1) != cache.size(2))
@@ -254,17 +267,21 @@ fgqa_kv_cache check_caches(const at::Tensor& k, const at::Tensor* v, PyObject* k
     std::memset(&c, 0, sizeof c);
     int dtype = 0;
     check_cache(k, "k_cache", &dtype);
+    // (both scales in one way)
+    const bool numbers = dtype != FGQA_KV_INT8 && may_be_number(k_scale) && (v == nullptr || may_be_number(v_scale)) &&
+                         !(dtype == FGQA_KV_FP8_E4M3 && may_be_blocks(k_scale, k) &&
+                           (v == nullptr || may_be_blocks(v_scale, *v)));
     if (v != nullptr) {
         if (v->scalar_type() != k.scalar_type() || v->sizes() != k.sizes())
             refuse("k_cache and v_cache must share dtype and shape");
         check_cache(*v, "v_cache", &dtype);
-        if (is_tensor(k_scale) != is_tensor(v_scale) && dtype != FGQA_KV_INT8)
+        if (!numbers && is_tensor(k_scale) != is_tensor(v_scale) && dtype != FGQA_KV_INT8)
             refuse("k_scale and v_scale must both be tensors or both numbers");
-        c.v_scales = check_scale(v_scale, *v, dtype, "v_scale", &c.v_scale, c.v_scales_stride);
+        c.v_scales = check_scale(v_scale, numbers, *v, dtype, "v_scale", &c.v_scale, c.v_scales_stride);
         c.v = address(*v);
         for (int i = 0; i < 3; ++i) c.v_stride[i] = v->stride(i);
     }
-    c.k_scales = check_scale(k_scale, k, dtype, "k_scale", &c.k_scale, c.k_scales_stride);
+    c.k_scales = check_scale(k_scale, numbers, k, dtype, "k_scale", &c.k_scale, c.k_scales_stride);
     c.k = address(k);
     for (int i = 0; i < 3; ++i) c.k_stride[i] = k.stride(i);
     c.kv_dtype = dtype;
@@ -340,13 +357,14 @@ PyObject* append(PyObject* const* o) {
         refuse("k_scale and v_scale must be positive");
     check_written(kc);
     check_written(vc);
-    check_written_scales(o[7], o[8]);
-    check_apart(kc, vc, o[7], o[8]);
+    PyObject *const ks = blocks_or_none(a.cache.k_scales, o[7]), *const vs = blocks_or_none(a.cache.v_scales, o[8]);
+    check_written_scales(ks, vs);
+    check_apart(kc, vc, ks, vs);
     for (const at::Tensor* t : {&k, &v})
         if (meet(*t, kc) || meet(*t, vc)) refuse("K and V must be apart from the caches");
     Device dev;
     for (const at::Tensor* t : {&k, &v, &kc, &vc, &table, &lens}) dev.add(*t);
-    for (int i = 6; i < 9; ++i) dev.add_if(o[i]);
+    for (PyObject* x : {o[6], ks, vs}) dev.add_if(x);
     void* stream = nullptr;
     if (!dev.current(&stream)) return not_here();
     const at::Tensor kr = ready(k), vr = ready(v);
@@ -405,7 +423,8 @@ PyObject* decode(PyObject* const* o) {
     }
     Device dev;
     for (const at::Tensor* t : {&q, &kc, &vc, &table, &lens}) dev.add(*t);
-    for (int i : {6, 7, 8, 9, 12}) dev.add_if(o[i]);
+    for (PyObject* x : {blocks_or_none(a.cache.k_scales, o[6]), blocks_or_none(a.cache.v_scales, o[7]), o[8], o[9], o[12]})
+        dev.add_if(x);
     void* stream = nullptr;
     if (!dev.current(&stream)) return not_here();
     const at::Tensor qr = ready(q);
@@ -459,10 +478,11 @@ PyObject* weights(PyObject* const* o) {
     a.max_seqlen = check_max_seqlen(o[8], tokens, std::min(tokens, W));
     if (W < a.max_seqlen) refuse("weights must hold max_seqlen tokens");
     check_written(w);
-    if (meet(w, lse) || meet(w, q) || meet(w, table) || meet(w, lens) || meet_any(w, {o[1], o[7]})) refuse("weights must be apart from the inputs");
+    PyObject* const ks = blocks_or_none(a.cache.k_scales, o[7]);
+    if (meet(w, lse) || meet(w, q) || meet(w, table) || meet(w, lens) || meet_any(w, {o[1], ks})) refuse("weights must be apart from the inputs");
     Device dev;
     for (const at::Tensor* t : {&q, &kc, &lse, &table, &lens, &w}) dev.add(*t);
-    dev.add_if(o[7]);
+    dev.add_if(ks);
     void* stream = nullptr;
     if (!dev.current(&stream)) return not_here();
     const at::Tensor qr = ready(q);
@@ -510,9 +530,10 @@ PyObject* evict(PyObject* const* o) {
     a.new_tokens = (int32_t)new_tokens;
     check_written(kc);
     check_written(vc);
-    check_written_scales(o[8], o[9]);
-    check_apart(kc, vc, o[8], o[9]);
-    if (meet_any(w, {o[0], o[1], o[8], o[9]})) refuse("weights must be apart from the caches and scales");
+    PyObject *const ks = blocks_or_none(a.cache.k_scales, o[8]), *const vs = blocks_or_none(a.cache.v_scales, o[9]);
+    check_written_scales(ks, vs);
+    check_apart(kc, vc, ks, vs);
+    if (meet_any(w, {o[0], o[1], ks, vs})) refuse("weights must be apart from the caches and scales");
     at::Tensor given[3];   // new_seqlens, new_weights, kept
     if (o[10] != Py_None) {
         given[0] = tensor(o[10], "new_seqlens");
@@ -533,13 +554,13 @@ PyObject* evict(PyObject* const* o) {
     for (int i = 0; i < 3; ++i) {
         if (!given[i].defined()) continue;
         bool met = meet(given[i], w) || meet(given[i], lens) || meet(given[i], table) || meet(given[i], new_table) ||
-                   meet_any(given[i], {o[0], o[1], o[8], o[9]});
+                   meet_any(given[i], {o[0], o[1], ks, vs});
         for (int j = 0; j < i; ++j) met = met || (given[j].defined() && meet(given[i], given[j]));
         if (met) refuse("new_seqlens, new_weights and kept must be apart from each other and from the inputs");
     }
     Device dev;
     for (const at::Tensor* t : {&w, &kc, &vc, &table, &lens, &new_table}) dev.add(*t);
-    for (int i = 8; i < 13; ++i) dev.add_if(o[i]);
+    for (PyObject* x : {ks, vs, o[10], o[11], o[12]}) dev.add_if(x);
     void* stream = nullptr;
     if (!dev.current(&stream)) return not_here();
     if (!given[0].defined()) given[0] = at::empty({B}, lens.options());

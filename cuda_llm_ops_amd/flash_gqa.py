@@ -278,9 +278,13 @@ def _has_block_scales(k_cache, k_scale, v_scale) -> bool:
         return True
     if isinstance(k_scale, float) and isinstance(v_scale, float):
         return False
-    # (a tensor of one element that is no [num_pages, Hkv] stands for a number)
-    return any(isinstance(s, torch.Tensor) and (s.numel() != 1 or s.shape == k_cache.shape[::2])
-               for s in (k_scale, v_scale))
+    # A tensor of one element stands for a number, unless it and the other are all
+    # block scales of an e4m3 cache of one page and head.
+    if any(isinstance(s, torch.Tensor) and s.numel() != 1 for s in (k_scale, v_scale)):
+        return True
+    return k_cache.dtype != torch.bfloat16 and all(
+        isinstance(s, torch.Tensor) and s.dtype == torch.float32 and s.shape == k_cache.shape[::2]
+        and s.device == k_cache.device for s in (k_scale, v_scale))
 
 
 def decode_flash_gqa_paged(q, k_cache, v_cache, block_table, seqlens, scale=None, k_scale=1.0, v_scale=1.0,

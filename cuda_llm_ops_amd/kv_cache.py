@@ -5,8 +5,10 @@ torch.float8_e4m3fn or torch.int8) and a block table int32 [B, max_pages]: token
 t of sequence b is slot t % page_size of page block_table[b, t // page_size].
 8-bit caches hold codes; ``k_scale`` and ``v_scale`` are fp32 tensors
 [num_pages, Hkv], a scale for each page of each KV head, or (float8_e4m3fn
-only) two numbers for the whole cache.  Calls that write a cache (append, evict)
-refuse K and V caches or scales that share memory.
+only) two numbers for the whole cache.  A tensor of one element counts as a number
+(the host reads it), unless both are the [num_pages, Hkv] scales of a cache of one
+page and head.  Calls that write a cache (append, evict) refuse K and V caches or
+scales that share memory.
 
     append_kv_paged              writes new tokens
     flash_gqa.decode_flash_gqa_paged   single-token attention
