@@ -185,6 +185,14 @@ struct Device {
     }
 };
 
+// Autograd learns that t was written (inference tensors have no version).
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written_if(PyObject* o) {
+    if (is_tensor(o)) written(THPVariable_Unpack(o));
+}
+
 PyObject* not_here() { Py_RETURN_NOTIMPLEMENTED; }
 
 void raise_status(int status, const char* where) {
@@ -378,6 +386,8 @@ PyObject* append(PyObject* const* o) {
     a.max_new = (int32_t)k.size(1);
     a.max_pages = (int32_t)pages;
     launch(fgqa_kv_append, a, stream, "fgqa_kv_append");
+    for (const at::Tensor* t : {&kc, &vc}) written(*t);
+    for (PyObject* x : {ks, vs}) written_if(x);
     Py_RETURN_NONE;
 }
 
@@ -497,6 +507,7 @@ PyObject* weights(PyObject* const* o) {
     a.num_q_heads = (int32_t)Hq;
     a.scale = o[6] == Py_None ? (float)(1.0 / std::sqrt(128.0)) : (float)number(o[6]);
     launch(fgqa_kv_weights, a, stream, "fgqa_kv_weights");
+    written(w);
     Py_RETURN_NONE;
 }
 
@@ -580,6 +591,8 @@ PyObject* evict(PyObject* const* o) {
     a.budget = (int32_t)budget;
     a.recent = (int32_t)std::min(recent, budget);
     launch(fgqa_kv_evict, a, stream, "fgqa_kv_evict");
+    for (const at::Tensor* t : {&kc, &vc}) written(*t);
+    for (PyObject* x : {ks, vs, o[10], o[11], o[12]}) written_if(x);
     return Py_BuildValue("(NNN)", THPVariable_Wrap(given[0]), THPVariable_Wrap(given[1]), THPVariable_Wrap(given[2]));
 }
 
