@@ -428,6 +428,7 @@ PyObject* decode(PyObject* const* o) {
     }
     if (o[12] != Py_None) {
         work = tensor(o[12], "workspace");
+        if (!work.is_contiguous()) refuse("workspace must be contiguous");   // (its bytes are all there)
         a.workspace = address(work);
         a.workspace_bytes = (size_t)work.numel() * work.element_size();
     }

@@ -108,6 +108,10 @@ def _decode_args(q, k, v, o, scale, seqlens, lse, split_tokens, workspace) -> _l
 
 def _workspace(workspace):
     """The workspace fields: its address and bytes, or none."""
+    if workspace is not None:
+        _require_cuda(workspace)
+        if not workspace.is_contiguous():   # (the bytes counted below are all there)
+            raise ValueError("workspace must be contiguous")
     return (0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
 
 
