@@ -101,7 +101,7 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
 
     float m_run = -INFINITY;
     float l_run = 0.f;   // this lane's share of the rowsum of head l16
-    // head l16's largest P sV so far, P relative to m_run, and 2^-112 at least: 2^14 /
+    // head l16's largest |P sV| so far, P relative to m_run, and 2^-112 at least: 2^14 /
     // vref is a number (blocks of zeros have the scale 2^-126)
     constexpr uint32_t kLeastRef = 0x07800000u;
     float vref = __uint_as_float(kLeastRef);
@@ -272,7 +272,7 @@ __device__ __forceinline__ void dec_item8(const DecodeParams& p, unsigned char* 
             const float e = fast_exp2(y[j] - m_sub);
             psum += e;
             pv[j] = e * vs[j];
-            pmax = fmaxf(pmax, pv[j]);
+            pmax = fmaxf(pmax, fabsf(pv[j]));
         }
         pmax = groups_max(pmax);
         // The sums so far are relative to vref, which a larger m_run lowers with them:
