@@ -534,9 +534,10 @@ PyObject* evict(PyObject* const* o) {
     const int64_t tokens = table_tokens(pages, a.cache);
     a.max_seqlen = check_max_seqlen(o[13], tokens, std::min(tokens, W));
     if (W < a.max_seqlen) refuse("weights must hold max_seqlen tokens");
-    // without a max_seqlen, tokens past the weights' rows are kept as recent ones are
-    a.max_tokens = o[13] == Py_None ? (int32_t)std::min<int64_t>(tokens, 1 << 30) : a.max_seqlen;
     const int64_t new_tokens = table_tokens(new_pages, a.cache);
+    // without a max_seqlen, tokens past the weights' rows are kept as recent ones are
+    // (no new pages at all, with weights of no tokens: nothing is kept)
+    a.max_tokens = o[13] == Py_None && new_tokens > 0 ? (int32_t)std::min<int64_t>(tokens, 1 << 30) : a.max_seqlen;
     if (new_tokens < std::min<int64_t>(budget, a.max_seqlen))
         refuse("new_block_table must have pages for min(budget, max_seqlen) tokens");
     a.new_tokens = (int32_t)new_tokens;

@@ -80,3 +80,19 @@ def test_long_rows_shared_by_workgroups(cuda):
         both = _table(rng, 1, width + 6, width + 6)
         w = torch.from_numpy(rng.exponential(size=(1, 1, W)).astype(np.float32))
         _run(cuda, c, both[:, :width], both[:, width:], [n], w, 3000, 10, 10 ** 9)
+
+
+def test_weights_of_no_tokens(cuda):
+    """All tokens are recent then; without new pages none is kept."""
+    import cuda_llm_ops_amd as fg
+    torch = _torch()
+    rng = np.random.default_rng(3400)
+    c = Cache(cuda, rng, "int8", 60, 16, 2)
+    both = _table(rng, 2, 24, 60)
+    w = torch.zeros((2, 2, 0))
+    _run(cuda, c, both[:, :20], both[:, 20:], [300, 7], w, 60, 3, 10 ** 9)
+    nl, nw, kept = fg.evict_kv_paged(c.t[0], c.t[1], _i32(cuda, both[:, :20]), _i32(cuda, [300, 7]), w.to(cuda),
+                                     _i32(cuda, both)[:, :0], budget=60, recent=3, **c.scales)
+    torch.cuda.synchronize()
+    assert nl.tolist() == [0, 0] and nw.shape == (2, 2, 0) and bool((kept == -1).all())
+    c.check("no new pages")
