@@ -547,7 +547,7 @@ __device__ __forceinline__ void fill_row(T* dst, int from, int to, T value, int 
 // took 22.1.)
 // The vector units of a row's one CU bound it: an operation on each of 32K keys
 // takes 0.2 us, the first histogram 3.5.  Shared out over workgroups, the
-// histograms would take a launch for each pass, about what a pass takes; but
+// histograms would take further launches (that form was not built or timed);
 // where there are fewer rows than CUs, `parts` workgroups find the same
 // threshold, and each writes its part of every wave's steps.  8 rows of 32K: 17.2
 // us (22.1 in one part), 256 of 8K 13.2, 4 of 600 6.9: the latency of loads, three
@@ -757,7 +757,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kernel(EvictParams p) {
 
 // Moves the kept tokens: one block of the new pages per item, as append_kernel,
 // its rows gathered through `kept` and the block table.  Memory bounds it: 32
-// sequences cut to 4000 tokens, 8 heads, e4m3 pages of 64: 530 MB in 111 us, 4.8 TB/s,
+// sequences cut to 4000 tokens, 8 heads, e4m3 pages of 64: 530 MB in 110 us, 4.8 TB/s,
 // the rate of a copy.
 template <int kCode, Scaling kScaling, typename Shape>
 __global__ __launch_bounds__(kThreads) void move_kernel(EvictParams p) {

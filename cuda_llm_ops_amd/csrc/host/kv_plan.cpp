@@ -226,12 +226,13 @@ fgqa_decode_paged_args as_decode_paged(const fgqa_decode_blocks_args* a) {
 // Splits of the tokens that a CU gets of a full batch, so that one round of
 // workgroups runs, down to a step of 8 waves; no splits where the sequences are
 // at most kSplitSlack longer (the combine's launch costs what those take).  Hq / Hkv,
-// 16-token pages, lengths up to S, us teams / splits: 16 / 1, 1 x 512 11.4 / 5.8; 32 / 8,
-// 4 x 1024 16.3 / 9.2, 1 x 32768 17.8 / 14.4, 16 x 4096 30.2 / 27.4.  Teams share
-// out uneven lengths, and 4 heads of theirs read side by side: they are taken
-// for more than kSplitMost tokens a CU (16 x 8192 39.8 / 45.5, 128 x 2048 61.9 / 72.2;
-// 28 / 4, 64 x 4096 the other way, 41.3 / 35.8) or two workgroups a CU (32 / 8, 128
-// x 512 25.2 / 28.7).
+// 16-token pages, lengths up to S, us teams / splits: 16 / 1, 1 x 512 11.1 / 6.0; 32 / 8,
+// 4 x 1024 16.0 / 9.4, 16 x 4096 30.7 / 28.1, 1 x 32768 25.0 / 21.6 (but 17.7 / 18.6
+// where the one sequence has 8806 tokens of them).  Teams share out uneven lengths,
+// and 4 heads of theirs read side by side: they are taken for more than kSplitMost
+// tokens a CU (16 x 8192 40.3 / 46.2, 128 x 2048 63.2 / 75.5) or two workgroups a CU
+// (32 / 8, 128 x 512 26.1 / 30.4).  The lines are those of 8 KV heads; 28 / 4, 64 x
+// 4096 is the other way, 41.3 / 36.5, which they do not tell apart.
 int blocks_split(int64_t batch, int64_t num_kv_heads, int64_t max_seqlen, int cus) {
     constexpr int64_t kSplitMost = 2048, kSplitSlack = 512;
     const i128 heads = (i128)batch * num_kv_heads;
