@@ -18,7 +18,8 @@ enum class KvCacheType { Bf16 = 0, Fp8E4m3 = 1, Int8 = 2 };
  * k, v: [numPages, pageSize, numKvHeads, 128] of `type`, 16-byte aligned.
  * kScales, vScales: fp32 [numPages, numKvHeads], the scale of each block (page
  * and KV head) of 8-bit codes; required for Int8, null for Bf16.  An Fp8E4m3
- * cache without them has kScale and vScale for all of it.
+ * cache without them has kScale and vScale for all of it.  K's and V's data and
+ * scales lie apart where a call writes them.
  */
 struct KvCache {
     void* k = nullptr;
