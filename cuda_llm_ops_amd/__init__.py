@@ -1,8 +1,9 @@
 """MI355X-native flash grouped-query attention (decode incl. paged/fp8/int8 KV caches, their writing and eviction, causal, sliding-window, MLA and sparse-index prefill, and the causal, sliding-window and MLA prefill backward).
 
 The kernels live in libfgqa.so (HIP, gfx950); ``flash_gqa`` is the Python host
-interface over its C ABI (include/fgqa.h), and ``kv_cache`` that of the paged
-cache's operators (include/fgqa_kv.h).
+interface over its C ABI (include/fgqa.h), ``kv_cache`` that of the paged
+cache's operators (include/fgqa_kv.h) and ``qk_rope`` that of the norm and rotation
+of queries and keys (include/fgqa_rope.h).
 """
 from ._lib import FgqaError, LIB_PATH, lib, native, status_string  # noqa: F401
 from .flash_gqa import (  # noqa: F401
@@ -37,6 +38,10 @@ from .kv_cache import (  # noqa: F401
     accumulate_kv_weights_paged,
     append_kv_paged,
     evict_kv_paged,
+)
+from .qk_rope import (  # noqa: F401
+    qk_norm_rope,
+    qk_norm_rope_backward,
 )
 
 __version__ = "0.1.0"

@@ -1,0 +1,526 @@
+// Queries and keys normalised for each head and rotated to their positions, in one
+// pass, and the gradients of that (include/fgqa_rope.h).
+//
+// A row is one token's query or key of one head, D elements of bf16.  A group of
+// 4, 8 or 16 lanes (D up to 64, 128, 256) holds a row, two 16-byte pieces a lane:
+// the pieces whose elements a rotation pairs, so nothing but the norm's sums goes
+// between lanes.  A lane group takes up to 4 rows of one token, with one set of
+// angles (8 pairs a lane).
+#include <algorithm>
+#include <math.h>
+
+#include <type_traits>
+
+#include "fgqa_device.h"
+#include "fgqa_internal.h"
+#include "../host/rope_plan.h"
+
+namespace fgqa {
+namespace {
+
+constexpr int kThreads = plan::kRopeThreads;
+
+// Rows of one tensor [B, S, H, D], strides in elements.
+struct Rows {
+    const __bf16* in;
+    const __bf16* grad;   // backward: of the outputs
+    __bf16* out;
+    const void* weight;
+    int64_t in_s[3], grad_s[3], out_s[3];
+    int heads;
+    int slices;            // items of a token: ceil(heads / heads an item takes)
+    FastDiv div_slices;
+    uint32_t items;
+};
+
+struct RopeParams {
+    Rows x[2];             // Q, K
+    unsigned first_k;      // workgroups from here on take K
+    const void* positions;
+    const float* inv_freq;
+    const int32_t* axes;
+    int64_t pos_a, pos_b, pos_s;
+    int pos64, weights_bf16, num_axes;
+    int seqlen, head_dim, rotary_dim, interleaved;
+    FastDiv div_seqlen;
+    float eps, inv_dim, sin_sign;
+    float* partial;        // backward: [workgroups, D], the workgroups' sums of the weights' gradients
+};
+
+// Sum over the lanes of a row, in each of them: neighbours, pairs, then mirrored
+// halves of 8 and 16 lanes (DPP, without LDS).
+template <int kLanes>
+__device__ __forceinline__ float row_sum(float v) {
+    auto add = [](float x, auto ctrl) {
+        const int o = __builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), decltype(ctrl)::value, 0xF, 0xF, true);
+        return x + __uint_as_float((uint32_t)o);
+    };
+    v = add(v, std::integral_constant<int, 0xB1>{});
+    v = add(v, std::integral_constant<int, 0x4E>{});
+    if constexpr (kLanes >= 8) v = add(v, std::integral_constant<int, 0x141>{});
+    if constexpr (kLanes >= 16) v = add(v, std::integral_constant<int, 0x140>{});
+    return v;
+}
+
+// cos and sin of t turns, |t| <= 1/2: with q the nearest quarter and x = 2 pi (t - q/4),
+// |x| <= pi/4, their Taylor sums to x^10 and x^11 (off by less than 2^-34), turned by q quarters.
+__device__ __forceinline__ void cos_sin_turns(float t, float* c, float* s) {
+    const float q = __builtin_rintf(4.f * t);
+    const float x = (t - 0.25f * q) * 6.28318530717958648f;
+    const float z = x * x;
+    float sp = fmaf(z, -1.f / 39916800.f, 1.f / 362880.f);
+    sp = fmaf(z, sp, -1.f / 5040.f);
+    sp = fmaf(z, sp, 1.f / 120.f);
+    sp = fmaf(z, sp, -1.f / 6.f);
+    sp = fmaf(x * z, sp, x);
+    float cp = fmaf(z, -1.f / 3628800.f, 1.f / 40320.f);
+    cp = fmaf(z, cp, -1.f / 720.f);
+    cp = fmaf(z, cp, 1.f / 24.f);
+    cp = fmaf(z, cp, -0.5f);
+    cp = fmaf(z, cp, 1.f);
+    const int n = (int)q;
+    const float u = (n & 1) ? sp : cp, v = (n & 1) ? cp : sp;
+    *c = ((n + 1) & 2) ? -u : u;
+    *s = (n & 2) ? -v : v;
+}
+
+typedef float f32x4u_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef int i32x4u_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4u_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// What a lane holds of each row: 16 elements, those of pieces off[0] and off[1].
+struct LaneShape {
+    int off[2];
+    int pair0;      // its first pair
+    bool rotated;
+    bool active;    // (lanes past the row's end hold nothing)
+};
+
+__device__ __forceinline__ LaneShape lane_shape(const RopeParams& p, int l) {
+    LaneShape s;
+    s.rotated = 16 * l < p.rotary_dim;
+    s.active = 16 * l < p.head_dim;
+    const bool split = s.rotated && !p.interleaved;
+    s.off[0] = split ? 8 * l : 16 * l;
+    s.off[1] = split ? p.rotary_dim / 2 + 8 * l : 16 * l + 8;
+    s.pair0 = 8 * l;
+    return s;
+}
+
+// The lane's 8 angles: positions times inverse frequencies in turns, in 64 bits as
+// far as the fraction (a position of 2^20 would leave 32-bit angles 2^-4 off).
+__device__ __forceinline__ void lane_angles(const RopeParams& p, const LaneShape& ls, int b, int s, float (&cs)[8],
+                                            float (&sn)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        cs[j] = 1.f;
+        sn[j] = 0.f;
+    }
+    if (!ls.rotated) return;
+    const int64_t at = b * p.pos_b + s * p.pos_s;
+    auto position = [&](int axis) {
+        const int64_t i = at + axis * p.pos_a;
+        return p.pos64 ? (double)static_cast<const int64_t*>(p.positions)[i]
+                       : (double)static_cast<const int32_t*>(p.positions)[i];
+    };
+    double pos[8];
+    if (p.axes != nullptr) {
+        const i32x4u_t a0 = *reinterpret_cast<const i32x4u_t*>(p.axes + ls.pair0);
+        const i32x4u_t a1 = *reinterpret_cast<const i32x4u_t*>(p.axes + ls.pair0 + 4);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pos[j] = position(min(max(j < 4 ? a0[j & 3] : a1[j & 3], 0), p.num_axes - 1));
+    } else {
+        const double one = position(0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pos[j] = one;
+    }
+    const f32x4u_t f0 = *reinterpret_cast<const f32x4u_t*>(p.inv_freq + ls.pair0);
+    const f32x4u_t f1 = *reinterpret_cast<const f32x4u_t*>(p.inv_freq + ls.pair0 + 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const double turns = pos[j] * ((double)(j < 4 ? f0[j & 3] : f1[j & 3]) * 0.15915494309189533577);
+        cos_sin_turns((float)(turns - __builtin_rint(turns)), &cs[j], &sn[j]);
+        sn[j] *= p.sin_sign;
+    }
+}
+
+// Two 16-byte pieces <-> 16 fp32: v[0..7] the first's, v[8..15] the second's.
+__device__ __forceinline__ void widen(const u32x4_t (&raw)[2], float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[8 * i + 2 * j] = __uint_as_float(raw[i][j] << 16);
+            v[8 * i + 2 * j + 1] = __uint_as_float(raw[i][j] & 0xffff0000u);
+        }
+}
+
+__device__ __forceinline__ u32x4_t narrow8(const float* v) {
+    bf16x8_t r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (__bf16)v[i];
+    return __builtin_bit_cast(u32x4_t, r);
+}
+
+__device__ __forceinline__ void lane_weights(const RopeParams& p, const Rows& x, const LaneShape& ls, float (&w)[16]) {
+    if (p.weights_bf16) {
+        u32x4_t raw[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            raw[i] = *reinterpret_cast<const u32x4u_t*>(static_cast<const __bf16*>(x.weight) + ls.off[i]);
+        widen(raw, w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const f32x4u_t f = *reinterpret_cast<const f32x4u_t*>(static_cast<const float*>(x.weight) + ls.off[i] + 4 * j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[8 * i + 4 * j + e] = f[e];
+            }
+    }
+}
+
+// Pairs (a, b) turned by the lane's angles: elements (v[j], v[8 + j]), or, interleaved,
+// (v[2j], v[2j + 1]).  Elements that are not rotated stay as they are (an infinity
+// times sin 0 would not).
+template <bool kInterleaved, bool kBack>
+__device__ __forceinline__ void rotate(float (&v)[16], const float (&cs)[8], const float (&sn)[8], bool rotated) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float& a = v[kInterleaved ? 2 * j : j];
+        float& b = v[kInterleaved ? 2 * j + 1 : 8 + j];
+        const float s = kBack ? -sn[j] : sn[j];
+        const float ra = a * cs[j] - b * s, rb = b * cs[j] + a * s;
+        a = rotated ? ra : a;
+        b = rotated ? rb : b;
+    }
+}
+
+struct Item {
+    int b, s, h0, rows;
+};
+
+template <int kHeads>
+__device__ __forceinline__ Item item_of(const RopeParams& p, const Rows& x, uint32_t item) {
+    Item r;
+    const int token = fast_div((int)item, x.div_slices);
+    r.h0 = ((int)item - token * x.slices) * kHeads;
+    r.rows = min(kHeads, x.heads - r.h0);
+    r.b = fast_div(token, p.div_seqlen);
+    r.s = token - r.b * p.seqlen;
+    return r;
+}
+
+// Forward; without a norm and with sin negated, also the gradients of a rotation alone.
+template <int kLanes, int kHeads, bool kInterleaved, bool kNorm>
+__global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
+    const int which = blockIdx.x >= p.first_k ? 1 : 0;
+    const Rows& x = p.x[which];
+    const unsigned block = blockIdx.x - (which ? p.first_k : 0u);
+    const uint32_t item = block * (uint32_t)(kThreads / kLanes) + threadIdx.x / kLanes;
+    const LaneShape ls = lane_shape(p, threadIdx.x % kLanes);
+    const bool mine = item < x.items && ls.active;   // (all lanes of a row stay for its sum)
+    const Item it = item_of<kHeads>(p, x, item < x.items ? item : 0u);
+
+    u32x4_t raw[kHeads][2];
+    const __bf16* src = x.in + it.b * x.in_s[0] + it.s * x.in_s[1] + it.h0 * x.in_s[2];
+#pragma unroll
+    for (int r = 0; r < kHeads; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            raw[r][i] = u32x4_t{0u, 0u, 0u, 0u};
+            if (mine && r < it.rows) raw[r][i] = *reinterpret_cast<const u32x4_t*>(src + r * x.in_s[2] + ls.off[i]);
+        }
+    float w[16];
+    if constexpr (kNorm) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = 0.f;
+        if (ls.active) lane_weights(p, x, ls, w);
+    }
+    float cs[8], sn[8];
+    lane_angles(p, ls, it.b, it.s, cs, sn);
+
+    __bf16* dst = x.out + it.b * x.out_s[0] + it.s * x.out_s[1] + it.h0 * x.out_s[2];
+#pragma unroll
+    for (int r = 0; r < kHeads; ++r) {
+        float v[16];
+        widen(raw[r], v);
+        if constexpr (kNorm) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum = fmaf(v[i], v[i], sum);
+            const float inv = rsqrtf(row_sum<kLanes>(sum) * p.inv_dim + p.eps);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = v[i] * inv * w[i];
+        }
+        rotate<kInterleaved, false>(v, cs, sn, ls.rotated);
+        if (mine && r < it.rows) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(dst + r * x.out_s[2] + ls.off[i]) = narrow8(v + 8 * i);
+        }
+    }
+}
+
+// Backward with a norm.  With g = R^T dy, u = x / sqrt(mean(x^2) + eps) = x r:
+//   dw = sum over rows of g u,   dx = r (w g - u mean(w g u)).
+// A workgroup walks items of one tensor and keeps its sums of dw in registers, each
+// lane those of its 16 elements, so that no gradient goes through an atomic.
+template <int kLanes, int kHeads, bool kInterleaved>
+__global__ __launch_bounds__(kThreads) void rope_backward_kernel(RopeParams p) {
+    __shared__ float s_dw[kThreads / kWave][plan::kRopeMaxHeadDim];
+    const int which = blockIdx.x >= p.first_k ? 1 : 0;
+    const Rows& x = p.x[which];
+    const unsigned block = blockIdx.x - (which ? p.first_k : 0u);
+    const uint32_t blocks = which ? gridDim.x - p.first_k : p.first_k;
+    constexpr uint32_t kGroups = kThreads / kLanes;
+    const LaneShape ls = lane_shape(p, threadIdx.x % kLanes);
+    float w[16], dw[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = dw[i] = 0.f;
+    if (ls.active) lane_weights(p, x, ls, w);
+
+    for (uint32_t first = block * kGroups; first < x.items; first += blocks * kGroups) {   // (items + a round stay below 2^32)
+        const uint32_t item = first + threadIdx.x / kLanes;
+        const bool mine = item < x.items && ls.active;
+        const Item it = item_of<kHeads>(p, x, item < x.items ? item : 0u);
+        u32x4_t raw[kHeads][2], graw[kHeads][2];
+        const __bf16* src = x.in + it.b * x.in_s[0] + it.s * x.in_s[1] + it.h0 * x.in_s[2];
+        const __bf16* gsrc = x.grad + it.b * x.grad_s[0] + it.s * x.grad_s[1] + it.h0 * x.grad_s[2];
+#pragma unroll
+        for (int r = 0; r < kHeads; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                raw[r][i] = graw[r][i] = u32x4_t{0u, 0u, 0u, 0u};
+                if (mine && r < it.rows) {
+                    raw[r][i] = *reinterpret_cast<const u32x4_t*>(src + r * x.in_s[2] + ls.off[i]);
+                    graw[r][i] = *reinterpret_cast<const u32x4_t*>(gsrc + r * x.grad_s[2] + ls.off[i]);
+                }
+            }
+        float cs[8], sn[8];
+        lane_angles(p, ls, it.b, it.s, cs, sn);
+        __bf16* dst = x.out + it.b * x.out_s[0] + it.s * x.out_s[1] + it.h0 * x.out_s[2];
+#pragma unroll
+        for (int r = 0; r < kHeads; ++r) {
+            float v[16], g[16];
+            widen(raw[r], v);
+            widen(graw[r], g);
+            rotate<kInterleaved, true>(g, cs, sn, ls.rotated);
+            float sum = 0.f, dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum = fmaf(v[i], v[i], sum);
+            const float inv = rsqrtf(row_sum<kLanes>(sum) * p.inv_dim + p.eps);
+            const bool here = mine && r < it.rows;   // (rows that are not there: eps 0 makes inv infinite)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                v[i] *= inv;
+                const float d = g[i] * v[i];
+                dw[i] += here ? d : 0.f;
+                g[i] *= w[i];
+                dot = fmaf(g[i], v[i], dot);
+            }
+            const float mean = row_sum<kLanes>(dot) * p.inv_dim;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) g[i] = inv * (g[i] - v[i] * mean);
+            if (here) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(dst + r * x.out_s[2] + ls.off[i]) = narrow8(g + 8 * i);
+            }
+        }
+    }
+
+    // the wave's lane groups, then the waves in order
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+#pragma unroll
+        for (int m = kLanes; m < kWave; m *= 2) dw[i] = xor_sum(dw[i], m);
+    }
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    if (lane < kLanes && ls.active) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s_dw[wave][ls.off[i / 8] + i % 8] = dw[i];
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < p.head_dim; d += kThreads) {
+        float sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < kThreads / kWave; ++v) sum += s_dw[v][d];
+        p.partial[(int64_t)blockIdx.x * p.head_dim + d] = sum;
+    }
+}
+
+// The workgroups' sums to the weights' gradients, 16 elements of one tensor a workgroup.
+constexpr int kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void rope_weights_kernel(const float* partial, int head_dim, int blocks_q, int blocks_k,
+                                                                   float* dq, float* dk) {
+    __shared__ float s_sum[kSumThreads / 16][17];
+    const int slices = head_dim / 16;
+    const bool k = (int)blockIdx.x >= slices;
+    const int d0 = 16 * ((int)blockIdx.x - (k ? slices : 0));
+    const int col = threadIdx.x % 16, row = threadIdx.x / 16;
+    const int n = k ? blocks_k : blocks_q;
+    const float* src = partial + (int64_t)(k ? blocks_q : 0) * head_dim + d0 + col;
+    float sum = 0.f;
+#pragma unroll 4
+    for (int i = row; i < n; i += kSumThreads / 16) sum += src[(int64_t)i * head_dim];
+    s_sum[row][col] = sum;
+    __syncthreads();
+    for (int m = kSumThreads / 32; m > 0; m /= 2) {
+        if (row < m) s_sum[row][col] += s_sum[row + m][col];
+        __syncthreads();
+    }
+    if (row == 0) (k ? dk : dq)[d0 + col] = s_sum[0][col];
+}
+
+// Calls f with the compile-time lanes of a row, heads of an item and pairing.
+template <typename F>
+void with_shape(const fgqa_rope_args& a, int heads_per, F&& f) {
+    auto heads = [&](auto lanes) {
+        auto pairing = [&](auto h) {
+            if (a.interleaved) f(lanes, h, std::true_type{});
+            else f(lanes, h, std::false_type{});
+        };
+        if (heads_per == 4) pairing(std::integral_constant<int, 4>{});
+        else if (heads_per == 2) pairing(std::integral_constant<int, 2>{});
+        else pairing(std::integral_constant<int, 1>{});
+    };
+    const int lanes = plan::rope_row_lanes(a.head_dim);
+    if (lanes == 4) heads(std::integral_constant<int, 4>{});
+    else if (lanes == 8) heads(std::integral_constant<int, 8>{});
+    else heads(std::integral_constant<int, 16>{});
+}
+
+RopeParams rope_params(const fgqa_rope_args& a, int heads_per) {
+    RopeParams p = {};
+    const int64_t tokens = (int64_t)a.batch * a.seqlen;
+    const int heads[2] = {a.num_q_heads, a.num_kv_heads};
+    const void* weights[2] = {a.q_weight, a.k_weight};
+    for (int i = 0; i < 2; ++i) {
+        Rows& x = p.x[i];
+        x.weight = weights[i];
+        x.heads = heads[i];
+        x.slices = (int)ceil_div(heads[i], heads_per);
+        x.div_slices = make_fast_div(x.slices);
+        x.items = (uint32_t)plan::rope_items(tokens, heads[i], heads_per);
+    }
+    p.positions = a.positions;
+    p.inv_freq = a.inv_freq;
+    p.axes = a.axes;
+    p.pos_a = a.positions_stride[0];
+    p.pos_b = a.positions_stride[1];
+    p.pos_s = a.positions_stride[2];
+    p.pos64 = a.positions_int64;
+    p.weights_bf16 = a.weights_bf16;
+    p.num_axes = a.num_axes;
+    p.seqlen = a.seqlen;
+    p.head_dim = a.head_dim;
+    p.rotary_dim = a.rotary_dim;
+    p.interleaved = a.interleaved;
+    p.div_seqlen = make_fast_div(a.seqlen);
+    p.eps = a.eps;
+    p.inv_dim = 1.f / (float)a.head_dim;
+    p.sin_sign = 1.f;
+    return p;
+}
+
+void set_rows(Rows* x, const void* in, const int64_t (&is)[3], void* out, const int64_t (&os)[3]) {
+    x->in = static_cast<const __bf16*>(in);
+    x->out = static_cast<__bf16*>(out);
+    for (int i = 0; i < 3; ++i) {
+        x->in_s[i] = is[i];
+        x->out_s[i] = os[i];
+    }
+}
+
+template <bool kNorm>
+void launch_rope(const fgqa_rope_args& a, RopeParams p, int heads_per, hipStream_t s) {
+    with_shape(a, heads_per, [&](auto lanes, auto h, auto inter) {
+        constexpr int kLanes = decltype(lanes)::value, kHeads = decltype(h)::value;
+        const int64_t groups = kThreads / kLanes;
+        p.first_k = (unsigned)ceil_div(p.x[0].items, groups);
+        const unsigned grid = p.first_k + (unsigned)ceil_div(p.x[1].items, groups);
+        hipLaunchKernelGGL((rope_kernel<kLanes, kHeads, decltype(inter)::value, kNorm>), dim3(grid), dim3(kThreads), 0, s, p);
+    });
+}
+
+}  // namespace
+}  // namespace fgqa
+
+using namespace fgqa;
+
+extern "C" int fgqa_qk_norm_rope(const fgqa_rope_args* a, void* stream) {
+    const int st = plan::validate_rope(a);
+    if (st != FGQA_OK) return st;
+    if (a->batch == 0 || a->seqlen == 0) return FGQA_OK;
+    const int heads_per = plan::rope_heads_per(*a);
+    RopeParams p = rope_params(*a, heads_per);
+    set_rows(&p.x[0], a->q, a->q_stride, a->q_out, a->q_out_stride);
+    set_rows(&p.x[1], a->k, a->k_stride, a->k_out, a->k_out_stride);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a->q_weight != nullptr) launch_rope<true>(*a, p, heads_per, s);
+    else launch_rope<false>(*a, p, heads_per, s);
+    return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
+}
+
+extern "C" int fgqa_qk_norm_rope_backward_workspace_bytes(const fgqa_rope_backward_args* a, size_t* bytes) {
+    if (a == nullptr || bytes == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
+    const int st = plan::validate_rope_sizes(a->fwd);
+    if (st != FGQA_OK) return st;
+    *bytes = a->fwd.q_weight != nullptr ? plan::rope_grad_plan(a->fwd).ws_bytes : 0;
+    return FGQA_OK;
+}
+
+extern "C" int fgqa_qk_norm_rope_backward(const fgqa_rope_backward_args* a, void* stream) {
+    const int st = plan::validate_rope_backward(a);
+    if (st != FGQA_OK) return st;
+    const fgqa_rope_args& f = a->fwd;
+    const bool norm = f.q_weight != nullptr, empty = f.batch == 0 || f.seqlen == 0;
+    if (empty && !norm) return FGQA_OK;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (!norm) {
+        const int heads_per = plan::rope_heads_per(f);
+        RopeParams p = rope_params(f, heads_per);
+        set_rows(&p.x[0], a->grad_q_out, a->grad_q_out_stride, a->grad_q, a->grad_q_stride);
+        set_rows(&p.x[1], a->grad_k_out, a->grad_k_out_stride, a->grad_k, a->grad_k_stride);
+        p.sin_sign = -1.f;
+        launch_rope<false>(f, p, heads_per, s);
+        return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
+    }
+    const plan::RopeGradPlan pl = plan::rope_grad_plan(f);
+    std::unique_lock<std::mutex> lock;
+    void* ws = a->workspace;
+    if (pl.ws_bytes > 0) {
+        if (ws == nullptr && a->workspace_bytes == 0) {
+            lock = workspace_lock();
+            int got = FGQA_OK;
+            ws = internal_workspace(pl.ws_bytes, &got);
+            if (got != FGQA_OK) return got;
+        } else if (ws == nullptr || a->workspace_bytes < pl.ws_bytes) {
+            return FGQA_ERR_WORKSPACE;
+        } else if ((reinterpret_cast<uintptr_t>(ws) & 255u) != 0) {
+            return FGQA_ERR_UNSUPPORTED;
+        }
+    }
+    const int heads_per = 1;
+    if (!empty) {
+        RopeParams p = rope_params(f, heads_per);
+        set_rows(&p.x[0], f.q, f.q_stride, a->grad_q, a->grad_q_stride);
+        set_rows(&p.x[1], f.k, f.k_stride, a->grad_k, a->grad_k_stride);
+        p.x[0].grad = static_cast<const __bf16*>(a->grad_q_out);
+        p.x[1].grad = static_cast<const __bf16*>(a->grad_k_out);
+        for (int i = 0; i < 3; ++i) {
+            p.x[0].grad_s[i] = a->grad_q_out_stride[i];
+            p.x[1].grad_s[i] = a->grad_k_out_stride[i];
+        }
+        p.partial = static_cast<float*>(ws);
+        p.first_k = (unsigned)pl.blocks[0];
+        with_shape(f, heads_per, [&](auto lanes, auto h, auto inter) {
+            hipLaunchKernelGGL((rope_backward_kernel<decltype(lanes)::value, decltype(h)::value, decltype(inter)::value>),
+                               dim3((unsigned)(pl.blocks[0] + pl.blocks[1])), dim3(kThreads), 0, s, p);
+        });
+    }
+    hipLaunchKernelGGL(rope_weights_kernel, dim3((unsigned)(2 * (f.head_dim / 16))), dim3(kSumThreads), 0, s,
+                       static_cast<const float*>(ws), f.head_dim, pl.blocks[0], pl.blocks[1], a->grad_q_weight,
+                       a->grad_k_weight);
+    return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
+}

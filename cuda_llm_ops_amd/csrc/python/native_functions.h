@@ -1,0 +1,13 @@
+// The native module's functions of other files: positional arguments as their Python
+// callers pass them.
+#pragma once
+
+#include <Python.h>
+
+namespace fgqa_native {
+
+// rope_native.cpp
+PyObject* rope(PyObject* const* o);
+PyObject* rope_backward(PyObject* const* o);
+
+}  // namespace fgqa_native
