@@ -2,7 +2,7 @@
 
 The kernels live in libfgqa.so (HIP, gfx950); ``flash_gqa`` is the Python host
 interface over its C ABI (include/fgqa.h), ``kv_cache`` that of the paged
-cache's operators (include/fgqa_kv.h) and ``qk_rope`` that of the norm and rotation
+cache's operators (include/fgqa_kv.h, include/fgqa_pages.h) and ``qk_rope`` that of the norm and rotation
 of queries and keys (include/fgqa_rope.h).
 """
 from ._lib import FgqaError, LIB_PATH, lib, native, status_string  # noqa: F401
@@ -37,7 +37,9 @@ from .flash_gqa import (  # noqa: F401
 from .kv_cache import (  # noqa: F401
     accumulate_kv_weights_paged,
     append_kv_paged,
+    compact_kv_paged,
     evict_kv_paged,
+    fork_kv_paged,
 )
 from .qk_rope import (  # noqa: F401
     qk_norm_rope,

@@ -491,27 +491,6 @@ __global__ __launch_bounds__(kPair ? 2 * kDecThreads : kDecThreads) void decode_
 constexpr int kPlanThreads = 256;
 constexpr int kPlanSortMax = 1024;   // remainders kept in LDS and length-sorted up to this batch size
 
-// Exclusive prefix sum of one value per thread over a workgroup of kThreads.
-// kAgain: another scan in s_wave follows (else a barrier does before s_wave's
-// memory is written again).
-template <int kThreads, bool kAgain, typename T>
-__device__ __forceinline__ T block_exclusive_scan(T v, T* s_wave, T* total) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = threadIdx.x / kWave;
-    const T incl = wave_fold(v, [](T a, T b) { return a + b; });
-    if (lane == kWave - 1) s_wave[wave] = incl;
-    __syncthreads();
-    T base = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / kWave; ++w) {
-        base += (w < wave) ? s_wave[w] : 0;
-        all += s_wave[w];
-    }
-    if constexpr (kAgain) __syncthreads();
-    *total = all;
-    return base + incl - v;
-}
-
 __global__ __launch_bounds__(kPlanThreads) void decode_plan_kernel(DecodeParams p, int32_t* work) {
     __shared__ int s_wave[kPlanThreads / kWave];
     __shared__ int s_rem[kPlanSortMax];   // len % chunk per sequence (batch <= kPlanSortMax)

@@ -31,8 +31,17 @@ bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0
 
 bool finite_positive(float x) { return isfinite(x) && x > 0.f; }
 
-// The cache's sizes, type, strides and which scales there are.
-// writes: codes are written, so a scale for the whole cache divides.
+// A launch has fewer than 2^31 workgroups and 2^32 threads.
+bool grid_ok(i128 workgroups, int threads) {
+    return workgroups < kLim31 && workgroups * threads < ((i128)1 << 32);
+}
+
+// Blocks of the append's and the eviction's pages.
+bool blocks_ok(i128 blocks, int page_size) {
+    return blocks < kLim31 && grid_ok(page_size <= kWavePageRows ? (blocks + 3) / 4 : blocks, 256);
+}
+}  // namespace
+
 int validate_cache(const fgqa_kv_cache& c, bool with_v, bool writes) {
     if (c.num_kv_heads <= 0 || c.head_dim <= 0 || c.page_size <= 0 || c.num_pages < 0) return FGQA_ERR_INVALID_ARGUMENT;
     if (c.kv_dtype != FGQA_KV_BF16 && c.kv_dtype != FGQA_KV_FP8_E4M3 && c.kv_dtype != FGQA_KV_INT8)
@@ -68,21 +77,9 @@ int validate_cache_pointers(const fgqa_kv_cache& c, bool with_v) {
     return FGQA_OK;
 }
 
-// K's and V's data and block scales, which the call writes, are not the same memory.
 bool written_apart(const fgqa_kv_cache& c) {
     return c.k != c.v && (c.k_scales == nullptr || c.k_scales != c.v_scales);
 }
-
-// A launch has fewer than 2^31 workgroups and 2^32 threads.
-bool grid_ok(i128 workgroups, int threads) {
-    return workgroups < kLim31 && workgroups * threads < ((i128)1 << 32);
-}
-
-// Blocks of the append's and the eviction's pages.
-bool blocks_ok(i128 blocks, int page_size) {
-    return blocks < kLim31 && grid_ok(page_size <= kWavePageRows ? (blocks + 3) / 4 : blocks, 256);
-}
-}  // namespace
 
 int validate_kv_append(const fgqa_kv_append_args* a) {
     if (a == nullptr) return FGQA_ERR_INVALID_ARGUMENT;

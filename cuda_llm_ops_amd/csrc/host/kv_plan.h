@@ -8,6 +8,13 @@
 namespace fgqa {
 namespace plan {
 
+// The cache's sizes, type, strides and which scales there are.
+// writes: codes are written, so a scale for the whole cache divides.
+int validate_cache(const fgqa_kv_cache& c, bool with_v, bool writes);
+int validate_cache_pointers(const fgqa_kv_cache& c, bool with_v);
+// K's and V's data and block scales, which the call writes, are not the same memory.
+bool written_apart(const fgqa_kv_cache& c);
+
 // Sizes and addresses of a call; FGQA_OK with batch (or what it would write)
 // zero, where nothing is launched and no address is looked at.
 int validate_kv_append(const fgqa_kv_append_args* a);

@@ -311,7 +311,8 @@ constexpr PyMethodDef method(const char* name) {
 
 PyMethodDef g_methods[] = {method<append, 9>("append"),   method<decode, 14>("decode"), method<weights, 9>("weights"),
                            method<evict, 14>("evict"),    method<rope, 11>("rope"),     method<rope_backward, 11>("rope_backward"),
-                           method<bind, 3>("bind"),       {nullptr, nullptr, 0, nullptr}};
+                           method<fgqa_native::fork, 13>("fork"),      method<compact, 9>("compact"), method<bind, 3>("bind"),
+                           {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_kv_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -10,4 +10,8 @@ namespace fgqa_native {
 PyObject* rope(PyObject* const* o);
 PyObject* rope_backward(PyObject* const* o);
 
+// pages_native.cpp
+PyObject* fork(PyObject* const* o);
+PyObject* compact(PyObject* const* o);
+
 }  // namespace fgqa_native

@@ -1,4 +1,4 @@
-"""The paged KV cache's operators, over the C ABI of include/fgqa_kv.h.
+"""The paged KV cache's operators, over the C ABI of include/fgqa_kv.h and include/fgqa_pages.h.
 
 A paged cache is a pair of tensors [num_pages, page_size, Hkv, 128] (bf16,
 torch.float8_e4m3fn or torch.int8) and a block table int32 [B, max_pages]: token
@@ -7,13 +7,15 @@ t of sequence b is slot t % page_size of page block_table[b, t // page_size].
 [num_pages, Hkv], a scale for each page of each KV head, or (float8_e4m3fn
 only) two numbers for the whole cache.  A tensor of one element counts as a number
 (the host reads it), unless both are the [num_pages, Hkv] scales of a cache of one
-page and head.  Calls that write a cache (append, evict) refuse K and V caches or
+page and head.  Calls that write a cache (append, evict, fork, compact) refuse K and V caches or
 scales that share memory.
 
     append_kv_paged              writes new tokens
     flash_gqa.decode_flash_gqa_paged   single-token attention
     accumulate_kv_weights_paged  the attention weight each cached token got
     evict_kv_paged               cuts sequences to a budget of tokens by weight
+    fork_kv_paged                rows that go on from others and share their pages; pages for new tokens
+    compact_kv_paged             moves the pages in use together
 
 No counterpart in the reference.  PyTorch only provides device memory and the
 current stream.  Every tensor of a call lives on one device; the call runs on that
@@ -26,7 +28,7 @@ import torch
 from . import _lib
 from .flash_gqa import PreparedLaunch, _get_device, _stream
 
-__all__ = ["append_kv_paged", "accumulate_kv_weights_paged", "evict_kv_paged"]
+__all__ = ["append_kv_paged", "accumulate_kv_weights_paged", "evict_kv_paged", "fork_kv_paged", "compact_kv_paged"]
 
 
 class DeviceLaunch(PreparedLaunch):
@@ -115,3 +117,43 @@ def evict_kv_paged(k_cache, v_cache, block_table, seqlens, weights, new_block_ta
     shares.  Blocks with scales are scaled anew, as in ``append_kv_paged``."""
     return call_native("evict", k_cache, k_cache, v_cache, block_table, seqlens, weights, new_block_table, budget, recent,
                        k_scale, v_scale, new_seqlens, new_weights, kept, max_seqlen)
+
+
+def fork_kv_paged(k_cache, v_cache, block_table, seqlens, parents=None, new_lens=None, held=None, max_pages=None,
+                  k_scale=1.0, v_scale=1.0, new_block_table=None, new_seqlens=None, num_free=None):
+    """Sequences that go on from others, and pages for their new tokens; returns
+    (new_block_table, new_seqlens, num_free).
+
+    parents: int32 [N]: new row i goes on from row parents[i] of block_table (None: row i
+    from row i); several may go on from one (samples, beams), a row that no new one goes
+    on from is dropped, and -1 is a new, empty sequence.  new_lens: int32 [N], the tokens
+    that each new row gets pages for (None: 0).
+
+    Full pages are shared.  A partly filled last page goes to the first new row of its old
+    one, the others get a page of their own with a copy of its filled slots and scales, so
+    that every row may be appended to.  Pages of its own are free ones, in ascending order:
+    those that no new row has from block_table, and that ``held`` (bool or uint8
+    [num_pages]: in use elsewhere, such as kept prefixes) does not name.  So the
+    pages of dropped rows are free at once.  A held page is copied rather than filled.
+
+    new_block_table: int32 [N, max_pages] (block_table's width when None), -1 past a row's
+    pages; new_seqlens: int32 [N], the tokens that the rows hold (without the new ones);
+    num_free: int32 [1], the free pages that are left or, below 0, missing: the last
+    cells are -1 then, and their tokens are not written by ``append_kv_paged``.  A partly
+    filled page must be in one place of block_table only, as this function leaves them."""
+    return call_native("fork", k_cache, k_cache, v_cache, block_table, seqlens, parents, new_lens, held, max_pages, k_scale,
+                       v_scale, new_block_table, new_seqlens, num_free)
+
+
+def compact_kv_paged(k_cache, v_cache, block_table, seqlens, held=None, k_scale=1.0, v_scale=1.0, new_block_table=None,
+                     num_used=None):
+    """Moves the pages in use to the lowest page numbers; returns (new_block_table, num_used).
+
+    In use are the pages that hold the sequences' tokens (``seqlens`` of them; shared ones
+    once).  Pages past their number move, in ascending order, to the free ones before it; the
+    others stay, and so do those that ``held`` names.  new_block_table: int32, block_table's
+    shape, -1 in cells past the tokens (pages for further tokens come from
+    ``fork_kv_paged``); num_used: int32 [1]: all pages from there on are free.  Pages that
+    were left keep their bytes."""
+    return call_native("compact", k_cache, k_cache, v_cache, block_table, seqlens, held, k_scale, v_scale, new_block_table,
+                       num_used)
