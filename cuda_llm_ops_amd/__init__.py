@@ -38,6 +38,7 @@ from .kv_cache import (  # noqa: F401
     accumulate_kv_weights_paged,
     append_kv_paged,
     compact_kv_paged,
+    decode_flash_gqa_paged_shared,
     evict_kv_paged,
     fork_kv_paged,
 )

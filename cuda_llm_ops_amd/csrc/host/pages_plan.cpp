@@ -118,5 +118,78 @@ int validate_kv_compact(const fgqa_kv_compact_args* a) {
     return FGQA_OK;
 }
 
+fgqa_decode_paged_args as_decode_paged(const fgqa_decode_shared_args* a) {
+    fgqa_decode_blocks_args b = {};
+    b.cache = a->cache;
+    b.q = a->q;
+    b.o = a->o;
+    b.lse = a->lse;
+    b.block_table = a->block_table;
+    b.seqlens = a->seqlens;
+    b.batch = a->batch;
+    b.max_seqlen = a->max_seqlen;
+    b.num_q_heads = a->num_q_heads;
+    b.scale = a->scale;
+    for (int i = 0; i < 2; ++i) {
+        b.q_stride[i] = a->q_stride[i];
+        b.o_stride[i] = a->o_stride[i];
+    }
+    b.block_table_stride = a->block_table_stride;
+    fgqa_decode_paged_args p = as_decode_paged(&b);
+    if (a->cache.kv_dtype == FGQA_KV_BF16) p.kv_dtype = FGQA_KV_BF16;
+    if (a->cache.kv_dtype == FGQA_KV_FP8_E4M3 && a->cache.k_scales == nullptr) {
+        p.k_scale = a->cache.k_scale;
+        p.v_scale = a->cache.v_scale;
+    }
+    return p;
+}
+
+int validate_decode_shared(const fgqa_decode_shared_args* a) {
+    if (a == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
+    int st = validate_cache(a->cache, true, false);
+    if (st != FGQA_OK) return st;
+    const fgqa_decode_paged_args p = as_decode_paged(a);
+    st = validate_paged(&p);
+    if (st != FGQA_OK) return st;
+    if (a->num_groups < 0) return FGQA_ERR_INVALID_ARGUMENT;
+    // (the merge's grid has a row for each sequence)
+    return a->num_groups <= kSharedMaxGroups && a->batch < (1 << 15) ? FGQA_OK : FGQA_ERR_UNSUPPORTED;
+}
+
+int validate_decode_shared_pointers(const fgqa_decode_shared_args* a) {
+    const fgqa_decode_paged_args p = as_decode_paged(a);
+    int st = validate_paged_pointers(&p);
+    if (st != FGQA_OK || a->batch == 0) return st;
+    if (a->num_groups > 0) {
+        if (a->group_starts == nullptr || a->shared_lens == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
+        if (!aligned4(a->group_starts) || !aligned4(a->shared_lens)) return FGQA_ERR_UNSUPPORTED;
+    }
+    return a->max_seqlen == 0 ? FGQA_OK : validate_cache_pointers(a->cache, true);
+}
+
+// With C tokens a chunk, C >= (all rows of tiles' and sequences' tokens) / slots, the items of one
+// KV head are at most slots + tiles + sequences (each cut leaves one rest), and their
+// rows of partials, at most 128 (and the batch's) a tile's chunk and the group's a sequence's.
+int plan_decode_shared(const fgqa_decode_shared_args* a, int cus, SharedPlan* plan) {
+    if (cus <= 0) cus = 256;
+    const int64_t hkv = a->cache.num_kv_heads, group = a->num_q_heads / hkv;
+    const int64_t rows = (int64_t)a->batch * group;   // of one KV head
+    const int64_t tiles = rows / kSharedRows + (a->num_groups < a->batch ? a->num_groups : a->batch);
+    const int64_t slots = ceil_div(2 * (int64_t)cus, hkv);
+    const int64_t items = slots + tiles + a->batch;
+    if ((i128)items * hkv >= ((i128)1 << 24)) return FGQA_ERR_UNSUPPORTED;
+    plan->slots = (int)slots;
+    plan->max_items = (int)items;
+    plan->max_rows = hkv * (slots * (rows < kSharedRows ? (rows > group ? rows : group) : kSharedRows) + 2 * rows);
+    if (plan->max_rows >= ((int64_t)1 << 31)) return FGQA_ERR_UNSUPPORTED;
+    auto round = [](size_t n) { return (n + 255) / 256 * 256; };
+    plan->part_ml_off = round((size_t)plan->max_rows * kHeadDim * 4);
+    plan->items_off = plan->part_ml_off + round((size_t)plan->max_rows * 2 * 4);
+    plan->seqs_off = plan->items_off + round((size_t)items * kSharedItemInts * 4);
+    plan->count_off = plan->seqs_off + round((size_t)a->batch * kSharedSeqInts * 4);
+    plan->total = plan->count_off + 256;
+    return FGQA_OK;
+}
+
 }  // namespace plan
 }  // namespace fgqa

@@ -36,5 +36,37 @@ int validate_kv_compact(const fgqa_kv_compact_args* a);
 int validate_kv_fork_sizes(const fgqa_kv_fork_args* a);
 int validate_kv_compact_sizes(const fgqa_kv_compact_args* a);
 
+// ---------------------------------------------------------------- decode of sequences that begin alike
+constexpr int kSharedRows = 128;       // query rows (sequences times heads of a KV head) of a workgroup
+constexpr int kSharedMaxGroups = 4096;
+constexpr int kSharedChunk = 128;      // tokens that the work is cut in multiples of
+
+// Tokens of a cut, of `total` of all row tiles and sequences.
+constexpr int64_t shared_chunk(int64_t total, int slots) {
+    const int64_t even = (total + slots - 1) / slots;
+    const int64_t c = (even + kSharedChunk - 1) / kSharedChunk * kSharedChunk;
+    return c < kSharedChunk ? kSharedChunk : c;
+}
+// What a range of n > 0 tokens is cut into: equal pieces of a multiple of `step` that are
+// at most a chunk (a multiple of step).
+constexpr int64_t shared_piece(int64_t n, int64_t chunk, int step) {
+    const int64_t pieces = (n + chunk - 1) / chunk;
+    return ((n + pieces - 1) / pieces + step - 1) / step * step;
+}
+
+// Sizes that a call's kernels and workspace are bounded by, whatever the lengths.
+struct SharedPlan {
+    int slots;             // workgroups of one KV head that run at once
+    int max_items;         // of one KV head
+    int64_t max_rows;      // of partials
+    size_t part_ml_off, items_off, seqs_off, count_off, total;   // bytes; partial O at 0
+};
+constexpr int kSharedItemInts = 8, kSharedSeqInts = 8;
+// What the decode checks of its arguments, an e4m3 cache of the same sizes for int8.
+fgqa_decode_paged_args as_decode_paged(const fgqa_decode_shared_args* a);
+int validate_decode_shared(const fgqa_decode_shared_args* a);
+int validate_decode_shared_pointers(const fgqa_decode_shared_args* a);
+int plan_decode_shared(const fgqa_decode_shared_args* a, int cus, SharedPlan* plan);
+
 }  // namespace plan
 }  // namespace fgqa

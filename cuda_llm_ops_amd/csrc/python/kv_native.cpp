@@ -309,9 +309,16 @@ constexpr PyMethodDef method(const char* name) {
     return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<f, kArgs>)), METH_FASTCALL, nullptr};
 }
 
-PyMethodDef g_methods[] = {method<append, 9>("append"),   method<decode, 14>("decode"), method<weights, 9>("weights"),
-                           method<evict, 14>("evict"),    method<rope, 11>("rope"),     method<rope_backward, 11>("rope_backward"),
-                           method<fgqa_native::fork, 13>("fork"),      method<compact, 9>("compact"), method<bind, 3>("bind"),
+PyMethodDef g_methods[] = {method<append, 9>("append"),
+                           method<decode, 14>("decode"),
+                           method<weights, 9>("weights"),
+                           method<evict, 14>("evict"),
+                           method<rope, 11>("rope"),
+                           method<rope_backward, 11>("rope_backward"),
+                           method<fgqa_native::fork, 13>("fork"),
+                           method<compact, 9>("compact"),
+                           method<decode_shared, 14>("decode_shared"),
+                           method<bind, 3>("bind"),
                            {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_kv_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

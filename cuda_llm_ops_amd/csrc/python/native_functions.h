@@ -13,5 +13,6 @@ PyObject* rope_backward(PyObject* const* o);
 // pages_native.cpp
 PyObject* fork(PyObject* const* o);
 PyObject* compact(PyObject* const* o);
+PyObject* decode_shared(PyObject* const* o);
 
 }  // namespace fgqa_native

@@ -172,4 +172,76 @@ PyObject* compact(PyObject* const* o) {
     return Py_BuildValue("(NN)", THPVariable_Wrap(new_table), THPVariable_Wrap(num_used));
 }
 
+// decode_shared(q, k_cache, v_cache, block_table, seqlens, group_starts, shared_lens, scale, k_scale, v_scale, out, lse,
+//               max_seqlen, workspace) -> out
+PyObject* decode_shared(PyObject* const* o) {
+    const at::Tensor &q = tensor(o[0], "q"), &kc = tensor(o[1], "k_cache"), &vc = tensor(o[2], "v_cache");
+    const at::Tensor &table = tensor(o[3], "block_table"), &lens = tensor(o[4], "seqlens");
+    const at::Tensor &starts = tensor(o[5], "group_starts"), &shared = tensor(o[6], "shared_lens");
+    if (q.scalar_type() != at::kBFloat16) refuse("paged decode expects a bf16 query");
+    if (q.dim() != 3) refuse("expected q [B,Hq,D] and k_cache/v_cache [num_pages, page_size, Hkv, D]");
+    fgqa_decode_shared_args a;
+    std::memset(&a, 0, sizeof a);
+    a.cache = check_caches(kc, &vc, o[8], o[9]);
+    const int64_t B = a.batch = check_batch(q.size(0));
+    const int64_t Hq = q.size(1);
+    if (q.size(2) != 128) refuse("the caches' head_dim must match Q");
+    if (Hq < 1 || Hq > INT_MAX || Hq % kc.size(2) != 0) refuse("Query heads must be divisible by KV heads");
+    int64_t pages;
+    a.block_table_stride = check_table(table, B, "block_table", &pages);
+    a.seqlens = check_lens(lens, B, "seqlens");
+    if (shared.dim() != 1) refuse("shared_lens must be a contiguous int32 tensor of one dim");
+    const int64_t N = shared.size(0);
+    if (N > 4096) refuse("at most 4096 groups");
+    a.num_groups = (int32_t)N;
+    a.shared_lens = check_lens(shared, N, "shared_lens");
+    if (starts.scalar_type() != at::kInt || starts.dim() != 1 || starts.size(0) != N + 1 || !starts.is_contiguous())
+        refuse("group_starts must be a contiguous int32 tensor of one element more than shared_lens");
+    a.group_starts = int32s(starts);
+    const int64_t tokens = table_tokens(pages, a.cache);
+    a.max_seqlen = check_max_seqlen(o[12], tokens, tokens);
+    at::Tensor out, work;
+    if (o[10] != Py_None) {
+        out = tensor(o[10], "out");
+        if (out.scalar_type() != at::kBFloat16 || out.sizes() != q.sizes() || !kernel_ready(out))
+            refuse("out must be a bf16 [B, Hq, D] tensor with contiguous rows");
+        check_out(out, "out", {o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[8], o[9], o[11], o[13]});
+    }
+    if (o[11] != Py_None) {
+        const at::Tensor& lse = tensor(o[11], "lse");
+        if (lse.scalar_type() != at::kFloat || lse.dim() != 2 || lse.size(0) != B || lse.size(1) != Hq || !lse.is_contiguous())
+            refuse("lse must be a contiguous fp32 [B, Hq] tensor");
+        check_out(lse, "lse", {o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[8], o[9], o[13]});
+        a.lse = floats(lse);
+    }
+    if (o[13] != Py_None) {
+        work = tensor(o[13], "workspace");
+        if (!work.is_contiguous()) refuse("workspace must be contiguous");
+        check_out(work, "workspace", {o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[8], o[9]});
+        a.workspace = address(work);
+        a.workspace_bytes = (size_t)work.numel() * work.element_size();
+    }
+    Device dev;
+    for (const at::Tensor* t : {&q, &kc, &vc, &table, &lens, &starts, &shared}) dev.add(*t);
+    for (PyObject* x : {blocks_or_none(a.cache.k_scales, o[8]), blocks_or_none(a.cache.v_scales, o[9]), o[10], o[11], o[13]})
+        dev.add_if(x);
+    void* stream = nullptr;
+    if (!dev.current(&stream)) return not_here();
+    const at::Tensor qr = ready(q);
+    if (!out.defined()) out = at::empty(q.sizes(), q.options());
+    a.q = address(qr);
+    a.o = address(out);
+    for (int i = 0; i < 2; ++i) {
+        a.q_stride[i] = qr.stride(i);
+        a.o_stride[i] = out.stride(i);
+    }
+    a.block_table = int32s(table);
+    a.num_q_heads = (int32_t)Hq;
+    a.scale = o[7] == Py_None ? (float)(1.0 / std::sqrt(128.0)) : (float)number(o[7]);
+    if (!work.defined() && B > 0) work = workspace_of(fgqa_decode_shared_workspace_bytes, &a, q, "fgqa_decode_shared_workspace_bytes");
+    launch(fgqa_decode_shared, a, stream, "fgqa_decode_shared");
+    for (PyObject* x : {o[10], o[11]}) written_if(x);
+    return THPVariable_Wrap(out);
+}
+
 }  // namespace fgqa_native

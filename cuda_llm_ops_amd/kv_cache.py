@@ -14,6 +14,7 @@ scales that share memory.
     flash_gqa.decode_flash_gqa_paged   single-token attention
     accumulate_kv_weights_paged  the attention weight each cached token got
     evict_kv_paged               cuts sequences to a budget of tokens by weight
+    decode_flash_gqa_paged_shared      the same for sequences that begin alike
     fork_kv_paged                rows that go on from others and share their pages; pages for new tokens
     compact_kv_paged             moves the pages in use together
 
@@ -28,7 +29,8 @@ import torch
 from . import _lib
 from .flash_gqa import PreparedLaunch, _get_device, _stream
 
-__all__ = ["append_kv_paged", "accumulate_kv_weights_paged", "evict_kv_paged", "fork_kv_paged", "compact_kv_paged"]
+__all__ = ["append_kv_paged", "accumulate_kv_weights_paged", "evict_kv_paged", "decode_flash_gqa_paged_shared",
+           "fork_kv_paged", "compact_kv_paged"]
 
 
 class DeviceLaunch(PreparedLaunch):
@@ -157,3 +159,25 @@ def compact_kv_paged(k_cache, v_cache, block_table, seqlens, held=None, k_scale=
     were left keep their bytes."""
     return call_native("compact", k_cache, k_cache, v_cache, block_table, seqlens, held, k_scale, v_scale, new_block_table,
                        num_used)
+
+
+def decode_flash_gqa_paged_shared(q, k_cache, v_cache, block_table, seqlens, group_starts, shared_lens, scale=None,
+                                  k_scale=1.0, v_scale=1.0, out=None, lse=None, max_seqlen=None, workspace=None):
+    """``decode_flash_gqa_paged`` for sequences that begin alike (samples of one prompt,
+    beams, questions on one document): what a group's sequences share is read once for
+    all of them.  Returns ``out``.
+
+    group_starts: int32 [N + 1], ascending, group n being sequences group_starts[n] ..
+    group_starts[n + 1] - 1 (those before the first and from the last on are on their own);
+    shared_lens: int32 [N], tokens for which the rows of block_table of a group's sequences
+    name the same pages, as ``fork_kv_paged`` leaves them: the pages of its
+    first sequence of any length are read for all.  Whole pages are taken of it, as far as
+    the group's shortest sequence reaches (empty ones aside).
+
+    The other arguments are those of ``decode_flash_gqa_paged``, over any cache (bf16, e4m3,
+    int8); lse: fp32 [B, Hq]; max_seqlen: at most the block table's tokens.  The workspace
+    (allocated when None) is 256-byte aligned; calls that may run at the same time
+    need one each.  Results may differ in rounding from those of ``decode_flash_gqa_paged``, and
+    with the other sequences of the batch."""
+    return call_native("decode_shared", q, q, k_cache, v_cache, block_table, seqlens, group_starts, shared_lens, scale,
+                       k_scale, v_scale, out, lse, max_seqlen, workspace)

@@ -105,6 +105,50 @@ int fgqa_kv_compact_workspace_bytes(const fgqa_kv_compact_args* args, size_t* by
 
 int fgqa_kv_compact(const fgqa_kv_compact_args* args, void* stream);
 
+/*
+ * Single-token attention over a paged cache, as fgqa_decode_paged and
+ * fgqa_decode_blocks, for sequences that begin alike: what group n's sequences,
+ * group_starts[n] .. group_starts[n + 1] - 1, share is read once for all of them.
+ *
+ *   group_starts  device int32 [num_groups + 1], ascending (each taken as at least the
+ *                 one before it, and as at most the batch); sequences outside have nothing in common
+ *   shared_lens   device int32 [num_groups]: the group's sequences of at least one token have the
+ *                 same pages for their first shared_lens[n] tokens: those of the
+ *                 first of them are read for all.  What is taken of it is whole pages, at most the shortest such
+ *                 sequence; a value of 0 or less is nothing.
+ *   cache         any of fgqa_kv.h's (v is read only, as K is)
+ *   q, o, lse, block_table, seqlens, max_seqlen, scale   as fgqa_decode_paged
+ *   workspace     256-byte aligned, fgqa_decode_shared_workspace_bytes (it depends on the
+ *                 sizes and the device, not on lengths); NULL and 0: the library's buffer
+ * Sums and statistics are fp32; P (times V's scale) is rounded to bf16 for P.V over
+ * shared tokens.  The work is cut as the lengths of all sequences ask: outputs may differ in
+ * rounding between batches, not between runs of one.  num_groups is at most 4096.
+ */
+typedef struct fgqa_decode_shared_args {
+    fgqa_kv_cache cache;
+    const void* q;
+    void* o;
+    float* lse;
+    const int32_t* block_table;
+    const int32_t* seqlens;
+    const int32_t* group_starts;
+    const int32_t* shared_lens;
+    int32_t batch;
+    int32_t max_seqlen;
+    int32_t num_q_heads;
+    int32_t num_groups;
+    float scale;
+    int64_t q_stride[2];
+    int64_t o_stride[2];
+    int64_t block_table_stride;
+    void* workspace;
+    size_t workspace_bytes;
+} fgqa_decode_shared_args;
+
+int fgqa_decode_shared_workspace_bytes(const fgqa_decode_shared_args* args, size_t* bytes);
+
+int fgqa_decode_shared(const fgqa_decode_shared_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
