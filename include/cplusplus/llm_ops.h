@@ -7,4 +7,6 @@
 #include "FlashGQA/flash_gqa_backward_kernel.h"
 #include "FlashGQA/flash_gqa_forward_kernel.h"
 #include "FlashGQA/kv_cache_kernel.h"
+#include "FlashGQA/kv_pages_kernel.h"
+#include "FlashGQA/qk_norm_rope_kernel.h"
 #include "Utils/utils.h"
