@@ -22,8 +22,7 @@ namespace fgqa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 64;             // shared tokens of a step
-constexpr int kPlanThreads = 1024;
+constexpr int kTile = 64, kBlock = 32;   // shared tokens of a barrier, and of a step
 
 // What runs on one workgroup for each KV head.
 struct Item {
@@ -53,6 +52,8 @@ struct SharedParams {
     const int32_t* shared_lens;
     int num_groups, slots;
     FastDiv div_group, div_hkv;
+    float scale_log2;    // shared tokens of caches without block scales: not negative, Q negated instead
+    uint32_t q_sign;
     Item* items;
     Seq* seqs;
     int32_t* count;
@@ -71,68 +72,75 @@ __device__ __forceinline__ int group_of(const int* starts, int n, int b) {
     return lo;
 }
 
-// Latency bounds it: a few dependent loads and scans of one workgroup.
+// Latency bounds it: a few dependent loads, barriers and scans of one workgroup, which
+// takes a thread for each group and sequence as far as they go (256 threads for up to 256 of each: a barrier of
+// 4 waves costs less than one of 16).
+template <int kPlanThreads>
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p) {
-    __shared__ int s_start[plan::kSharedMaxGroups + 1];
-    __shared__ int s_len[plan::kSharedMaxGroups];     // shortest of its sequences, then what is shared
-    __shared__ int s_first[plan::kSharedMaxGroups];   // its first sequence with tokens
-    __shared__ int s_more[plan::kSharedMaxGroups];    // its last one
-    __shared__ int64_t s_wave64[kPlanThreads / kWave];
-    __shared__ int s_wave[kPlanThreads / kWave];
+    constexpr int kGroups = kPlanThreads == 256 ? 256 : plan::kSharedMaxGroups;
+    __shared__ int s_start[kGroups + 1];
+    __shared__ int s_len[kGroups];     // shortest of its sequences, then what is shared
+    __shared__ int s_first[kGroups];   // its first sequence with tokens, then its first row of partials
+    __shared__ int s_count[kGroups];   // its sequences with tokens, then its pieces
+    __shared__ int64_t s_wave[kPlanThreads / kWave];
     const int tid = threadIdx.x, n = p.num_groups, batch = p.d.batch, group = p.d.group, hkv = p.d.hkv;
+    // (these loads are under way together)
+    const int len0 = tid < batch ? clamp_len(p.d, tid) : 0;
+    const int shared0 = tid < n ? p.shared_lens[tid] : 0;
     for (int i = tid; i <= n; i += kPlanThreads) {
         s_start[i] = n > 0 ? min(max(p.group_starts[i], 0), batch) : 0;
         if (i < n) {
             s_len[i] = s_first[i] = INT32_MAX;
-            s_more[i] = -1;
+            s_count[i] = 0;
         }
     }
     __syncthreads();
-    // each start at least the one before it
-    for (int d = 1; d <= n; d *= 2) {
-        int v[plan::kSharedMaxGroups / kPlanThreads + 1];
-        int k = 0;
-        for (int i = tid; i <= n; i += kPlanThreads) v[k++] = max(s_start[i], i >= d ? s_start[i - d] : 0);
-        __syncthreads();
-        k = 0;
-        for (int i = tid; i <= n; i += kPlanThreads) s_start[i] = v[k++];
-        __syncthreads();
+    int falls = 0;
+    for (int i = tid; i < n; i += kPlanThreads) falls |= s_start[i + 1] < s_start[i];
+    if (__syncthreads_or(falls)) {   // each start at least the one before it
+        for (int d = 1; d <= n; d *= 2) {
+            int v[kGroups / kPlanThreads + 1];
+            int k = 0;
+            for (int i = tid; i <= n; i += kPlanThreads) v[k++] = max(s_start[i], i >= d ? s_start[i - d] : 0);
+            __syncthreads();
+            k = 0;
+            for (int i = tid; i <= n; i += kPlanThreads) s_start[i] = v[k++];
+            __syncthreads();
+        }
     }
+    int64_t sum = 0, total;
     for (int b = tid; b < batch; b += kPlanThreads) {
-        const int len = clamp_len(p.d, b), g = group_of(s_start, n, b);
+        const int len = b == tid ? len0 : clamp_len(p.d, b), g = group_of(s_start, n, b);
+        sum += len;
         if (g < 0 || len == 0) continue;
         atomicMin(&s_len[g], len);
         atomicMin(&s_first[g], b);
-        atomicMax(&s_more[g], b);
+        atomicAdd(&s_count[g], 1);
     }
     __syncthreads();
-    int64_t sum = 0, total;
-    auto tiles_of = [&](int g) {
-        return (int)(((int64_t)(s_start[g + 1] - s_start[g]) * group + plan::kSharedRows - 1) / plan::kSharedRows);
-    };
+    auto rows_of = [&](int g) { return (s_start[g + 1] - s_start[g]) * group; };
+    auto tiles_of = [&](int g) { return (rows_of(g) + plan::kSharedRows - 1) / plan::kSharedRows; };
     for (int g = tid; g < n; g += kPlanThreads) {
         // (one sequence shares with none)
-        int len = s_more[g] > s_first[g] ? min(s_len[g], p.shared_lens[g]) : 0;
+        int len = s_count[g] > 1 ? min(s_len[g], g == tid ? shared0 : p.shared_lens[g]) : 0;
         len = max(len, 0) >> p.d.page_shift << p.d.page_shift;
-        s_len[g] = len < plan::kSharedChunk ? 0 : len;
-        sum += (int64_t)tiles_of(g) * s_len[g];
+        if (len < plan::kSharedChunk) len = 0;
+        s_len[g] = len;
+        sum += (int64_t)(tiles_of(g) - s_count[g]) * len;   // in the tiles instead of each sequence
     }
-    __syncthreads();
-    for (int b = tid; b < batch; b += kPlanThreads) {
-        const int g = group_of(s_start, n, b), len = clamp_len(p.d, b);
-        if (len > 0) sum += len - (g < 0 ? 0 : s_len[g]);
-    }
-    block_exclusive_scan<kPlanThreads, true>(sum, s_wave64, &total);
-    const int64_t chunk = plan::shared_chunk(total, p.slots);
-    int item = 0, row = 0;   // so far
+    block_exclusive_scan<kPlanThreads, true>(sum, s_wave, &total);
+    const int chunk = (int)min(plan::shared_chunk(total, p.slots), (int64_t)1 << 30);   // (longer than any sequence)
+    // Offsets of items, and, 32 bits up, of rows.
+    int64_t at = 0;
     for (int g0 = 0; g0 < n; g0 += kPlanThreads) {
         const int g = g0 + tid;
-        const int len = g < n ? s_len[g] : 0, tiles = len > 0 ? tiles_of(g) : 0;
-        const int rows = len > 0 ? (s_start[g + 1] - s_start[g]) * group : 0;
-        const int piece = len > 0 ? (int)plan::shared_piece(len, chunk, kTile) : 1, pieces = (len + piece - 1) / piece;
-        int all_items, all_rows;
-        int at = item + block_exclusive_scan<kPlanThreads, true>(pieces * tiles, s_wave, &all_items);
-        const int base = row + block_exclusive_scan<kPlanThreads, true>(pieces * hkv * rows, s_wave, &all_rows);
+        const int len = g < n ? s_len[g] : 0, tiles = len > 0 ? tiles_of(g) : 0, rows = len > 0 ? rows_of(g) : 0;
+        const int piece = len > 0 ? plan::shared_piece(len, chunk, kTile) : 1, pieces = (len + piece - 1) / piece;
+        int64_t all;
+        const int64_t mine = at + block_exclusive_scan<kPlanThreads, true>(
+                                      ((int64_t)pieces * hkv * rows << 32) + pieces * tiles, s_wave, &all);
+        int next = (int)(mine & 0xffffffff);
+        const int base = (int)(mine >> 32);
         for (int i = 0; i < pieces; ++i)
             for (int t = 0; t < tiles; ++t) {
                 Item it;
@@ -144,26 +152,27 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
                 it.rows = min(plan::kSharedRows, rows - it.row0);
                 it.slot = base + i * hkv * rows + it.row0;
                 it.stride = rows;
-                p.items[at++] = it;
+                p.items[next++] = it;
             }
         if (g < n) {
-            s_first[g] = base;      // (the first sequence is not needed any more)
-            s_more[g] = pieces;
+            s_first[g] = base;
+            s_count[g] = pieces;
         }
-        item += all_items;
-        row += all_rows;
+        at += all;
     }
     __syncthreads();
     for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
         const int b = b0 + tid;
         const bool here = b < batch;
-        const int g = here ? group_of(s_start, n, b) : -1, len = here ? clamp_len(p.d, b) : 0;
+        const int g = here ? group_of(s_start, n, b) : -1, len = b == tid ? len0 : here ? clamp_len(p.d, b) : 0;
         const int begin = g < 0 || len == 0 ? 0 : s_len[g], left = len - begin;
-        const int piece = left > 0 ? (int)plan::shared_piece(left, chunk, plan::kSharedChunk) : 1, pieces = (left + piece - 1) / piece;
+        const int piece = left > 0 ? plan::shared_piece(left, chunk, plan::kSharedChunk) : 1, pieces = (left + piece - 1) / piece;
         const bool whole = begin == 0 && pieces == 1;
-        int all_items, all_rows;
-        int at = item + block_exclusive_scan<kPlanThreads, true>(pieces, s_wave, &all_items);
-        const int base = row + block_exclusive_scan<kPlanThreads, true>(whole ? 0 : pieces * hkv * group, s_wave, &all_rows);
+        int64_t all;
+        const int64_t mine = at + block_exclusive_scan<kPlanThreads, true>(
+                                      ((int64_t)(whole ? 0 : pieces * hkv * group) << 32) + pieces, s_wave, &all);
+        int next = (int)(mine & 0xffffffff);
+        const int base = (int)(mine >> 32);
         for (int i = 0; i < pieces; ++i) {
             Item it;
             it.b = it.table = b;
@@ -172,12 +181,12 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
             it.slot = whole ? -1 : base + i * hkv * group;
             it.rows = it.row0 = 0;
             it.stride = group;
-            p.items[at++] = it;
+            p.items[next++] = it;
         }
         if (here) {
             Seq s;
-            s.n_shared = begin > 0 ? s_more[g] : 0;
-            s.head = begin > 0 ? (s_start[g + 1] - s_start[g]) * group : 0;
+            s.n_shared = begin > 0 ? s_count[g] : 0;
+            s.head = begin > 0 ? rows_of(g) : 0;
             s.step = hkv * s.head;
             s.shared = begin > 0 ? s_first[g] + (b - s_start[g]) * group : 0;
             s.own = base;
@@ -186,16 +195,17 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
             s.pad = 0;
             p.seqs[b] = s;
         }
-        item += all_items;
-        row += all_rows;
+        at += all;
     }
-    if (tid == 0) *p.count = item;
+    if (tid == 0) *p.count = (int)(at & 0xffffffff);
 }
 
 // ---------------------------------------------------------------- shared tokens
+// LDS rows are 256 bytes of bf16.  K's 16-byte piece c of row r lies at piece c ^ (r % 16), V's at
+// c ^ 4 (r % 4): b128 reads of a piece of 16 rows, transposed reads of 64 bytes of 4 rows, and
+// writes of whole rows then fall on all banks.
 constexpr int kTileBytes = kTile * kHeadDim * 2;
-constexpr int kBufBytes = 2 * kTileBytes + 2 * kTile * 4;   // K, V, their scales
-constexpr int kSharedSmem = 2 * kBufBytes;
+constexpr int kSharedSmem = 4 * kTileBytes + 4 * kTile * 4;   // K and V of two tiles, their scales
 
 // Loads of a tile: 16 bytes of a row each, bf16 rows by 16 threads, rows of codes by 8.
 template <int kKv>
@@ -204,10 +214,30 @@ struct TileShape {
     static constexpr bool blocks = kKv >= kKvBlocksFp8;
     static constexpr int row_threads = bf16 ? 16 : 8;
     static constexpr int rows = kThreads / row_threads;   // of one load
+    static constexpr int wave_rows = kWave / row_threads;
     static constexpr int loads = kTile / rows;
 };
 
-template <int kKv>
+// Tokens [it.t0, it.t1) of up to 128 query rows of one KV head.
+// kUni: the rows of a wave's load lie in one page (pages of at least 4 rows of bf16, 8 of codes, whose
+// bytes stay below 2^31), read through a buffer resource that ends at the last token (rows past
+// it are zeros); the wave's pages come 64 loads at a time from one vector load of the table.
+// Four scores times their tokens' scales.
+__device__ __forceinline__ void scale4(f32x16_t& s, int q, f32x4_t by) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[4 * q + i] *= by[i];
+}
+
+// f(integral_constant<int, 0>), ..., f(integral_constant<int, N - 1>)
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        static_for<N, I + 1>(f);
+    }
+}
+
+template <int kKv, bool kUni>
 __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned char* smem, const Item& it, int kvh) {
     using T = TileShape<kKv>;
     const DecodeParams& p = sp.d;
@@ -223,7 +253,10 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
         const int seq = fast_div(row, sp.div_group);
         const __bf16* q = p.q + (it.b + seq) * p.q_sb + (int64_t)(kvh * p.group + row - seq * p.group) * p.q_sh + 8 * half;
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) qop[ks] = as_bf16x8(*reinterpret_cast<const u32x4_t*>(q + 16 * ks));
+        for (int ks = 0; ks < 8; ++ks) {
+            const u32x4_t x = *reinterpret_cast<const u32x4_t*>(q + 16 * ks);
+            qop[ks] = as_bf16x8(T::blocks ? x : x ^ sp.q_sign);
+        }
     }
     float m_run = -INFINITY, l_run = 0.f;   // l: this lane's share
     f32x16_t oacc[4];
@@ -235,167 +268,285 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
     constexpr int kElem = T::bf16 ? 2 : 1;
     const unsigned char* kbase = reinterpret_cast<const unsigned char*>(p.k) + kvh * p.k_sh * kElem;
     const unsigned char* vbase = reinterpret_cast<const unsigned char*>(p.v) + kvh * p.v_sh * kElem;
+    const float* kscales = T::blocks ? p.k_scales + kvh * p.ks_sh : nullptr;
+    const float* vscales = T::blocks ? p.v_scales + kvh * p.vs_sh : nullptr;
     const int32_t* bt = p.block_table + (int64_t)it.table * p.bt_stride;
     const int pmask = (1 << p.page_shift) - 1;
     const int lrow = tid / T::row_threads, chunk = tid % T::row_threads;
-    const int tiles = (it.t1 - it.t0 + kTile - 1) / kTile;
-    u32x4_t kreg[T::loads], vreg[T::loads];
+    const int t0 = __builtin_amdgcn_readfirstlane(it.t0), t1 = __builtin_amdgcn_readfirstlane(it.t1);
+    const int tiles = (t1 - t0 + kTile - 1) / kTile;
+    // bf16 rows go straight to LDS; codes pass through registers, where they are widened
+    constexpr bool kDma = kUni && T::bf16;
+    [[maybe_unused]] u32x4_t kreg[T::loads], vreg[T::loads];
     [[maybe_unused]] float ksreg[T::loads], vsreg[T::loads];
-    int pg[T::loads];
-    // Tokens past the end read the last one again (their scores are masked; the rows are numbers).
-    auto token = [&](int j, int i) { return min(it.t0 + j * kTile + lrow + i * T::rows, it.t1 - 1); };
-    auto fetch_pages = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < T::loads; ++i) pg[i] = bt[token(j, i) >> p.page_shift];
+    const uint32_t kss = (uint32_t)(p.k_ss * kElem), vss = (uint32_t)(p.v_ss * kElem);
+    // (straight to LDS: lane l fills piece l % 16 of row l / 16 of the wave's four)
+    const int lane_row = lane / T::row_threads;
+    [[maybe_unused]] const uint32_t koff =
+        (uint32_t)lane_row * kss + 16 * (kDma ? chunk ^ (T::wave_rows * wave + lane_row) : chunk);
+    [[maybe_unused]] const uint32_t voff = (uint32_t)lane_row * vss + 16 * (kDma ? chunk ^ (4 * lane_row) : chunk);
+    [[maybe_unused]] const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem +
+                                           (uint32_t)(wave * T::wave_rows * kHeadDim * 2);
+    // The scores run one block of 32 tokens ahead of P.V, so K's tile j is tokens 64 j + 32 .. 64 j + 95 (from -1
+    // on, for the first block) and V's 64 j .. 64 j + 63: a step reads one of each.
+    // kUni: lane l holds the addresses of the first rows of the wave's loads pt_first + l (load i of tile j being
+    // (j + 1) * loads + i), the bytes of V's rows before the end (rows past it are zeros; K's may be any, in a page
+    // all the same), and their scales.  A load then takes a few scalar instructions, not thirty.
+    [[maybe_unused]] int pt_first = -kWave;
+    [[maybe_unused]] uint32_t pt_k[2] = {0u, 0u}, pt_v[2] = {0u, 0u}, pt_vbytes = 0u;
+    [[maybe_unused]] float pt_ks = 0.f, pt_vs = 0.f;
+    [[maybe_unused]] auto pt_load = [&](int first) {
+        const int n = first + lane;
+        const int tok_v = t0 + (n / T::loads - 1) * kTile + (n % T::loads) * T::rows + wave * T::wave_rows;
+        const int tok_k = max(tok_v + kBlock, t0);
+        const int page_k = min(max(bt[min(tok_k, t1 - 1) >> p.page_shift], 0), p.num_pages - 1);
+        const int page_v = min(max(bt[min(max(tok_v, t0), t1 - 1) >> p.page_shift], 0), p.num_pages - 1);
+        const uint64_t k = reinterpret_cast<uint64_t>(kbase + page_k * p.k_sb * kElem + (int64_t)(tok_k & pmask) * kss);
+        const uint64_t v = reinterpret_cast<uint64_t>(vbase + page_v * p.v_sb * kElem + (int64_t)(tok_v & pmask) * vss);
+        pt_k[0] = (uint32_t)k;
+        pt_k[1] = (uint32_t)(k >> 32);
+        pt_v[0] = (uint32_t)v;
+        pt_v[1] = (uint32_t)(v >> 32);
+        const int rows = min(T::wave_rows, t1 - tok_v);
+        pt_vbytes = rows > 0 ? (uint32_t)(rows - 1) * vss + kHeadDim * kElem : 0u;
+        if constexpr (T::blocks) {
+            pt_ks = kscales[page_k * p.ks_sp];
+            pt_vs = vscales[page_v * p.vs_sp];
+        }
+        pt_first = first;
     };
-    // The table's entries are loaded a tile before they are used, ahead of the rows between.
-    auto load = [&](int j, bool more) {
-        int64_t page[T::loads];
-#pragma unroll
-        for (int i = 0; i < T::loads; ++i) page[i] = min(max(pg[i], 0), p.num_pages - 1);
-        if (more) fetch_pages(j + 1);
+    // else each row's page is looked up.  Tokens past the end read the last one again (their scores are masked;
+    // the rows are numbers).
+    [[maybe_unused]] auto load_rows = [&](int first, const unsigned char* base, int64_t page_bytes, uint32_t row_bytes,
+                                          [[maybe_unused]] const float* scales, [[maybe_unused]] int64_t scale_page,
+                                          u32x4_t (&reg)[T::loads], [[maybe_unused]] float (&sreg)[T::loads]) {
 #pragma unroll
         for (int i = 0; i < T::loads; ++i) {
-            const int64_t slot = token(j, i) & pmask;
-            kreg[i] = *reinterpret_cast<const u32x4_t*>(kbase + (page[i] * p.k_sb + slot * p.k_ss) * kElem + chunk * 16);
-            vreg[i] = *reinterpret_cast<const u32x4_t*>(vbase + (page[i] * p.v_sb + slot * p.v_ss) * kElem + chunk * 16);
-            if constexpr (T::blocks) {
-                ksreg[i] = p.k_scales[page[i] * p.ks_sp + kvh * p.ks_sh];
-                vsreg[i] = p.v_scales[page[i] * p.vs_sp + kvh * p.vs_sh];
+            const int tok = min(max(first + lrow + i * T::rows, t0), t1 - 1);
+            const int64_t page = min(max(bt[tok >> p.page_shift], 0), p.num_pages - 1);
+            reg[i] = *reinterpret_cast<const u32x4_t*>(base + page * page_bytes + (int64_t)(tok & pmask) * row_bytes + chunk * 16);
+            if constexpr (T::blocks) sreg[i] = scales[page * scale_page];
+        }
+    };
+    // The loads of one cache's tile j: kUni, to registers or (kDma) to `lds`; else to registers.
+    [[maybe_unused]] auto load_uni = [&](int j, const uint32_t (&at)[2], bool v, uint32_t off, [[maybe_unused]] u32x4_t (&reg)[T::loads],
+                                         [[maybe_unused]] uint32_t lds) {
+        const int first = (j + 1) * T::loads - pt_first;
+#pragma unroll
+        for (int i = 0; i < T::loads; ++i) {
+            const uint64_t base = (uint64_t)__builtin_amdgcn_readlane(at[1], first + i) << 32 |
+                                  (uint32_t)__builtin_amdgcn_readlane(at[0], first + i);
+            const uint32_t bytes = v ? __builtin_amdgcn_readlane(pt_vbytes, first + i)
+                                     : (uint32_t)(T::wave_rows - 1) * kss + kHeadDim * kElem;
+            const __amdgpu_buffer_rsrc_t r = make_rsrc(reinterpret_cast<const void*>(base), bytes);
+            if constexpr (kDma) {
+                asm volatile("s_add_u32 m0, %0, %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                             :: "s"(lds), "v"(off), "s"(r), "i"(i * T::rows * kHeadDim * 2) : "memory", "scc");
+            } else {
+                reg[i] = buf_load16(r, off);
             }
         }
     };
-    // K's 16-byte piece c of row r lies at piece c ^ (r % 16), V's at c ^ 4 (r % 4): reads and
-    // writes then spread over all banks.
-    auto stage = [&](unsigned char* buf) {
-        __bf16* kl = reinterpret_cast<__bf16*>(buf);
-        __bf16* vl = kl + kTile * kHeadDim;
-        float* sl = reinterpret_cast<float*>(buf + 2 * kTileBytes);
+    auto load = [&](int j) {
+        if constexpr (kUni) {
+            if ((j + 2) * T::loads > pt_first + kWave) pt_load((j + 1) * T::loads);
+            load_uni(j, pt_k, false, koff, kreg, lds0 + (j & 1) * kTileBytes);
+            load_uni(j, pt_v, true, voff, vreg, lds0 + (2 + (j & 1)) * kTileBytes);
+        } else {
+            load_rows(t0 + j * kTile + kBlock, kbase, p.k_sb * kElem, kss, kscales, p.ks_sp, kreg, ksreg);
+            load_rows(t0 + j * kTile, vbase, p.v_sb * kElem, vss, vscales, p.vs_sp, vreg, vsreg);
+        }
+    };
+    float* const scale_lds = reinterpret_cast<float*>(smem + 4 * kTileBytes);   // K's of two tiles, V's
+    // Registers to buffer `at` (K: 0 and 1, V: 2 and 3).
+    [[maybe_unused]] auto stage_one = [&](int j, int at, const u32x4_t (&reg)[T::loads], [[maybe_unused]] const float (&sreg)[T::loads],
+                                      [[maybe_unused]] float pt_scale, [[maybe_unused]] float factor) {
+        const int turn = at < 2 ? lrow & 15 : 4 * (lrow & 3);   // (rows 16 on turn alike)
+        __bf16* d = reinterpret_cast<__bf16*>(smem + at * kTileBytes) + lrow * kHeadDim;
 #pragma unroll
         for (int i = 0; i < T::loads; ++i) {
-            const int r = lrow + i * T::rows;
-            __bf16* kr = kl + r * kHeadDim;
-            __bf16* vr = vl + r * kHeadDim;
+            __bf16* r = d + i * T::rows * kHeadDim;
             if constexpr (T::bf16) {
-                *reinterpret_cast<u32x4_t*>(kr + 8 * (chunk ^ (r & 15))) = kreg[i];
-                *reinterpret_cast<u32x4_t*>(vr + 8 * (chunk ^ (4 * (r & 3)))) = vreg[i];
+                *reinterpret_cast<u32x4_t*>(r + 8 * (chunk ^ turn)) = reg[i];
             } else {
                 constexpr int kCode = kKv == kKvBlocksInt8 ? kCodeInt8 : kCodeFp8;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int c = 2 * chunk + h;
-                    *reinterpret_cast<bf16x8_t*>(kr + 8 * (c ^ (r & 15))) = codes_to_bf16<kCode>(kreg[i][2 * h], kreg[i][2 * h + 1]);
-                    *reinterpret_cast<bf16x8_t*>(vr + 8 * (c ^ (4 * (r & 3)))) = codes_to_bf16<kCode>(vreg[i][2 * h], vreg[i][2 * h + 1]);
-                }
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<bf16x8_t*>(r + 8 * ((2 * chunk + h) ^ turn)) =
+                        codes_to_bf16<kCode>(reg[i][2 * h], reg[i][2 * h + 1]);
                 if constexpr (T::blocks) {
-                    if (chunk == 0) {
-                        sl[r] = ksreg[i] * p.scale_log2;
-                        sl[kTile + r] = vsreg[i];
-                    }
+                    // (kUni: the pages' vector is still the one of the loads)
+                    float x = 0.f;
+                    if constexpr (kUni)
+                        x = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pt_scale), (j + 1) * T::loads + i - pt_first));
+                    else x = sreg[i];
+                    if (chunk == 0) scale_lds[at * kTile + lrow + i * T::rows] = x * factor;
                 }
             }
         }
     };
+    auto stage = [&]([[maybe_unused]] int j) {
+        if constexpr (!kDma) {
+            stage_one(j, j & 1, kreg, ksreg, pt_ks, p.scale_log2);
+            stage_one(j, 2 + (j & 1), vreg, vsreg, pt_vs, 1.f);
+        }
+    };
+    // what went straight to LDS has landed
+    auto landed = [] {
+        if constexpr (kDma) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
 
-    auto compute = [&](const unsigned char* buf, int j) {
-        const __bf16* kl = reinterpret_cast<const __bf16*>(buf);
-        const __bf16* vl = kl + kTile * kHeadDim;
-        const float* sl = reinterpret_cast<const float*>(buf + 2 * kTileBytes);
-        // S^T: register i of block tb is token 32 tb + 8 (i / 4) + 4 half + i % 4, of row l32
-        f32x16_t s[2];
+    // Operands in LDS: K's piece 2 ks + half of row l32 (and 32 on), V's by transposed reads of rows
+    // 4 half + (lane % 16) / 4 (and 8 on), columns 32 db + 16 ((lane % 32) / 16) + 4 (lane % 4) .. +3.
+    int k_at[8], v_at[4];
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb) {
+    for (int ks = 0; ks < 8; ++ks) k_at[ks] = l32 * kHeadDim + 8 * ((2 * ks + half) ^ (l32 & 15));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[tb][i] = 0.f;
+    for (int db = 0; db < 4; ++db) {
+        const int r = 4 * half + ((lane & 15) >> 2), c = 4 * db + 2 * (l32 >> 4) + ((lane & 3) >> 1);
+        v_at[db] = r * kHeadDim + 8 * (c ^ (4 * (r & 3))) + 4 * (lane & 1);
+    }
+    // Block h (0, 1) of K's and of V's tile: operand ks of the scores; columns n % 4 of 16 tokens n / 4
+    auto k_operand = [&](int j, int h, int ks) {
+        return *reinterpret_cast<const bf16x8_t*>(reinterpret_cast<const __bf16*>(smem + (j & 1) * kTileBytes) + k_at[ks] +
+                                                  h * kBlock * kHeadDim);
+    };
+    auto v_operand = [&](int j, int h, int n) {
+        const __bf16* src = reinterpret_cast<const __bf16*>(smem + (2 + (j & 1)) * kTileBytes) + v_at[n & 3] +
+                            (h * kBlock + 16 * (n >> 2)) * kHeadDim;
+        return __builtin_shufflevector(lds_read_tr16(src), lds_read_tr16(src + 8 * kHeadDim), 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    // Of caches with block scales: those of K's or V's tokens 8 q + 4 half + {0..3} of a block.
+    auto scales_of = [&](int at, int h, int q) {
+        return *reinterpret_cast<const f32x4_t*>(scale_lds + at * kTile + h * kBlock + 8 * q + 4 * half);
+    };
+    auto mask = [&](int left, f32x16_t& s) {
+        left -= 4 * half;
+        asm volatile("" : "+v"(left));   // (else the comparands are kept in registers for the whole loop)
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                const bf16x8_t ka =
-                    *reinterpret_cast<const bf16x8_t*>(kl + (32 * tb + l32) * kHeadDim + 8 * ((2 * ks + half) ^ (l32 & 15)));
-                s[tb] = mfma32(ka, qop[ks], s[tb]);
-            }
+        for (int i = 0; i < 16; ++i)
+            if (8 * (i / 4) + i % 4 >= left) s[i] = -INFINITY;
+    };
+    auto largest = [&](const f32x16_t& s) {
+        float x = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) x = fmaxf(x, s[i]);
+        return x;
+    };
+
+    // Block b's tokens, half h of V's tile j: the scores of block b + 1 (half h of K's tile) and P.V of block b, with
+    // the softmax of block b and the largest of the next scores spread between the products.  S^T: register i is
+    // token 8 (i / 4) + 4 half + i % 4 of its block, of row l32.
+    // Written in the order that it is to be issued in: operands three or four products ahead (the first of the
+    // tile's second half at the end of its first), nothing that waits for a product right behind it.
+    bf16x8_t ring[4], vring[3];
+    auto step = [&](int j, auto half_c, f32x16_t& s, f32x16_t& next, float& top) {
+        constexpr int h = decltype(half_c)::value;
+        const int left = t1 - (t0 + j * kTile + h * kBlock);
+        if (left < kBlock) {
+            mask(left, s);
+            top = largest(s);
         }
-        float top = -INFINITY;
+        if constexpr (h == 0) {
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                [[maybe_unused]] f32x4_t ks4;
-                if constexpr (T::blocks) ks4 = *reinterpret_cast<const f32x4_t*>(sl + 32 * tb + 8 * q + 4 * half);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[tb][4 * q + i] *= T::blocks ? ks4[i] : p.scale_log2;
-            }
-        const int left = it.t1 - (it.t0 + j * kTile);
-        if (left < kTile) {
-#pragma unroll
-            for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (32 * tb + 8 * (i / 4) + 4 * half + i % 4 >= left) s[tb][i] = -INFINITY;
+            for (int ks = 0; ks < 4; ++ks) ring[ks] = k_operand(j, 0, ks);
         }
+        const float c = T::blocks ? 1.f : sp.scale_log2;
+        float sum[2] = {0.f, 0.f}, m_sub = 0.f;
+        bf16x8_t pop[2];
+        [[maybe_unused]] f32x4_t by;
+        auto softmax = [&](auto ec) {
+            constexpr int e = decltype(ec)::value;
+            if constexpr (T::blocks && e % 4 == 0) by = scales_of(2 + (j & 1), h, e / 4);
+            const float w = fast_exp2(T::blocks ? s[e] - m_sub : fmaf(s[e], c, -m_sub));
+            sum[e & 1] += w;
+            pop[e >> 3][e & 7] = (__bf16)(T::blocks ? w * by[e & 3] : w);
+        };
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
+        for (int i = 0; i < 16; ++i) next[i] = 0.f;
+        static_for<8>([&](auto ic) {
+            constexpr int n = decltype(ic)::value;
+            __builtin_amdgcn_sched_barrier(0);
+            next = mfma32(ring[n & 3], qop[n], next);
+            if constexpr (n < 4) ring[n & 3] = k_operand(j, h, n + 4);
+            else if constexpr (n >= 5) vring[n - 5] = v_operand(j, h, n - 5);
+            if constexpr (n == 0) {
+                const float m_block = half_max(top) * c;
+                // The maximum moves only where it is exceeded by more than 2^8 (P is at most 2^8 then).
+                if (__any(m_block > m_run + 8.f)) {
+                    const float m_new = fmaxf(m_run, m_block);
+                    const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new));
+                    m_run = m_new;
+                    l_run *= alpha;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[tb][i]);
-        top = half_max(top);
-        // The maximum moves only where it is exceeded by more than 2^8 (P is at most 2^8 then).
-        if (__any(top > m_run + 8.f)) {
-            const float m_new = fmaxf(m_run, top);
-            const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new));
-            m_run = m_new;
-            l_run *= alpha;
-#pragma unroll
-            for (int db = 0; db < 4; ++db) oacc[db] *= alpha;
-        }
-        const float m_sub = m_run == -INFINITY ? 0.f : m_run;
-        float sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[tb][i] = fast_exp2(s[tb][i] - m_sub);
-                sum[i & 1] += s[tb][i];
+                    for (int db = 0; db < 4; ++db) oacc[db] *= alpha;
+                }
+                m_sub = m_run == -INFINITY ? 0.f : m_run;
+            } else if constexpr (n < 6) {
+                softmax(std::integral_constant<int, 2 * n - 2>{});
+                softmax(std::integral_constant<int, 2 * n - 1>{});
+            } else {
+                softmax(std::integral_constant<int, n + 4>{});
             }
-        l_run += sum[0] + sum[1];
+        });
         // V^T as the A operand: lane holds column 32 db + l32 of the tokens whose P it holds
-        const int l16 = lane & 15;
+        float most = 0.f;
+        static_for<8>([&](auto ic) {
+            constexpr int n = decltype(ic)::value;
+            __builtin_amdgcn_sched_barrier(0);
+            oacc[n & 3] = mfma32(vring[n % 3], pop[n >> 2], oacc[n & 3]);
+            if constexpr (n + 3 < 8) vring[n % 3] = v_operand(j, h, n + 3);
+            else if constexpr (h == 0) ring[n - 5] = k_operand(j, 1, n - 5);
+            if constexpr (n < 2) {
+                softmax(std::integral_constant<int, 12 + 2 * n>{});
+                softmax(std::integral_constant<int, 13 + 2 * n>{});
+            } else if constexpr (n < 6) {   // (4 scores each)
+                if constexpr (T::blocks) scale4(next, n - 2, scales_of(j & 1, h, n - 2));
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                bf16x8_t pop;
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    [[maybe_unused]] f32x4_t vs4;
-                    if constexpr (T::blocks)
-                        vs4 = *reinterpret_cast<const f32x4_t*>(sl + kTile + 32 * tb + 16 * h + 8 * q + 4 * half);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = s[tb][8 * h + 4 * q + i];
-                        pop[4 * q + i] = (__bf16)(T::blocks ? x * vs4[i] : x);
-                    }
-                }
-                // rows 32 tb + 16 h + 4 half + {0..3} and 8 more; lane l16 / 4 of its 16 names the row
-                const int row = 32 * tb + 16 * h + 4 * half + (l16 >> 2);
-#pragma unroll
-                for (int db = 0; db < 4; ++db) {
-                    // columns 32 db + 16 (l32 / 16) + 4 (l16 % 4) .. +3: half a 16-byte piece
-                    const int c = 4 * db + 2 * (l32 >> 4) + ((l16 & 3) >> 1);
-                    const __bf16* src = vl + row * kHeadDim + 8 * (c ^ (4 * (row & 3))) + 4 * (l16 & 1);
-                    const bf16x4_t lo = lds_read_tr16(src);
-                    const bf16x4_t hi = lds_read_tr16(src + 8 * kHeadDim);
-                    oacc[db] = mfma32(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), pop, oacc[db]);
-                }
+                for (int i = 4 * (n - 2); i < 4 * (n - 1); ++i) most = i == 0 ? next[0] : fmaxf(most, next[i]);
             }
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (h == 0) ring[3] = k_operand(j, 1, 3);
+        l_run += sum[0] + sum[1];
+        top = most;
     };
 
-    fetch_pages(0);
-    load(0, tiles > 1);
+    load(-1);
+    landed();
+    stage(-1);
+    load(0);
+    landed();
+    stage(0);
+    if constexpr (!kDma) {
+        if (tiles > 1) load(1);
+    }
+    __syncthreads();
+    f32x16_t s0, s1;
+    float top = -INFINITY;
+    if (active) {   // block 0: the second half of K's tile -1
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s0[i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) s0 = mfma32(k_operand(-1, 1, ks), qop[ks], s0);
+        if constexpr (T::blocks) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) scale4(s0, q, scales_of(1, 1, q));
+        }
+        top = largest(s0);
+    }
     for (int j = 0; j < tiles; ++j) {
-        unsigned char* buf = smem + (j & 1) * kBufBytes;
-        stage(buf);
-        if (j + 1 < tiles) load(j + 1, j + 2 < tiles);
-        __syncthreads();   // (the buffer before this one is written again only after the next barrier)
-        if (active) compute(buf, j);
+        __syncthreads();   // (tile j - 1 has been read, tile j is there)
+        if (j + 1 < tiles) {
+            stage(j + 1);
+            if constexpr (kDma) load(j + 1);
+            else if (j + 2 < tiles) load(j + 2);
+        }
+        if (active) {
+            step(j, std::integral_constant<int, 0>{}, s0, s1, top);
+            if (t0 + j * kTile + kBlock < t1) step(j, std::integral_constant<int, 1>{}, s1, s0, top);
+        }
+        landed();
     }
 
     if (!active) return;
@@ -427,7 +578,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
     const Item it = p.items[at];   // (there is room for every workgroup's)
     if (at >= *p.count) return;
     if (it.rows > 0) {
-        shared_item<kKv>(p, smem, it, kvh);
+        shared_item<kKv, (kSeg > 0)>(p, smem, it, kvh);
     } else {
         const bool whole = it.slot < 0;
         dec_item_of<kKv, kSeg, kDecWaves, true>(p.d, smem, it.t0, it.t1, kvh, it.b, threadIdx.x, whole,
@@ -606,6 +757,8 @@ extern "C" int fgqa_decode_shared(const fgqa_decode_shared_args* a, void* stream
     const bool blocks = c.k_scales != nullptr, whole = c.kv_dtype == FGQA_KV_FP8_E4M3 && !blocks;
     d.scale_log2 = a->scale * (whole ? c.k_scale : 1.f) * kLog2e;
     d.v_scale = whole ? c.v_scale : 1.f;
+    p.scale_log2 = score_scale(fabsf(d.scale_log2));
+    p.q_sign = d.scale_log2 < 0.f ? 0x80008000u : 0u;
     d.block_table = a->block_table;
     d.bt_stride = a->block_table_stride;
     d.page_shift = plan::log2_of(c.page_size);
@@ -629,7 +782,8 @@ extern "C" int fgqa_decode_shared(const fgqa_decode_shared_args* a, void* stream
     p.count = reinterpret_cast<int32_t*>(ws + pl.count_off);
 
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
+    if (d.batch <= 256 && p.num_groups <= 255) hipLaunchKernelGGL(shared_plan_kernel<256>, dim3(1), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(shared_plan_kernel<1024>, dim3(1), dim3(1024), 0, s, p);
     if (a->max_seqlen > 0) {
         const unsigned grid = (unsigned)(pl.max_items * d.hkv);
         const int seg = page_segment(c);

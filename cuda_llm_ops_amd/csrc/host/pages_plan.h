@@ -48,10 +48,11 @@ constexpr int64_t shared_chunk(int64_t total, int slots) {
     return c < kSharedChunk ? kSharedChunk : c;
 }
 // What a range of n > 0 tokens is cut into: equal pieces of a multiple of `step` that are
-// at most a chunk (a multiple of step).
-constexpr int64_t shared_piece(int64_t n, int64_t chunk, int step) {
-    const int64_t pieces = (n + chunk - 1) / chunk;
-    return ((n + pieces - 1) / pieces + step - 1) / step * step;
+// at most a chunk (a multiple of step, and 2^30 at most).
+constexpr int shared_piece(int n, int chunk, int step) {
+    const int pieces = (int)(((uint32_t)n + (uint32_t)chunk - 1) / (uint32_t)chunk);
+    const uint32_t even = ((uint32_t)n + (uint32_t)pieces - 1) / (uint32_t)pieces;
+    return (int)((even + (uint32_t)step - 1) / (uint32_t)step * (uint32_t)step);
 }
 
 // Sizes that a call's kernels and workspace are bounded by, whatever the lengths.

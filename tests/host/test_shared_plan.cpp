@@ -84,6 +84,7 @@ int main() {
     CHECK(check([](A& a) { a.cache.kv_dtype = FGQA_KV_FP8_E4M3; a.cache.v_scale = 1.f / 0.f; }) == kBad);
 
     CHECK(shared_chunk(0, 64) == 128 && shared_chunk(64 * 128, 64) == 128 && shared_chunk(64 * 128 + 1, 64) == 256);
+    CHECK(shared_piece(1 << 30, 1 << 30, 64) == 1 << 30 && shared_piece((1 << 30) - 1, 1 << 29, 64) == 1 << 29);
     CHECK(shared_piece(1, 128, 64) == 64 && shared_piece(129, 128, 64) == 128 && shared_piece(1000, 384, 128) == 384);
 
     std::mt19937_64 rng(5);
@@ -119,11 +120,11 @@ int main() {
             for (int b = cut[g]; b < cut[g + 1]; ++b) left[b] -= n;
         }
         for (int64_t n : left) total += n;
-        const int64_t chunk = shared_chunk(total, pl.slots);
+        const int chunk = (int)std::min<int64_t>(shared_chunk(total, pl.slots), 1 << 30);
         int64_t items = 0, rows = 0;
         for (int g = 0; g < a.num_groups; ++g) {
             if (shared[g] == 0) continue;
-            const int64_t piece = shared_piece(shared[g], chunk, 64), pieces = (shared[g] + piece - 1) / piece;
+            const int64_t piece = shared_piece((int)shared[g], chunk, 64), pieces = (shared[g] + piece - 1) / piece;
             const int64_t r = (int64_t)(cut[g + 1] - cut[g]) * group;
             CHECK(piece <= chunk && piece % 64 == 0);
             items += pieces * ((r + kSharedRows - 1) / kSharedRows);
@@ -131,7 +132,7 @@ int main() {
         }
         for (int64_t n : left) {
             if (n == 0) continue;
-            const int64_t piece = shared_piece(n, chunk, kSharedChunk), pieces = (n + piece - 1) / piece;
+            const int64_t piece = shared_piece((int)n, chunk, kSharedChunk), pieces = (n + piece - 1) / piece;
             CHECK(piece <= chunk && piece % kSharedChunk == 0);
             items += pieces;
             rows += pieces * a.cache.num_kv_heads * group;
