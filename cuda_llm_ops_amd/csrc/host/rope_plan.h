@@ -14,15 +14,24 @@ constexpr int kRopeThreads = 256;
 // Lanes of a row, 16 elements each: the power of two from 4 that holds head_dim.
 constexpr int rope_row_lanes(int head_dim) { return head_dim <= 64 ? 4 : head_dim <= 128 ? 8 : 16; }
 
-// Items of one tensor: a lane group takes up to heads_per rows of one token.
-inline int64_t rope_items(int64_t tokens, int heads, int heads_per) { return tokens * ceil_div(heads, heads_per); }
+// An item is up to `per` heads' rows of one token, `count` items a token.
+struct RopeSlices {
+    int per, count;
+};
 
-// Heads of an item: 4 (1 where that leaves fewer than kRopeFullWaves waves).
+// Even slices of at most `most` heads.
+inline RopeSlices rope_slices(int heads, int most) {
+    const int count = (int)ceil_div(heads, most);
+    return {(int)ceil_div(heads, count), count};
+}
+
+// Heads that a lane group of the forward takes: 4 (1 where that leaves fewer than kRopeFullWaves waves).
 int rope_heads_per(const fgqa_rope_args& a);
 
-// Workgroups of the backward with weights, for Q and for K: the items shared out over
-// at most kRopeGradBlocks, in proportion.
+// Backward with weights: Q's and K's items, walked by at most kRopeGradBlocks
+// workgroups that are shared out in proportion to their heads.
 struct RopeGradPlan {
+    RopeSlices slices[2];
     int blocks[2];
     size_t ws_bytes;   // fp32 [blocks[0] + blocks[1], head_dim]
 };

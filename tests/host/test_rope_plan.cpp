@@ -56,8 +56,8 @@ static fgqa_rope_backward_args backward_args() {
     a.grad_k_out = g_mem + 2304;
     a.grad_q = g_mem + 2560;
     a.grad_k = g_mem + 2816;
-    a.grad_q_weight = reinterpret_cast<float*>(g_mem + 3072);
-    a.grad_k_weight = reinterpret_cast<float*>(g_mem + 3328);
+    a.grad_q_weight = reinterpret_cast<float*>(g_mem + 3584);
+    a.grad_k_weight = reinterpret_cast<float*>(g_mem + 3840);
     for (int i = 0; i < 3; ++i) {
         a.grad_q_out_stride[i] = a.grad_q_stride[i] = a.fwd.q_stride[i];
         a.grad_k_out_stride[i] = a.grad_k_stride[i] = a.fwd.k_stride[i];
