@@ -5,6 +5,18 @@
 // page; a free page's number is found from the bits and a running count of them by words
 // (a search over the words, then over one word's bits).  So there is no list of free
 // pages to keep, and equal tables give equal results.
+//
+// With tables that one workgroup reads in passing, a call is one launch: each
+// workgroup works the bits and counts out for itself, in LDS, and then takes its share of
+// cells and copies.  Larger ones do that once, in three launches before the last.
+//
+// Small calls are bound by one launch and the chain of reads behind it (lengths, table,
+// bits, counts): 16 beams of up to 700 tokens forked 8.4 us, a cache of 8 sequences made
+// compact 8.6 us (17.8 and 17.0 us in four launches).  Large ones are bound by the pages'
+// bytes: 256 samples of 16 prompts of 8000 tokens 14 us (31 MB read and written; 40 us in
+// four launches, their threads after the free pages through the L2), 48 conversations of
+// 8000 tokens of bf16 171 us, the copies at 5 TB/s.  A page's pieces are dealt out to
+// threads a slice's width apart: consecutive ones took 181 us.
 #include <algorithm>
 
 #include "fgqa_device.h"
@@ -16,7 +28,7 @@ namespace fgqa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kScanThreads = 1024;
+constexpr int kScanThreads = plan::kAloneThreads;
 constexpr int kWordsPerScan = 4;   // of a thread
 
 // A page's rows as 16-byte pieces, and how many slots of it are copied.
@@ -25,12 +37,13 @@ struct CopyShape {
     FastDiv div_heads;
 };
 
-// Slots [0, slots) of page src to page dst, K and V and their scales: pieces first,
+constexpr int kAhead = 4;   // pieces of K and of V that a thread has in flight
+
+// Slots [0, slots) of page src to page dst, K and V and their scales: 16-byte pieces first,
 // first + step, ... of all.
 __device__ __forceinline__ void copy_slots(const CacheParams& c, const CopyShape& sh, int src, int dst, int slots, int first,
                                            int step) {
     const int total = (slots * c.hkv) << sh.piece_log2;   // (a page's bytes / 16 stay below 2^31)
-    constexpr int kAhead = 4;
     for (int x0 = first; x0 < total; x0 += kAhead * step) {
         u32x4_t v[kAhead][2];
         int64_t at[kAhead][2];
@@ -194,23 +207,35 @@ __global__ __launch_bounds__(kThreads) void fork_mark_kernel(ForkParams p) {
     }
 }
 
-// Counts of free pages by words and of fresh ones by rows.
-__global__ __launch_bounds__(kScanThreads) void fork_scan_kernel(ForkParams p) {
+// Counts of free pages by words and of fresh ones by rows (row(i, fresh pages, those of rows
+// before it, cells kept)); the free pages that are left.  A workgroup.
+template <typename F>
+__device__ __forceinline__ int fork_scan(const ForkParams& p, const uint32_t* bits, const int32_t* first, int32_t* before, F&& row) {
     __shared__ int s_wave[kScanThreads / kWave];
-    const int free_pages = scan_words(p.words, p.before, s_wave,
-                                      [&](int w) { return __popc(~p.bits[w] & word_mask(w, p.c.num_pages)); });
+    const int free_pages = scan_words(p.words, before, s_wave, [&](int w) { return __popc(~bits[w] & word_mask(w, p.c.num_pages)); });
     __shared__ int64_t s_wave64[kScanThreads / kWave];
     int64_t wanted = 0;   // (rows times cells can pass 2^31)
     for (int i0 = 0; i0 < p.new_batch; i0 += kScanThreads) {
         const int i = i0 + (int)threadIdx.x;
-        int kept;
+        int kept = 0;
         int64_t total;
-        const int64_t n = i < p.new_batch ? fresh_pages(p, fork_row(p, i), i, p.first, &kept) : 0;
+        const int64_t n = i < p.new_batch ? fresh_pages(p, fork_row(p, i), i, first, &kept) : 0;
         const int64_t at = block_exclusive_scan<kScanThreads, true>(n, s_wave64, &total);
-        if (i < p.new_batch) p.row_first[i] = (int)min(wanted + at, (int64_t)INT32_MAX);
+        if (i < p.new_batch) row(i, (int)n, (int)min(wanted + at, (int64_t)INT32_MAX), kept);
         wanted += total;
     }
-    if (threadIdx.x == 0) *p.num_free = (int)max((int64_t)free_pages - wanted, (int64_t)INT32_MIN);
+    return (int)max((int64_t)free_pages - wanted, (int64_t)INT32_MIN);
+}
+
+__global__ __launch_bounds__(kScanThreads) void fork_scan_kernel(ForkParams p) {
+    const int left = fork_scan(p, p.bits, p.first, p.before, [&](int i, int, int at, int) { p.row_first[i] = at; });
+    if (threadIdx.x == 0) *p.num_free = left;
+}
+
+// The k-th free page.
+__device__ __forceinline__ int free_page(const ForkParams& p, const uint32_t* bits, const int32_t* before, int k) {
+    const int w = word_of(p.words, k, [&](int x) { return before[x]; });
+    return 32 * w + bit_of(~bits[w] & word_mask(w, p.c.num_pages), k - before[w]);
 }
 
 // The rows' other cells, and the copies of partly filled pages.
@@ -220,12 +245,7 @@ __global__ __launch_bounds__(kThreads) void fork_fill_kernel(ForkParams p) {
     int kept;
     const int fresh = fresh_pages(p, r, i, p.first, &kept);
     const int first = p.row_first[i], free_pages = p.before[p.words];
-    auto fresh_page = [&](int n) {
-        if (n >= free_pages - first) return -1;
-        const int k = first + n;
-        const int w = word_of(p.words, k, [&](int x) { return p.before[x]; });
-        return 32 * w + bit_of(~p.bits[w] & word_mask(w, p.c.num_pages), k - p.before[w]);
-    };
+    auto fresh_page = [&](int n) { return n < free_pages - first ? free_page(p, p.bits, p.before, first + n) : -1; };
     const int at = blockIdx.y * kThreads + threadIdx.x, step = gridDim.y * kThreads;
     for (int j = r.full + at; j < p.new_max_pages; j += step)
         p.new_table[i * p.new_stride + j] = j < kept ? p.table[r.p * p.stride + j] : j - kept < fresh ? fresh_page(j - kept) : -1;
@@ -235,7 +255,80 @@ __global__ __launch_bounds__(kThreads) void fork_fill_kernel(ForkParams p) {
     if (dst >= 0) copy_slots(p.c, p.shape, p.table[r.p * p.stride + r.full], dst, r.part, at, step);
 }
 
+// All of it, each workgroup planning for itself.  LDS: plan::fork_alone_ints.
+__global__ __launch_bounds__(kScanThreads) void fork_alone_kernel(ForkParams p, FastDiv div_width, int width, FastDiv div_new_width,
+                                                                  int slices) {
+    extern __shared__ int32_t smem[];
+    uint32_t* bits = reinterpret_cast<uint32_t*>(smem);
+    int32_t* before = smem + p.words;
+    int32_t* first = before + p.words + 1;   // [batch]
+    int32_t* lens = first + p.batch;         // [batch]
+    int32_t* row = lens + p.batch;           // [new_batch][4]: old row, fresh pages, those of rows before it, cells kept
+    const int tid = threadIdx.x;
+    for (int w = tid; w < p.words; w += kScanThreads) bits[w] = held_word(p.held, w, p.c.num_pages);
+    for (int b = tid; b < p.batch; b += kScanThreads) {
+        first[b] = INT32_MAX;
+        lens[b] = min(max(p.seqlens[b], 0), p.max_tokens);
+    }
+    __syncthreads();
+    for (int i = tid; i < p.new_batch; i += kScanThreads) {
+        const int parent = p.parents != nullptr ? p.parents[i] : i;
+        const bool there = parent >= 0 && parent < p.batch;
+        row[4 * i] = there ? parent : -1;
+        if (there) atomicMin(&first[parent], i);
+    }
+    __syncthreads();
+    const int round = (1 << p.c.page_shift) - 1, old_cells = p.batch * width;
+#pragma unroll 4
+    for (int x = tid; x < old_cells; x += kScanThreads) {
+        const int b = fast_div(x, div_width), j = x - b * width;
+        if (j <= (lens[b] - 1) >> p.c.page_shift && first[b] != INT32_MAX) {
+            const int page = p.table[b * p.stride + j];
+            if (is_page(p.c, page)) atomicOr(&bits[page >> 5], 1u << (page & 31));
+        }
+    }
+    __syncthreads();
+    const int left = fork_scan(p, bits, first, before, [&](int i, int n, int at, int kept) {
+        row[4 * i + 1] = n;
+        row[4 * i + 2] = at;
+        row[4 * i + 3] = kept;
+    });
+    if (blockIdx.x == 0 && tid == 0) *p.num_free = left;
+    __syncthreads();
+    const int free_pages = before[p.words];
+    auto fresh_page = [&](int at, int n) { return n < free_pages - at ? free_page(p, bits, before, at + n) : -1; };
+
+    // slices of the copied pages, one to a wave
+    const int lane = tid % kWave, waves = gridDim.x * (kScanThreads / kWave);
+    for (int64_t t = (tid / kWave) * gridDim.x + blockIdx.x; t < (int64_t)p.new_batch * slices; t += waves) {
+        const int i = (int)(t / slices), slice = (int)(t - (int64_t)i * slices);
+        const int parent = row[4 * i], len = parent >= 0 ? lens[parent] : 0, full = len >> p.c.page_shift;
+        const bool copied = (len & round) != 0 && row[4 * i + 3] == full;
+        const int dst = copied ? fresh_page(row[4 * i + 2], 0) : -1;
+        if (slice == 0 && lane == 0) p.new_seqlens[i] = copied && dst < 0 ? full << p.c.page_shift : len;
+        if (dst >= 0)
+            copy_slots(p.c, p.shape, p.table[parent * p.stride + full], dst, len & round, slice * kWave + lane, slices * kWave);
+    }
+    const int cells = p.new_batch * p.new_max_pages;
+    for (int x = blockIdx.x * kScanThreads + tid; x < cells; x += gridDim.x * kScanThreads) {
+        const int i = fast_div(x, div_new_width), j = x - i * p.new_max_pages;
+        const int fresh = row[4 * i + 1], kept = row[4 * i + 3];
+        p.new_table[i * p.new_stride + j] = j < kept          ? p.table[row[4 * i] * p.stride + j]
+                                            : j - kept < fresh ? fresh_page(row[4 * i + 2], j - kept)
+                                                               : -1;
+    }
+}
+
 // ---------------------------------------------------------------- compact
+// The pages' bits and counts by words.
+struct PageWords {
+    int words, num_pages;
+    uint32_t* live;
+    uint32_t* held;
+    int32_t* live_before;
+    int32_t* open_before;
+};
+
 struct CompactParams {
     CacheParams c;
     CopyShape shape;
@@ -246,11 +339,8 @@ struct CompactParams {
     int32_t* num_used;
     int64_t stride, new_stride;
     int batch, max_pages, max_tokens;
-    int words, slices, table_blocks;
-    uint32_t* live;
-    uint32_t* held_bits;
-    int32_t* live_before;
-    int32_t* open_before;
+    int slices, table_blocks;
+    PageWords words;
     int32_t* edge;
 };
 
@@ -260,9 +350,9 @@ __device__ __forceinline__ int compact_cells(const CompactParams& p, int b) {
 }
 
 __global__ __launch_bounds__(kThreads) void compact_clear_kernel(CompactParams p) {
-    for (int64_t w = (int64_t)blockIdx.x * kThreads + threadIdx.x; w < p.words; w += (int64_t)gridDim.x * kThreads) {
-        p.live[w] = 0;
-        p.held_bits[w] = held_word(p.held, (int)w, p.c.num_pages);
+    for (int64_t w = (int64_t)blockIdx.x * kThreads + threadIdx.x; w < p.words.words; w += (int64_t)gridDim.x * kThreads) {
+        p.words.live[w] = 0;
+        p.words.held[w] = held_word(p.held, (int)w, p.c.num_pages);
     }
 }
 
@@ -270,75 +360,124 @@ __global__ __launch_bounds__(kThreads) void compact_mark_kernel(CompactParams p)
     const int b = blockIdx.x, cells = compact_cells(p, b);
     for (int j = blockIdx.y * kThreads + threadIdx.x; j < cells; j += gridDim.y * kThreads) {
         const int page = p.table[b * p.stride + j];
-        if (is_page(p.c, page)) atomicOr(&p.live[page >> 5], 1u << (page & 31));
+        if (is_page(p.c, page)) atomicOr(&p.words.live[page >> 5], 1u << (page & 31));
     }
 }
 
 // (held pages are not counted as live: they stay)
-__device__ __forceinline__ uint32_t live_word(const CompactParams& p, int w) { return p.live[w] & ~p.held_bits[w]; }
-__device__ __forceinline__ uint32_t open_word(const CompactParams& p, int w) {
-    return ~p.held_bits[w] & word_mask(w, p.c.num_pages);
-}
+__device__ __forceinline__ uint32_t live_word(const PageWords& s, int w) { return s.live[w] & ~s.held[w]; }
+__device__ __forceinline__ uint32_t open_word(const PageWords& s, int w) { return ~s.held[w] & word_mask(w, s.num_pages); }
 
-// Counts by words; the edge, behind the first L pages that are not held (L: live ones).
-__global__ __launch_bounds__(kScanThreads) void compact_scan_kernel(CompactParams p) {
+// Counts by words; *edge, behind the first L pages that are not held (L: live ones); how many
+// pages are in use or held up to the last such one.  A workgroup.
+__device__ __forceinline__ int compact_scan(const PageWords& s, int32_t* edge) {
     __shared__ int s_wave[kScanThreads / kWave];
     __shared__ int s_last;
     if (threadIdx.x == 0) s_last = -1;
-    const int live = scan_words(p.words, p.live_before, s_wave, [&](int w) { return __popc(live_word(p, w)); });
-    scan_words(p.words, p.open_before, s_wave, [&](int w) { return __popc(open_word(p, w)); });
+    const int live = scan_words(s.words, s.live_before, s_wave, [&](int w) { return __popc(live_word(s, w)); });
+    scan_words(s.words, s.open_before, s_wave, [&](int w) { return __popc(open_word(s, w)); });
     __syncthreads();
-    for (int w = threadIdx.x; w < p.words; w += kScanThreads) {
-        if (p.held_bits[w] != 0) atomicMax(&s_last, 32 * w + 31 - __builtin_clz(p.held_bits[w]));
-        const int n = live - 1 - p.open_before[w];
-        if (live > 0 && n >= 0 && n < __popc(open_word(p, w))) {   // (one word's)
-            *p.edge = 32 * w + bit_of(open_word(p, w), n) + 1;
-            atomicMax(&s_last, 32 * w + bit_of(open_word(p, w), n));
+    for (int w = threadIdx.x; w < s.words; w += kScanThreads) {
+        if (s.held[w] != 0) atomicMax(&s_last, 32 * w + 31 - __builtin_clz(s.held[w]));
+        const int n = live - 1 - s.open_before[w];
+        if (live > 0 && n >= 0 && n < __popc(open_word(s, w))) {   // (one word's)
+            *edge = 32 * w + bit_of(open_word(s, w), n) + 1;
+            atomicMax(&s_last, 32 * w + bit_of(open_word(s, w), n));
         }
     }
+    if (threadIdx.x == 0 && live == 0) *edge = 0;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        if (live == 0) *p.edge = 0;
-        *p.num_used = s_last + 1;
-    }
+    return s_last + 1;
+}
+
+__global__ __launch_bounds__(kScanThreads) void compact_scan_kernel(CompactParams p) {
+    const int used = compact_scan(p.words, p.edge);
+    if (threadIdx.x == 0) *p.num_used = used;
 }
 
 // Live pages before page x.
-__device__ __forceinline__ int live_rank(const CompactParams& p, int x) {
-    if (x >= 32 * p.words) return p.live_before[p.words];
-    return p.live_before[x >> 5] + __popc(live_word(p, x >> 5) & ((1u << (x & 31)) - 1));
+__device__ __forceinline__ int live_rank(const PageWords& s, int x) {
+    if (x >= 32 * s.words) return s.live_before[s.words];
+    return s.live_before[x >> 5] + __popc(live_word(s, x >> 5) & ((1u << (x & 31)) - 1));
 }
 
 // The t-th page before the edge that is neither held nor live.
-__device__ __forceinline__ int hole(const CompactParams& p, int t) {
-    const int w = word_of(p.words, t, [&](int x) { return p.open_before[x] - p.live_before[x]; });
-    return 32 * w + bit_of(open_word(p, w) & ~p.live[w], t - (p.open_before[w] - p.live_before[w]));
+__device__ __forceinline__ int hole(const PageWords& s, int t) {
+    const int w = word_of(s.words, t, [&](int x) { return s.open_before[x] - s.live_before[x]; });
+    return 32 * w + bit_of(open_word(s, w) & ~s.live[w], t - (s.open_before[w] - s.live_before[w]));
+}
+
+// The new number of page `page` of the old table.
+__device__ __forceinline__ int moved_to(const CompactParams& p, const PageWords& s, int page, int edge, int stay) {
+    if (!is_page(p.c, page) || page < edge || ((s.held[page >> 5] >> (page & 31)) & 1)) return page;
+    return hole(s, live_rank(s, page) - stay);
+}
+
+// Slice t % slices of the page that is the (t / slices)-th to move, by `threads` threads.
+__device__ __forceinline__ void move_slice(const CompactParams& p, const PageWords& s, int64_t t, int stay, int thread, int threads) {
+    const int mover = (int)(t / p.slices), slice = (int)(t - (int64_t)mover * p.slices);
+    const int w = word_of(s.words, stay + mover, [&](int x) { return s.live_before[x]; });
+    const int src = 32 * w + bit_of(live_word(s, w), stay + mover - s.live_before[w]);
+    copy_slots(p.c, p.shape, src, hole(s, mover), 1 << p.c.page_shift, slice * threads + thread, p.slices * threads);
 }
 
 // Workgroups up to table_blocks renumber the table; the others copy, a slice of a page at a time.
 __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p) {
+    const PageWords& s = p.words;
     const int edge = *p.edge;
-    const int stay = live_rank(p, edge), live = p.live_before[p.words];
+    const int stay = live_rank(s, edge), live = s.live_before[s.words];
     if ((int)blockIdx.x < p.table_blocks) {
         const int64_t cells = (int64_t)p.batch * p.max_pages;
         for (int64_t x = (int64_t)blockIdx.x * kThreads + threadIdx.x; x < cells; x += (int64_t)p.table_blocks * kThreads) {
             const int b = (int)(x / p.max_pages), j = (int)(x - (int64_t)b * p.max_pages);
-            int page = -1;
-            if (j < compact_cells(p, b)) {
-                page = p.table[b * p.stride + j];
-                if (is_page(p.c, page) && page >= edge && !((p.held_bits[page >> 5] >> (page & 31)) & 1))
-                    page = hole(p, live_rank(p, page) - stay);
-            }
-            p.new_table[b * p.new_stride + j] = page;
+            p.new_table[b * p.new_stride + j] =
+                j < compact_cells(p, b) ? moved_to(p, s, p.table[b * p.stride + j], edge, stay) : -1;
         }
         return;
     }
     const int64_t tasks = (int64_t)(live - stay) * p.slices;
-    for (int64_t t = (int)blockIdx.x - p.table_blocks; t < tasks; t += gridDim.x - p.table_blocks) {
-        const int mover = (int)(t / p.slices), slice = (int)(t - (int64_t)mover * p.slices);
-        const int w = word_of(p.words, stay + mover, [&](int x) { return p.live_before[x]; });
-        const int src = 32 * w + bit_of(live_word(p, w), stay + mover - p.live_before[w]);
-        copy_slots(p.c, p.shape, src, hole(p, mover), 1 << p.c.page_shift, slice * kThreads + threadIdx.x, p.slices * kThreads);
+    for (int64_t t = (int)blockIdx.x - p.table_blocks; t < tasks; t += gridDim.x - p.table_blocks)
+        move_slice(p, s, t, stay, threadIdx.x, kThreads);
+}
+
+// All of it, each workgroup planning for itself.  LDS: plan::compact_alone_ints.
+__global__ __launch_bounds__(kScanThreads) void compact_alone_kernel(CompactParams p, FastDiv div_width) {
+    extern __shared__ int32_t smem[];
+    __shared__ int32_t s_edge;
+    PageWords s = p.words;
+    s.live = reinterpret_cast<uint32_t*>(smem);
+    s.held = s.live + s.words;
+    s.live_before = smem + 2 * s.words;
+    s.open_before = s.live_before + s.words + 1;
+    int32_t* cells_of = s.open_before + s.words + 1;   // [batch]
+    const int tid = threadIdx.x;
+    for (int w = tid; w < s.words; w += kScanThreads) {
+        s.live[w] = 0;
+        s.held[w] = held_word(p.held, w, p.c.num_pages);
+    }
+    for (int b = tid; b < p.batch; b += kScanThreads) cells_of[b] = compact_cells(p, b);
+    __syncthreads();
+    const int cells = p.batch * p.max_pages;
+#pragma unroll 4
+    for (int x = tid; x < cells; x += kScanThreads) {
+        const int b = fast_div(x, div_width), j = x - b * p.max_pages;
+        if (j < cells_of[b]) {
+            const int page = p.table[b * p.stride + j];
+            if (is_page(p.c, page)) atomicOr(&s.live[page >> 5], 1u << (page & 31));
+        }
+    }
+    __syncthreads();
+    const int used = compact_scan(s, &s_edge);
+    if (blockIdx.x == 0 && tid == 0) *p.num_used = used;
+    const int edge = s_edge;
+    const int stay = live_rank(s, edge);
+    const int64_t tasks = (int64_t)(s.live_before[s.words] - stay) * p.slices;
+    const int waves = gridDim.x * (kScanThreads / kWave);
+    for (int64_t t = (tid / kWave) * gridDim.x + blockIdx.x; t < tasks; t += waves)   // (a wave's)
+        move_slice(p, s, t, stay, tid % kWave, kWave);
+    for (int x = blockIdx.x * kScanThreads + tid; x < cells; x += gridDim.x * kScanThreads) {
+        const int b = fast_div(x, div_width), j = x - b * p.max_pages;
+        p.new_table[b * p.new_stride + j] = j < cells_of[b] ? moved_to(p, s, p.table[b * p.stride + j], edge, stay) : -1;
     }
 }
 
@@ -364,6 +503,12 @@ int take_workspace(void* given, size_t given_bytes, size_t bytes, std::unique_lo
 
 unsigned blocks_for(int64_t n, int64_t most) { return (unsigned)std::max<int64_t>(1, std::min(ceil_div(n, kThreads), most)); }
 
+// Workgroups that plan for themselves: 4 waves' slices or 1024 cells each, and at most `most`.
+unsigned alone_blocks(int64_t slices, int64_t cells, int64_t most) {
+    const int64_t n = std::max(ceil_div(slices, 4), ceil_div(cells, kScanThreads));
+    return (unsigned)std::max<int64_t>(1, std::min(n, most));
+}
+
 }  // namespace
 }  // namespace fgqa
 
@@ -372,20 +517,14 @@ using namespace fgqa;
 extern "C" int fgqa_kv_fork_workspace_bytes(const fgqa_kv_fork_args* a, size_t* bytes) {
     const int st = plan::validate_kv_fork_sizes(a);
     if (st != FGQA_OK || bytes == nullptr) return st != FGQA_OK ? st : FGQA_ERR_INVALID_ARGUMENT;
-    *bytes = (size_t)plan::fork_layout(*a).total * 4;
+    *bytes = plan::fork_alone_ints(*a) > 0 ? 0 : (size_t)plan::fork_layout(*a).total * 4;
     return FGQA_OK;
 }
 
 extern "C" int fgqa_kv_fork(const fgqa_kv_fork_args* a, void* stream) {
     int st = plan::validate_kv_fork(a);
     if (st != FGQA_OK) return st;
-    const plan::ForkLayout l = plan::fork_layout(*a);
-    std::unique_lock<std::mutex> lock;
-    void* ws = nullptr;
-    st = take_workspace(a->workspace, a->workspace_bytes, (size_t)l.total * 4, &lock, &ws);
-    if (st != FGQA_OK) return st;
-    int32_t* w = static_cast<int32_t*>(ws);
-    ForkParams p;
+    ForkParams p = {};
     p.c = cache_params(a->cache);
     p.shape = copy_shape(a->cache);
     p.table = a->block_table;
@@ -403,11 +542,26 @@ extern "C" int fgqa_kv_fork(const fgqa_kv_fork_args* a, void* stream) {
     p.new_max_pages = a->new_max_pages;
     p.max_tokens = std::min(a->max_pages, a->new_max_pages) * a->cache.page_size;
     p.words = (int)plan::page_words(a->cache.num_pages);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const int alone = plan::fork_alone_ints(*a);
+    if (alone > 0) {
+        const int width = plan::fork_width(*a);
+        const int slices = (int)ceil_div(page_pieces(a->cache), kAhead * kWave);
+        const int64_t cells = (int64_t)a->new_batch * a->new_max_pages;
+        hipLaunchKernelGGL(fork_alone_kernel, dim3(alone_blocks((int64_t)a->new_batch * slices, cells, 256)), dim3(kScanThreads), (size_t)alone * 4, s, p,
+                           make_fast_div(std::max(width, 1)), width, make_fast_div(std::max(a->new_max_pages, 1)), slices);
+        return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
+    }
+    const plan::ForkLayout l = plan::fork_layout(*a);
+    std::unique_lock<std::mutex> lock;
+    void* ws = nullptr;
+    st = take_workspace(a->workspace, a->workspace_bytes, (size_t)l.total * 4, &lock, &ws);
+    if (st != FGQA_OK) return st;
+    int32_t* w = static_cast<int32_t*>(ws);
     p.bits = reinterpret_cast<uint32_t*>(w + l.bits);
     p.before = w + l.before;
     p.row_first = w + l.row_first;
     p.first = w + l.first;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned rows = (unsigned)a->new_batch;
     const unsigned cells = blocks_for(a->new_max_pages, 16);
     hipLaunchKernelGGL(fork_clear_kernel, dim3(blocks_for(std::max<int64_t>(p.words, a->batch), 1024)), dim3(kThreads), 0, s, p);
@@ -423,20 +577,14 @@ extern "C" int fgqa_kv_fork(const fgqa_kv_fork_args* a, void* stream) {
 extern "C" int fgqa_kv_compact_workspace_bytes(const fgqa_kv_compact_args* a, size_t* bytes) {
     const int st = plan::validate_kv_compact_sizes(a);
     if (st != FGQA_OK || bytes == nullptr) return st != FGQA_OK ? st : FGQA_ERR_INVALID_ARGUMENT;
-    *bytes = (size_t)plan::compact_layout(*a).total * 4;
+    *bytes = plan::compact_alone_ints(*a) > 0 ? 0 : (size_t)plan::compact_layout(*a).total * 4;
     return FGQA_OK;
 }
 
 extern "C" int fgqa_kv_compact(const fgqa_kv_compact_args* a, void* stream) {
     int st = plan::validate_kv_compact(a);
     if (st != FGQA_OK) return st;
-    const plan::CompactLayout l = plan::compact_layout(*a);
-    std::unique_lock<std::mutex> lock;
-    void* ws = nullptr;
-    st = take_workspace(a->workspace, a->workspace_bytes, (size_t)l.total * 4, &lock, &ws);
-    if (st != FGQA_OK) return st;
-    int32_t* w = static_cast<int32_t*>(ws);
-    CompactParams p;
+    CompactParams p = {};
     p.c = cache_params(a->cache);
     p.shape = copy_shape(a->cache);
     p.table = a->block_table;
@@ -449,22 +597,35 @@ extern "C" int fgqa_kv_compact(const fgqa_kv_compact_args* a, void* stream) {
     p.batch = a->batch;
     p.max_pages = a->max_pages;
     p.max_tokens = a->max_pages * a->cache.page_size;
-    p.words = (int)plan::page_words(a->cache.num_pages);
-    p.live = reinterpret_cast<uint32_t*>(w + l.live);
-    p.held_bits = reinterpret_cast<uint32_t*>(w + l.held);
-    p.live_before = w + l.live_before;
-    p.open_before = w + l.open_before;
-    p.edge = w + l.edge;
+    p.words.words = (int)plan::page_words(a->cache.num_pages);
+    p.words.num_pages = a->cache.num_pages;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t cells = (int64_t)a->batch * a->max_pages;
-    hipLaunchKernelGGL(compact_clear_kernel, dim3(blocks_for(p.words, 1024)), dim3(kThreads), 0, s, p);
+    const int64_t pieces = page_pieces(a->cache), moves = plan::compact_moves(*a);
+    const int alone = plan::compact_alone_ints(*a);
+    if (alone > 0) {
+        p.slices = (int)ceil_div(pieces, kAhead * kWave);
+        hipLaunchKernelGGL(compact_alone_kernel, dim3(alone_blocks(moves * p.slices, cells, 256)), dim3(kScanThreads), (size_t)alone * 4, s, p,
+                           make_fast_div(std::max(a->max_pages, 1)));
+        return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
+    }
+    const plan::CompactLayout l = plan::compact_layout(*a);
+    std::unique_lock<std::mutex> lock;
+    void* ws = nullptr;
+    st = take_workspace(a->workspace, a->workspace_bytes, (size_t)l.total * 4, &lock, &ws);
+    if (st != FGQA_OK) return st;
+    int32_t* w = static_cast<int32_t*>(ws);
+    p.words.live = reinterpret_cast<uint32_t*>(w + l.live);
+    p.words.held = reinterpret_cast<uint32_t*>(w + l.held);
+    p.words.live_before = w + l.live_before;
+    p.words.open_before = w + l.open_before;
+    p.edge = w + l.edge;
+    hipLaunchKernelGGL(compact_clear_kernel, dim3(blocks_for(p.words.words, 1024)), dim3(kThreads), 0, s, p);
     if (cells > 0)
         hipLaunchKernelGGL(compact_mark_kernel, dim3((unsigned)a->batch, blocks_for(a->max_pages, 16)), dim3(kThreads), 0, s, p);
     hipLaunchKernelGGL(compact_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, p);
     if (cells > 0) {
-        // (at most half of the pages move, and no more than the table has cells)
-        const int64_t pieces = page_pieces(a->cache), moves = std::min<int64_t>(a->cache.num_pages / 2, cells);
-        p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(pieces / (4 * kThreads), 16));
+        p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(pieces / (kAhead * kThreads), 16));
         p.table_blocks = (int)blocks_for(cells, 256);
         const int64_t copy_blocks = std::min<int64_t>(moves * p.slices, 4096);
         hipLaunchKernelGGL(compact_move_kernel, dim3((unsigned)(p.table_blocks + copy_blocks)), dim3(kThreads), 0, s, p);

@@ -57,6 +57,30 @@ CompactLayout compact_layout(const fgqa_kv_compact_args& a) {
     return l;
 }
 
+namespace {
+// A table that a workgroup of kAloneThreads reads in passing, and LDS for its rows and bits
+// that any kernel has.  Planning in each workgroup and in launches of its own took, on
+// tables of n cells: fork 8.4 and 17.5 us (n = 2,016), 18 and 21 (n = 32,256), compact 9.6
+// and 16.4, 18 and 24.
+constexpr int64_t kAloneCells = 32768, kAloneInts = 15360;
+// Bytes of pages that may move: past that, copies by smaller workgroups give more than the
+// launches cost (1.2 GB: 170 against 176 us).
+constexpr int64_t kAloneMoves = (int64_t)1 << 29;
+}  // namespace
+
+int fork_alone_ints(const fgqa_kv_fork_args& a) {
+    const int64_t ints = 2 * page_words(a.cache.num_pages) + 1 + 2 * (int64_t)a.batch + 4 * (int64_t)a.new_batch;
+    const bool small = (int64_t)a.batch * fork_width(a) <= kAloneCells && (int64_t)a.new_batch * a.new_max_pages < ((int64_t)1 << 30);
+    return small && ints <= kAloneInts ? (int)ints : 0;
+}
+
+int compact_alone_ints(const fgqa_kv_compact_args& a) {
+    const int64_t ints = 4 * page_words(a.cache.num_pages) + 2 + a.batch, cells = (int64_t)a.batch * a.max_pages;
+    if (cells > kAloneCells || ints > kAloneInts) return 0;
+    const int64_t page = (int64_t)a.cache.page_size * a.cache.num_kv_heads * (a.cache.kv_dtype == FGQA_KV_BF16 ? 512 : 256);
+    return compact_moves(a) <= kAloneMoves / page ? (int)ints : 0;
+}
+
 int validate_kv_fork_sizes(const fgqa_kv_fork_args* a) {
     if (a == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
     int st = validate_cache(a->cache, true, false);

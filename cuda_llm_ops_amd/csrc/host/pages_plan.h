@@ -29,6 +29,19 @@ struct CompactLayout {
 };
 CompactLayout compact_layout(const fgqa_kv_compact_args& a);
 
+// int32 of LDS of a workgroup that plans for itself; 0 where the call's sizes are too large
+// for that (the general form, with a workspace).
+constexpr int kAloneThreads = 1024;
+int fork_alone_ints(const fgqa_kv_fork_args& a);
+int compact_alone_ints(const fgqa_kv_compact_args& a);
+// Pages that can move: at most half of all, and no more than the table has cells.
+inline int64_t compact_moves(const fgqa_kv_compact_args& a) {
+    const int64_t cells = (int64_t)a.batch * a.max_pages;
+    return cells < a.cache.num_pages / 2 ? cells : a.cache.num_pages / 2;
+}
+// Cells of an old row that a new one can hold.
+inline int fork_width(const fgqa_kv_fork_args& a) { return a.max_pages < a.new_max_pages ? a.max_pages : a.new_max_pages; }
+
 // FGQA_OK with new_batch 0 too (num_free is still written); a cache without pages is refused.
 int validate_kv_fork(const fgqa_kv_fork_args* a);
 int validate_kv_compact(const fgqa_kv_compact_args* a);

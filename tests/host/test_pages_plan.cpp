@@ -138,6 +138,7 @@ int main() {
               m.edge - m.open_before >= words + 1 && m.total > m.edge);
         CHECK(l.total % 4 == 0 && m.total % 4 == 0);
     }
+    int alone = 0;
     std::mt19937_64 rng(11);
     const int32_t sizes[] = {0, 1, 3, 16, 128, 1 << 19, 1 << 20, INT_MAX, -1};
     auto pick = [&] { return sizes[rng() % 9]; };
@@ -151,14 +152,32 @@ int main() {
         a.new_block_table_stride = (int64_t)(rng() >> (rng() % 64));
         a.cache.num_pages = pick();
         a.cache.page_size = pick();
-        if (validate_kv_fork(&a) == FGQA_OK) CHECK(fork_layout(a).total > 0);
+        if (validate_kv_fork(&a) == FGQA_OK) {
+            CHECK(fork_layout(a).total > 0);
+            const int64_t n = fork_alone_ints(a);
+            if (n > 0) {
+                ++alone;
+                CHECK(n * 4 <= 61440 && n >= 2 * page_words(a.cache.num_pages) + 1 + 2 * (int64_t)a.batch + 4 * (int64_t)a.new_batch);
+                CHECK((int64_t)a.batch * fork_width(a) < INT_MAX - kAloneThreads);
+                CHECK((int64_t)a.new_batch * a.new_max_pages < INT_MAX - 256 * kAloneThreads);
+            }
+        }
         fgqa_kv_compact_args c = compact_args();
         c.batch = a.batch;
         c.max_pages = a.max_pages;
         c.new_block_table_stride = a.new_block_table_stride;
         c.cache = a.cache;
-        if (validate_kv_compact(&c) == FGQA_OK) CHECK(compact_layout(c).total > 0);
+        if (validate_kv_compact(&c) == FGQA_OK) {
+            CHECK(compact_layout(c).total > 0);
+            const int64_t n = compact_alone_ints(c);
+            if (n > 0) {
+                ++alone;
+                CHECK(n * 4 <= 61440 && n >= 4 * page_words(c.cache.num_pages) + 2 + c.batch);
+                CHECK((int64_t)c.batch * c.max_pages < INT_MAX - 256 * kAloneThreads);
+            }
+        }
     }
+    CHECK(alone > 100);
     std::printf("%d failed\n", g_failed);
     return g_failed != 0;
 }

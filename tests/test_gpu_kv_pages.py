@@ -325,3 +325,117 @@ def test_fork_then_append(cuda):
             pages = table[i, :-(-len(h) // P)].long()
             assert k[pages].reshape(-1, H, 128)[:len(h), 1, 77].tolist() == h, (step, i)
             assert v[pages].reshape(-1, H, 128)[:len(h), 0, 3].tolist() == [-a for a in h], (step, i)
+
+
+def _page_structs():
+    import ctypes as C
+    two, three = C.c_int64 * 2, C.c_int64 * 3
+
+    class Cache(C.Structure):
+        _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scales", "v_scales")] + [
+            (n, C.c_int32) for n in ("kv_dtype", "num_kv_heads", "head_dim", "page_size", "num_pages")] + [
+            ("k_scale", C.c_float), ("v_scale", C.c_float), ("k_stride", three), ("v_stride", three),
+            ("k_scales_stride", two), ("v_scales_stride", two)]
+
+    class Fork(C.Structure):
+        _fields_ = [("cache", Cache)] + [(n, C.c_void_p) for n in (
+            "block_table", "seqlens", "parents", "new_lens", "held", "new_block_table", "new_seqlens", "num_free")] + [
+            ("block_table_stride", C.c_int64), ("new_block_table_stride", C.c_int64)] + [
+            (n, C.c_int32) for n in ("batch", "max_pages", "new_batch", "new_max_pages")] + [
+            ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+    class Compact(C.Structure):
+        _fields_ = [("cache", Cache)] + [(n, C.c_void_p) for n in (
+            "block_table", "seqlens", "held", "new_block_table", "num_used")] + [
+            ("block_table_stride", C.c_int64), ("new_block_table_stride", C.c_int64)] + [
+            (n, C.c_int32) for n in ("batch", "max_pages")] + [("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+    return Cache, Fork, Compact
+
+
+CacheArgs, ForkArgs, CompactArgs = _page_structs()
+
+
+@pytest.mark.parametrize("width", (9, 9000))
+def test_workspaces_of_the_c_abi(cuda, width):
+    """A narrow table needs no workspace; of a wide one (planned in launches of its own) too small and
+    misaligned ones are refused, and one that is large enough gives what the library's gives."""
+    import ctypes
+    import torch
+    import cuda_llm_ops_amd as fg
+    L = ctypes.CDLL(fg.LIB_PATH)
+    r = random.Random(width)
+    B, N, W, P, H, pages = 4, 6, 9, 16, 2, 60
+    table, lens = _random_rows(r, B, W, P, pages)
+    table = [row + [5] * (width - W) for row in table]
+    parents, new = [3, 0, 0, -1, 2, 0], [4, 0, 40, 17, 1, 3]
+    stream = torch.cuda.current_stream().cuda_stream
+    for kind in ("fork", "compact"):
+        k, v, _ = _cache(torch, cuda, pages, P, H, "bf16")
+        state = _state(k, v, {})
+        t, ln, pa, nw = (_t(torch, cuda, x) for x in (table, lens, parents, new))
+        a = ForkArgs() if kind == "fork" else CompactArgs()
+        a.cache.kv_dtype, a.cache.num_kv_heads, a.cache.head_dim, a.cache.page_size, a.cache.num_pages = 0, H, 128, P, pages
+        a.cache.k, a.cache.v, a.cache.k_scale, a.cache.v_scale = k.data_ptr(), v.data_ptr(), 1.0, 1.0
+        a.cache.k_stride[:], a.cache.v_stride[:] = [P * H * 128, H * 128, 128], [P * H * 128, H * 128, 128]
+        a.block_table, a.seqlens, a.block_table_stride, a.batch, a.max_pages = t.data_ptr(), ln.data_ptr(), width, B, width
+        rows = N if kind == "fork" else B
+        out, out_lens, count = (torch.empty(n, dtype=torch.int32, device=cuda) for n in ((rows, width), (rows,), (1,)))
+        a.new_block_table, a.new_block_table_stride = out.data_ptr(), width
+        if kind == "fork":
+            a.parents, a.new_lens, a.new_seqlens, a.num_free = pa.data_ptr(), nw.data_ptr(), out_lens.data_ptr(), count.data_ptr()
+            a.new_batch, a.new_max_pages = N, width
+            want, want_lens, copies, want_count = ref.fork(table, lens, P, pages, parents, new)
+        else:
+            a.num_used = count.data_ptr()
+            want, moves, want_count = ref.compact(table, lens, P, pages)
+            copies = [(s, d, None) for s, d in moves]
+        fn = getattr(L, f"fgqa_kv_{kind}")
+        fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        need = ctypes.c_size_t(1 << 40)
+        assert getattr(L, f"fgqa_kv_{kind}_workspace_bytes")(ctypes.byref(a), ctypes.byref(need)) == 0
+        assert (need.value > 0) == (width > 9) and need.value < 1 << 20
+        work = torch.empty(need.value + 256, dtype=torch.uint8, device=cuda)
+        if need.value > 0:
+            for ws, n, status in ((work.data_ptr(), need.value - 1, -3), (work.data_ptr() + 4, need.value, -2), (None, need.value, -3)):
+                a.workspace, a.workspace_bytes = ws, n
+                assert fn(ctypes.byref(a), stream) == status
+        for ws, n in ((work.data_ptr(), need.value), (None, 0)):
+            for x, s in zip((k, v), state):
+                x.copy_(s)
+            for x in (out, out_lens, count):
+                x.fill_(-77)
+            a.workspace, a.workspace_bytes = ws, n
+            assert fn(ctypes.byref(a), stream) == 0
+            assert out.tolist() == want and count.tolist() == [want_count]
+            assert kind == "compact" or out_lens.tolist() == want_lens
+            assert _same([k, v], _expect(state, copies))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("with_held", (False, True))
+def test_wide_tables(cuda, dtype, with_held):
+    """Rows that could be long: the same calls planned in launches of their own."""
+    import torch
+    import cuda_llm_ops_amd as fg
+    for seed, (B, N, W, P, H, width) in enumerate(((4, 16, 9, 32, 4, 9000), (40, 50, 5, 8, 2, 1000), (1, 3, 6, 64, 8, 40000))):
+        r = random.Random(f"{dtype} {with_held} {seed}")
+        num_pages = 2 * B * W + 40
+        table, lens = _random_rows(r, B, W, P, num_pages)
+        parents = [r.choice((-1, B, r.randrange(B), 0)) for _ in range(N)]
+        new = [r.choice((-3, 0, 1, P, r.randint(0, 3 * P))) for _ in range(N)]
+        held = [r.random() < 0.3 for _ in range(num_pages)] if with_held else None
+        held_t = None if held is None else torch.tensor(held, device=cuda)
+        wide = [row + [-1] * (width - W) for row in table]
+        k, v, scales = _cache(torch, cuda, num_pages, P, H, dtype, seed)
+        state = _state(k, v, scales)
+        want, want_lens, copies, left = ref.fork(wide, lens, P, num_pages, parents, new, held)
+        out = fg.fork_kv_paged(k, v, _t(torch, cuda, wide), _t(torch, cuda, lens), parents=_t(torch, cuda, parents),
+                               new_lens=_t(torch, cuda, new), held=held_t, **scales)
+        assert out[0].tolist() == want and out[1].tolist() == want_lens and out[2].tolist() == [left]
+        state = _expect(state, copies)
+        assert _same([k, v, *scales.values()], state)
+        want, moves, used = ref.compact(wide, lens, P, num_pages, held)
+        out = fg.compact_kv_paged(k, v, _t(torch, cuda, wide), _t(torch, cuda, lens), held=held_t, **scales)
+        assert out[0].tolist() == want and out[1].tolist() == [used]
+        assert _same([k, v, *scales.values()], _expect(state, [(s, d, None) for s, d in moves]))
