@@ -8,8 +8,11 @@
 // S^T = K Q^T and O^T += V^T P^T on 32x32x16 MFMAs, 32 rows a wave, each K and V row read
 // once from memory for all of them, widened to bf16 and staged in LDS for the four waves.
 //
-// One planning workgroup finds the groups and cuts all work into pieces of about equal
-// token counts that fill the chip; one launch runs them; one merges the partials.
+// A plan finds the groups and cuts all work into pieces of about equal token counts that
+// fill the chip; one launch runs them; one merges the partials.  The running launch's
+// workgroups plan for themselves up to 256 sequences: 8 samples of a prompt of 2000 tokens,
+// 2 KV heads of int8, took 17.4 us, with the plan in a launch of its own 22.0 (4 prompts of 8000 tokens, 16 samples each:
+// 52.4 and 54.2; 128 questions to one document of 32,768: 247 and 250).
 #include <algorithm>
 #include <type_traits>
 
@@ -22,6 +25,7 @@ namespace fgqa {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kPlanThreads = 1024;       // of a planning workgroup of its own
 constexpr int kTile = 64, kBlock = 32;   // shared tokens of a barrier, and of a step
 
 // What runs on one workgroup for each KV head.
@@ -72,22 +76,25 @@ __device__ __forceinline__ int group_of(const int* starts, int n, int b) {
     return lo;
 }
 
-// Latency bounds it: a few dependent loads, barriers and scans of one workgroup, which
-// takes a thread for each group and sequence as far as they go (256 threads for up to 256 of each: a barrier of
-// 4 waves costs less than one of 16).
-template <int kPlanThreads>
-__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p) {
-    constexpr int kGroups = kPlanThreads == 256 ? 256 : plan::kSharedMaxGroups;
+// A workgroup of kN threads plans all work: items(first, n, item) has a range of items,
+// of which item(i) makes one; seqs(b, s) a sequence's partials.  The number of items.
+//
+// Latency bounds it: a few dependent loads, barriers and scans, with a thread for each
+// group and sequence as far as they go.  Where 256 threads go that far each workgroup of the
+// decode plans for itself and makes its own item: a launch less.
+template <int kN, typename Items, typename Seqs>
+__device__ __forceinline__ int shared_plan(const SharedParams& p, Items&& items, Seqs&& seqs) {
+    constexpr int kGroups = kN == kThreads ? kThreads : plan::kSharedMaxGroups;
     __shared__ int s_start[kGroups + 1];
     __shared__ int s_len[kGroups];     // shortest of its sequences, then what is shared
     __shared__ int s_first[kGroups];   // its first sequence with tokens, then its first row of partials
     __shared__ int s_count[kGroups];   // its sequences with tokens, then its pieces
-    __shared__ int64_t s_wave[kPlanThreads / kWave];
+    __shared__ int64_t s_wave[kN / kWave];
     const int tid = threadIdx.x, n = p.num_groups, batch = p.d.batch, group = p.d.group, hkv = p.d.hkv;
     // (these loads are under way together)
     const int len0 = tid < batch ? clamp_len(p.d, tid) : 0;
     const int shared0 = tid < n ? p.shared_lens[tid] : 0;
-    for (int i = tid; i <= n; i += kPlanThreads) {
+    for (int i = tid; i <= n; i += kN) {
         s_start[i] = n > 0 ? min(max(p.group_starts[i], 0), batch) : 0;
         if (i < n) {
             s_len[i] = s_first[i] = INT32_MAX;
@@ -96,20 +103,20 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
     }
     __syncthreads();
     int falls = 0;
-    for (int i = tid; i < n; i += kPlanThreads) falls |= s_start[i + 1] < s_start[i];
+    for (int i = tid; i < n; i += kN) falls |= s_start[i + 1] < s_start[i];
     if (__syncthreads_or(falls)) {   // each start at least the one before it
         for (int d = 1; d <= n; d *= 2) {
-            int v[kGroups / kPlanThreads + 1];
+            int v[kGroups / kN + 1];
             int k = 0;
-            for (int i = tid; i <= n; i += kPlanThreads) v[k++] = max(s_start[i], i >= d ? s_start[i - d] : 0);
+            for (int i = tid; i <= n; i += kN) v[k++] = max(s_start[i], i >= d ? s_start[i - d] : 0);
             __syncthreads();
             k = 0;
-            for (int i = tid; i <= n; i += kPlanThreads) s_start[i] = v[k++];
+            for (int i = tid; i <= n; i += kN) s_start[i] = v[k++];
             __syncthreads();
         }
     }
     int64_t sum = 0, total;
-    for (int b = tid; b < batch; b += kPlanThreads) {
+    for (int b = tid; b < batch; b += kN) {
         const int len = b == tid ? len0 : clamp_len(p.d, b), g = group_of(s_start, n, b);
         sum += len;
         if (g < 0 || len == 0) continue;
@@ -120,7 +127,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
     __syncthreads();
     auto rows_of = [&](int g) { return (s_start[g + 1] - s_start[g]) * group; };
     auto tiles_of = [&](int g) { return (rows_of(g) + plan::kSharedRows - 1) / plan::kSharedRows; };
-    for (int g = tid; g < n; g += kPlanThreads) {
+    for (int g = tid; g < n; g += kN) {
         // (one sequence shares with none)
         int len = s_count[g] > 1 ? min(s_len[g], g == tid ? shared0 : p.shared_lens[g]) : 0;
         len = max(len, 0) >> p.d.page_shift << p.d.page_shift;
@@ -128,32 +135,32 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         s_len[g] = len;
         sum += (int64_t)(tiles_of(g) - s_count[g]) * len;   // in the tiles instead of each sequence
     }
-    block_exclusive_scan<kPlanThreads, true>(sum, s_wave, &total);
+    block_exclusive_scan<kN, true>(sum, s_wave, &total);
     const int chunk = (int)min(plan::shared_chunk(total, p.slots), (int64_t)1 << 30);   // (longer than any sequence)
     // Offsets of items, and, 32 bits up, of rows.
     int64_t at = 0;
-    for (int g0 = 0; g0 < n; g0 += kPlanThreads) {
+    for (int g0 = 0; g0 < n; g0 += kN) {
         const int g = g0 + tid;
         const int len = g < n ? s_len[g] : 0, tiles = len > 0 ? tiles_of(g) : 0, rows = len > 0 ? rows_of(g) : 0;
         const int piece = len > 0 ? plan::shared_piece(len, chunk, kTile) : 1, pieces = (len + piece - 1) / piece;
         int64_t all;
-        const int64_t mine = at + block_exclusive_scan<kPlanThreads, true>(
+        const int64_t mine = at + block_exclusive_scan<kN, true>(
                                       ((int64_t)pieces * hkv * rows << 32) + pieces * tiles, s_wave, &all);
-        int next = (int)(mine & 0xffffffff);
         const int base = (int)(mine >> 32);
-        for (int i = 0; i < pieces; ++i)
-            for (int t = 0; t < tiles; ++t) {
-                Item it;
-                it.b = s_start[g];
-                it.table = s_first[g];
-                it.t0 = i * piece;
-                it.t1 = min(len, it.t0 + piece);
-                it.row0 = t * plan::kSharedRows;
-                it.rows = min(plan::kSharedRows, rows - it.row0);
-                it.slot = base + i * hkv * rows + it.row0;
-                it.stride = rows;
-                p.items[next++] = it;
-            }
+        items((int)(mine & 0xffffffff), pieces * tiles, [&](int i) {
+            const int t = i % tiles;
+            i /= tiles;
+            Item it;
+            it.b = s_start[g];
+            it.table = s_first[g];
+            it.t0 = i * piece;
+            it.t1 = min(len, it.t0 + piece);
+            it.row0 = t * plan::kSharedRows;
+            it.rows = min(plan::kSharedRows, rows - it.row0);
+            it.slot = base + i * hkv * rows + it.row0;
+            it.stride = rows;
+            return it;
+        });
         if (g < n) {
             s_first[g] = base;
             s_count[g] = pieces;
@@ -161,7 +168,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         at += all;
     }
     __syncthreads();
-    for (int b0 = 0; b0 < batch; b0 += kPlanThreads) {
+    for (int b0 = 0; b0 < batch; b0 += kN) {
         const int b = b0 + tid;
         const bool here = b < batch;
         const int g = here ? group_of(s_start, n, b) : -1, len = b == tid ? len0 : here ? clamp_len(p.d, b) : 0;
@@ -169,11 +176,10 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
         const int piece = left > 0 ? plan::shared_piece(left, chunk, plan::kSharedChunk) : 1, pieces = (left + piece - 1) / piece;
         const bool whole = begin == 0 && pieces == 1;
         int64_t all;
-        const int64_t mine = at + block_exclusive_scan<kPlanThreads, true>(
+        const int64_t mine = at + block_exclusive_scan<kN, true>(
                                       ((int64_t)(whole ? 0 : pieces * hkv * group) << 32) + pieces, s_wave, &all);
-        int next = (int)(mine & 0xffffffff);
         const int base = (int)(mine >> 32);
-        for (int i = 0; i < pieces; ++i) {
+        items((int)(mine & 0xffffffff), pieces, [&](int i) {
             Item it;
             it.b = it.table = b;
             it.t0 = begin + i * piece;
@@ -181,8 +187,8 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
             it.slot = whole ? -1 : base + i * hkv * group;
             it.rows = it.row0 = 0;
             it.stride = group;
-            p.items[next++] = it;
-        }
+            return it;
+        });
         if (here) {
             Seq s;
             s.n_shared = begin > 0 ? s_count[g] : 0;
@@ -193,11 +199,21 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams 
             s.n_own = pieces;
             s.whole = whole;
             s.pad = 0;
-            p.seqs[b] = s;
+            seqs(b, s);
         }
         at += all;
     }
-    if (tid == 0) *p.count = (int)(at & 0xffffffff);
+    return (int)(at & 0xffffffff);
+}
+
+__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedParams p) {
+    const int count = shared_plan<kPlanThreads>(
+        p,
+        [&](int first, int n, auto&& item) {
+            for (int i = 0; i < n; ++i) p.items[first + i] = item(i);
+        },
+        [&](int b, const Seq& s) { p.seqs[b] = s; });
+    if (threadIdx.x == 0) *p.count = count;
 }
 
 // ---------------------------------------------------------------- shared tokens
@@ -575,8 +591,24 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
     __shared__ __attribute__((aligned(16))) unsigned char smem[max_int(kSharedSmem, kDecItemSmem<kKv, kDecWaves>)];
     const int at = fast_div((int)blockIdx.x, p.div_hkv);
     const int kvh = (int)blockIdx.x - at * p.d.hkv;
-    const Item it = p.items[at];   // (there is room for every workgroup's)
-    if (at >= *p.count) return;
+    Item it;
+    if (p.items == nullptr) {
+        __shared__ Item s_item;
+        const int count = shared_plan<kThreads>(
+            p,
+            [&](int first, int n, auto&& item) {
+                if (at >= first && at - first < n) s_item = item(at - first);
+            },
+            [&](int b, const Seq& s) {
+                if (blockIdx.x == 0) p.seqs[b] = s;
+            });
+        if (at >= count) return;
+        __syncthreads();
+        it = s_item;
+    } else {
+        it = p.items[at];   // (there is room for every workgroup's)
+        if (at >= *p.count) return;
+    }
     if (it.rows > 0) {
         shared_item<kKv, (kSeg > 0)>(p, smem, it, kvh);
     } else {
@@ -782,8 +814,8 @@ extern "C" int fgqa_decode_shared(const fgqa_decode_shared_args* a, void* stream
     p.count = reinterpret_cast<int32_t*>(ws + pl.count_off);
 
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (d.batch <= 256 && p.num_groups <= 255) hipLaunchKernelGGL(shared_plan_kernel<256>, dim3(1), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL(shared_plan_kernel<1024>, dim3(1), dim3(1024), 0, s, p);
+    if (d.batch <= kThreads && p.num_groups < kThreads && a->max_seqlen > 0) p.items = nullptr;   // (the workgroups plan)
+    else hipLaunchKernelGGL(shared_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p);
     if (a->max_seqlen > 0) {
         const unsigned grid = (unsigned)(pl.max_items * d.hkv);
         const int seg = page_segment(c);

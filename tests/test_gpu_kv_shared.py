@@ -181,6 +181,21 @@ def test_many_groups(cuda):
     c.check(*c.run())
 
 
+def test_odd_groups_of_many(cuda):
+    """As test_odd_groups, of more sequences or groups than the decode's workgroups plan for themselves."""
+    import torch
+    c = Case(torch, cuda, "int8", 4, 2, 16, [256], [[1 + i % 5 for i in range(300)]], [40, 300])
+    for starts, n in (([0, 300], 1), ([-5, 300], 1), ([0, 200, 100, 300], 3), ([299, 1, 300, 9999], 3),
+                      (list(range(0, 302, 2)) + [300] * 250, 400)):
+        print(starts[:4], n, flush=True)
+        c.check(*c.run(starts, [256] * n))
+    now = [0 if i % 3 == 0 else 3 if i == 7 else n for i, n in enumerate(c.lens)]
+    c.n.copy_(c.ints(now))
+    c.check(*c.run(), lens=now)
+    c = Case(torch, cuda, "int8", 4, 2, 16, [256], [[1 + i % 5 for i in range(30)]], [40])
+    c.check(*c.run([0, 20, 10, 30] + [30] * 297, [256] * 300))
+
+
 def test_long_and_large(cuda):
     """A long document: many cuts of the shared tokens; a large group: many row tiles."""
     import torch
