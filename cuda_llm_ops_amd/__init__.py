@@ -1,4 +1,4 @@
-"""MI355X-native flash grouped-query attention (decode incl. paged/fp8/int8 KV caches, their writing and eviction, causal, sliding-window, MLA and sparse-index prefill, and the causal, sliding-window and MLA prefill backward).
+"""MI355X-native flash grouped-query attention (decode incl. paged/fp8/int8 KV caches, their writing, eviction and forking, causal, sliding-window, MLA and sparse-index prefill, the causal, sliding-window and MLA prefill backward, and norm and rotation of queries and keys).
 
 The kernels live in libfgqa.so (HIP, gfx950); ``flash_gqa`` is the Python host
 interface over its C ABI (include/fgqa.h), ``kv_cache`` that of the paged
