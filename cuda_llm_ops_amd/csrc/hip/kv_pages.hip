@@ -99,12 +99,27 @@ __device__ __forceinline__ uint32_t word_mask(int w, int num_pages) {
     return left >= 32 ? 0xffffffffu : (1u << left) - 1;
 }
 
+typedef uint32_t u32x4b_t __attribute__((ext_vector_type(4), aligned(1)));
+
 // held[32w .. 32w + 31] as bits.
 __device__ __forceinline__ uint32_t held_word(const uint8_t* held, int w, int num_pages) {
+    if (held == nullptr) return 0;
+    const uint8_t* src = held + (int64_t)32 * w;
+    const int n = min(32, num_pages - 32 * w);
     uint32_t bits = 0;
-    if (held != nullptr) {
-        const int n = min(32, num_pages - 32 * w);
-        for (int i = 0; i < n; ++i) bits |= (held[(int64_t)32 * w + i] != 0 ? 1u : 0u) << i;
+    if (n == 32) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const u32x4b_t x = *reinterpret_cast<const u32x4b_t*>(src + 16 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // bytes other than 0 have their top bits in m, which the product brings together
+                const uint32_t m = ((((x[j] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x[j]) & 0x80808080u) >> 7;
+                bits |= ((m * 0x01020408u) >> 24 & 15u) << (16 * i + 4 * j);
+            }
+        }
+    } else {
+        for (int i = 0; i < n; ++i) bits |= (src[i] != 0 ? 1u : 0u) << i;
     }
     return bits;
 }

@@ -132,6 +132,28 @@ def test_fork_forms(cuda):
     assert _same([k, v], _expect(state, want[2]))
 
 
+@pytest.mark.parametrize("offset", (0, 1, 3))
+def test_held_of_any_value_and_address(cuda, offset):
+    import torch
+    import cuda_llm_ops_amd as fg
+    r = random.Random(offset)
+    B, W, P, H, pages = 3, 30, 1, 1, 211
+    table, lens = _random_rows(r, B, W, P, pages)
+    marks = [r.choice((0, 0, 1, 0x7F, 0x80, 0xFF)) for _ in range(pages)]
+    held = torch.tensor([9] * offset + marks, dtype=torch.uint8, device=cuda)[offset:]
+    new = [5, 0, 40]
+    k, v, _ = _cache(torch, cuda, pages, P, H, "bf16")
+    state = _state(k, v, {})
+    want, want_lens, copies, left = ref.fork(table, lens, P, pages, None, new, marks, 70)
+    out = fg.fork_kv_paged(k, v, _t(torch, cuda, table), _t(torch, cuda, lens), new_lens=_t(torch, cuda, new), held=held, max_pages=70)
+    assert out[0].tolist() == want and out[1].tolist() == want_lens and out[2].tolist() == [left]
+    state = _expect(state, copies)
+    want, moves, used = ref.compact(table, lens, P, pages, marks)
+    out = fg.compact_kv_paged(k, v, _t(torch, cuda, table), _t(torch, cuda, lens), held=held)
+    assert out[0].tolist() == want and out[1].tolist() == [used]
+    assert _same([k, v], _expect(state, [(a, b, None) for a, b in moves]))
+
+
 def test_fork_large(cuda):
     """Many pages (more words than one round of the scan), long rows, many rows, nothing free."""
     import torch
