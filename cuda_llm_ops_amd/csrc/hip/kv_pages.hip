@@ -552,7 +552,7 @@ extern "C" int fgqa_kv_fork(const fgqa_kv_fork_args* a, void* stream) {
     p.num_free = a->num_free;
     p.stride = a->block_table_stride;
     p.new_stride = a->new_block_table_stride;
-    p.batch = a->batch;
+    p.batch = a->new_batch > 0 ? a->batch : 0;   // (with no new row the old ones are not read, and may be NULL)
     p.new_batch = a->new_batch;
     p.new_max_pages = a->new_max_pages;
     p.max_tokens = std::min(a->max_pages, a->new_max_pages) * a->cache.page_size;

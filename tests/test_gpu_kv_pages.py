@@ -434,6 +434,28 @@ def test_workspaces_of_the_c_abi(cuda, width):
             assert _same([k, v], _expect(state, copies))
 
 
+@pytest.mark.parametrize("width", (9, 9000))
+def test_no_new_rows_of_the_c_abi(cuda, width):
+    """Every sequence is dropped: the old rows are not read (here there are none), the pages are counted."""
+    import ctypes
+    import torch
+    import cuda_llm_ops_amd as fg
+    P, H, pages = 16, 2, 60
+    k, v, _ = _cache(torch, cuda, pages, P, H, "bf16")
+    a = ForkArgs()
+    a.cache.kv_dtype, a.cache.num_kv_heads, a.cache.head_dim, a.cache.page_size, a.cache.num_pages = 0, H, 128, P, pages
+    a.cache.k, a.cache.v, a.cache.k_scale, a.cache.v_scale = k.data_ptr(), v.data_ptr(), 1.0, 1.0
+    a.cache.k_stride[:], a.cache.v_stride[:] = [P * H * 128, H * 128, 128], [P * H * 128, H * 128, 128]
+    held = torch.tensor([1] * 7 + [0] * (pages - 7), dtype=torch.uint8, device=cuda)
+    count = torch.full((1,), -77, dtype=torch.int32, device=cuda)
+    a.held, a.num_free = held.data_ptr(), count.data_ptr()
+    a.block_table_stride, a.new_block_table_stride, a.batch, a.max_pages, a.new_max_pages = width, width, 4, width, width
+    fn = ctypes.CDLL(fg.LIB_PATH).fgqa_kv_fork
+    fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    assert fn(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+    assert count.tolist() == [pages - 7]
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("with_held", (False, True))
 def test_wide_tables(cuda, dtype, with_held):
