@@ -13,6 +13,8 @@
 // workgroups plan for themselves up to 256 sequences: 8 samples of a prompt of 2000 tokens,
 // 2 KV heads of int8, took 17.4 us, with the plan in a launch of its own 22.0 (4 prompts of 8000 tokens, 16 samples each:
 // 52.4 and 54.2; 128 questions to one document of 32,768: 247 and 250).
+#include <float.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -234,10 +236,6 @@ struct TileShape {
     static constexpr int loads = kTile / rows;
 };
 
-// Tokens [it.t0, it.t1) of up to 128 query rows of one KV head.
-// kUni: the rows of a wave's load lie in one page (pages of at least 4 rows of bf16, 8 of codes, whose
-// bytes stay below 2^31), read through a buffer resource that ends at the last token (rows past
-// it are zeros); the wave's pages come 64 loads at a time from one vector load of the table.
 // Four scores times their tokens' scales.
 __device__ __forceinline__ void scale4(f32x16_t& s, int q, f32x4_t by) {
 #pragma unroll
@@ -253,9 +251,17 @@ __device__ __forceinline__ void static_for(F&& f) {
     }
 }
 
-template <int kKv, bool kUni>
+// Tokens [it.t0, it.t1) of up to 128 query rows of one KV head.
+// kUni: the rows of a wave's load lie in one page (pages of at least 4 rows of bf16, 8 of codes, whose
+// bytes stay below 2^31), read through a buffer resource that ends at the last token (rows past
+// it are zeros); the wave's pages come 64 loads at a time from one vector load of the table.
+// kFlat: 32 tokens of a block-scaled cache lie in one page, so that a step's scores have one factor, as they
+// have without block scales, and its P one too (128 questions to 32,768 tokens of e4m3: 244 us, with a
+// factor for each token 258).
+template <int kKv, int kSeg>
 __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned char* smem, const Item& it, int kvh) {
     using T = TileShape<kKv>;
+    constexpr bool kUni = kSeg > 0, kFlat = T::blocks && kSeg >= kBlock, kScaled = T::blocks && !kFlat;
     const DecodeParams& p = sp.d;
     const int tid = threadIdx.x, lane = tid & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -271,7 +277,7 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
             const u32x4_t x = *reinterpret_cast<const u32x4_t*>(q + 16 * ks);
-            qop[ks] = as_bf16x8(T::blocks ? x : x ^ sp.q_sign);
+            qop[ks] = as_bf16x8(kScaled ? x : x ^ sp.q_sign);
         }
     }
     float m_run = -INFINITY, l_run = 0.f;   // l: this lane's share
@@ -403,7 +409,7 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
     };
     auto stage = [&]([[maybe_unused]] int j) {
         if constexpr (!kDma) {
-            stage_one(j, j & 1, kreg, ksreg, pt_ks, p.scale_log2);
+            stage_one(j, j & 1, kreg, ksreg, pt_ks, kScaled ? p.scale_log2 : sp.scale_log2);
             stage_one(j, 2 + (j & 1), vreg, vsreg, pt_vs, 1.f);
         }
     };
@@ -456,7 +462,10 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
     // Written in the order that it is to be issued in: operands three or four products ahead (the first of the
     // tile's second half at the end of its first), nothing that waits for a product right behind it.
     bf16x8_t ring[4], vring[3];
-    auto step = [&](int j, auto half_c, f32x16_t& s, f32x16_t& next, float& top) {
+    // kFlat: block h's factor of the scores (above 0: masked scores stay -inf), and of P
+    [[maybe_unused]] auto k_factor = [&](int at, int h) { return fmaxf(scale_lds[at * kTile + h * kBlock], FLT_MIN); };
+    auto step = [&](int j, auto half_c, f32x16_t& s, f32x16_t& next, float& top, [[maybe_unused]] float factor,
+                    [[maybe_unused]] float& next_factor) {
         constexpr int h = decltype(half_c)::value;
         const int left = t1 - (t0 + j * kTile + h * kBlock);
         if (left < kBlock) {
@@ -467,16 +476,17 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) ring[ks] = k_operand(j, 0, ks);
         }
-        const float c = T::blocks ? 1.f : sp.scale_log2;
+        const float c = kFlat ? factor : kScaled ? 1.f : sp.scale_log2;
+        [[maybe_unused]] const float by_all = kFlat ? scale_lds[(2 + (j & 1)) * kTile + h * kBlock] : 1.f;
         float sum[2] = {0.f, 0.f}, m_sub = 0.f;
         bf16x8_t pop[2];
         [[maybe_unused]] f32x4_t by;
         auto softmax = [&](auto ec) {
             constexpr int e = decltype(ec)::value;
-            if constexpr (T::blocks && e % 4 == 0) by = scales_of(2 + (j & 1), h, e / 4);
-            const float w = fast_exp2(T::blocks ? s[e] - m_sub : fmaf(s[e], c, -m_sub));
+            if constexpr (kScaled && e % 4 == 0) by = scales_of(2 + (j & 1), h, e / 4);
+            const float w = fast_exp2(kScaled ? s[e] - m_sub : fmaf(s[e], c, -m_sub));
             sum[e & 1] += w;
-            pop[e >> 3][e & 7] = (__bf16)(T::blocks ? w * by[e & 3] : w);
+            pop[e >> 3][e & 7] = (__bf16)(kScaled ? w * by[e & 3] : kFlat ? w * by_all : w);
         };
 #pragma unroll
         for (int i = 0; i < 16; ++i) next[i] = 0.f;
@@ -517,7 +527,8 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
                 softmax(std::integral_constant<int, 12 + 2 * n>{});
                 softmax(std::integral_constant<int, 13 + 2 * n>{});
             } else if constexpr (n < 6) {   // (4 scores each)
-                if constexpr (T::blocks) scale4(next, n - 2, scales_of(j & 1, h, n - 2));
+                if constexpr (kScaled) scale4(next, n - 2, scales_of(j & 1, h, n - 2));
+                if constexpr (kFlat && n == 2) next_factor = k_factor(j & 1, h);
 #pragma unroll
                 for (int i = 4 * (n - 2); i < 4 * (n - 1); ++i) most = i == 0 ? next[0] : fmaxf(most, next[i]);
             }
@@ -539,16 +550,17 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
     }
     __syncthreads();
     f32x16_t s0, s1;
-    float top = -INFINITY;
+    float top = -INFINITY, f0 = 1.f, f1 = 1.f;
     if (active) {   // block 0: the second half of K's tile -1
 #pragma unroll
         for (int i = 0; i < 16; ++i) s0[i] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) s0 = mfma32(k_operand(-1, 1, ks), qop[ks], s0);
-        if constexpr (T::blocks) {
+        if constexpr (kScaled) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) scale4(s0, q, scales_of(1, 1, q));
         }
+        if constexpr (kFlat) f0 = k_factor(1, 1);
         top = largest(s0);
     }
     for (int j = 0; j < tiles; ++j) {
@@ -559,8 +571,8 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
             else if (j + 2 < tiles) load(j + 2);
         }
         if (active) {
-            step(j, std::integral_constant<int, 0>{}, s0, s1, top);
-            if (t0 + j * kTile + kBlock < t1) step(j, std::integral_constant<int, 1>{}, s1, s0, top);
+            step(j, std::integral_constant<int, 0>{}, s0, s1, top, f0, f1);
+            if (t0 + j * kTile + kBlock < t1) step(j, std::integral_constant<int, 1>{}, s1, s0, top, f1, f0);
         }
         landed();
     }
@@ -610,7 +622,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
         if (at >= *p.count) return;
     }
     if (it.rows > 0) {
-        shared_item<kKv, (kSeg > 0)>(p, smem, it, kvh);
+        shared_item<kKv, kSeg>(p, smem, it, kvh);
     } else {
         const bool whole = it.slot < 0;
         dec_item_of<kKv, kSeg, kDecWaves, true>(p.d, smem, it.t0, it.t1, kvh, it.b, threadIdx.x, whole,
