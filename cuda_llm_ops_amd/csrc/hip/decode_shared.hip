@@ -10,9 +10,10 @@
 //
 // A plan finds the groups and cuts all work into pieces of about equal token counts that
 // fill the chip; one launch runs them; one merges the partials.  The running launch's
-// workgroups plan for themselves up to 256 sequences: 8 samples of a prompt of 2000 tokens,
-// 2 KV heads of int8, took 17.4 us, with the plan in a launch of its own 22.0 (4 prompts of 8000 tokens, 16 samples each:
-// 52.4 and 54.2; 128 questions to one document of 32,768: 247 and 250).
+// workgroups plan for themselves up to 256 sequences: 4 samples of a prompt of 1000 tokens
+// of bf16, 8 KV heads, took 14.6 us, with the plan in a launch of its own 17.2 (128 of 8000,
+// one KV head: 35.4 and 53.7; 4 prompts of 8000 tokens of e4m3, 16 samples each: 52.4 and
+// 54.2; 128 questions to one document of 32,768 of bf16: 247 and 250).
 #include <float.h>
 
 #include <algorithm>
@@ -745,6 +746,10 @@ using namespace fgqa;
 extern "C" int fgqa_decode_shared_workspace_bytes(const fgqa_decode_shared_args* a, size_t* bytes) {
     int st = plan::validate_decode_shared(a);
     if (st != FGQA_OK || bytes == nullptr) return st != FGQA_OK ? st : FGQA_ERR_INVALID_ARGUMENT;
+    if (plan::shared_as_blocks(a, device_cu_count())) {
+        const fgqa_decode_blocks_args b = plan::as_decode_blocks(a);
+        return fgqa_decode_blocks_workspace_bytes(&b, bytes);
+    }
     plan::SharedPlan pl;
     st = plan::plan_decode_shared(a, device_cu_count(), &pl);
     if (st != FGQA_OK) return st;
@@ -757,6 +762,10 @@ extern "C" int fgqa_decode_shared(const fgqa_decode_shared_args* a, void* stream
     if (st == FGQA_OK) st = plan::validate_decode_shared_pointers(a);
     if (st != FGQA_OK) return st;
     if (a->batch == 0) return FGQA_OK;
+    if (plan::shared_as_blocks(a, device_cu_count())) {
+        const fgqa_decode_blocks_args b = plan::as_decode_blocks(a);
+        return fgqa_decode_blocks(&b, stream);
+    }
     plan::SharedPlan pl;
     st = plan::plan_decode_shared(a, device_cu_count(), &pl);
     if (st != FGQA_OK) return st;

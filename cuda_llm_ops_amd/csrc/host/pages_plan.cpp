@@ -142,7 +142,7 @@ int validate_kv_compact(const fgqa_kv_compact_args* a) {
     return FGQA_OK;
 }
 
-fgqa_decode_paged_args as_decode_paged(const fgqa_decode_shared_args* a) {
+fgqa_decode_blocks_args as_decode_blocks(const fgqa_decode_shared_args* a) {
     fgqa_decode_blocks_args b = {};
     b.cache = a->cache;
     b.q = a->q;
@@ -159,6 +159,23 @@ fgqa_decode_paged_args as_decode_paged(const fgqa_decode_shared_args* a) {
         b.o_stride[i] = a->o_stride[i];
     }
     b.block_table_stride = a->block_table_stride;
+    b.workspace = a->workspace;
+    b.workspace_bytes = a->workspace_bytes;
+    return b;
+}
+
+bool shared_as_blocks(const fgqa_decode_shared_args* a, int cus) {
+    // Tokens of a KV head for each CU, of sequences as long as they may be.  8 samples of 2000 tokens, 2 KV
+    // heads of int8: 10.6 us each on their own, 16.3 together; 137,000 tokens of all KV heads 12.9 to 14.4 and 19.3 to
+    // 21.5, 263,000 to 294,000 tokens 12.0 to 17.1 and 15.8 to 22.2, 550,000 28.6 to 36.4 and 18.8 to 25.7.
+    // (Without block scales the decode on their own takes longer from the start: 23.1 and 13.8.)
+    constexpr int64_t kAloneTokens = 1152;
+    return a->cache.k_scales != nullptr &&
+           (i128)a->batch * a->cache.num_kv_heads * a->max_seqlen <= (i128)kAloneTokens * (cus > 0 ? cus : 256);
+}
+
+fgqa_decode_paged_args as_decode_paged(const fgqa_decode_shared_args* a) {
+    const fgqa_decode_blocks_args b = as_decode_blocks(a);
     fgqa_decode_paged_args p = as_decode_paged(&b);
     if (a->cache.kv_dtype == FGQA_KV_BF16) p.kv_dtype = FGQA_KV_BF16;
     if (a->cache.kv_dtype == FGQA_KV_FP8_E4M3 && a->cache.k_scales == nullptr) {

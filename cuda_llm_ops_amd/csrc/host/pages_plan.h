@@ -76,6 +76,11 @@ struct SharedPlan {
     size_t part_ml_off, items_off, seqs_off, count_off, total;   // bytes; partial O at 0
 };
 constexpr int kSharedItemInts = 8, kSharedSeqInts = 8;
+// The call without its groups, over a cache with block scales.
+fgqa_decode_blocks_args as_decode_blocks(const fgqa_decode_shared_args* a);
+// Whether a call is that one: with few tokens its launch and chain of loads cost more than
+// reading what is shared once for each sequence.
+bool shared_as_blocks(const fgqa_decode_shared_args* a, int cus);
 // What the decode checks of its arguments, an e4m3 cache of the same sizes for int8.
 fgqa_decode_paged_args as_decode_paged(const fgqa_decode_shared_args* a);
 int validate_decode_shared(const fgqa_decode_shared_args* a);

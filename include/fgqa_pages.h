@@ -123,6 +123,8 @@ int fgqa_kv_compact(const fgqa_kv_compact_args* args, void* stream);
  * Sums and statistics are fp32; P (times V's scale) is rounded to bf16 for P.V over
  * shared tokens.  The work is cut as the lengths of all sequences ask: outputs may differ in
  * rounding between batches, not between runs of one.  num_groups is at most 4096.
+ * Over a cache with block scales a call of few tokens (batch * KV heads * max_seqlen at most
+ * 1152 a CU) is fgqa_decode_blocks, which then takes less time.
  */
 typedef struct fgqa_decode_shared_args {
     fgqa_kv_cache cache;

@@ -87,6 +87,28 @@ int main() {
     CHECK(shared_piece(1 << 30, 1 << 30, 64) == 1 << 30 && shared_piece((1 << 30) - 1, 1 << 29, 64) == 1 << 29);
     CHECK(shared_piece(1, 128, 64) == 64 && shared_piece(129, 128, 64) == 128 && shared_piece(1000, 384, 128) == 384);
 
+    {
+        fgqa_decode_shared_args a = args();
+        float scale = 1.f;
+        a.cache.num_kv_heads = 8;
+        a.batch = 16;
+        a.max_seqlen = 2304;
+        CHECK(!shared_as_blocks(&a, 256));
+        a.cache.k_scales = a.cache.v_scales = &scale;
+        CHECK(shared_as_blocks(&a, 256) && shared_as_blocks(&a, 0) && !shared_as_blocks(&a, 255));
+        a.max_seqlen = 2305;
+        CHECK(!shared_as_blocks(&a, 256));
+        a.batch = (1 << 15) - 1;
+        a.max_seqlen = 1 << 30;
+        CHECK(!shared_as_blocks(&a, 256));
+        a.max_seqlen = 0;
+        CHECK(shared_as_blocks(&a, 256));
+        a.workspace = &scale;
+        a.workspace_bytes = 77;
+        const fgqa_decode_blocks_args b = as_decode_blocks(&a);
+        CHECK(b.batch == a.batch && b.cache.k_scales == &scale && b.workspace == &scale && b.workspace_bytes == 77);
+    }
+
     std::mt19937_64 rng(5);
     auto some = [&](int64_t n) { return (int64_t)(rng() % (uint64_t)n); };
     for (int turn = 0; turn < 20000; ++turn) {

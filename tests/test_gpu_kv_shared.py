@@ -21,8 +21,10 @@ class Case:
     """Sequences on pages of a cache, groups of which share their first pages; everything else is filled
     with NaN (bf16, e4m3) or the largest codes."""
 
-    def __init__(self, torch, dev, dtype, Hq, Hkv, P, shared, groups, alone=(), seed=1, scales="blocks", sigma=1.0, extra=3):
-        """shared: tokens of each group; groups: each group's sequences' own tokens; alone: of those without."""
+    def __init__(self, torch, dev, dtype, Hq, Hkv, P, shared, groups, alone=(), seed=1, scales="blocks", sigma=1.0, extra=3,
+                 wide=True):
+        """shared: tokens of each group; groups: each group's sequences' own tokens; alone: of those without;
+        wide: rows that could be long, which small calls over block scales are not decoded one by one with."""
         r = random.Random(seed)
         self.torch, self.dev, self.dtype, self.P, self.Hq, self.Hkv = torch, dev, dtype, P, Hq, Hkv
         self.starts, self.shared = [0], list(shared)
@@ -42,6 +44,8 @@ class Case:
             lens.append(n)
         self.lens = lens
         W = max([len(x) for x in rows] + [1]) + extra
+        if wide and dtype != "bf16" and scales == "blocks" and rows:
+            W = max(W, 1152 * 256 // (len(rows) * Hkv * P) + 1)
         # (entries behind a sequence's pages are nobody's)
         self.table = torch.tensor([x + [r.choice((-1, need + 5, 0))] * (W - len(x)) for x in rows], dtype=torch.int32,
                                   device=dev).reshape(len(rows), W)
@@ -136,6 +140,26 @@ def test_against_float64(cuda, dtype, scales, Hq, Hkv, P, shared, groups, alone)
     c.check(out, lse)
     again, lse2 = c.run()
     assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("dtype", ("e4m3", "int8"))
+def test_small_calls(cuda, dtype):
+    """Block scales and few tokens: each sequence on its own, as decode_flash_gqa_paged has it."""
+    import torch
+    import cuda_llm_ops_amd as fg
+    for Hq, Hkv, P, shared, groups, alone in ((16, 2, 16, [400], [[3, 50, 1, 130, 0, 17, 64, 9]], []), (8, 8, 64, [300], [[1, 2]], [33]),
+                                              (4, 1, 8, [137], [[40] * 5], []), (6, 3, 1, [0], [[1]], [7])):
+        c = Case(torch, cuda, dtype, Hq, Hkv, P, shared, groups, alone, wide=False)
+        out, lse = c.run()
+        c.check(out, lse)
+        want_lse = torch.empty_like(lse)
+        want = fg.decode_flash_gqa_paged(c.q, *c.cache, c.table, c.n, lse=want_lse, **c.kw)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+        work = torch.empty(64 << 20, dtype=torch.uint8, device=cuda)
+        again, lse2 = c.run(workspace=work)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+        c.n[0] = 0
+        c.check(*c.run(), lens=[0] + c.lens[1:])
 
 
 @pytest.mark.parametrize("dtype", ("bf16", "int8"))
