@@ -184,22 +184,29 @@ __device__ __forceinline__ ForkRow fork_row(const ForkParams& p, int i) {
     r.part = r.len & ((1 << p.c.page_shift) - 1);
     return r;
 }
+__device__ __forceinline__ ForkRow fork_row(const ForkParams& p, int old, const int32_t* lens) {   // old: -1, or a row
+    ForkRow r;
+    r.p = old;
+    r.there = old >= 0;
+    r.len = r.there ? lens[old] : 0;
+    r.full = r.len >> p.c.page_shift;
+    r.part = r.len & ((1 << p.c.page_shift) - 1);
+    return r;
+}
 __device__ __forceinline__ bool is_page(const CacheParams& c, int page) { return page >= 0 && page < c.num_pages; }
 
-// The partly filled page of a row (its cell r.full), and whether the row keeps it.
-__device__ __forceinline__ bool keeps_last(const ForkParams& p, const ForkRow& r, int i, const int32_t* first, int* page) {
-    *page = p.table[r.p * p.stride + r.full];
-    if (!is_page(p.c, *page)) return true;
-    return first[r.p] == i && (p.held == nullptr || p.held[*page] == 0);
-}
-
-// Pages of its own that row i wants; *kept: cells before them.
-__device__ __forceinline__ int fresh_pages(const ForkParams& p, const ForkRow& r, int i, const int32_t* first, int* kept) {
-    int page;
-    *kept = r.full + (r.part > 0 && keeps_last(p, r, i, first, &page) ? 1 : 0);
+// Pages of its own that row i wants; *kept: cells before them.  last: the old row's partly filled page (its
+// cell r.full), which its first new row keeps.
+__device__ __forceinline__ int fresh_pages(const ForkParams& p, const ForkRow& r, int i, int first, int last, int* kept) {
+    const bool keeps = !is_page(p.c, last) || (first == i && (p.held == nullptr || p.held[last] == 0));
+    *kept = r.full + (r.part > 0 && keeps ? 1 : 0);
     const int64_t more = p.new_lens != nullptr ? max(p.new_lens[i], 0) : 0;
     const int64_t cells = (r.len + more + (1 << p.c.page_shift) - 1) >> p.c.page_shift;
     return (int)min(cells, (int64_t)p.new_max_pages) - *kept;
+}
+__device__ __forceinline__ int fresh_pages(const ForkParams& p, const ForkRow& r, int i, int* kept) {
+    const bool part = r.part > 0;   // (of an old row, then)
+    return fresh_pages(p, r, i, part ? p.first[r.p] : -1, part ? p.table[r.p * p.stride + r.full] : -1, kept);
 }
 
 __global__ __launch_bounds__(kThreads) void fork_clear_kernel(ForkParams p) {
@@ -222,10 +229,10 @@ __global__ __launch_bounds__(kThreads) void fork_mark_kernel(ForkParams p) {
     }
 }
 
-// Counts of free pages by words and of fresh ones by rows (row(i, fresh pages, those of rows
-// before it, cells kept)); the free pages that are left.  A workgroup.
-template <typename F>
-__device__ __forceinline__ int fork_scan(const ForkParams& p, const uint32_t* bits, const int32_t* first, int32_t* before, F&& row) {
+// Counts of free pages by words and of fresh ones by rows (fresh(i, &cells kept) has a row's, row(i, fresh
+// pages, those of rows before it, cells kept) takes them); the free pages that are left.  A workgroup.
+template <typename Fresh, typename Row>
+__device__ __forceinline__ int fork_scan(const ForkParams& p, const uint32_t* bits, int32_t* before, Fresh&& fresh, Row&& row) {
     __shared__ int s_wave[kScanThreads / kWave];
     const int free_pages = scan_words(p.words, before, s_wave, [&](int w) { return __popc(~bits[w] & word_mask(w, p.c.num_pages)); });
     __shared__ int64_t s_wave64[kScanThreads / kWave];
@@ -234,7 +241,7 @@ __device__ __forceinline__ int fork_scan(const ForkParams& p, const uint32_t* bi
         const int i = i0 + (int)threadIdx.x;
         int kept = 0;
         int64_t total;
-        const int64_t n = i < p.new_batch ? fresh_pages(p, fork_row(p, i), i, first, &kept) : 0;
+        const int64_t n = i < p.new_batch ? fresh(i, &kept) : 0;
         const int64_t at = block_exclusive_scan<kScanThreads, true>(n, s_wave64, &total);
         if (i < p.new_batch) row(i, (int)n, (int)min(wanted + at, (int64_t)INT32_MAX), kept);
         wanted += total;
@@ -243,7 +250,9 @@ __device__ __forceinline__ int fork_scan(const ForkParams& p, const uint32_t* bi
 }
 
 __global__ __launch_bounds__(kScanThreads) void fork_scan_kernel(ForkParams p) {
-    const int left = fork_scan(p, p.bits, p.first, p.before, [&](int i, int, int at, int) { p.row_first[i] = at; });
+    const int left = fork_scan(
+        p, p.bits, p.before, [&](int i, int* kept) { return fresh_pages(p, fork_row(p, i), i, kept); },
+        [&](int i, int, int at, int) { p.row_first[i] = at; });
     if (threadIdx.x == 0) *p.num_free = left;
 }
 
@@ -258,7 +267,7 @@ __global__ __launch_bounds__(kThreads) void fork_fill_kernel(ForkParams p) {
     const int i = blockIdx.x;
     const ForkRow r = fork_row(p, i);
     int kept;
-    const int fresh = fresh_pages(p, r, i, p.first, &kept);
+    const int fresh = fresh_pages(p, r, i, &kept);
     const int first = p.row_first[i], free_pages = p.before[p.words];
     auto fresh_page = [&](int n) { return n < free_pages - first ? free_page(p, p.bits, p.before, first + n) : -1; };
     const int at = blockIdx.y * kThreads + threadIdx.x, step = gridDim.y * kThreads;
@@ -278,7 +287,8 @@ __global__ __launch_bounds__(kScanThreads) void fork_alone_kernel(ForkParams p, 
     int32_t* before = smem + p.words;
     int32_t* first = before + p.words + 1;   // [batch]
     int32_t* lens = first + p.batch;         // [batch]
-    int32_t* row = lens + p.batch;           // [new_batch][4]: old row, fresh pages, those of rows before it, cells kept
+    int32_t* last = lens + p.batch;          // [batch]: their partly filled pages
+    int32_t* row = last + p.batch;           // [new_batch][4]: old row, fresh pages, those of rows before it, cells kept
     const int tid = threadIdx.x;
     for (int w = tid; w < p.words; w += kScanThreads) bits[w] = held_word(p.held, w, p.c.num_pages);
     for (int b = tid; b < p.batch; b += kScanThreads) {
@@ -293,21 +303,29 @@ __global__ __launch_bounds__(kScanThreads) void fork_alone_kernel(ForkParams p, 
         if (there) atomicMin(&first[parent], i);
     }
     __syncthreads();
-    const int round = (1 << p.c.page_shift) - 1, old_cells = p.batch * width;
+    const int old_cells = p.batch * width;
 #pragma unroll 4
     for (int x = tid; x < old_cells; x += kScanThreads) {
         const int b = fast_div(x, div_width), j = x - b * width;
         if (j <= (lens[b] - 1) >> p.c.page_shift && first[b] != INT32_MAX) {
             const int page = p.table[b * p.stride + j];
             if (is_page(p.c, page)) atomicOr(&bits[page >> 5], 1u << (page & 31));
+            if (j == lens[b] >> p.c.page_shift) last[b] = page;
         }
     }
     __syncthreads();
-    const int left = fork_scan(p, bits, first, before, [&](int i, int n, int at, int kept) {
-        row[4 * i + 1] = n;
-        row[4 * i + 2] = at;
-        row[4 * i + 3] = kept;
-    });
+    const int left = fork_scan(
+        p, bits, before,
+        [&](int i, int* kept) {
+            const ForkRow r = fork_row(p, row[4 * i], lens);
+            const bool part = r.part > 0;
+            return fresh_pages(p, r, i, part ? first[r.p] : -1, part ? last[r.p] : -1, kept);
+        },
+        [&](int i, int n, int at, int kept) {
+            row[4 * i + 1] = n;
+            row[4 * i + 2] = at;
+            row[4 * i + 3] = kept;
+        });
     if (blockIdx.x == 0 && tid == 0) *p.num_free = left;
     __syncthreads();
     const int free_pages = before[p.words];
@@ -317,12 +335,11 @@ __global__ __launch_bounds__(kScanThreads) void fork_alone_kernel(ForkParams p, 
     const int lane = tid % kWave, waves = gridDim.x * (kScanThreads / kWave);
     for (int64_t t = (tid / kWave) * gridDim.x + blockIdx.x; t < (int64_t)p.new_batch * slices; t += waves) {
         const int i = (int)(t / slices), slice = (int)(t - (int64_t)i * slices);
-        const int parent = row[4 * i], len = parent >= 0 ? lens[parent] : 0, full = len >> p.c.page_shift;
-        const bool copied = (len & round) != 0 && row[4 * i + 3] == full;
+        const ForkRow r = fork_row(p, row[4 * i], lens);
+        const bool copied = r.part > 0 && row[4 * i + 3] == r.full;
         const int dst = copied ? fresh_page(row[4 * i + 2], 0) : -1;
-        if (slice == 0 && lane == 0) p.new_seqlens[i] = copied && dst < 0 ? full << p.c.page_shift : len;
-        if (dst >= 0)
-            copy_slots(p.c, p.shape, p.table[parent * p.stride + full], dst, len & round, slice * kWave + lane, slices * kWave);
+        if (slice == 0 && lane == 0) p.new_seqlens[i] = copied && dst < 0 ? r.full << p.c.page_shift : r.len;
+        if (dst >= 0) copy_slots(p.c, p.shape, last[r.p], dst, r.part, slice * kWave + lane, slices * kWave);
     }
     const int cells = p.new_batch * p.new_max_pages;
     for (int x = blockIdx.x * kScanThreads + tid; x < cells; x += gridDim.x * kScanThreads) {

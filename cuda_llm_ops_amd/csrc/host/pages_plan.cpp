@@ -69,7 +69,7 @@ constexpr int64_t kAloneMoves = (int64_t)1 << 29;
 }  // namespace
 
 int fork_alone_ints(const fgqa_kv_fork_args& a) {
-    const int64_t ints = 2 * page_words(a.cache.num_pages) + 1 + 2 * (int64_t)a.batch + 4 * (int64_t)a.new_batch;
+    const int64_t ints = 2 * page_words(a.cache.num_pages) + 1 + 3 * (int64_t)a.batch + 4 * (int64_t)a.new_batch;
     const bool small = (int64_t)a.batch * fork_width(a) <= kAloneCells && (int64_t)a.new_batch * a.new_max_pages < ((int64_t)1 << 30);
     return small && ints <= kAloneInts ? (int)ints : 0;
 }

@@ -157,7 +157,7 @@ int main() {
             const int64_t n = fork_alone_ints(a);
             if (n > 0) {
                 ++alone;
-                CHECK(n * 4 <= 61440 && n >= 2 * page_words(a.cache.num_pages) + 1 + 2 * (int64_t)a.batch + 4 * (int64_t)a.new_batch);
+                CHECK(n * 4 <= 61440 && n >= 2 * page_words(a.cache.num_pages) + 1 + 3 * (int64_t)a.batch + 4 * (int64_t)a.new_batch);
                 CHECK((int64_t)a.batch * fork_width(a) < INT_MAX - kAloneThreads);
                 CHECK((int64_t)a.new_batch * a.new_max_pages < INT_MAX - 256 * kAloneThreads);
             }
