@@ -279,6 +279,44 @@ __global__ __launch_bounds__(kThreads) void fork_fill_kernel(ForkParams p) {
     if (dst >= 0) copy_slots(p.c, p.shape, p.table[r.p * p.stride + r.full], dst, r.part, at, step);
 }
 
+// The cells of a table of `cells` = rows x width, x = threadIdx.x, + kScanThreads, ...:
+// use(row, column, entry) for each.  begin() reads the first kCellsAhead rounds, so that they are under way together with
+// what else a kernel reads first.  (Columns past a sequence's cells are read and not used.)
+constexpr int kCellsAhead = 4;
+struct TableCells {
+    const int32_t* table;
+    int64_t stride;
+    FastDiv div_width;
+    int width, cells;
+    int ahead[kCellsAhead];
+
+    __device__ __forceinline__ int entry(int x) const {
+        const int b = fast_div(x, div_width);
+        return table[b * stride + (x - b * width)];
+    }
+    __device__ __forceinline__ void begin() {
+#pragma unroll
+        for (int i = 0; i < kCellsAhead; ++i) {
+            const int x = (int)threadIdx.x + i * kScanThreads;
+            ahead[i] = x < cells ? entry(x) : -1;
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F&& use) const {
+#pragma unroll
+        for (int i = 0; i < kCellsAhead; ++i) {
+            const int x = (int)threadIdx.x + i * kScanThreads;
+            const int b = fast_div(min(x, max(cells - 1, 0)), div_width);
+            if (x < cells) use(b, x - b * width, ahead[i]);
+        }
+#pragma unroll 4
+        for (int x = (int)threadIdx.x + kCellsAhead * kScanThreads; x < cells; x += kScanThreads) {
+            const int b = fast_div(x, div_width);
+            use(b, x - b * width, entry(x));
+        }
+    }
+};
+
 // All of it, each workgroup planning for itself.  LDS: plan::fork_alone_ints.
 __global__ __launch_bounds__(kScanThreads) void fork_alone_kernel(ForkParams p, FastDiv div_width, int width, FastDiv div_new_width,
                                                                   int slices) {
@@ -290,6 +328,10 @@ __global__ __launch_bounds__(kScanThreads) void fork_alone_kernel(ForkParams p, 
     int32_t* last = lens + p.batch;          // [batch]: their partly filled pages
     int32_t* row = last + p.batch;           // [new_batch][4]: old row, fresh pages, those of rows before it, cells kept
     const int tid = threadIdx.x;
+    auto parent_of = [&](int i) { return p.parents != nullptr ? p.parents[i] : i; };
+    TableCells old{p.table, p.stride, div_width, width, p.batch * width};
+    old.begin();
+    const int parent0 = tid < p.new_batch ? parent_of(tid) : -1;
     for (int w = tid; w < p.words; w += kScanThreads) bits[w] = held_word(p.held, w, p.c.num_pages);
     for (int b = tid; b < p.batch; b += kScanThreads) {
         first[b] = INT32_MAX;
@@ -297,22 +339,18 @@ __global__ __launch_bounds__(kScanThreads) void fork_alone_kernel(ForkParams p, 
     }
     __syncthreads();
     for (int i = tid; i < p.new_batch; i += kScanThreads) {
-        const int parent = p.parents != nullptr ? p.parents[i] : i;
+        const int parent = i == tid ? parent0 : parent_of(i);
         const bool there = parent >= 0 && parent < p.batch;
         row[4 * i] = there ? parent : -1;
         if (there) atomicMin(&first[parent], i);
     }
     __syncthreads();
-    const int old_cells = p.batch * width;
-#pragma unroll 4
-    for (int x = tid; x < old_cells; x += kScanThreads) {
-        const int b = fast_div(x, div_width), j = x - b * width;
+    old.each([&](int b, int j, int page) {
         if (j <= (lens[b] - 1) >> p.c.page_shift && first[b] != INT32_MAX) {
-            const int page = p.table[b * p.stride + j];
             if (is_page(p.c, page)) atomicOr(&bits[page >> 5], 1u << (page & 31));
             if (j == lens[b] >> p.c.page_shift) last[b] = page;
         }
-    }
+    });
     __syncthreads();
     const int left = fork_scan(
         p, bits, before,
@@ -483,21 +521,18 @@ __global__ __launch_bounds__(kScanThreads) void compact_alone_kernel(CompactPara
     s.open_before = s.live_before + s.words + 1;
     int32_t* cells_of = s.open_before + s.words + 1;   // [batch]
     const int tid = threadIdx.x;
+    const int cells = p.batch * p.max_pages;
+    TableCells old{p.table, p.stride, div_width, p.max_pages, cells};
+    old.begin();
     for (int w = tid; w < s.words; w += kScanThreads) {
         s.live[w] = 0;
         s.held[w] = held_word(p.held, w, p.c.num_pages);
     }
     for (int b = tid; b < p.batch; b += kScanThreads) cells_of[b] = compact_cells(p, b);
     __syncthreads();
-    const int cells = p.batch * p.max_pages;
-#pragma unroll 4
-    for (int x = tid; x < cells; x += kScanThreads) {
-        const int b = fast_div(x, div_width), j = x - b * p.max_pages;
-        if (j < cells_of[b]) {
-            const int page = p.table[b * p.stride + j];
-            if (is_page(p.c, page)) atomicOr(&s.live[page >> 5], 1u << (page & 31));
-        }
-    }
+    old.each([&](int b, int j, int page) {
+        if (j < cells_of[b] && is_page(p.c, page)) atomicOr(&s.live[page >> 5], 1u << (page & 31));
+    });
     __syncthreads();
     const int used = compact_scan(s, &s_edge);
     if (blockIdx.x == 0 && tid == 0) *p.num_used = used;
