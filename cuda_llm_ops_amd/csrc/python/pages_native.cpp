@@ -25,6 +25,7 @@ template <typename Args>
 at::Tensor workspace_of(int (*bytes_of)(const Args*, size_t*), Args* a, const at::Tensor& like, const char* where) {
     size_t bytes = 0;
     raise_status(bytes_of(a, &bytes), where);
+    if (bytes == 0) return at::Tensor();   // (NULL and 0: none is needed)
     at::Tensor work = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
     a->workspace = address(work);
     a->workspace_bytes = bytes;
