@@ -124,28 +124,28 @@ __device__ __forceinline__ uint32_t held_word(const uint8_t* held, int w, int nu
     return bits;
 }
 
-// before[w]: the sum of count(0 .. w - 1), for w <= words; a workgroup.
-template <typename F>
-__device__ __forceinline__ int scan_words(int words, int32_t* before, int* s_wave, F&& count) {
-    int carry = 0;
+// store(w, the sum of count(0 .. w - 1)), for w <= words; the sum of all.  A workgroup.
+template <typename T, typename Count, typename Store>
+__device__ __forceinline__ T scan_words(int words, T* s_wave, Count&& count, Store&& store) {
+    T carry = 0;
     for (int w0 = 0; w0 < words; w0 += kScanThreads * kWordsPerScan) {
-        int n[kWordsPerScan], sum = 0, total;
+        T n[kWordsPerScan], sum = 0, total;
 #pragma unroll
         for (int i = 0; i < kWordsPerScan; ++i) {
             const int w = w0 + (int)threadIdx.x * kWordsPerScan + i;
             n[i] = w < words ? count(w) : 0;
             sum += n[i];
         }
-        int at = carry + block_exclusive_scan<kScanThreads, true>(sum, s_wave, &total);
+        T at = carry + block_exclusive_scan<kScanThreads, true>(sum, s_wave, &total);
 #pragma unroll
         for (int i = 0; i < kWordsPerScan; ++i) {
             const int w = w0 + (int)threadIdx.x * kWordsPerScan + i;
-            if (w < words) before[w] = at;
+            if (w < words) store(w, at);
             at += n[i];
         }
         carry += total;
     }
-    if (threadIdx.x == 0) before[words] = carry;
+    if (threadIdx.x == 0) store(words, carry);
     return carry;
 }
 
@@ -234,7 +234,8 @@ __global__ __launch_bounds__(kThreads) void fork_mark_kernel(ForkParams p) {
 template <typename Fresh, typename Row>
 __device__ __forceinline__ int fork_scan(const ForkParams& p, const uint32_t* bits, int32_t* before, Fresh&& fresh, Row&& row) {
     __shared__ int s_wave[kScanThreads / kWave];
-    const int free_pages = scan_words(p.words, before, s_wave, [&](int w) { return __popc(~bits[w] & word_mask(w, p.c.num_pages)); });
+    const int free_pages = scan_words(
+        p.words, s_wave, [&](int w) { return __popc(~bits[w] & word_mask(w, p.c.num_pages)); }, [&](int w, int n) { before[w] = n; });
     __shared__ int64_t s_wave64[kScanThreads / kWave];
     int64_t wanted = 0;   // (rows times cells can pass 2^31)
     for (int i0 = 0; i0 < p.new_batch; i0 += kScanThreads) {
@@ -441,11 +442,15 @@ __device__ __forceinline__ uint32_t open_word(const PageWords& s, int w) { retur
 // Counts by words; *edge, behind the first L pages that are not held (L: live ones); how many
 // pages are in use or held up to the last such one.  A workgroup.
 __device__ __forceinline__ int compact_scan(const PageWords& s, int32_t* edge) {
-    __shared__ int s_wave[kScanThreads / kWave];
+    __shared__ int64_t s_wave[kScanThreads / kWave];
     __shared__ int s_last;
     if (threadIdx.x == 0) s_last = -1;
-    const int live = scan_words(s.words, s.live_before, s_wave, [&](int w) { return __popc(live_word(s, w)); });
-    scan_words(s.words, s.open_before, s_wave, [&](int w) { return __popc(open_word(s, w)); });
+    const int live = (int)scan_words(
+        s.words, s_wave, [&](int w) { return (int64_t)__popc(open_word(s, w)) << 32 | __popc(live_word(s, w)); },
+        [&](int w, int64_t n) {
+            s.live_before[w] = (int)n;   // (counts stay below 2^31)
+            s.open_before[w] = (int)(n >> 32);
+        });
     __syncthreads();
     for (int w = threadIdx.x; w < s.words; w += kScanThreads) {
         if (s.held[w] != 0) atomicMax(&s_last, 32 * w + 31 - __builtin_clz(s.held[w]));
