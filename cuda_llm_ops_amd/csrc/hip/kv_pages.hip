@@ -10,12 +10,12 @@
 // workgroup works the bits and counts out for itself, in LDS, and then takes its share of
 // cells and copies.  Larger ones do that once, in three launches before the last.
 //
-// Small calls are bound by one launch and the chain of reads behind it (lengths, table,
-// bits, counts): 16 beams of up to 700 tokens forked 8.4 us, a cache of 8 sequences made
-// compact 8.6 us (17.8 and 17.0 us in four launches).  Large ones are bound by the pages'
-// bytes: 256 samples of 16 prompts of 8000 tokens 14 us (38 MB read and written; 40 us in
+// Small calls are bound by one launch and the chain behind it (lengths, table, bits,
+// counts, copies): 16 beams of up to 700 tokens forked 6.6 us, a cache of 8 sequences made
+// compact 7.9 us (18.2 and 17.1 us with four launches).  Large ones are bound by the pages'
+// bytes: 256 samples of 16 prompts of 8000 tokens 12 us (38 MB read and written; 40 us in
 // four launches, their threads after the free pages through the L2), 48 conversations of
-// 8000 tokens of bf16 171 us, the copies at 5 TB/s.  A page's pieces are dealt out to
+// 8000 tokens of bf16 171 us, the copies at 5.3 TB/s.  A page's pieces are dealt out to
 // threads a slice's width apart: consecutive ones took 181 us.
 #include <algorithm>
 
