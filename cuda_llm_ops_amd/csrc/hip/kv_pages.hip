@@ -8,15 +8,16 @@
 //
 // With tables that one workgroup reads in passing, a call is one launch: each
 // workgroup works the bits and counts out for itself, in LDS, and then takes its share of
-// cells and copies.  Larger ones do that once, in three launches before the last.
+// cells and copies.  Larger ones do that once, in three launches before the last (one, if
+// only the pages that may move are many).
 //
 // Small calls are bound by one launch and the chain behind it (lengths, table, bits,
 // counts, copies): 16 beams of up to 700 tokens forked 6.6 us, a cache of 8 sequences made
 // compact 7.9 us (18.2 and 17.1 us with four launches).  Large ones are bound by the pages'
 // bytes: 256 samples of 16 prompts of 8000 tokens 12 us (38 MB read and written; 40 us in
 // four launches, their threads after the free pages through the L2), 48 conversations of
-// 8000 tokens of bf16 171 us, the copies at 5.3 TB/s.  A page's pieces are dealt out to
-// threads a slice's width apart: consecutive ones took 181 us.
+// 8000 tokens of bf16 166 us, the copies at 5.3 TB/s.  A page's pieces are dealt out to
+// threads a slice's width apart: consecutive ones took 11 us more.
 #include <algorithm>
 
 #include "fgqa_device.h"
@@ -515,7 +516,9 @@ __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p)
         move_slice(p, s, t, stay, threadIdx.x, kThreads);
 }
 
-// All of it, each workgroup planning for itself.  LDS: plan::compact_alone_ints.
+// All of it, each workgroup planning for itself.  LDS: plan::compact_alone_ints.  kPlan: the words and the edge
+// alone, to memory, by one workgroup.
+template <bool kPlan>
 __global__ __launch_bounds__(kScanThreads) void compact_alone_kernel(CompactParams p, FastDiv div_width) {
     extern __shared__ int32_t smem[];
     __shared__ int32_t s_edge;
@@ -542,6 +545,18 @@ __global__ __launch_bounds__(kScanThreads) void compact_alone_kernel(CompactPara
     const int used = compact_scan(s, &s_edge);
     if (blockIdx.x == 0 && tid == 0) *p.num_used = used;
     const int edge = s_edge;
+    if constexpr (kPlan) {
+        for (int w = tid; w <= s.words; w += kScanThreads) {
+            if (w < s.words) {
+                p.words.live[w] = s.live[w];
+                p.words.held[w] = s.held[w];
+            }
+            p.words.live_before[w] = s.live_before[w];
+            p.words.open_before[w] = s.open_before[w];
+        }
+        if (tid == 0) *p.edge = edge;
+        return;
+    }
     const int stay = live_rank(s, edge);
     const int64_t tasks = (int64_t)(s.live_before[s.words] - stay) * p.slices;
     const int waves = gridDim.x * (kScanThreads / kWave);
@@ -649,7 +664,8 @@ extern "C" int fgqa_kv_fork(const fgqa_kv_fork_args* a, void* stream) {
 extern "C" int fgqa_kv_compact_workspace_bytes(const fgqa_kv_compact_args* a, size_t* bytes) {
     const int st = plan::validate_kv_compact_sizes(a);
     if (st != FGQA_OK || bytes == nullptr) return st != FGQA_OK ? st : FGQA_ERR_INVALID_ARGUMENT;
-    *bytes = plan::compact_alone_ints(*a) > 0 ? 0 : (size_t)plan::compact_layout(*a).total * 4;
+    const bool none = plan::compact_alone_ints(*a) > 0 && plan::compact_moves_little(*a);
+    *bytes = none ? 0 : (size_t)plan::compact_layout(*a).total * 4;
     return FGQA_OK;
 }
 
@@ -675,9 +691,9 @@ extern "C" int fgqa_kv_compact(const fgqa_kv_compact_args* a, void* stream) {
     const int64_t cells = (int64_t)a->batch * a->max_pages;
     const int64_t pieces = page_pieces(a->cache), moves = plan::compact_moves(*a);
     const int alone = plan::compact_alone_ints(*a);
-    if (alone > 0) {
+    if (alone > 0 && plan::compact_moves_little(*a)) {
         p.slices = (int)ceil_div(pieces, kAhead * kWave);
-        hipLaunchKernelGGL(compact_alone_kernel, dim3(alone_blocks(moves * p.slices, cells, 256)), dim3(kScanThreads), (size_t)alone * 4, s, p,
+        hipLaunchKernelGGL(compact_alone_kernel<false>, dim3(alone_blocks(moves * p.slices, cells, 256)), dim3(kScanThreads), (size_t)alone * 4, s, p,
                            make_fast_div(std::max(a->max_pages, 1)));
         return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
     }
@@ -692,10 +708,15 @@ extern "C" int fgqa_kv_compact(const fgqa_kv_compact_args* a, void* stream) {
     p.words.live_before = w + l.live_before;
     p.words.open_before = w + l.open_before;
     p.edge = w + l.edge;
-    hipLaunchKernelGGL(compact_clear_kernel, dim3(blocks_for(p.words.words, 1024)), dim3(kThreads), 0, s, p);
-    if (cells > 0)
-        hipLaunchKernelGGL(compact_mark_kernel, dim3((unsigned)a->batch, blocks_for(a->max_pages, 16)), dim3(kThreads), 0, s, p);
-    hipLaunchKernelGGL(compact_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, p);
+    if (alone > 0) {
+        hipLaunchKernelGGL(compact_alone_kernel<true>, dim3(1), dim3(kScanThreads), (size_t)alone * 4, s, p,
+                           make_fast_div(std::max(a->max_pages, 1)));
+    } else {
+        hipLaunchKernelGGL(compact_clear_kernel, dim3(blocks_for(p.words.words, 1024)), dim3(kThreads), 0, s, p);
+        if (cells > 0)
+            hipLaunchKernelGGL(compact_mark_kernel, dim3((unsigned)a->batch, blocks_for(a->max_pages, 16)), dim3(kThreads), 0, s, p);
+        hipLaunchKernelGGL(compact_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, p);
+    }
     if (cells > 0) {
         p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(pieces / (kAhead * kThreads), 16));
         p.table_blocks = (int)blocks_for(cells, 256);

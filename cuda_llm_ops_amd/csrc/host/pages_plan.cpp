@@ -63,9 +63,6 @@ namespace {
 // tables of n cells: fork 8.4 and 17.5 us (n = 2,016), 18 and 21 (n = 32,256), compact 9.6
 // and 16.4, 18 and 24.
 constexpr int64_t kAloneCells = 32768, kAloneInts = 15360;
-// Bytes of pages that may move: past that, copies by smaller workgroups give more than the
-// launches cost (1.2 GB: 170 against 176 us).
-constexpr int64_t kAloneMoves = (int64_t)1 << 29;
 }  // namespace
 
 int fork_alone_ints(const fgqa_kv_fork_args& a) {
@@ -75,10 +72,15 @@ int fork_alone_ints(const fgqa_kv_fork_args& a) {
 }
 
 int compact_alone_ints(const fgqa_kv_compact_args& a) {
-    const int64_t ints = 4 * page_words(a.cache.num_pages) + 2 + a.batch, cells = (int64_t)a.batch * a.max_pages;
-    if (cells > kAloneCells || ints > kAloneInts) return 0;
+    const int64_t ints = 4 * page_words(a.cache.num_pages) + 2 + a.batch;
+    return (int64_t)a.batch * a.max_pages <= kAloneCells && ints <= kAloneInts ? (int)ints : 0;
+}
+
+bool compact_moves_little(const fgqa_kv_compact_args& a) {
+    // Bytes of the pages: with 1.2 GB workgroups of 256 threads take 160 us and 1024 threads, which plan too, 176.
+    constexpr int64_t kAloneMoves = (int64_t)1 << 29;
     const int64_t page = (int64_t)a.cache.page_size * a.cache.num_kv_heads * (a.cache.kv_dtype == FGQA_KV_BF16 ? 512 : 256);
-    return compact_moves(a) <= kAloneMoves / page ? (int)ints : 0;
+    return compact_moves(a) <= kAloneMoves / page;
 }
 
 int validate_kv_fork_sizes(const fgqa_kv_fork_args* a) {

@@ -39,6 +39,8 @@ inline int64_t compact_moves(const fgqa_kv_compact_args& a) {
     const int64_t cells = (int64_t)a.batch * a.max_pages;
     return cells < a.cache.num_pages / 2 ? cells : a.cache.num_pages / 2;
 }
+// Whether workgroups that plan for themselves move them: smaller ones copy large amounts faster.
+bool compact_moves_little(const fgqa_kv_compact_args& a);
 // Cells of an old row that a new one can hold.
 inline int fork_width(const fgqa_kv_fork_args& a) { return a.max_pages < a.new_max_pages ? a.max_pages : a.new_max_pages; }
 

@@ -138,6 +138,20 @@ int main() {
               m.edge - m.open_before >= words + 1 && m.total > m.edge);
         CHECK(l.total % 4 == 0 && m.total % 4 == 0);
     }
+    {
+        fgqa_kv_compact_args c = compact_args();
+        c.batch = 10;
+        c.max_pages = 10;
+        c.cache.num_pages = 128;   // (64 move at most, of 2^23 bytes each)
+        c.cache.page_size = 4096;
+        c.cache.num_kv_heads = 4;
+        c.cache.kv_dtype = FGQA_KV_BF16;
+        CHECK(compact_moves(c) == 64 && compact_moves_little(c) && compact_alone_ints(c) > 0);
+        c.cache.num_pages = 130;
+        CHECK(!compact_moves_little(c) && compact_alone_ints(c) > 0);
+        c.batch = 6;
+        CHECK(compact_moves(c) == 60 && compact_moves_little(c));
+    }
     int alone = 0;
     std::mt19937_64 rng(11);
     const int32_t sizes[] = {0, 1, 3, 16, 128, 1 << 19, 1 << 20, INT_MAX, -1};

@@ -244,6 +244,25 @@ def test_compact_large(cuda):
         assert torch.equal(t, s)
 
 
+@pytest.mark.parametrize("with_held", (False, True))
+def test_compact_many_bytes(cuda, with_held):
+    """A small table of large pages: planned in one launch and copied in another."""
+    import torch
+    import cuda_llm_ops_amd as fg
+    r = random.Random(7)
+    B, W, P, H, pages = 5, 9, 4096, 8, 90
+    table, lens = _random_rows(r, B, W, P, pages, share=True)
+    held = [r.random() < 0.2 for _ in range(pages)] if with_held else None
+    k, v, _ = _cache(torch, cuda, pages, P, H, "bf16")
+    state = _state(k, v, {})
+    want, moves, used = ref.compact(table, lens, P, pages, held)
+    assert moves
+    out = fg.compact_kv_paged(k, v, _t(torch, cuda, table), _t(torch, cuda, lens),
+                              held=None if held is None else torch.tensor(held, device=cuda))
+    assert out[0].tolist() == want and out[1].tolist() == [used]
+    assert _same([k, v], _expect(state, [(a, b, None) for a, b in moves]))
+
+
 def test_strided_caches(cuda):
     """K and V interleaved in one tensor, heads before slots, scales by columns."""
     import torch
