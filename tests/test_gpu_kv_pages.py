@@ -263,6 +263,36 @@ def test_compact_many_bytes(cuda, with_held):
     assert _same([k, v], _expect(state, [(a, b, None) for a, b in moves]))
 
 
+@pytest.mark.parametrize("width", (3, 20000))
+def test_offsets_past_32_bits(cuda, width):
+    """Pages at both ends of a cache of more than 2^32 bytes, planned in either form."""
+    import torch
+    import cuda_llm_ops_amd as fg
+    P, H, pages = 64, 8, 40_000
+    k, v = (torch.zeros(pages, P, H, 128, dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    top = pages - 6
+    for i, page in enumerate((top, top + 1, top + 2)):
+        k[page] = i + 1
+        v[page] = -i - 1
+    table, lens = [[top, top + 1] + [-1] * (width - 2), [top, top + 2] + [-1] * (width - 2)], [100, 70]
+    held = torch.ones(pages, dtype=torch.bool, device=cuda)
+    held[top:] = False
+    want, want_lens, copies, left = ref.fork(table, lens, P, pages, [0, 0, 1], [30, 0, 0], held.tolist())
+    assert [c[1] > top for c in copies] == [True]
+    out = fg.fork_kv_paged(k, v, _t(torch, cuda, table), _t(torch, cuda, lens), parents=_t(torch, cuda, [0, 0, 1]),
+                           new_lens=_t(torch, cuda, [30, 0, 0]), held=held)
+    assert out[0].tolist() == want and out[1].tolist() == want_lens and out[2].tolist() == [left]
+    src, dst, slots = copies[0]
+    assert bool((k[dst, :slots] == k[src, :slots]).all()) and bool((v[dst, :slots] == -2).all())
+    assert not bool(k[dst, slots:].any())
+    moved, moves, used = ref.compact(want, want_lens, P, pages)
+    was = {s: (k[s].clone(), v[s].clone()) for s, _ in moves}
+    out = fg.compact_kv_paged(k, v, out[0], out[1])
+    assert out[0].tolist() == moved and out[1].tolist() == [used] == [len(moves)]
+    for s, d in moves:
+        assert torch.equal(k[d], was[s][0]) and torch.equal(v[d], was[s][1])
+
+
 def test_strided_caches(cuda):
     """K and V interleaved in one tensor, heads before slots, scales by columns."""
     import torch

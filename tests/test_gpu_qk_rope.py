@@ -205,6 +205,31 @@ def test_rows_of_other_strides(cuda):
     assert all(torch.equal(a, b) for a, b in zip(fg.qk_norm_rope(**d), want))
 
 
+def test_offsets_past_32_bits(cuda):
+    """Batches and heads more than 2^32 bytes apart, outputs too."""
+    import torch
+    import cuda_llm_ops_amd as fg
+    c = _make(torch, cuda, (3, 40), 8, 2, 128, 128, fused=False)
+    want = fg.qk_norm_rope(**c)
+    gq, gk = torch.randn_like(c["q"]), torch.randn_like(c["k"])
+    grads = fg.qk_norm_rope_backward(gq, gk, **c)
+    far = (1 << 31) + 256   # elements
+    room = torch.empty(2 * far + 40 * 8 * 128, dtype=torch.bfloat16, device=cuda)
+
+    def spread(t):
+        return room.as_strided(t.shape, (far, t.shape[2] * 128, 128, 1)).copy_(t)
+
+    d = dict(c, q=spread(c["q"]))
+    assert all(torch.equal(a, b) for a, b in zip(fg.qk_norm_rope(**d), want))
+    assert all(torch.equal(a, b) for a, b in zip(fg.qk_norm_rope_backward(gq, gk, **d), grads))
+    assert all(torch.equal(a, b) for a, b in zip(fg.qk_norm_rope_backward(spread(gq), gk, **c), grads))
+    out = room.as_strided(c["q"].shape, (far, 8 * 128, 128, 1))
+    assert torch.equal(fg.qk_norm_rope(**c, q_out=out)[0], want[0])
+    heads = room.as_strided((3, 40, 2, 128), (40 * 128, 128, far, 1)).copy_(c["k"])
+    assert all(torch.equal(a, b) for a, b in zip(fg.qk_norm_rope(**dict(c, k=heads)), want))
+    assert all(torch.equal(a, b) for a, b in zip(fg.qk_norm_rope_backward(gq, gk, **dict(c, k=heads)), grads))
+
+
 def test_empty_and_odd_values(cuda):
     import torch
     import cuda_llm_ops_amd as fg
