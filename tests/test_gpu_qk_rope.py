@@ -113,6 +113,28 @@ def test_forward_and_backward(cuda, lead, Hq, Hkv, D, R, axes, interleaved, weig
     assert all(a is b or torch.equal(a, b) for a, b in zip(grads, again))
 
 
+@pytest.mark.parametrize("lead,Hq,Hkv,D,R,axes,interleaved,weights", [
+    ((2, 4501), 16, 8, 128, 128, 3, True, "bf16"),
+    ((1, 10007), 17, 3, 128, 96, None, False, "fp32"),
+    ((1, 4500), 9, 2, 256, 256, None, False, "bf16"),
+    ((20000,), 4, 2, 64, 64, None, True, "bf16"),
+])
+def test_many_rows(cuda, lead, Hq, Hkv, D, R, axes, interleaved, weights):
+    """Items of many rows, more than one for each workgroup.  Of a weight's gradient an fp32 sum has up to 24
+    rows of a lane, its 8 groups, 4 waves, 12 workgroups of a thread and their tree: some 50 additions, 2^-18.3 of
+    the sum of magnitudes, within the reference's 2^-17."""
+    import torch
+    import cuda_llm_ops_amd as fg
+    c = _make(torch, cuda, lead, Hq, Hkv, D, R, axes=axes, weights=weights)
+    outs = fg.qk_norm_rope(**c, interleaved=interleaved)
+    _check_forward(c, outs, interleaved=interleaved)
+    gq, gk = torch.randn_like(outs[0]), torch.randn_like(outs[1])
+    grads = fg.qk_norm_rope_backward(gq, gk, **c, interleaved=interleaved)
+    _check_backward(c, gq, gk, grads, interleaved=interleaved)
+    again = fg.qk_norm_rope_backward(gq, gk, **c, interleaved=interleaved)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
 def test_norm_alone(cuda):
     import torch
     import cuda_llm_ops_amd as fg
