@@ -90,9 +90,11 @@ static int64_t waves(const fgqa_rope_args& a, int most) {
 }
 
 int rope_heads_per(const fgqa_rope_args& a) {
-    // Lane groups that keep the loads of 4 rows in flight, as far as they fill the chip.
-    constexpr int64_t kRopeFullWaves = 4096;
-    return waves(a, 4) >= kRopeFullWaves ? 4 : 1;
+    // 4 rows share a lane group's angles and have their loads in flight together, as far as there is a wave
+    // of them for each SIMD: 1 and 4 rows took 10.2 and 9.3 us on 81,920 rows of 128 (2,560 waves of 4), 6.5 and 6.3
+    // on 40,960, but 4.8 and 5.4 on 10,240 (320 waves).
+    constexpr int64_t kRopeWaves = 1024;
+    return waves(a, 4) >= kRopeWaves ? 4 : 1;
 }
 
 RopeGradPlan rope_grad_plan(const fgqa_rope_args& a) {

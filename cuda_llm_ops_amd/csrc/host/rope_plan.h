@@ -25,7 +25,7 @@ inline RopeSlices rope_slices(int heads, int most) {
     return {(int)ceil_div(heads, count), count};
 }
 
-// Heads that a lane group of the forward takes: 4 (1 where that leaves fewer than kRopeFullWaves waves).
+// Heads that a lane group of the forward takes: 4 (1 where that leaves fewer than kRopeWaves waves).
 int rope_heads_per(const fgqa_rope_args& a);
 
 // Backward with weights: Q's and K's items, walked by at most kRopeGradBlocks
