@@ -8,9 +8,9 @@
 // angles (8 pairs a lane; the backward's up to 8 rows).
 //
 // Both directions are bound by the bytes of the rows.  Forward, [4, 6001] tokens of 28
-// and 4 heads of 128: 85 us for 393 MB, 4.6 TB/s; one token of 64 conversations, 64 and
-// 8 heads: 5.9 us, of a launch.  Backward, [3, 5003] tokens of 32 and 8 heads: 108 us
-// for 461 MB with its second launch, 4.3 TB/s.  A large copy reaches 4.9 TB/s.
+// and 4 heads of 128: 75 us for 393 MB, 5.2 TB/s; one token of 64 conversations, 64 and
+// 8 heads: 3.4 us, of a launch.  Backward, [3, 5003] tokens of 32 and 8 heads: 110 us
+// for 461 MB with its second launch, 4.2 TB/s.  A large copy reaches 4.96 TB/s.
 #include <algorithm>
 #include <math.h>
 
@@ -77,6 +77,20 @@ __device__ __forceinline__ void cos_sin_turns(float t, float* c, float* s) {
 typedef float f32x4u_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef int i32x4u_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4u_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// 16 bytes of a row; kStream: past the caches, which more rows than they hold would only churn.
+template <bool kStream>
+__device__ __forceinline__ u32x4_t load16(const __bf16* at) {
+    const u32x4_t* p = reinterpret_cast<const u32x4_t*>(at);
+    if constexpr (kStream) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool kStream>
+__device__ __forceinline__ void store16(__bf16* at, u32x4_t v) {
+    u32x4_t* p = reinterpret_cast<u32x4_t*>(at);
+    if constexpr (kStream) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
 
 // What a lane holds of each row: 16 elements, those of pieces off[0] and off[1].
 struct LaneShape {
@@ -202,7 +216,7 @@ __device__ __forceinline__ Item item_of(const RopeParams& p, const Rows& x, uint
 }
 
 // Forward; without a norm and with sin negated, also the gradients of a rotation alone.
-template <int kLanes, int kHeads, bool kInterleaved, bool kNorm>
+template <int kLanes, int kHeads, bool kInterleaved, bool kNorm, bool kStream>
 __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
     const int which = blockIdx.x >= p.first_k ? 1 : 0;
     const Rows& x = p.x[which];
@@ -219,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             raw[r][i] = u32x4_t{0u, 0u, 0u, 0u};
-            if (mine && r < it.rows) raw[r][i] = *reinterpret_cast<const u32x4_t*>(src + r * x.in_s[2] + ls.off[i]);
+            if (mine && r < it.rows) raw[r][i] = load16<kStream>(src + r * x.in_s[2] + ls.off[i]);
         }
     float w[16];
     if constexpr (kNorm) {
@@ -246,7 +260,7 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
         rotate<kInterleaved, false>(v, cs, sn, ls.rotated);
         if (mine && r < it.rows) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(dst + r * x.out_s[2] + ls.off[i]) = narrow8(v + 8 * i);
+            for (int i = 0; i < 2; ++i) store16<kStream>(dst + r * x.out_s[2] + ls.off[i], narrow8(v + 8 * i));
         }
     }
 }
@@ -257,7 +271,7 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
 // lane those of its 16 elements, so that no gradient goes through an atomic.  A lane
 // group goes through its item's rows one by one with one set of angles, and has the
 // next row's loads in flight.
-template <int kLanes, bool kInterleaved>
+template <int kLanes, bool kInterleaved, bool kStream>
 __global__ __launch_bounds__(kThreads) void rope_backward_kernel(RopeParams p) {
     __shared__ float s_dw[kThreads / kWave][plan::kRopeMaxHeadDim];
     const int which = blockIdx.x >= p.first_k ? 1 : 0;
@@ -294,8 +308,8 @@ __global__ __launch_bounds__(kThreads) void rope_backward_kernel(RopeParams p) {
         for (int i = 0; i < 2; ++i) {
             raw[i] = graw[i] = u32x4_t{0u, 0u, 0u, 0u};
             if (r < at.rows) {
-                raw[i] = *reinterpret_cast<const u32x4_t*>(at.src + r * x.in_s[2] + ls.off[i]);
-                graw[i] = *reinterpret_cast<const u32x4_t*>(at.grad + r * x.grad_s[2] + ls.off[i]);
+                raw[i] = load16<kStream>(at.src + r * x.in_s[2] + ls.off[i]);
+                graw[i] = load16<kStream>(at.grad + r * x.grad_s[2] + ls.off[i]);
             }
         }
     };
@@ -331,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void rope_backward_kernel(RopeParams p) {
             for (int i = 0; i < 16; ++i) g[i] = inv * (g[i] - v[i] * mean);
             if (r < at.rows) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(at.dst + r * x.out_s[2] + ls.off[i]) = narrow8(g + 8 * i);
+                for (int i = 0; i < 2; ++i) store16<false>(at.dst + r * x.out_s[2] + ls.off[i], narrow8(g + 8 * i));
             }
         }
         at = after;
@@ -445,8 +459,13 @@ void launch_rope(const fgqa_rope_args& a, RopeParams p, int heads_per, hipStream
         const int64_t groups = kThreads / kLanes;
         p.first_k = (unsigned)ceil_div(p.x[0].items, groups);
         const unsigned grid = p.first_k + (unsigned)ceil_div(p.x[1].items, groups);
-        if (heads_per == 4) hipLaunchKernelGGL((rope_kernel<kLanes, 4, kInter, kNorm>), dim3(grid), dim3(kThreads), 0, s, p);
-        else hipLaunchKernelGGL((rope_kernel<kLanes, 1, kInter, kNorm>), dim3(grid), dim3(kThreads), 0, s, p);
+        auto launch = [&](auto h, auto stream) {
+            hipLaunchKernelGGL((rope_kernel<kLanes, decltype(h)::value, kInter, kNorm, decltype(stream)::value>), dim3(grid),
+                               dim3(kThreads), 0, s, p);
+        };
+        if (heads_per != 4) launch(std::integral_constant<int, 1>{}, std::false_type{});
+        else if (plan::rope_streams(a, 2)) launch(std::integral_constant<int, 4>{}, std::true_type{});
+        else launch(std::integral_constant<int, 4>{}, std::false_type{});
     });
 }
 
@@ -527,8 +546,12 @@ extern "C" int fgqa_qk_norm_rope_backward(const fgqa_rope_backward_args* a, void
         p.partial = static_cast<float*>(ws);
         p.first_k = (unsigned)pl.blocks[0];
         with_shape(f, [&](auto lanes, auto inter) {
-            hipLaunchKernelGGL((rope_backward_kernel<decltype(lanes)::value, decltype(inter)::value>),
-                               dim3((unsigned)(pl.blocks[0] + pl.blocks[1])), dim3(kThreads), 0, s, p);
+            auto launch = [&](auto stream) {
+                hipLaunchKernelGGL((rope_backward_kernel<decltype(lanes)::value, decltype(inter)::value, decltype(stream)::value>),
+                                   dim3((unsigned)(pl.blocks[0] + pl.blocks[1])), dim3(kThreads), 0, s, p);
+            };
+            if (plan::rope_streams(f, 3)) launch(std::true_type{});
+            else launch(std::false_type{});
         });
     }
     hipLaunchKernelGGL(rope_weights_kernel, dim3((unsigned)(2 * (f.head_dim / 16))), dim3(kSumThreads), 0, s,

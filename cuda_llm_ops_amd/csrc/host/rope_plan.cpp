@@ -97,6 +97,15 @@ int rope_heads_per(const fgqa_rope_args& a) {
     return waves(a, 4) >= kRopeWaves ? 4 : 1;
 }
 
+bool rope_streams(const fgqa_rope_args& a, int passes) {
+    // The last cache holds 2^28 bytes.  Loads and stores of the forward through the caches and past them took 28.8
+    // and 30.7 us for 168 MB, 43.8 and 44.8 for 256, 51.9 and 50.7 for 287, 92.3 and 86.1 for 492; loads of the
+    // backward (its stores are better in the caches) 47.6 and 52.5 for 252, 70.0 and 67.6 for 307, 98 and 80 for 430.
+    constexpr int64_t kRopeCache = (int64_t)1 << 28;
+    const int64_t rows = (int64_t)a.batch * a.seqlen * ((int64_t)a.num_q_heads + a.num_kv_heads);   // (below 2^31)
+    return rows * a.head_dim * 2 * passes > kRopeCache;
+}
+
 RopeGradPlan rope_grad_plan(const fgqa_rope_args& a) {
     // As many workgroups as the kernel's registers let on the chip at once (3 waves a SIMD);
     // 1024, of which the last wait for a place, took 120 against 108 us on 600,360 rows.

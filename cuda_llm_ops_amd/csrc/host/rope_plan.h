@@ -28,6 +28,9 @@ inline RopeSlices rope_slices(int heads, int most) {
 // Heads that a lane group of the forward takes: 4 (1 where that leaves fewer than kRopeWaves waves).
 int rope_heads_per(const fgqa_rope_args& a);
 
+// Whether the rows, read and written `passes` times, are more than the caches hold.
+bool rope_streams(const fgqa_rope_args& a, int passes);
+
 // Backward with weights: Q's and K's items, walked by at most kRopeGradBlocks
 // workgroups that are shared out in proportion to their heads.
 struct RopeGradPlan {

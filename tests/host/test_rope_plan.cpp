@@ -169,6 +169,14 @@ int main() {
             CHECK(p.blocks[0] >= 1 && p.blocks[1] >= 1 && p.blocks[0] + p.blocks[1] <= 1026);
             CHECK(p.ws_bytes == (size_t)(p.blocks[0] + p.blocks[1]) * 128 * 4);
         }
+    {
+        fgqa_rope_args a = forward_args();   // 10 heads of 128
+        a.batch = 1;
+        a.seqlen = 52428;
+        CHECK(!rope_streams(a, 2) && rope_streams(a, 3) && rope_heads_per(a) == 4);
+        a.seqlen = 52429;
+        CHECK(rope_streams(a, 2));
+    }
     std::mt19937_64 rng(7);
     const int64_t sizes[] = {0, 1, 2, 5, 127, 128, 4096, INT_MAX, -1};
     auto pick = [&] { return (int32_t)sizes[rng() % 9]; };
