@@ -2,15 +2,15 @@
 // pass, and the gradients of that (include/fgqa_rope.h).
 //
 // A row is one token's query or key of one head, D elements of bf16.  A group of
-// 4, 8 or 16 lanes (D up to 64, 128, 256) holds a row, two 16-byte pieces a lane:
-// the pieces whose elements a rotation pairs, so nothing but the norm's sums goes
+// 4, 8 or 16 lanes (D up to 64, 128, 256) holds a row, two 16-byte pieces a lane
+// with the elements that a rotation pairs, so nothing but the norm's sums goes
 // between lanes.  A lane group takes up to 4 rows of one token, with one set of
 // angles (8 pairs a lane; the backward's up to 8 rows).
 //
 // Both directions are bound by the bytes of the rows.  Forward, [4, 6001] tokens of 28
 // and 4 heads of 128: 75 us for 393 MB, 5.2 TB/s; one token of 64 conversations, 64 and
-// 8 heads: 3.4 us, of a launch.  Backward, [3, 5003] tokens of 32 and 8 heads: 110 us
-// for 461 MB with its second launch, 4.2 TB/s.  A large copy reaches 4.96 TB/s.
+// 8 heads: 3.4 us, of a launch.  Backward, [3, 5003] tokens of 32 and 8 heads: 99 us
+// for 461 MB with its second launch, 4.7 TB/s.  A large copy reaches 4.96 TB/s.
 #include <algorithm>
 #include <math.h>
 
@@ -95,7 +95,7 @@ __device__ __forceinline__ void store16(__bf16* at, u32x4_t v) {
 // What a lane holds of each row: 16 elements, those of pieces off[0] and off[1].
 struct LaneShape {
     int off[2];
-    int pair0;      // its first pair
+    int pair[2];    // its first pair and its fifth
     bool rotated;
     bool active;    // (lanes past the row's end hold nothing)
 };
@@ -104,10 +104,14 @@ __device__ __forceinline__ LaneShape lane_shape(const RopeParams& p, int l) {
     LaneShape s;
     s.rotated = 16 * l < p.rotary_dim;
     s.active = 16 * l < p.head_dim;
-    const bool split = s.rotated && !p.interleaved;
-    s.off[0] = split ? 8 * l : 16 * l;
-    s.off[1] = split ? p.rotary_dim / 2 + 8 * l : 16 * l + 8;
-    s.pair0 = 8 * l;
+    // A piece of each half of what is rotated, or of what is not, side by side with the next lanes' (where
+    // neighbours are pairs any two would do: the backward of [3, 5003] tokens took 11 us more with two that follow
+    // each other).
+    const int base = s.rotated ? 0 : p.rotary_dim, span = s.rotated ? p.rotary_dim : p.head_dim - p.rotary_dim;
+    s.off[0] = base + 8 * (l - base / 16);
+    s.off[1] = s.off[0] + span / 2;
+    s.pair[0] = p.interleaved ? 4 * l : 8 * l;
+    s.pair[1] = p.interleaved ? p.rotary_dim / 4 + 4 * l : 8 * l + 4;
     return s;
 }
 
@@ -129,8 +133,8 @@ __device__ __forceinline__ void lane_angles(const RopeParams& p, const LaneShape
     };
     double pos[8];
     if (p.axes != nullptr) {
-        const i32x4u_t a0 = *reinterpret_cast<const i32x4u_t*>(p.axes + ls.pair0);
-        const i32x4u_t a1 = *reinterpret_cast<const i32x4u_t*>(p.axes + ls.pair0 + 4);
+        const i32x4u_t a0 = *reinterpret_cast<const i32x4u_t*>(p.axes + ls.pair[0]);
+        const i32x4u_t a1 = *reinterpret_cast<const i32x4u_t*>(p.axes + ls.pair[1]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) pos[j] = position(min(max(j < 4 ? a0[j & 3] : a1[j & 3], 0), p.num_axes - 1));
     } else {
@@ -138,8 +142,8 @@ __device__ __forceinline__ void lane_angles(const RopeParams& p, const LaneShape
 #pragma unroll
         for (int j = 0; j < 8; ++j) pos[j] = one;
     }
-    const f32x4u_t f0 = *reinterpret_cast<const f32x4u_t*>(p.inv_freq + ls.pair0);
-    const f32x4u_t f1 = *reinterpret_cast<const f32x4u_t*>(p.inv_freq + ls.pair0 + 4);
+    const f32x4u_t f0 = *reinterpret_cast<const f32x4u_t*>(p.inv_freq + ls.pair[0]);
+    const f32x4u_t f1 = *reinterpret_cast<const f32x4u_t*>(p.inv_freq + ls.pair[1]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const double turns = pos[j] * ((double)(j < 4 ? f0[j & 3] : f1[j & 3]) * 0.15915494309189533577);
