@@ -16,7 +16,7 @@
 // compact 7.9 us (18.2 and 17.1 us with four launches).  Large ones are bound by the pages'
 // bytes: 256 samples of 16 prompts of 8000 tokens 12 us (38 MB read and written; 40 us in
 // four launches, their threads after the free pages through the L2), 48 conversations of
-// 8000 tokens of bf16 166 us, the copies at 5.3 TB/s.  A page's pieces are dealt out to
+// 8000 tokens of bf16 155 us, the copies at 5.7 TB/s.  A page's pieces are dealt out to
 // threads a slice's width apart: consecutive ones took 11 us more.
 #include <algorithm>
 
@@ -41,7 +41,8 @@ struct CopyShape {
 constexpr int kAhead = 4;   // pieces of K and of V that a thread has in flight
 
 // Slots [0, slots) of page src to page dst, K and V and their scales: 16-byte pieces first,
-// first + step, ... of all.
+// first + step, ... of all.  kStream: past the caches.
+template <bool kStream = false>
 __device__ __forceinline__ void copy_slots(const CacheParams& c, const CopyShape& sh, int src, int dst, int slots, int first,
                                            int step) {
     const int total = (slots * c.hkv) << sh.piece_log2;   // (a page's bytes / 16 stay below 2^31)
@@ -57,14 +58,20 @@ __device__ __forceinline__ void copy_slots(const CacheParams& c, const CopyShape
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
                 at[i][kv] = slot * c.slot[kv] + h * c.head[kv] + 16 * (x & ((1 << sh.piece_log2) - 1));
-                v[i][kv] = *reinterpret_cast<const u32x4_t*>(c.data[kv] + src * c.page[kv] + at[i][kv]);
+                const u32x4_t* from = reinterpret_cast<const u32x4_t*>(c.data[kv] + src * c.page[kv] + at[i][kv]);
+                if constexpr (kStream) v[i][kv] = __builtin_nontemporal_load(from);
+                else v[i][kv] = *from;
             }
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv)
-                if (x0 + i * step < total) *reinterpret_cast<u32x4_t*>(c.data[kv] + dst * c.page[kv] + at[i][kv]) = v[i][kv];
+                if (x0 + i * step < total) {
+                    u32x4_t* to = reinterpret_cast<u32x4_t*>(c.data[kv] + dst * c.page[kv] + at[i][kv]);
+                    if constexpr (kStream) __builtin_nontemporal_store(v[i][kv], to);
+                    else *to = v[i][kv];
+                }
     }
     if (c.scales[0] != nullptr) {
         for (int h = first; h < c.hkv; h += step)
@@ -490,14 +497,17 @@ __device__ __forceinline__ int moved_to(const CompactParams& p, const PageWords&
 }
 
 // Slice t % slices of the page that is the (t / slices)-th to move, by `threads` threads.
+template <bool kStream>
 __device__ __forceinline__ void move_slice(const CompactParams& p, const PageWords& s, int64_t t, int stay, int thread, int threads) {
     const int mover = (int)(t / p.slices), slice = (int)(t - (int64_t)mover * p.slices);
     const int w = word_of(s.words, stay + mover, [&](int x) { return s.live_before[x]; });
     const int src = 32 * w + bit_of(live_word(s, w), stay + mover - s.live_before[w]);
-    copy_slots(p.c, p.shape, src, hole(s, mover), 1 << p.c.page_shift, slice * threads + thread, p.slices * threads);
+    copy_slots<kStream>(p.c, p.shape, src, hole(s, mover), 1 << p.c.page_shift, slice * threads + thread, p.slices * threads);
 }
 
-// Workgroups up to table_blocks renumber the table; the others copy, a slice of a page at a time.
+// Workgroups up to table_blocks renumber the table; the others copy, a slice of a page at a time (with kStream,
+// where many bytes may move, past the caches: 155 us where 166).
+template <bool kStream>
 __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p) {
     const PageWords& s = p.words;
     const int edge = *p.edge;
@@ -513,7 +523,7 @@ __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p)
     }
     const int64_t tasks = (int64_t)(live - stay) * p.slices;
     for (int64_t t = (int)blockIdx.x - p.table_blocks; t < tasks; t += gridDim.x - p.table_blocks)
-        move_slice(p, s, t, stay, threadIdx.x, kThreads);
+        move_slice<kStream>(p, s, t, stay, threadIdx.x, kThreads);
 }
 
 // All of it, each workgroup planning for itself.  LDS: plan::compact_alone_ints.  kPlan: the words and the edge
@@ -561,7 +571,7 @@ __global__ __launch_bounds__(kScanThreads) void compact_alone_kernel(CompactPara
     const int64_t tasks = (int64_t)(s.live_before[s.words] - stay) * p.slices;
     const int waves = gridDim.x * (kScanThreads / kWave);
     for (int64_t t = (tid / kWave) * gridDim.x + blockIdx.x; t < tasks; t += waves)   // (a wave's)
-        move_slice(p, s, t, stay, tid % kWave, kWave);
+        move_slice<false>(p, s, t, stay, tid % kWave, kWave);
     for (int x = blockIdx.x * kScanThreads + tid; x < cells; x += gridDim.x * kScanThreads) {
         const int b = fast_div(x, div_width), j = x - b * p.max_pages;
         p.new_table[b * p.new_stride + j] = j < cells_of[b] ? moved_to(p, s, p.table[b * p.stride + j], edge, stay) : -1;
@@ -721,7 +731,9 @@ extern "C" int fgqa_kv_compact(const fgqa_kv_compact_args* a, void* stream) {
         p.slices = (int)std::max<int64_t>(1, std::min<int64_t>(pieces / (kAhead * kThreads), 16));
         p.table_blocks = (int)blocks_for(cells, 256);
         const int64_t copy_blocks = std::min<int64_t>(moves * p.slices, 4096);
-        hipLaunchKernelGGL(compact_move_kernel, dim3((unsigned)(p.table_blocks + copy_blocks)), dim3(kThreads), 0, s, p);
+        const dim3 grid((unsigned)(p.table_blocks + copy_blocks));
+        if (plan::compact_moves_little(*a)) hipLaunchKernelGGL(compact_move_kernel<false>, grid, dim3(kThreads), 0, s, p);
+        else hipLaunchKernelGGL(compact_move_kernel<true>, grid, dim3(kThreads), 0, s, p);
     }
     return hipGetLastError() == hipSuccess ? FGQA_OK : FGQA_ERR_HIP;
 }
