@@ -8,9 +8,9 @@
 // angles (8 pairs a lane; the backward's up to 8 rows).
 //
 // Both directions are bound by the bytes of the rows.  Forward, [4, 6001] tokens of 28
-// and 4 heads of 128: 75 us for 393 MB, 5.2 TB/s; one token of 64 conversations, 64 and
-// 8 heads: 3.4 us, of a launch.  Backward, [3, 5003] tokens of 32 and 8 heads: 99 us
-// for 461 MB with its second launch, 4.7 TB/s.  A large copy reaches 4.96 TB/s.
+// and 4 heads of 128: 72 us for 393 MB, 5.4 TB/s; one token of 64 conversations, 64 and
+// 8 heads: 3.4 us, of a launch.  Backward, [3, 5003] tokens of 32 and 8 heads: 103 us
+// for 461 MB with its second launch, 4.5 TB/s.  A large copy reaches 4.96 TB/s.
 #include <algorithm>
 #include <math.h>
 
@@ -105,8 +105,8 @@ __device__ __forceinline__ LaneShape lane_shape(const RopeParams& p, int l) {
     s.rotated = 16 * l < p.rotary_dim;
     s.active = 16 * l < p.head_dim;
     // A piece of each half of what is rotated, or of what is not, side by side with the next lanes' (where
-    // neighbours are pairs any two would do: the backward of [3, 5003] tokens took 11 us more with two that follow
-    // each other).
+    // neighbours are pairs any two would do: the backward of [3, 5003] tokens took 11 to 18 us more with two that
+    // follow each other).
     const int base = s.rotated ? 0 : p.rotary_dim, span = s.rotated ? p.rotary_dim : p.head_dim - p.rotary_dim;
     s.off[0] = base + 8 * (l - base / 16);
     s.off[1] = s.off[0] + span / 2;
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(kThreads) void rope_backward_kernel(RopeParams p) {
             for (int i = 0; i < 16; ++i) g[i] = inv * (g[i] - v[i] * mean);
             if (r < at.rows) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) store16<false>(at.dst + r * x.out_s[2] + ls.off[i], narrow8(g + 8 * i));
+                for (int i = 0; i < 2; ++i) store16<kStream>(at.dst + r * x.out_s[2] + ls.off[i], narrow8(g + 8 * i));
             }
         }
         at = after;
