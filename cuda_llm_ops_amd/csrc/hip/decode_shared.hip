@@ -355,6 +355,7 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
     [[maybe_unused]] auto load_uni = [&](int j, const uint32_t (&at)[2], bool v, uint32_t off, [[maybe_unused]] u32x4_t (&reg)[T::loads],
                                          [[maybe_unused]] uint32_t lds) {
         const int first = (j + 1) * T::loads - pt_first;
+        [[maybe_unused]] __amdgpu_buffer_rsrc_t rs[T::loads];
 #pragma unroll
         for (int i = 0; i < T::loads; ++i) {
             const uint64_t base = (uint64_t)__builtin_amdgcn_readlane(at[1], first + i) << 32 |
@@ -362,12 +363,14 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
             const uint32_t bytes = v ? __builtin_amdgcn_readlane(pt_vbytes, first + i)
                                      : (uint32_t)(T::wave_rows - 1) * kss + kHeadDim * kElem;
             const __amdgpu_buffer_rsrc_t r = make_rsrc(reinterpret_cast<const void*>(base), bytes);
-            if constexpr (kDma) {
-                asm volatile("s_add_u32 m0, %0, %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                             :: "s"(lds), "v"(off), "s"(r), "i"(i * T::rows * kHeadDim * 2) : "memory", "scc");
-            } else {
-                reg[i] = buf_load16(r, off);
-            }
+            if constexpr (kDma) rs[i] = r;
+            else reg[i] = buf_load16(r, off);
+        }
+        if constexpr (kDma) {
+            static_for<T::loads>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                lds_load16<i * T::rows * kHeadDim * 2>(lds, off, rs[i]);
+            });
         }
     };
     auto load = [&](int j) {

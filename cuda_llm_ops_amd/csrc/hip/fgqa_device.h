@@ -78,6 +78,31 @@ __device__ __forceinline__ u32x4_t buf_load16_nt(__amdgpu_buffer_rsrc_t r, uint3
     return __builtin_amdgcn_raw_buffer_load_b128(r, byte_off, 0, kCachePolicyNT);
 }
 
+// 16 bytes of each lane straight to LDS, to lds + kOff + 16 * lane (m0 = lds + kOff).  Inline
+// asm, so that the compiler does not make every later LDS read wait for it: the caller waits
+// (s_waitcnt vmcnt) before the barrier that publishes what was loaded.
+// gfx950 asks for 1 wait state between the write of m0 and the load, and the compiler counts
+// none around inline asm: the asm holds it.  tests/test_lds_load_isa.py reads the built code for it.
+template <int kOff = 0>
+__device__ __forceinline__ void lds_load16(uint32_t lds, uint32_t voffset, __amdgpu_buffer_rsrc_t r) {
+    if constexpr (kOff == 0)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :: "s"(lds), "v"(voffset), "s"(r) : "memory");
+    else
+        asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                     :: "s"(lds), "v"(voffset), "s"(r), "i"(kOff) : "memory", "scc");
+}
+template <int kOff = 0>
+__device__ __forceinline__ void lds_load16(uint32_t lds, uint32_t voffset, uint32_t soffset, __amdgpu_buffer_rsrc_t r) {
+    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(lds), "v"(voffset), "s"(r), "s"(soffset), "i"(kOff) : "memory", "scc");
+}
+// 4 bytes of each lane, to lds + 4 * lane.
+__device__ __forceinline__ void lds_load4(uint32_t lds, uint32_t voffset, __amdgpu_buffer_rsrc_t r) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :: "s"(lds), "v"(voffset), "s"(r) : "memory");
+}
+
 __device__ __forceinline__ bf16x8_t as_bf16x8(u32x4_t v) { return __builtin_bit_cast(bf16x8_t, v); }
 
 __device__ __forceinline__ f32x4_t mfma16(bf16x8_t a, bf16x8_t b, f32x4_t c) {

@@ -232,9 +232,7 @@ __device__ __forceinline__ void pf_unit(const PrefillParams& p, unsigned char* s
     // one SGPR per tile buffer stays live (one SGPR per instruction made the
     // compiler spill them and reload each with v_readlane in the loop).
     auto dma16 = [](auto ic, uint32_t base, uint32_t voffset, uint32_t soffset, __amdgpu_buffer_rsrc_t rsrc) {
-        constexpr int kOff = decltype(ic)::value * 4096;
-        asm volatile("s_add_u32 m0, %0, %4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                     :: "s"(base), "v"(voffset), "s"(rsrc), "s"(soffset), "i"(kOff) : "memory", "scc");
+        lds_load16<decltype(ic)::value * 4096>(base, voffset, soffset, rsrc);
     };
     // Instruction i of this wave fills the 1 KB at slot 64*(wave + 4*i) of a
     // tile; lane l writes slot 64*(wave + 4*i) + l, i.e. row r = slot / chunks,
@@ -498,9 +496,7 @@ __device__ __forceinline__ void pf_unit(const PrefillParams& p, unsigned char* s
         // (head dim 192: Q came straight into registers above)
         if constexpr (kStageQ) {
             auto dmaq = [](auto ic, uint32_t base, uint32_t voffset, __amdgpu_buffer_rsrc_t rsrc) {
-                constexpr int kOff = decltype(ic)::value * 1024;
-                asm volatile("s_add_u32 m0, %0, %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                             :: "s"(base), "v"(voffset), "s"(rsrc), "i"(kOff) : "memory", "scc");
+                lds_load16<decltype(ic)::value * 1024>(base, voffset, rsrc);
             };
             static_for<D::kRowBytes / 32>([&](auto ic) { dmaq(ic, q_lds, q_voff(decltype(ic)::value), qrs); });
         }
@@ -516,9 +512,7 @@ __device__ __forceinline__ void pf_unit(const PrefillParams& p, unsigned char* s
         }
     } else if constexpr (kStageQ) {
         auto dmaq = [](auto ic, uint32_t base, uint32_t voffset, __amdgpu_buffer_rsrc_t rsrc) {
-            constexpr int kOff = decltype(ic)::value * 1024;
-            asm volatile("s_add_u32 m0, %0, %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :: "s"(base), "v"(voffset), "s"(rsrc), "i"(kOff) : "memory", "scc");
+            lds_load16<decltype(ic)::value * 1024>(base, voffset, rsrc);
         };
         constexpr int kHalf = D::kRowBytes / 64;   // a group's share of the instructions
         static_for<kHalf>([&](auto ic) {

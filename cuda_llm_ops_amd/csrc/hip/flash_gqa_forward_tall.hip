@@ -110,8 +110,7 @@ __device__ __forceinline__ void o_scale(f32x16_t (&o)[4], float alpha) {
 // before the barrier that publishes the tile.
 template <int kOff>
 __device__ __forceinline__ void tl_dma(uint32_t base, uint32_t voffset, uint32_t soffset, __amdgpu_buffer_rsrc_t rsrc) {
-    asm volatile("s_add_u32 m0, %0, %4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :: "s"(base), "v"(voffset), "s"(rsrc), "s"(soffset), "i"(kOff) : "memory", "scc");
+    lds_load16<kOff>(base, voffset, soffset, rsrc);
 }
 
 // One segment (tiles [seg.lo, seg.hi) of the KV range) of 256-row unit
