@@ -367,6 +367,7 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
             else reg[i] = buf_load16(r, off);
         }
         if constexpr (kDma) {
+            lds_load_settle(rs);
             static_for<T::loads>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 lds_load16<i * T::rows * kHeadDim * 2>(lds, off, rs[i]);

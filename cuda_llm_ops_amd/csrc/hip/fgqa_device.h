@@ -81,8 +81,11 @@ __device__ __forceinline__ u32x4_t buf_load16_nt(__amdgpu_buffer_rsrc_t r, uint3
 // 16 bytes of each lane straight to LDS, to lds + kOff + 16 * lane (m0 = lds + kOff).  Inline
 // asm, so that the compiler does not make every later LDS read wait for it: the caller waits
 // (s_waitcnt vmcnt) before the barrier that publishes what was loaded.
-// gfx950 asks for 1 wait state between the write of m0 and the load, and the compiler counts
-// none around inline asm: the asm holds it.  tests/test_lds_load_isa.py reads the built code for it.
+// gfx950 asks for 1 wait state between the write of m0 and the load, and for 5 between a VALU write
+// of an SGPR (a descriptor taken from a lane, or a spilled one read back from one) and a
+// load that reads it, and the compiler counts neither around inline asm.  The asm holds the first;
+// lds_load_settle ahead of a group of loads the second (all 5 in each load took 3 to 5 %
+// of the prefill's and the backward's time).  tests/test_lds_load_isa.py reads the built code for both.
 template <int kOff = 0>
 __device__ __forceinline__ void lds_load16(uint32_t lds, uint32_t voffset, __amdgpu_buffer_rsrc_t r) {
     if constexpr (kOff == 0)
@@ -96,6 +99,13 @@ template <int kOff = 0>
 __device__ __forceinline__ void lds_load16(uint32_t lds, uint32_t voffset, uint32_t soffset, __amdgpu_buffer_rsrc_t r) {
     asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :: "s"(lds), "v"(voffset), "s"(r), "s"(soffset), "i"(kOff) : "memory", "scc");
+}
+// What the next loads read has been written 4 states before, 5 with their own write of m0.
+__device__ __forceinline__ void lds_load_settle(__amdgpu_buffer_rsrc_t a, __amdgpu_buffer_rsrc_t b, uint32_t c, uint32_t d) {
+    asm volatile("s_nop 3" :: "s"(a), "s"(b), "s"(c), "s"(d));
+}
+__device__ __forceinline__ void lds_load_settle(const __amdgpu_buffer_rsrc_t (&r)[4]) {
+    asm volatile("s_nop 3" :: "s"(r[0]), "s"(r[1]), "s"(r[2]), "s"(r[3]));
 }
 // 4 bytes of each lane, to lds + 4 * lane.
 __device__ __forceinline__ void lds_load4(uint32_t lds, uint32_t voffset, __amdgpu_buffer_rsrc_t r) {

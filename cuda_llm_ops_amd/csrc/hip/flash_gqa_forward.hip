@@ -264,6 +264,7 @@ __device__ __forceinline__ void pf_unit(const PrefillParams& p, unsigned char* s
         const uint32_t vdst = lds_base + 2 * D::kKTileBytes + vb * D::kVTileBytes + 1024 * wave;
         // K and V instructions interleaved, K first
         if (t0 + kPfTile - 1 <= kv_last) {   // whole tile in range
+            lds_load_settle(krs, vrs, (uint32_t)t0 * kss, (uint32_t)t0 * vss);
             static_for<D::kDmaK>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 if (kb >= 0) dma16(ic, kdst, koff_dma[i], (uint32_t)t0 * kss, krs);

@@ -135,15 +135,17 @@ def built(tmp_path_factory):
 
 
 def test_lds_load_wait_states(built):
-    counts, found_m0 = {}, []
+    counts, found_m0, found_sgprs = {}, [], []
     for name, asm in built.items():
-        loads, near_m0, _ = lds_load_hazards(asm)
+        loads, near_m0, near_sgprs = lds_load_hazards(asm)
         counts[name] = len(loads)
         found_m0 += [f"{name}: {x}" for x in near_m0 + m0_reads(asm)[1]]
+        found_sgprs += [f"{name}: {x}" for x in near_sgprs]
     with_loads = {n for n, c in counts.items() if c}
     assert {"decode_shared.hip", "flash_gqa_forward.hip", "flash_gqa_forward_tall.hip", "flash_gqa_backward.hip",
             "flash_gqa_backward_dkdv.hip"} <= with_loads, f"no load to LDS found: the check would pass vacuously ({counts})"
     assert not found_m0, f"{len(found_m0)}\n" + "\n".join(found_m0[:20])
+    assert not found_sgprs, f"{len(found_sgprs)}\n" + "\n".join(found_sgprs[:20])
 
 
 def test_scan_finds_planted_cases():
