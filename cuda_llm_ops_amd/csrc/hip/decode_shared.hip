@@ -302,7 +302,7 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
     constexpr bool kDma = kUni && T::bf16;
     [[maybe_unused]] u32x4_t kreg[T::loads], vreg[T::loads];
     [[maybe_unused]] float ksreg[T::loads], vsreg[T::loads];
-    const uint32_t kss = (uint32_t)(p.k_ss * kElem), vss = (uint32_t)(p.v_ss * kElem);
+    [[maybe_unused]] const uint32_t kss = (uint32_t)(p.k_ss * kElem), vss = (uint32_t)(p.v_ss * kElem);   // (kUni: below 2^31)
     // (straight to LDS: lane l fills piece l % 16 of row l / 16 of the wave's four)
     const int lane_row = lane / T::row_threads;
     [[maybe_unused]] const uint32_t koff =
@@ -340,14 +340,14 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
     };
     // else each row's page is looked up.  Tokens past the end read the last one again (their scores are masked;
     // the rows are numbers).
-    [[maybe_unused]] auto load_rows = [&](int first, const unsigned char* base, int64_t page_bytes, uint32_t row_bytes,
+    [[maybe_unused]] auto load_rows = [&](int first, const unsigned char* base, int64_t page_bytes, int64_t row_bytes,
                                           [[maybe_unused]] const float* scales, [[maybe_unused]] int64_t scale_page,
                                           u32x4_t (&reg)[T::loads], [[maybe_unused]] float (&sreg)[T::loads]) {
 #pragma unroll
         for (int i = 0; i < T::loads; ++i) {
             const int tok = min(max(first + lrow + i * T::rows, t0), t1 - 1);
             const int64_t page = min(max(bt[tok >> p.page_shift], 0), p.num_pages - 1);
-            reg[i] = *reinterpret_cast<const u32x4_t*>(base + page * page_bytes + (int64_t)(tok & pmask) * row_bytes + chunk * 16);
+            reg[i] = *reinterpret_cast<const u32x4_t*>(base + page * page_bytes + (tok & pmask) * row_bytes + chunk * 16);
             if constexpr (T::blocks) sreg[i] = scales[page * scale_page];
         }
     };
@@ -380,8 +380,8 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
             load_uni(j, pt_k, false, koff, kreg, lds0 + (j & 1) * kTileBytes);
             load_uni(j, pt_v, true, voff, vreg, lds0 + (2 + (j & 1)) * kTileBytes);
         } else {
-            load_rows(t0 + j * kTile + kBlock, kbase, p.k_sb * kElem, kss, kscales, p.ks_sp, kreg, ksreg);
-            load_rows(t0 + j * kTile, vbase, p.v_sb * kElem, vss, vscales, p.vs_sp, vreg, vsreg);
+            load_rows(t0 + j * kTile + kBlock, kbase, p.k_sb * kElem, p.k_ss * kElem, kscales, p.ks_sp, kreg, ksreg);
+            load_rows(t0 + j * kTile, vbase, p.v_sb * kElem, p.v_ss * kElem, vscales, p.vs_sp, vreg, vsreg);
         }
     };
     float* const scale_lds = reinterpret_cast<float*>(smem + 4 * kTileBytes);   // K's of two tiles, V's
