@@ -503,9 +503,11 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
             else if constexpr (n >= 5) vring[n - 5] = v_operand(j, h, n - 5);
             if constexpr (n == 0) {
                 const float m_block = half_max(top) * c;
-                // The maximum moves only where it is exceeded by more than 2^8 (P is at most 2^8 then).
-                if (__any(m_block > m_run + 8.f)) {
-                    const float m_new = fmaxf(m_run, m_block);
+                // What is subtracted is set 8 above a largest score and moves only where one exceeds it: P is
+                // at most 1 (P above 1 made sums of values near bf16's largest, and P times a large block's
+                // scale, infinite), and 2^-8 at least where it counts, which costs a float no bits.
+                if (__any(m_block > m_run)) {
+                    const float m_new = m_block > m_run ? m_block + 8.f : m_run;
                     const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new));
                     m_run = m_new;
                     l_run *= alpha;
