@@ -120,8 +120,8 @@ int fgqa_kv_compact(const fgqa_kv_compact_args* args, void* stream);
  *   q, o, lse, block_table, seqlens, max_seqlen, scale   as fgqa_decode_paged
  *   workspace     256-byte aligned, fgqa_decode_shared_workspace_bytes (it depends on the
  *                 sizes and the device, not on lengths); NULL and 0: the library's buffer
- * Sums and statistics are fp32; P (times V's scale) is rounded to bf16 for P.V over
- * shared tokens.  The work is cut as the lengths of all sequences ask: outputs may differ in
+ * Sums and statistics are fp32.  For P.V over shared tokens P is rounded to bf16 or, with block
+ * scales, held times V's scale in two bf16 numbers (16 bits, products below 2^-126 as 0).  The work is cut as the lengths of all sequences ask: outputs may differ in
  * rounding between batches, not between runs of one.  num_groups is at most 4096.
  * Over a cache with block scales a call of few tokens (batch * KV heads * max_seqlen at most
  * 1152 a CU) is fgqa_decode_blocks, which then takes less time.
