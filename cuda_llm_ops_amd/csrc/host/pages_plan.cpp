@@ -30,6 +30,25 @@ bool rows_apart(int n, int pages, int64_t stride) { return n <= 1 || stride >= p
 // Rows of a launch of up to 16 workgroups each.
 bool grid_ok(int64_t rows) { return rows < ((int64_t)1 << 20); }
 
+// An address, and whether the call uses it.
+struct Used {
+    const void* at;
+    bool used;
+};
+
+// Each output is at an address of its own (workgroups that plan for themselves would read what others write).
+template <size_t kOut, size_t kIn>
+bool outputs_apart(const Used (&out)[kOut], const Used (&in)[kIn]) {
+    for (size_t i = 0; i < kOut; ++i) {
+        if (!out[i].used) continue;
+        for (size_t j = 0; j < i; ++j)
+            if (out[j].used && out[i].at == out[j].at) return false;
+        for (const Used& x : in)
+            if (x.used && x.at == out[i].at) return false;
+    }
+    return true;
+}
+
 // A page's 16-byte pieces are counted in 32 bits.
 bool pages_ok(const fgqa_kv_cache& c) { return (i128)c.page_size * c.num_kv_heads * 16 < ((i128)1 << 30); }
 }  // namespace
@@ -111,10 +130,10 @@ int validate_kv_fork(const fgqa_kv_fork_args* a) {
                           (const void*)a->new_lens, (const void*)a->new_block_table, (const void*)a->new_seqlens,
                           (const void*)a->num_free})
         if (!aligned4(p)) return FGQA_ERR_UNSUPPORTED;
-    if (rows && (a->new_block_table == a->block_table || a->new_seqlens == a->seqlens || a->new_seqlens == a->new_lens ||
-                 a->new_seqlens == a->parents))
-        if (a->batch > 0) return FGQA_ERR_INVALID_ARGUMENT;
-    return FGQA_OK;
+    const bool old = rows && a->batch > 0, cells = rows && a->new_max_pages > 0;
+    const Used out[] = {{a->num_free, true}, {a->new_seqlens, rows}, {a->new_block_table, cells}};
+    const Used in[] = {{a->seqlens, old}, {a->block_table, old}, {a->parents, rows}, {a->new_lens, rows}, {a->held, true}};
+    return outputs_apart(out, in) ? FGQA_OK : FGQA_ERR_INVALID_ARGUMENT;
 }
 
 int validate_kv_compact_sizes(const fgqa_kv_compact_args* a) {
@@ -135,9 +154,11 @@ int validate_kv_compact(const fgqa_kv_compact_args* a) {
     if (st != FGQA_OK) return st;
     if (!written_apart(a->cache) || a->num_used == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
     if (a->batch > 0 && a->seqlens == nullptr) return FGQA_ERR_INVALID_ARGUMENT;
-    if (a->batch > 0 && a->max_pages > 0 &&
-        (a->block_table == nullptr || a->new_block_table == nullptr || a->new_block_table == a->block_table))
-        return FGQA_ERR_INVALID_ARGUMENT;
+    const bool cells = a->batch > 0 && a->max_pages > 0;
+    if (cells && (a->block_table == nullptr || a->new_block_table == nullptr)) return FGQA_ERR_INVALID_ARGUMENT;
+    const Used out[] = {{a->num_used, true}, {a->new_block_table, cells}};
+    const Used in[] = {{a->seqlens, a->batch > 0}, {a->block_table, cells}, {a->held, true}};
+    if (!outputs_apart(out, in)) return FGQA_ERR_INVALID_ARGUMENT;
     for (const void* p : {(const void*)a->block_table, (const void*)a->seqlens, (const void*)a->new_block_table,
                           (const void*)a->num_used})
         if (!aligned4(p)) return FGQA_ERR_UNSUPPORTED;

@@ -46,7 +46,7 @@ extern "C" {
  *   new_seqlens   device int32 [new_batch]
  *   num_free      device int32 [1]: free pages that are left, or, below 0, how many were missing
  *   workspace     16-byte aligned, fgqa_kv_fork_workspace_bytes; NULL and 0: the library's buffer
- * What is written lies apart from all that is read, and from each other.
+ * What is written lies apart from all that is read, and from each other (one address for two is refused).
  */
 typedef struct fgqa_kv_fork_args {
     fgqa_kv_cache cache;
@@ -84,7 +84,7 @@ int fgqa_kv_fork(const fgqa_kv_fork_args* args, void* stream);
  *   new_block_table  device int32 [batch, max_pages]: the new numbers; -1 in cells
  *                    past a sequence's tokens; entries outside [0, num_pages) as they are
  *   num_used         device int32 [1]: all pages from there on are free
- * What is written lies apart from all that is read.
+ * What is written lies apart from all that is read, and from each other (as above).
  */
 typedef struct fgqa_kv_compact_args {
     fgqa_kv_cache cache;
