@@ -1,5 +1,6 @@
-// One decode item over a paged cache of 8-bit codes with block scales (included
-// by decode_flash_gqa.hip, whose kernels share the work out and merge the items).
+// One decode item over a paged cache of 8-bit codes with block scales (included by
+// decode_item.h; the kernels of decode_flash_gqa.hip and decode_shared.hip share the work
+// out and merge the items).
 //
 // The mathematics is that of dec_item, on codes: with K = sK c_K and V = sV c_V
 // (one scale per page and KV head),
@@ -66,8 +67,8 @@ struct Step8 {
     float ks[4], vs[4];
 };
 
-// As dec_item: tokens [t_begin, t_end) (not empty, t_begin a multiple of 128)
-// of one sequence and kv head, by kNw waves.  Two steps' loads are in flight per
+// As dec_item: tokens [t_begin, t_end) (not empty, t_begin the first of a page or a
+// multiple of 128 from there) of one sequence and kv head, by kNw waves.  Two steps' loads are in flight per
 // wave.
 // kSeg (32, 16 or 8, for pages of at least that many rows whose bytes stay below
 // 2^31): a step is 1, 2 or 4 page segments, read through buffer resources that

@@ -11,9 +11,9 @@
 // A plan finds the groups and cuts all work into pieces of about equal token counts that
 // fill the chip; one launch runs them; one merges the partials.  The running launch's
 // workgroups plan for themselves up to 256 sequences: 4 samples of a prompt of 1000 tokens
-// of bf16, 8 KV heads, took 14.6 us, with the plan in a launch of its own 17.2 (128 of 8000,
-// one KV head: 35.4 and 53.7; 4 prompts of 8000 tokens of e4m3, 16 samples each: 52.4 and
-// 54.2; 128 questions to one document of 32,768 of bf16: 247 and 250).
+// of bf16, 8 KV heads, took 14.5 us, with the plan in a launch of its own 18.2 (128 of 8000,
+// one KV head: 34.3 and 64.4; 4 prompts of 8000 tokens of e4m3, 16 samples each: 55.6 and
+// 57.4; 128 questions to one document of 32,768 of bf16: 208 and 209, of e4m3: 276 and 283).
 #include <float.h>
 
 #include <algorithm>
@@ -257,8 +257,8 @@ __device__ __forceinline__ void static_for(F&& f) {
 // bytes stay below 2^31), read through a buffer resource that ends at the last token (rows past
 // it are zeros); the wave's pages come 64 loads at a time from one vector load of the table.
 // kFlat: 32 tokens of a block-scaled cache lie in one page, so that a step's scores have one factor, as they
-// have without block scales, and its P one too (128 questions to 32,768 tokens of e4m3: 244 us, with a
-// factor for each token 258).
+// have without block scales, and its P one too (128 questions to 32,768 tokens of e4m3: 276 us, with a
+// factor for each token 281).
 template <int kKv, int kSeg>
 __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned char* smem, const Item& it, int kvh) {
     using T = TileShape<kKv>;

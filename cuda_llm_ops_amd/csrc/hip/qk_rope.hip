@@ -9,7 +9,7 @@
 //
 // Both directions are bound by the bytes of the rows.  Forward, [4, 6001] tokens of 28
 // and 4 heads of 128: 72 us for 393 MB, 5.4 TB/s; one token of 64 conversations, 64 and
-// 8 heads: 3.4 us, of a launch.  Backward, [3, 5003] tokens of 32 and 8 heads: 103 us
+// 8 heads: 3.7 us, of a launch.  Backward, [3, 5003] tokens of 32 and 8 heads: 103 us
 // for 461 MB with its second launch, 4.5 TB/s.  A large copy reaches 4.96 TB/s.
 #include <algorithm>
 #include <math.h>

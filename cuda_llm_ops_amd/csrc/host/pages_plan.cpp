@@ -188,9 +188,10 @@ fgqa_decode_blocks_args as_decode_blocks(const fgqa_decode_shared_args* a) {
 }
 
 bool shared_as_blocks(const fgqa_decode_shared_args* a, int cus) {
-    // Tokens of a KV head for each CU, of sequences as long as they may be.  8 samples of 2000 tokens, 2 KV
-    // heads of int8: 10.6 us each on their own, 16.3 together; 137,000 tokens of all KV heads 12.9 to 14.4 and 19.3 to
-    // 21.5, 263,000 to 294,000 tokens 12.0 to 17.1 and 15.8 to 22.2, 550,000 28.6 to 36.4 and 18.8 to 25.7.
+    // Tokens of a KV head for each CU, of sequences as long as they may be.  Each on their own and together, e4m3
+    // to int8: 33,600 tokens of all KV heads 13.2 and 16.7 to 17.5 us (8 samples), 134,000 14 and 19.3 to 19.9, 282,000 17 to
+    // 18.9 and 22.6 to 23.1, 352,000 17.7 to 19.9 and 23.3 to 23.7, 422,000 (24 samples) 18.3 to 35.2 and 28.5 to 26.6,
+    // 480,000 20.5 to 23.6 and 23.6 to 24.5, 550,000 31.8 to 36 and 27.2 to 27.7: the rule ends where the first are always less.
     // (Without block scales the decode on their own takes longer from the start: 23.1 and 13.8.)
     constexpr int64_t kAloneTokens = 1152;
     return a->cache.k_scales != nullptr &&

@@ -102,6 +102,9 @@ bool rope_streams(const fgqa_rope_args& a, int passes) {
     // and 30.7 us for 168 MB, 43.8 and 44.8 for 256, 51.9 and 50.7 for 287, 92.3 and 86.1 for 492; those of the
     // backward 47.6 and 54.0 for 252, 70.0 and 69.0 for 307, 98 and 83.5 for 430, 148 and 136 for 737.  (Its loads alone
     // past them took 80 for 430, but 113 for 461 between other calls' data, where both took 103 and neither 110.)
+    // A prefill behind the forward, which reads what was written, takes the difference back: [4, 6001] tokens of 28 and 4
+    // heads 71 and 81 us, with the prefill 1020 and 1022 (window 512: 362 and 353), [2, 8192] of 32 and 8 heads 62 and 71,
+    // 967 and 964 (252 and 251).
     constexpr int64_t kRopeCache = (int64_t)1 << 28;
     const int64_t rows = (int64_t)a.batch * a.seqlen * ((int64_t)a.num_q_heads + a.num_kv_heads);   // (below 2^31)
     return rows * a.head_dim * 2 * passes > kRopeCache;

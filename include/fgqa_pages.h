@@ -122,7 +122,7 @@ int fgqa_kv_compact(const fgqa_kv_compact_args* args, void* stream);
  *                 sizes and the device, not on lengths); NULL and 0: the library's buffer
  * Sums and statistics are fp32.  For P.V over shared tokens P is rounded to bf16 or, with block
  * scales, held times V's scale in two bf16 numbers (16 bits, products below 2^-126 as 0).  The work is cut as the lengths of all sequences ask: outputs may differ in
- * rounding between batches, not between runs of one.  num_groups is at most 4096.
+ * rounding between batches, not between runs of one.  num_groups is at most 4096, batch below 32768.
  * Over a cache with block scales a call of few tokens (batch * KV heads * max_seqlen at most
  * 1152 a CU) is fgqa_decode_blocks, which then takes less time.
  */
