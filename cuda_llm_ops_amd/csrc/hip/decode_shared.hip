@@ -14,8 +14,6 @@
 // of bf16, 8 KV heads, took 14.5 us, with the plan in a launch of its own 18.2 (128 of 8000,
 // one KV head: 34.3 and 64.4; 4 prompts of 8000 tokens of e4m3, 16 samples each: 55.6 and
 // 57.4; 128 questions to one document of 32,768 of bf16: 208 and 209, of e4m3: 276 and 283).
-#include <float.h>
-
 #include <algorithm>
 #include <type_traits>
 
@@ -467,8 +465,9 @@ __device__ __forceinline__ void shared_item(const SharedParams& sp, unsigned cha
     // Written in the order that it is to be issued in: operands three or four products ahead (the first of the
     // tile's second half at the end of its first), nothing that waits for a product right behind it.
     bf16x8_t ring[4], vring[3];
-    // kFlat: block h's factor of the scores (above 0: masked scores stay -inf), and of P
-    [[maybe_unused]] auto k_factor = [&](int at, int h) { return fmaxf(scale_lds[at * kTile + h * kBlock], FLT_MIN); };
+    // kFlat: block h's factor of the scores (above 0: masked scores stay -inf; the least scale times the scores' is no
+    // normal number), and of P
+    [[maybe_unused]] auto k_factor = [&](int at, int h) { return fmaxf(scale_lds[at * kTile + h * kBlock], __FLT_DENORM_MIN__); };
     auto step = [&](int j, auto half_c, f32x16_t& s, f32x16_t& next, float& top, [[maybe_unused]] float factor,
                     [[maybe_unused]] float& next_factor) {
         constexpr int h = decltype(half_c)::value;
